@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define Q1ENV_ABI_VERSION 6
+#define Q1ENV_ABI_VERSION 7
 
 /* Environment variables the library reads (ALL of them; each is an A/B measurement knob read once per process, none changes a result bit):
  *   Q1ENV_HOST_DIRECT=0           the small-batch *_host paths stage through copy commands instead of the host-coherent block (csrc/q1env_core.hip)
@@ -580,6 +580,58 @@ typedef struct q1env_resident_args {
     double timeout_s;
 } q1env_resident_args;
 int q1env_sample_resident(q1env_t* env, const q1env_resident_args* args);
+
+/* ---- (ABI v7) wide categorical head and gradient clipping: training operators without an environment handle ---------------------
+ * These calls take a device index and a hipStream_t (NULL = the device's default stream) instead of a handle, are asynchronous on that stream,
+ * keep nothing between calls, allocate nothing and may be captured into a graph.  Two calls may run at the same time if they share no workspace
+ * or state.  Element types: */
+enum { Q1ENV_DT_F32 = 0, Q1ENV_DT_BF16 = 1, Q1ENV_DT_F16 = 2 };
+enum { Q1ENV_REDUCE_MEAN = 0, Q1ENV_REDUCE_SUM = 1 };
+
+/* A categorical distribution over `classes` per row of hidden, logits l = hidden weight^T + bias, which are never stored: what the discrete
+ * mouse's child distribution of Q1PhysActionDist (q1physrl/action_dist.py:221-222; Discrete(2S+1), env.py:216-219) is over logits that exist.
+ *   lse_i = log sum_j exp l_ij    logp_i = l_i,target(i) - lse_i    H_i = lse_i - sum_j p_ij l_ij
+ * hidden, weight, bias have one element type; products are accumulated and all statistics are held in float32.  float32 operands keep their
+ * 24 bits (three bfloat16 pieces, six matrix products).  A class whose bias is -inf takes no part; a row without any class left is NaN, as is a
+ * row whose target lies outside 0 .. classes - 1 (and its gradients).  Rows with target == ignore_index are padding: logp = H = 0, no
+ * gradient, not counted by the mean, whatever their hidden row holds (NaN included).  Results do not depend on how the device is occupied:
+ * the same call gives the same bits. */
+typedef struct q1env_head {
+    int32_t dtype;                       /* Q1ENV_DT_* of hidden, weight, bias and their gradients */
+    int32_t target_bits;                 /* 32 or 64: int32 / int64 targets */
+    int64_t rows, width, classes;        /* 0 .. 2^22, 1 .. 2^16, 1 .. 2^22 */
+    int64_t ignore_index;
+    const void* hidden_dev; int64_t hidden_stride;       /* [rows][width], elements from row to row (>= width) */
+    const void* weight_dev; int64_t weight_stride;       /* [classes][width] */
+    const void* bias_dev;                /* [classes] or NULL */
+    const void* target_dev;              /* [rows]; not read by the backward call */
+    void* state_dev;                     /* q1env_head_state_bytes: written by the forward call, read by the backward call */
+    void* ws_dev; uint64_t ws_bytes;     /* q1env_head_workspace_bytes: nothing in it outlives a call */
+} q1env_head;
+/* host arithmetic; 0 for arguments out of range.  backward = 0 / 1: of the forward / backward call */
+uint64_t q1env_head_state_bytes(int64_t rows);
+uint64_t q1env_head_workspace_bytes(int dtype, int64_t rows, int64_t width, int64_t classes, int backward);
+/* logp float[rows]; entropy float[rows] or NULL; loss (one float) or NULL: minus the sum (Q1ENV_REDUCE_SUM) of logp, or minus its mean over the
+ * rows that are not ignored (Q1ENV_REDUCE_MEAN; 0 when all are). */
+int q1env_head_forward(int device, void* stream, const q1env_head* head, int reduction, float* logp_dev, float* entropy_dev, float* loss_dev);
+/* The gradients of hidden, weight and bias (each may be NULL) for EITHER dlogp / dentropy (float[rows], one may be NULL) OR dloss (one float: the
+ * gradient of the loss the forward call wrote).  The head is the one the forward call had, with its state; results are overwritten. */
+int q1env_head_backward(int device, void* stream, const q1env_head* head, const float* dlogp_dev, const float* dentropy_dev, const float* dloss_dev,
+                        void* dhidden_dev, int64_t dhidden_stride, void* dweight_dev, int64_t dweight_stride, void* dbias_dev);
+
+/* The global norm of `count` gradient tensors, |scale| sqrt(sum of squares) (squares summed in float64), and clipping by it - RLlib's `grad_clip`
+ * (tf.clip_by_global_norm in its TF policies; the reference leaves it unset, data/params.yml:2-13):
+ *   dst = src x scale x (norm <= max_norm ? 1 : max_norm / norm)
+ * Tensor i holds values[i] elements of type dtype[i] at src[i] (device addresses in HOST arrays, read before the call returns): contiguous, or -
+ * where cols is given and cols[i] != 0 - rows of cols[i] elements, src_pitch[i] / dst_pitch[i] elements apart.  dst[i] == src[i] clips in place (nothing
+ * is written when there is nothing to scale); a result that overlaps another tensor is refused.  A norm that is not finite is reported as it is:
+ * a NaN norm makes every result NaN, an infinite one turns finite values to zero.  norm: one float on the device. */
+uint64_t q1env_grad_norm_workspace_bytes(int count);
+int q1env_grad_norm(int device, void* stream, int count, const void* const* src, const int64_t* values, const int32_t* dtype, const int64_t* cols,
+                    const int64_t* pitch, double scale, float* norm_dev, void* ws_dev, uint64_t ws_bytes);
+int q1env_grad_clip(int device, void* stream, int count, const void* const* src, void* const* dst, const int64_t* values, const int32_t* dtype,
+                    const int64_t* cols, const int64_t* src_pitch, const int64_t* dst_pitch, double scale, double max_norm, float* norm_dev,
+                    void* ws_dev, uint64_t ws_bytes);
 
 /* ---- persistent tick server (experimental) -----------------------------------------------------
  * One resident grid serves `ticks` ticks without a kernel boundary per tick: the env state stays in registers and tick t's action is

@@ -13,7 +13,9 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 # Q1ENV_LIB_PATH selects another build of the SAME library (tools/asan_check.sh: the AddressSanitizer build of the host side)
 LIB_PATH = os.environ.get("Q1ENV_LIB_PATH") or os.path.join(_PKG, "libq1env.so")
 
-ABI_VERSION = 6
+ABI_VERSION = 7
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+REDUCE_MEAN, REDUCE_SUM = 0, 1
 ACT_F64_ROWS, ACT_F32_ROWS, ACT_PACKED, ACT_RANDOM = 0, 1, 2, 3
 OBS_F64, OBS_F32 = 0, 1
 TIMER_START, TIMER_STOP = 4, 8     # q1env_step_many use_graph flags: record the handle's start / stop timer event around the launches
@@ -66,6 +68,12 @@ class Q1LearnerBatch(C.Structure):   # q1env_learner_batch
                 ("value_old_dev", C.c_void_p), ("vtarg_dev", C.c_void_p),
                 ("clip_param", C.c_float), ("vf_clip_param", C.c_float), ("vf_loss_coeff", C.c_float), ("entropy_coeff", C.c_float),
                 ("kl_coeff_dev", C.c_void_p), ("stats_partials_dev", C.c_void_p), ("skip_reduce", C.c_int), ("saturation_dev", C.c_void_p)]
+
+
+class Q1Head(C.Structure):           # q1env_head
+    _fields_ = [("dtype", C.c_int32), ("target_bits", C.c_int32), ("rows", C.c_int64), ("width", C.c_int64), ("classes", C.c_int64), ("ignore_index", C.c_int64),
+                ("hidden_dev", C.c_void_p), ("hidden_stride", C.c_int64), ("weight_dev", C.c_void_p), ("weight_stride", C.c_int64),
+                ("bias_dev", C.c_void_p), ("target_dev", C.c_void_p), ("state_dev", C.c_void_p), ("ws_dev", C.c_void_p), ("ws_bytes", C.c_uint64)]
 
 
 STATE_FIELDS = (("vel_x", np.float32, 1), ("vel_y", np.float32, 1), ("vel_z", np.float32, 1),
@@ -148,6 +156,13 @@ _SIGNATURES = {
     "q1env_signal_mark": (C.c_int, [_P]),
     "q1env_signal_wait": (C.c_int, [_P, C.c_double]),
     "q1env_signal_read": (C.c_int, [_P, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), C.POINTER(C.c_double)]),
+    "q1env_head_state_bytes": (C.c_uint64, [C.c_int64]),
+    "q1env_head_workspace_bytes": (C.c_uint64, [C.c_int] + [C.c_int64] * 3 + [C.c_int]),
+    "q1env_head_forward": (C.c_int, [C.c_int, _P, C.POINTER(Q1Head), C.c_int, _P, _P, _P]),
+    "q1env_head_backward": (C.c_int, [C.c_int, _P, C.POINTER(Q1Head), _P, _P, _P, _P, C.c_int64, _P, C.c_int64, _P]),
+    "q1env_grad_norm_workspace_bytes": (C.c_uint64, [C.c_int]),
+    "q1env_grad_norm": (C.c_int, [C.c_int, _P, C.c_int] + [_P] * 5 + [C.c_double, _P, _P, C.c_uint64]),
+    "q1env_grad_clip": (C.c_int, [C.c_int, _P, C.c_int] + [_P] * 7 + [C.c_double] * 2 + [_P, _P, C.c_uint64]),
     "q1env_build_id": (C.c_char_p, []),
     "q1env_timer_start": (C.c_int, [_P]),
     "q1env_timer_stop": (C.c_int, [_P, C.POINTER(C.c_float)]),

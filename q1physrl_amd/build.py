@@ -40,6 +40,9 @@ TU_FLAGS = {"q1env_learner.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
             # the persistent learner: the same register form (its step loop read 220 accumulator registers back per step), and NO atomic
             # optimizer: that pass rewrites a uniform-address atomic into a wave reduction + s_waitcnt vmcnt(0) + readfirstlane, i.e. it
             # makes the barrier poll that is requested early and looked at late (q1learner_persist.hpp, barrier 3) synchronous again
+            # the training operators: without the packed float32 instructions, which the compiler otherwise forms from ordinary float code
+            "q1env_head.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
+            "q1env_clip.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
             "q1env_plearner.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]}
 LINK_FLAGS = ["--offload-arch=gfx950", "-shared", "-fPIC"]
 HIPCC_FLAGS = COMPILE_FLAGS + ["-shared"]     # (kept for tools that compile a single file the old way, e.g. tools/asan_check.sh)

@@ -1,0 +1,324 @@
+// q1env_clip.hip - the global norm of many gradient tensors and clipping by it (include/q1env.h q1env_grad_norm / q1env_grad_clip).
+//
+//   norm = |scale| sqrt(sum over all tensors of g^2);   out = g x scale x (norm <= max_norm ? 1 : max_norm / norm)
+//
+// Two passes: squares summed in float64 (no overflow or underflow of a float32 gradient's square, and an order fixed by the sizes alone: the
+// same bits every time), one partial per workgroup; then every workgroup adds the partials up in the same order - cheaper than a third
+// launch - and writes its share.  The tensors travel in the kernel arguments, so nothing is uploaded, nothing is kept between calls and a captured launch holds
+// its own table.
+#include "q1env_host.hpp"
+
+#include <algorithm>
+
+namespace {
+
+constexpr int TENSORS = 96;                       // per launch: 96 x 40 bytes, under 4 KB of kernel arguments
+constexpr int THREADS = 256;
+constexpr int MAX_BLOCKS = 2048;                  // eight workgroups per CU
+constexpr int64_t UNIT_MIN = 1024, UNIT_MAX = 8192;      // values a workgroup takes at a time
+
+struct __attribute__((packed, aligned(4))) Tensor {
+    const void* src;
+    void* dst;
+    int64_t count;
+    int32_t cols;                                 // 0 = contiguous, else values per row of the pitched form
+    int32_t src_pitch, dst_pitch;                 // values from row to row
+};
+
+struct Table {
+    Tensor t[TENSORS];
+    uint32_t first[TENSORS];                      // first unit of each tensor
+    uint32_t n, units, unit;
+    uint32_t dtype;
+};
+static_assert(sizeof(Table) <= 4000, "the table has to fit the kernel arguments");
+
+template <int DT> struct El { typedef uint16_t type; };
+template <> struct El<Q1ENV_DT_F32> { typedef float type; };
+template <int DT> __device__ __forceinline__ float value(typename El<DT>::type v) {
+    if constexpr (DT == Q1ENV_DT_F32) return v;
+    else if constexpr (DT == Q1ENV_DT_BF16) return __builtin_bit_cast(float, (uint32_t)v << 16);
+    else return (float)__builtin_bit_cast(_Float16, v);
+}
+template <int DT> __device__ __forceinline__ typename El<DT>::type rounded(float v) {
+    if constexpr (DT == Q1ENV_DT_F32) return v;
+    else if constexpr (DT == Q1ENV_DT_BF16) return __builtin_bit_cast(uint16_t, (__bf16)v);
+    else return __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+__device__ __forceinline__ double block_sum(double a, double* red) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) a += __shfl_down(a, off, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
+// runs f(tensor, first value, end) over the units of workgroup blockIdx.x: an even share, in the order of the table
+template <typename F> __device__ __forceinline__ void each_unit(const Table& tb, F f) {
+    const uint32_t per = (tb.units + gridDim.x - 1) / gridDim.x;
+    uint32_t u = blockIdx.x * per;
+    const uint32_t end = u + per < tb.units ? u + per : tb.units;
+    if (u >= end) return;
+    uint32_t lo = 0, hi = tb.n;                   // the last tensor whose first unit is <= u
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (tb.first[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    for (; u < end; ++u) {
+        while (lo + 1 < tb.n && tb.first[lo + 1] <= u) ++lo;
+        const int64_t a = (int64_t)(u - tb.first[lo]) * tb.unit;
+        const int64_t b = a + tb.unit < tb.t[lo].count ? a + tb.unit : tb.t[lo].count;
+        f(tb.t[lo], a, b);
+    }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(THREADS) squares_kernel(Table tb, double* __restrict__ partial) {
+    typedef typename El<DT>::type E;
+    constexpr int V = 16 / sizeof(E);
+    __shared__ double red[4];
+    double acc = 0.0;
+    each_unit(tb, [&](const Tensor& t, int64_t a, int64_t b) {
+        const E* p = (const E*)t.src;
+        if (t.cols) {
+            for (int64_t i = a + threadIdx.x; i < b; i += THREADS) {
+                const int64_t r = i / t.cols;
+                const double x = (double)value<DT>(p[r * t.src_pitch + (i - r * t.cols)]);
+                acc = fma(x, x, acc);
+            }
+            return;
+        }
+        int64_t i = a + (int64_t)threadIdx.x * V;
+        for (; i + V <= b; i += THREADS * V) {
+            E v[V];
+            __builtin_memcpy(v, p + i, 16);
+#pragma unroll
+            for (int j = 0; j < V; ++j) { const double x = (double)value<DT>(v[j]); acc = fma(x, x, acc); }
+        }
+        for (; i < b; ++i) { const double x = (double)value<DT>(p[i]); acc = fma(x, x, acc); }
+    });
+    acc = block_sum(acc, red);
+    if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+// the norm from the partials, the same in every workgroup
+__device__ __forceinline__ double norm_of(const double* __restrict__ partial, int n, double scale, double* red) {
+    double a = 0.0;
+    for (int i = threadIdx.x; i < n; i += THREADS) a += partial[i];
+    return sqrt(block_sum(a, red)) * fabs(scale);
+}
+
+__global__ void __launch_bounds__(THREADS) norm_kernel(const double* __restrict__ partial, int n, double scale, float* __restrict__ norm) {
+    __shared__ double red[4];
+    const double v = norm_of(partial, n, scale, red);
+    if (threadIdx.x == 0) *norm = (float)v;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(THREADS) clip_kernel(Table tb, const double* __restrict__ partial, int n, double scale, double max_norm, float* __restrict__ norm) {
+    typedef typename El<DT>::type E;
+    constexpr int V = 16 / sizeof(E);
+    __shared__ double red[4];
+    const double v = norm_of(partial, n, scale, red);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+    const float c = (float)(scale * (v <= max_norm ? 1.0 : max_norm / v));       // a NaN norm makes every value NaN
+    each_unit(tb, [&](const Tensor& t, int64_t a, int64_t b) {
+        const E* p = (const E*)t.src;
+        E* q = (E*)t.dst;
+        if (c == 1.0f && (const E*)q == p) return;                               // in place and nothing to clip
+        if (t.cols) {
+            for (int64_t i = a + threadIdx.x; i < b; i += THREADS) {
+                const int64_t r = i / t.cols, k = i - r * t.cols;
+                q[r * t.dst_pitch + k] = rounded<DT>(value<DT>(p[r * t.src_pitch + k]) * c);
+            }
+            return;
+        }
+        int64_t i = a + (int64_t)threadIdx.x * V;
+        for (; i + V <= b; i += THREADS * V) {
+            E w[V];
+            __builtin_memcpy(w, p + i, 16);
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = rounded<DT>(value<DT>(w[j]) * c);
+            __builtin_memcpy(q + i, w, 16);
+        }
+        for (; i < b; ++i) q[i] = rounded<DT>(value<DT>(p[i]) * c);
+    });
+}
+
+size_t elem_size(int dt) { return dt == Q1ENV_DT_F32 ? 4 : 2; }
+
+// what a call hands over, and how it is cut into launches
+struct Job {
+    int count;
+    const void* const* src;
+    void* const* dst;
+    const int64_t* values;
+    const int32_t* dtype;
+    const int64_t *cols, *src_pitch, *dst_pitch;
+};
+
+struct Span { uintptr_t a, b; int i; uintptr_t pitch, row; };        // bytes
+
+// two pitched tensors of the same pitch may interleave: column slices of one matrix
+bool apart(const Span& x, const Span& y) {
+    if (x.b <= y.a || y.b <= x.a) return true;
+    if (!x.pitch || x.pitch != y.pitch) return false;
+    const uintptr_t off = y.a >= x.a ? (y.a - x.a) % x.pitch : (x.pitch - (x.a - y.a) % x.pitch) % x.pitch;      // y's columns within x's rows
+    return off >= x.row && off + y.row <= x.pitch;
+}
+
+int check_job(const char* who, const Job& j, bool write) {
+    if (j.count < 0 || j.count > 65536) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": tensor count out of range (0 .. 65536)");
+    if (j.count > 0 && (!j.src || !j.values || !j.dtype || (write && !j.dst))) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": null argument");
+    if (j.cols && (!j.src_pitch || (write && !j.dst_pitch))) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": pitched tensors need their pitches");
+    int64_t total = 0;
+    for (int i = 0; i < j.count; ++i) {
+        const int dt = j.dtype[i];
+        if (dt != Q1ENV_DT_F32 && dt != Q1ENV_DT_BF16 && dt != Q1ENV_DT_F16) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": unknown dtype");
+        if (j.values[i] < 0 || j.values[i] > (int64_t)1 << 40) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": a tensor's size is out of range");
+        total += j.values[i];
+        if (j.values[i] == 0) continue;
+        if (!j.src[i] || (write && !j.dst[i])) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": a tensor's address is NULL");
+        if ((uintptr_t)j.src[i] % elem_size(dt) || (write && (uintptr_t)j.dst[i] % elem_size(dt)))
+            return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": an address is not aligned to its element size");
+        if (j.cols && j.cols[i] != 0) {
+            const int64_t c = j.cols[i];
+            if (c < 0 || c > INT32_MAX || j.values[i] % c || j.src_pitch[i] < c || j.src_pitch[i] > INT32_MAX || (write && (j.dst_pitch[i] < c || j.dst_pitch[i] > INT32_MAX)))
+                return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": bad columns / pitch of a pitched tensor");
+        }
+    }
+    if (total > (int64_t)1 << 42) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": more than 2^42 values");
+    if (!write) return 0;
+    // no value is written by one tensor and read or written by another: every destination against all spans
+    std::vector<Span> s;
+    s.reserve(2 * (size_t)j.count);
+    for (int i = 0; i < j.count; ++i) {
+        if (j.values[i] == 0) continue;
+        const uintptr_t es = elem_size(j.dtype[i]);
+        const int64_t c = j.cols && j.cols[i] ? j.cols[i] : j.values[i], rows = j.values[i] / c;
+        const uintptr_t sp = j.cols && j.cols[i] ? (uintptr_t)j.src_pitch[i] * es : 0, dp = j.cols && j.cols[i] ? (uintptr_t)j.dst_pitch[i] * es : 0;
+        const uintptr_t sa = (uintptr_t)j.src[i], da = (uintptr_t)j.dst[i];
+        s.push_back({da, da + (rows - 1) * dp + c * es, i, dp, c * es});
+        if (sa != da || sp != dp) s.push_back({sa, sa + (rows - 1) * sp + c * es, ~i, sp, c * es});      // ~i: a source
+    }
+    std::sort(s.begin(), s.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
+    std::vector<size_t> open;
+    for (size_t k = 0; k < s.size(); ++k) {
+        size_t kept = 0;
+        for (size_t o : open) {
+            if (s[o].b <= s[k].a) continue;
+            open[kept++] = o;
+            if ((s[o].i >= 0 || s[k].i >= 0) && !apart(s[o], s[k]))
+                return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": a result overlaps another tensor (the same tensor twice, or a destination that is not its own source)");
+        }
+        open.resize(kept);
+        open.push_back(k);
+    }
+    return 0;
+}
+
+// cuts the tensors into tables of one dtype and at most TENSORS entries and launches go(table, blocks, first block) for each
+template <typename F> int each_table(const Job& j, int64_t unit, int max_blocks, F go) {
+    int at = 0, block0 = 0;
+    int64_t all_units = 0;
+    for (int i = 0; i < j.count; ++i) all_units += (j.values[i] + unit - 1) / unit;
+    Table tb;
+    while (at < j.count) {
+        tb.n = 0;
+        tb.unit = (uint32_t)unit;
+        tb.dtype = (uint32_t)j.dtype[at];
+        uint64_t units = 0;
+        for (; at < j.count && tb.n < TENSORS && (uint32_t)j.dtype[at] == tb.dtype; ++at) {
+            if (j.values[at] == 0) continue;
+            Tensor& t = tb.t[tb.n];
+            t.src = j.src[at];
+            t.dst = j.dst ? j.dst[at] : nullptr;
+            t.count = j.values[at];
+            t.cols = j.cols ? (int32_t)j.cols[at] : 0;
+            t.src_pitch = t.cols ? (int32_t)j.src_pitch[at] : 0;
+            t.dst_pitch = t.cols && j.dst ? (int32_t)j.dst_pitch[at] : 0;
+            tb.first[tb.n++] = (uint32_t)units;
+            units += (uint64_t)((j.values[at] + unit - 1) / unit);
+        }
+        if (tb.n == 0) continue;
+        tb.units = (uint32_t)units;
+        int64_t blocks = (int64_t)((double)max_blocks * (double)units / (double)all_units);      // this table's share
+        blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)units));
+        if (int rc = go(tb, (unsigned)blocks, block0)) return rc;
+        block0 += (int)blocks;
+    }
+    return 0;
+}
+
+int64_t unit_of(const Job& j) {
+    int64_t total = 0;
+    for (int i = 0; i < j.count; ++i) total += j.values[i];
+    int64_t unit = UNIT_MIN;
+    while (unit < UNIT_MAX && total / unit > MAX_BLOCKS) unit *= 2;
+    return unit;
+}
+
+int run(const char* who, int device, hipStream_t stream, const Job& j, bool write, double scale, double max_norm, float* norm, void* ws, uint64_t ws_bytes) {
+    if (int rc = check_job(who, j, write)) return rc;
+    if (!norm) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": norm is NULL");
+    if (!(scale > 0.0) || std::isinf(scale)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": scale must be positive and finite");
+    if (write && !(max_norm >= 0.0)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": max_norm must not be negative or NaN");
+    if (!ws || ws_bytes < q1env_grad_norm_workspace_bytes(j.count)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": workspace smaller than q1env_grad_norm_workspace_bytes");
+    const int64_t unit = unit_of(j);
+    for (int i = 0; i < j.count; ++i)
+        if (j.values[i] / unit > (int64_t)1 << 30) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": a tensor's size is out of range");
+    int n = 0;
+    if (hipGetDeviceCount(&n) != hipSuccess || n == 0) return fail(Q1ENV_ERR_NO_DEVICE, std::string(who) + ": no HIP device (there is no CPU fallback)");
+    if (device < 0 || device >= n) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": no such device");
+    DeviceGuard guard(device);
+    double* partial = (double*)ws;
+    int parts = 0;
+    int rc = each_table(j, unit, MAX_BLOCKS, [&](const Table& tb, unsigned blocks, int block0) -> int {
+        parts = block0 + (int)blocks;
+        if (tb.dtype == Q1ENV_DT_F32) hipLaunchKernelGGL((squares_kernel<Q1ENV_DT_F32>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial + block0);
+        else if (tb.dtype == Q1ENV_DT_BF16) hipLaunchKernelGGL((squares_kernel<Q1ENV_DT_BF16>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial + block0);
+        else hipLaunchKernelGGL((squares_kernel<Q1ENV_DT_F16>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial + block0);
+        HIP_TRY(hipGetLastError());
+        return 0;
+    });
+    if (rc) return rc;
+    if (!write || parts == 0) {
+        hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(THREADS), 0, stream, partial, parts, scale, norm);
+        HIP_TRY(hipGetLastError());
+        return Q1ENV_OK;
+    }
+    return each_table(j, unit, MAX_BLOCKS, [&](const Table& tb, unsigned blocks, int block0) -> int {
+        float* out = block0 == 0 ? norm : nullptr;
+        if (tb.dtype == Q1ENV_DT_F32) hipLaunchKernelGGL((clip_kernel<Q1ENV_DT_F32>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial, parts, scale, max_norm, out);
+        else if (tb.dtype == Q1ENV_DT_BF16) hipLaunchKernelGGL((clip_kernel<Q1ENV_DT_BF16>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial, parts, scale, max_norm, out);
+        else hipLaunchKernelGGL((clip_kernel<Q1ENV_DT_F16>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial, parts, scale, max_norm, out);
+        HIP_TRY(hipGetLastError());
+        return 0;
+    });
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t q1env_grad_norm_workspace_bytes(int count) {
+    // one partial per workgroup: MAX_BLOCKS shares, and one more for each table that is too small for a share (a table per TENSORS tensors or change of dtype)
+    return count < 0 || count > 65536 ? 0 : 8ull * (MAX_BLOCKS + (uint64_t)count + 1);
+}
+
+int q1env_grad_norm(int device, void* stream, int count, const void* const* src, const int64_t* values, const int32_t* dtype, const int64_t* cols, const int64_t* pitch, double scale,
+                    float* norm, void* ws, uint64_t ws_bytes) {
+    const Job j{count, src, nullptr, values, dtype, cols, pitch, nullptr};
+    return run("q1env_grad_norm", device, (hipStream_t)stream, j, false, scale, 0.0, norm, ws, ws_bytes);
+}
+
+int q1env_grad_clip(int device, void* stream, int count, const void* const* src, void* const* dst, const int64_t* values, const int32_t* dtype, const int64_t* cols,
+                    const int64_t* src_pitch, const int64_t* dst_pitch, double scale, double max_norm, float* norm, void* ws, uint64_t ws_bytes) {
+    const Job j{count, src, dst, values, dtype, cols, src_pitch, dst_pitch};
+    return run("q1env_grad_clip", device, (hipStream_t)stream, j, true, scale, max_norm, norm, ws, ws_bytes);
+}
+
+}  // extern "C"

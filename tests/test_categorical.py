@@ -1,0 +1,402 @@
+"""The wide categorical head (q1physrl_amd/categorical.py, q1env_head_*): against the definition in float64, at the sizes, masks, strides and types
+where tiles end, and its refusals (those need no GPU).
+
+Tolerances, from the arithmetic alone (u = 2^-24, float32's half step; ut = the type's half step):
+  a logit: D products and sums in float32, the accumulator possibly truncating: at most (D + 8) 2u S with S = sum_k |h_k w_k| + |b| -> el
+  log-sum-exp: the largest el, the sum of the exponentials with at most 256 + V / 2048 additions in a chain and one exponential of 4u per term,
+    the logarithm and the final sums at their own magnitude: el + (256 + V / 2048 + 16) 2u + 8u |lse|
+  log-probability: that and el again; entropy: each p (log p) to the relative error e of p plus the error of log p
+  a gradient of a logit: its parts to e relative, and half a step ut of the type it is stored in (float32: 2^-24); a product over K of them: (K + 8) 2u of
+    the sum of the absolute products more, half a step ut of the result, and in float16 the subnormal step 2^-25 of the result and of the scaled store."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from q1physrl_amd import _lib, categorical
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+IGN = -100
+gpu = pytest.mark.gpu
+
+
+def make(n, d, v, dtype, bias=True, seed=0, ignored=0.1, spread=2.5):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    h = torch.tanh(torch.randn(n, d, device="cuda", generator=g)).to(dtype)
+    w = (torch.randn(v, d, device="cuda", generator=g) * (spread / math.sqrt(d))).to(dtype)
+    b = torch.randn(v, device="cuda", generator=g).to(dtype) if bias else None
+    t = torch.randint(0, v, (n,), device="cuda", generator=g)
+    t[torch.rand(n, device="cuda", generator=g) < ignored] = IGN
+    return h, w, b, t
+
+
+class Truth:
+    """The definition in float64, and how far each result may be off."""
+
+    def __init__(self, h, w, b, t, ignore=IGN):
+        self.dtype, self.d, self.v = h.dtype, h.shape[1], w.shape[0]
+        self.ok = t != ignore
+        self.t = torch.where(self.ok, t.long(), 0)
+        self.h = torch.where(self.ok[:, None], h.detach().double(), 0.0)       # what an ignored row holds does not matter
+        self.w = w.detach().double()
+        self.b = torch.zeros(self.v, dtype=torch.float64, device=h.device) if b is None else b.detach().double()
+        z = self.h @ self.w.T + self.b
+        self.lse = torch.logsumexp(z, 1)
+        self.lp = z - self.lse[:, None]
+        self.p = self.lp.exp()
+        self.lp = torch.where(self.p > 0, self.lp, 0.0)                        # a class at -inf takes no part
+        self.logp = torch.where(self.ok, z.gather(1, self.t[:, None])[:, 0] - self.lse, 0.0)
+        self.entropy = torch.where(self.ok, -(self.p * self.lp).sum(1), 0.0)
+        fin = torch.where(torch.isfinite(self.b), self.b.abs(), 0.0)
+        self.el = ((self.d + 8) * 2 * U * (self.h.abs() @ self.w.abs().T + fin)).amax(1)
+        self.elogp = 2 * self.el + (256 + self.v / 2048 + 16) * 2 * U + 8 * U * (self.lse.abs() + self.logp.abs() + 1)
+        self.e = 2 * self.elogp                                                # relative error of a probability
+        self.eent = self.e * (self.p * (self.lp.abs() + 1)).sum(1) + self.elogp
+
+    def grads(self, A, E):
+        """(dh, dw, db) and their tolerances for upstream A = d/dlogp, E = d/dentropy (rows)."""
+        A, E = (torch.where(self.ok, x.double(), 0.0) for x in (A, E))
+        g = -self.p * (A[:, None] + E[:, None] * (self.lp + self.entropy[:, None]))
+        g.scatter_add_(1, self.t[:, None], A[:, None])
+        size = self.p * (A.abs()[:, None] + E.abs()[:, None] * (self.lp.abs() + self.entropy[:, None] + 1))
+        ut = HALF[self.dtype]
+        n = self.h.shape[0]
+        off = size * self.e[:, None] + g.abs() * ut + 4 * U * size.scatter_add(1, self.t[:, None], A.abs()[:, None])
+        if self.dtype == torch.float16:                                        # the scaled store's smallest step: at most 2^-25 of 2^-13 of the largest bound
+            off = off + torch.where(self.ok, 2.0 ** -38 * (A.abs() + 16 * E.abs()).max(), 0.0)[:, None]
+        tiny = 2.0 ** -25 if self.dtype == torch.float16 else 0.0
+
+        def tol(k, err, size_, ref):
+            return err * (1 + 1e-3) + (k + 8) * 2 * U * size_ + ut * ref.abs() * 1.01 + tiny + 1e-30
+        dh, dw, db = g @ self.w, g.T @ self.h, g.sum(0)
+        return ((dh, tol(self.v, off @ self.w.abs(), (g.abs() + off) @ self.w.abs(), dh)), (dw, tol(n, off.T @ self.h.abs(), (g.abs() + off).T @ self.h.abs(), dw)),
+                (db, tol(n, off.sum(0), (g.abs() + off).sum(0), db)))
+
+
+def near(got, ref, tol, what):
+    got = got.detach().double()
+    assert got.shape == ref.shape, what
+    assert bool(torch.isfinite(got).all()), f"{what}: not finite"
+    over = (got - ref).abs() - tol
+    assert float(over.max() if over.numel() else -1.0) <= 0.0, f"{what}: {float((got - ref).abs().max()):.3g} off, {float(over.max()):.3g} over what the arithmetic allows"
+
+
+SIZES = [(1, 1, 1), (1, 16, 2), (3, 5, 7), (1, 256, 721), (33, 64, 129), (127, 256, 361), (130, 200, 1000), (257, 72, 65), (64, 128, 5003), (5, 1000, 300), (2001, 40, 34),
+         (700, 264, 520), (300, 65, 255), (256, 64, 256)]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", SIZES)
+def test_rows_and_gradients(n, d, v, dtype):
+    h, w, b, t = make(n, d, v, dtype, bias=(n % 2 == 1), seed=n + v)
+    leaves = [x.requires_grad_() for x in (h, w, b) if x is not None]
+    logp, ent = categorical.linear_categorical(h, w, t, b)
+    assert logp.dtype == ent.dtype == torch.float32
+    T = Truth(h, w, b, t)
+    near(logp, T.logp, T.elogp, "logp")
+    near(ent, T.entropy, T.eent, "entropy")
+    g = torch.Generator(device="cuda").manual_seed(7)
+    A, E = torch.randn(n, device="cuda", generator=g), torch.randn(n, device="cuda", generator=g) * 0.1
+    got = torch.autograd.grad((logp, ent), leaves, (A, E))
+    ref = T.grads(A, E)
+    for name, x, (r, tol) in zip(("dh", "dw", "db"), got, ref):
+        assert x.dtype == dtype
+        near(x, r, tol, name)
+    assert bool((got[0][t == IGN] == 0).all()) and bool((logp[t == IGN] == 0).all()) and bool((ent[t == IGN] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(1, 16, 3), (200, 256, 361), (129, 100, 1025)])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_cross_entropy(n, d, v, dtype, reduction):
+    h, w, b, t = make(n, d, v, dtype, seed=3)
+    leaves = [x.requires_grad_() for x in (h, w, b)]
+    loss = categorical.linear_cross_entropy(h, w, t, b, reduction=reduction)
+    T = Truth(h, w, b, t)
+    live = T.ok.double()
+    count = live.sum().clamp(min=1)
+    if reduction == "none":
+        near(loss, -T.logp, T.elogp, "loss")
+        up = torch.linspace(0.5, 1.5, n, device="cuda")
+        A = -up
+    else:
+        k = count if reduction == "mean" else torch.ones((), device="cuda", dtype=torch.float64)
+        near(loss, -T.logp.sum() / k, (T.elogp * live).sum() / k + 2 * U * T.logp.abs().sum() / k, "loss")
+        up = torch.tensor(0.75, device="cuda")
+        A = (-0.75 / k).expand(n)
+    got = torch.autograd.grad(loss, leaves, up)
+    for name, x, (r, tol) in zip(("dh", "dw", "db"), got, T.grads(A, torch.zeros(n, device="cuda"))):
+        near(x, r, tol, name)
+    if reduction != "none":
+        l2, dh, dw, db = categorical.linear_cross_entropy_grad(h, w, t, b, reduction=reduction, grad_scale=up)
+        assert torch.equal(l2, loss.detach()) and all(map(torch.equal, (dh, dw, db), got))
+
+
+@gpu
+def test_pieces_of_the_classes_and_splits():
+    """more classes x rows than one piece holds (float32: 256 MiB), and a sum split over many workgroups"""
+    n, d, v = 30000, 24, 3000
+    h, w, b, t = make(n, d, v, torch.float32)
+    T = Truth(h, w, b, t)
+    loss, dh, dw, db = categorical.linear_cross_entropy_grad(h, w, t, b)
+    live = T.ok.double()
+    near(loss, -T.logp.sum() / live.sum(), (T.elogp * live).mean() + 4 * U * T.logp.abs().mean(), "loss")
+    for name, x, (r, tol) in zip(("dh", "dw", "db"), (dh, dw, db), T.grads((-1.0 / live.sum()).expand(n), torch.zeros(n, device="cuda"))):
+        near(x, r, tol, name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_what_padding_rows_hold_does_not_matter(dtype):
+    h, w, b, t = make(150, 96, 333, dtype, seed=5, ignored=0.3)
+    a = categorical.linear_cross_entropy_grad(h, w, t, b)
+    bad = h.clone()
+    bad[t == IGN] = torch.tensor([float("nan"), float("inf"), -float("inf")], dtype=dtype, device="cuda").repeat(32)
+    c = categorical.linear_cross_entropy_grad(bad, w, t, b)
+    assert all(map(torch.equal, a, c))
+    h2 = bad.requires_grad_()
+    logp, ent = categorical.linear_categorical(h2, w, t, b)
+    (g,) = torch.autograd.grad((logp, ent), (h2,), (torch.ones_like(logp), torch.ones_like(ent)))
+    assert bool(torch.isfinite(logp).all() & torch.isfinite(ent).all() & torch.isfinite(g).all()) and bool((g[t == IGN] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_all_rows_ignored_and_no_rows(dtype):
+    h, w, b, t = make(40, 32, 70, dtype)
+    loss, dh, dw, db = categorical.linear_cross_entropy_grad(h, w, torch.full_like(t, IGN), b)
+    assert float(loss) == 0.0 and not any(bool(x.any()) for x in (dh, dw, db))
+    e = h[:0].requires_grad_()
+    w.requires_grad_(), b.requires_grad_()
+    loss = categorical.linear_cross_entropy(e, w, t[:0], b)
+    gs = torch.autograd.grad(loss, (e, w, b))
+    assert float(loss) == 0.0 and gs[0].shape == (0, 32) and not bool(gs[1].any()) and not bool(gs[2].any())
+    logp, ent = categorical.linear_categorical(e, w, t[:0], b)
+    assert logp.shape == ent.shape == (0,)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_masked_classes(dtype):
+    """a bias of -inf takes a class out; the type's lowest value does the same to rounding; whole tiles of them, and a row's own class"""
+    n, d, v = 60, 64, 700
+    h, w, b, t = make(n, d, v, dtype, seed=11, ignored=0.0)
+    b[128:400] = -float("inf")
+    b[500] = -float("inf")
+    t = torch.where((t >= 128) & (t < 400) | (t == 500), 3, t)
+    T = Truth(h, w, b, t)
+    loss, dh, dw, db = categorical.linear_cross_entropy_grad(h, w, t, b)
+    for name, x, (r, tol) in zip(("dh", "dw", "db"), (dh, dw, db), T.grads(torch.full((n,), -1.0 / n, device="cuda"), torch.zeros(n, device="cuda"))):
+        near(x, r, tol, name)
+    assert not bool(dw[128:400].any()) and not bool(db[128:400].any())
+    logp, ent = categorical.linear_categorical(h, w, t, b)
+    near(logp, T.logp, T.elogp, "logp")
+    near(ent, T.entropy, T.eent, "entropy")
+    low = b.clone()
+    low[torch.isinf(low)] = torch.finfo(dtype).min
+    logp2, ent2 = categorical.linear_categorical(h, w, t, low)
+    near(logp2, T.logp, T.elogp, "logp, lowest value")
+    near(ent2, T.entropy, T.eent, "entropy, lowest value")
+    own = t.clone()
+    own[0] = 200                                                              # a class that takes no part: no chance at all
+    assert float(categorical.linear_categorical(h, w, own, b)[0][0]) == -float("inf")
+    nothing = torch.full_like(b, -float("inf"))
+    assert bool(torch.isnan(categorical.linear_categorical(h, w, t, nothing)[0]).all())
+
+
+@gpu
+@pytest.mark.parametrize("bad", [-1, 700, 2 ** 40])
+def test_classes_that_do_not_exist_are_nan(bad):
+    h, w, b, t = make(20, 64, 700, torch.float32, ignored=0.0)
+    good = categorical.linear_categorical(h, w, t, b)
+    t2 = t.clone()
+    t2[7] = bad
+    h.requires_grad_()
+    logp, ent = categorical.linear_categorical(h, w, t2, b)
+    keep = torch.arange(20, device="cuda") != 7
+    assert math.isnan(float(logp[7])) and math.isnan(float(ent[7])) and torch.equal(logp[keep], good[0][keep]) and torch.equal(ent[keep], good[1][keep])
+    (dh,) = torch.autograd.grad(logp.sum(), h)
+    assert bool(torch.isnan(dh[7]).all()) and bool(torch.isfinite(dh[keep]).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 61, 8])
+def test_strides_and_alignment(dtype, d):
+    """rows at a pitch, a base address one element off, a transposed weight (copied), leading dimensions, int32 classes"""
+    n, v = 77, 190
+    h, w, b, t = make(n, d, v, dtype, seed=2)
+    ref = categorical.linear_cross_entropy_grad(h, w, t, b)
+    wide = torch.zeros(n, 2 * d + 3, dtype=dtype, device="cuda")
+    wide[:, 1:d + 1] = h
+    flat = torch.zeros(v * d + 1, dtype=dtype, device="cuda")
+    flat[1:] = w.reshape(-1)
+    b1 = torch.zeros(v + 1, dtype=dtype, device="cuda")
+    b1[1:] = b
+    for args in ((wide[:, 1:d + 1], w, t, b), (h, flat[1:].view(v, d), t, b), (h, w.t().contiguous().t(), t, b1[1:]), (wide[:, 1:d + 1], flat[1:].view(v, d), t.int(), b1[1:])):
+        got = categorical.linear_cross_entropy_grad(*args)
+        assert all(map(torch.equal, got, ref))
+    got = categorical.linear_cross_entropy_grad(h.view(7, 11, d), w, t.view(7, 11), b)
+    assert got[1].shape == (7, 11, d) and torch.equal(got[1].view(n, d), ref[1]) and torch.equal(got[2], ref[2])
+    logp, ent = categorical.linear_categorical(h.view(7, 11, d), w, t.view(7, 11), b)
+    assert logp.shape == ent.shape == (7, 11)
+
+
+@gpu
+def test_gradients_against_differences():
+    """central differences of the float32 loss in float64-summed directions: step 2^-6 along a unit direction, third-order term and two roundings of the loss"""
+    n, d, v = 40, 32, 50
+    h, w, b, t = make(n, d, v, torch.float32, seed=9, ignored=0.2)
+    leaves = [x.requires_grad_() for x in (h, w, b)]
+    c = torch.linspace(-1, 1, n, device="cuda")
+
+    def f(h_, w_, b_):
+        logp, ent = categorical.linear_categorical(h_, w_, t, b_)
+        return (logp * c).double().sum() + 0.3 * ent.double().sum()
+    grads = torch.autograd.grad(f(*leaves), leaves)
+    step = 2.0 ** -6
+    for i, g in enumerate(grads):
+        gen = torch.Generator(device="cuda").manual_seed(i)
+        u = torch.randn(g.shape, device="cuda", generator=gen)
+        u = u / u.norm()
+        with torch.no_grad():
+            up, dn = ([x + s * step * u if k == i else x for k, x in enumerate(leaves)] for s in (1, -1))
+            diff = float(f(*up) - f(*dn)) / (2 * step)
+        want = float((g.double() * u.double()).sum())
+        # the loss: n rows of about log(v) + |l| each to 2^-20; the third derivative of n rows along a unit direction is below n x 8 |h or w|^3 / n^0
+        assert abs(diff - want) <= n * 8 * 2.0 ** -20 / (2 * step) + step * step / 6 * n * 8, (i, diff, want)
+
+
+@gpu
+def test_only_what_is_asked_for_and_partial_upstreams():
+    h, w, b, t = make(90, 64, 200, torch.float32, seed=4)
+    T = Truth(h, w, b, t)
+    w.requires_grad_()
+    logp, ent = categorical.linear_categorical(h, w, t, b)
+    (dw,) = torch.autograd.grad(ent.sum(), (w,))
+    r, tol = T.grads(torch.zeros(90, device="cuda"), torch.ones(90, device="cuda"))[1]
+    near(dw, r, tol, "dw of the entropy alone")
+    logp, ent = categorical.linear_categorical(h, w, t, b)
+    (dw,) = torch.autograd.grad(logp.sum(), (w,))
+    r, tol = T.grads(torch.ones(90, device="cuda"), torch.zeros(90, device="cuda"))[1]
+    near(dw, r, tol, "dw of logp alone")
+    with pytest.raises(RuntimeError):
+        x = categorical.linear_cross_entropy(h, w, t, b)
+        (g,) = torch.autograd.grad(x, (w,), create_graph=True)
+        g.sum().backward()
+
+
+@gpu
+def test_same_bits_every_time_and_two_streams_at_once():
+    h, w, b, t = make(500, 128, 3001, torch.bfloat16, seed=6)
+    h2, w2, b2, t2 = make(333, 256, 900, torch.bfloat16, seed=8)
+    ref, ref2 = categorical.linear_cross_entropy_grad(h, w, t, b), categorical.linear_cross_entropy_grad(h2, w2, t2, b2)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    s1.wait_stream(torch.cuda.current_stream()), s2.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            a = categorical.linear_cross_entropy_grad(h, w, t, b)
+        with torch.cuda.stream(s2):
+            c = categorical.linear_cross_entropy_grad(h2, w2, t2, b2)
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, a, ref)) and all(map(torch.equal, c, ref2))
+
+
+@gpu
+def test_captured_and_replayed():
+    h, w, b, t = make(200, 64, 777, torch.float32, seed=1)
+    other = make(200, 64, 777, torch.float32, seed=2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        categorical.linear_cross_entropy_grad(h, w, t, b)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):                                                       # two graphs of the same call share nothing
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = categorical.linear_cross_entropy_grad(h, w, t, b)
+        graphs.append((g, out))
+    with torch.no_grad():
+        for k in range(4):
+            src = other if k % 2 else make(200, 64, 777, torch.float32, seed=20 + k)
+            for x, y in zip((h, w, b, t), src):
+                x.copy_(y)
+            want = categorical.linear_cross_entropy_grad(h, w, t, b)
+            for g, out in graphs:
+                g.replay()
+            torch.cuda.synchronize()
+            for g, out in graphs:
+                assert all(map(torch.equal, out, want))
+    w.requires_grad_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="captured"):
+            categorical.linear_cross_entropy(h, w, t, b)
+        keep = torch.zeros(1, device="cuda")
+    assert keep is not None
+
+
+# ---- refusals: no GPU needed
+
+def test_refuses_what_does_not_fit():
+    h, w, t = torch.zeros(4, 8), torch.zeros(5, 8), torch.zeros(4, dtype=torch.int64)
+    f = categorical.linear_categorical
+    for args, err in (((h, w.double(), t), TypeError), ((h.double(), w.double(), t), TypeError), ((h, w, t.float()), TypeError), ((h, w.bfloat16(), t), TypeError),
+                      ((h, w[:, :7], t), ValueError), ((h, w[:0], t), ValueError), ((h, w, t[:3]), ValueError), ((h, w, t, torch.zeros(4)), ValueError),
+                      ((h, w, t, torch.zeros(5, dtype=torch.float16)), TypeError), ((h, None, t), TypeError), ((h, w, t), _lib.Q1EnvError)):
+        with pytest.raises(err):
+            f(*args)
+    with pytest.raises(ValueError):
+        categorical.linear_cross_entropy(h, w, t, reduction="avg")
+    with pytest.raises(ValueError):
+        f(h, w, t, ignore_index=0.5)
+
+
+def test_sizes_are_host_arithmetic():
+    lib = _lib.load()
+    assert lib.q1env_head_state_bytes(-1) == 0 and lib.q1env_head_state_bytes(2 ** 22 + 1) == 0 and lib.q1env_head_state_bytes(0) > 0
+    ws = lib.q1env_head_workspace_bytes
+    assert ws(0, 100, 64, 1000, 0) > 0 and ws(1, 100, 64, 1000, 1) > 0 and ws(2, 0, 64, 1000, 1) > 0
+    for bad in ((3, 1, 1, 1), (0, -1, 1, 1), (0, 1, 0, 1), (0, 1, 2 ** 16 + 1, 1), (0, 1, 1, 0), (0, 1, 1, 2 ** 22 + 1), (0, 2 ** 22 + 1, 1, 1)):
+        assert ws(*bad, 0) == 0
+    # the logits are not in it: 8192 x 131072 float32 logits are 4.3 GB
+    assert ws(1, 8192, 2048, 131072, 0) < 2 ** 28 and ws(1, 8192, 2048, 131072, 1) < 2 ** 29
+
+
+def head(**kw):
+    a = dict(dtype=0, target_bits=64, rows=4, width=8, classes=5, ignore_index=-100, hidden_dev=4096, hidden_stride=8, weight_dev=4096, weight_stride=8, bias_dev=None, target_dev=4096,
+             state_dev=4096, ws_dev=4096, ws_bytes=1 << 30)
+    a.update(kw)
+    return _lib.Q1Head(*[a[k] for k, _ in _lib.Q1Head._fields_])
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(width=0), dict(classes=0), dict(hidden_dev=None), dict(weight_dev=None), dict(hidden_stride=7),
+                                dict(weight_stride=7), dict(state_dev=None), dict(ws_dev=None), dict(ws_bytes=16), dict(target_bits=16), dict(target_dev=None), dict(hidden_dev=4097),
+                                dict(rows=2 ** 22 + 1)])
+def test_the_library_refuses(kw):
+    lib = _lib.load()
+    assert lib.q1env_head_forward(0, None, C.byref(head(**kw)), 0, 4096, None, None) == -1
+    if not {"target_bits", "target_dev"} & set(kw):
+        assert lib.q1env_head_backward(0, None, C.byref(head(**kw)), 4096, None, None, 4096, 8, None, 8, None) == -1
+
+
+def test_the_library_refuses_results():
+    lib = _lib.load()
+    h = head()
+    assert lib.q1env_head_forward(0, None, None, 0, 4096, None, None) == -1
+    assert lib.q1env_head_forward(0, None, C.byref(h), 2, 4096, None, None) == -1
+    assert lib.q1env_head_forward(0, None, C.byref(h), 0, None, None, None) == -1
+    b = lib.q1env_head_backward
+    assert b(0, None, C.byref(h), None, None, None, 4096, 8, None, 8, None) == -1           # no upstream gradient
+    assert b(0, None, C.byref(h), 4096, None, 4096, 4096, 8, None, 8, None) == -1           # two kinds of it
+    assert b(0, None, C.byref(h), 4096, None, None, None, 8, None, 8, None) == -1           # nothing asked for
+    assert b(0, None, C.byref(h), 4096, None, None, 4096, 7, None, 8, None) == -1
+    assert b(0, None, C.byref(h), 4096, None, None, None, 8, 4096, 7, None) == -1
+    assert b(0, None, C.byref(h), 4096, None, None, 4098, 8, None, 8, None) == -1
+    assert b"alignment" in lib.q1env_last_error() or b"aligned" in lib.q1env_last_error()
