@@ -3,78 +3,122 @@
 #include "q1env_host.hpp"
 #include "q1head.hpp"
 
+#include <algorithm>
+#include <atomic>
+
 using namespace q1head;
 
 namespace {
 
 constexpr uint64_t PIECE_BYTES = 256ull << 20;     // of the gradient of one piece of the classes
+constexpr uint64_t LAID_BYTES = 96ull << 20;       // of the laid-out weights of one piece
 constexpr int64_t MAX_ROWS = 1 << 22, MAX_WIDTH = 1 << 16, MAX_CLASSES = 1 << 22;
-constexpr int64_t WORKGROUPS = 512;                // two per CU: what a launch should have before its sums are split further
+constexpr int64_t PIECE_STEP = 256;                // pieces are whole tiles of every configuration
+
+typedef Config<256, 256, 2, 4, 2> Large;           // 128 KB of LDS: one workgroup of eight waves per CU
+typedef Config<128, 128, 2, 2, 2> Middle;          // 64 KB: two workgroups of four waves per CU, one computes while the other waits
+typedef Config<128, 64, 4, 1, 3> Few;              // up to 64 rows: 72 KB, two workgroups per CU
+typedef Config<128, 32, 4, 1, 4> Fewest;           // up to 32 rows: 80 KB, two workgroups per CU
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return div_up(a, b) * b; }
 uint64_t aligned(uint64_t x) { return (x + 255) & ~255ull; }
 size_t elem_size(int dt) { return dt == F32 ? 4 : 2; }
+int planes_of(int dt) { return dt == F32 ? 3 : 1; }
 
 // the forward pass's results as the backward pass reads them (q1env_head_state_bytes)
 struct State {
     float *lse, *entropy, *each;
     int64_t* target;
     uint8_t* live;
-    static uint64_t bytes(int64_t n) { return 2 * aligned(4 * n) + aligned(8 * n) + aligned(n) + 256; }
+    uint64_t* bits;
+    static uint64_t bytes(int64_t n) { return 2 * aligned(4 * n) + aligned(8 * n) + aligned(n) + aligned(8 * div_up(n, 64)) + 256; }
     State(void* p, int64_t n) {
         char* c = (char*)p;
         lse = (float*)c; c += aligned(4 * n);
         entropy = (float*)c; c += aligned(4 * n);
         target = (int64_t*)c; c += aligned(8 * n);
         live = (uint8_t*)c; c += aligned(n);
+        bits = (uint64_t*)c; c += aligned(8 * div_up(n, 64));
         each = (float*)c;
     }
 };
 
-struct Plan {
-    int64_t piece, pieces;             // classes per piece (a multiple of BM)
-    int dh_split, dw_split;
-    int64_t dh_k, dw_k;                // classes / rows per split
-    uint64_t part, own, scale, g, db, dh_slab, dw_slab;        // byte offsets in the workspace
-    uint64_t forward_bytes, backward_bytes;
-};
+// which tile a product of m x n results with k terms takes
+enum Size { LARGE, MIDDLE, FEW, FEWEST };
+Size size_of(int64_t m, int64_t n, int64_t k) {
+    if (n <= 32) return FEWEST;
+    if (n <= 64) return FEW;
+    return k >= 512 && div_up(m, 256) * div_up(n, 256) >= 384 ? LARGE : MIDDLE;
+}
+int64_t bm_of(Size s) { return s == LARGE ? 256 : 128; }
+int64_t bn_of(Size s) { return s == LARGE ? 256 : s == MIDDLE ? 128 : s == FEW ? 64 : 32; }
 
+// how the sums of a product are split over workgroups when its result has few tiles
 void split(int64_t tiles, int64_t k, int& n, int64_t& len) {
-    int64_t s = div_up(WORKGROUPS, tiles), most = div_up(k, 512);        // a part shorter than 512 costs more in its slab than it gains
+    int64_t s = div_up(512, tiles), most = div_up(k, 512);        // two workgroups per CU; a part shorter than 512 costs more in its slab than it gains
     if (s > most) s = most;
     if (s < 1) s = 1;
-    len = div_up(div_up(k, s), BK) * BK;
+    len = round_up(div_up(k, s), BK);
     n = (int)div_up(k, len);
 }
 
-Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes) {
+bool in_place(int dt, const void* p, int64_t stride, int64_t width) {       // whether the loads can take an operand as it lies
+    return dt != F32 && ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && width % 8 == 0 && stride < (1 << 21);
+}
+
+struct Plan {
+    int64_t padded;                    // width of laid-out rows
+    int64_t piece;                     // classes per piece
+    int64_t pieces;
+    Size logits, dh, dw;
+    int dh_split, dw_split;
+    int64_t dh_k, dw_k;                // classes / rows per split
+    uint64_t part, own, scale, g, db, dh_slab, dw_slab, h_laid, w_laid;        // byte offsets in the workspace
+    uint64_t bytes;
+};
+
+// w_in_place / h_in_place: the workspace has to suffice for any address, so its size is asked for with both false
+Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward, bool h_in_place, bool w_in_place) {
     Plan p{};
-    const int64_t ct = div_up(classes, BM);
-    p.own = 0;
-    p.part = aligned(4 * rows);
-    p.forward_bytes = p.part + aligned(12 * (uint64_t)ct * rows);
-    int64_t piece = (int64_t)(PIECE_BYTES / (elem_size(dt) * rows)) / BM * BM;
-    if (piece < BM) piece = BM;
-    if (piece > ct * BM) piece = ct * BM;
+    p.padded = round_up(width, 64);
+    const int64_t all = round_up(classes, PIECE_STEP);
+    int64_t piece = all;
+    const int64_t laid = planes_of(dt) * 2 * p.padded;                        // bytes of a laid-out row
+    if (!w_in_place) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(LAID_BYTES / laid) / PIECE_STEP * PIECE_STEP));
+    if (backward) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(PIECE_BYTES / (2 * planes_of(dt) * rows)) / PIECE_STEP * PIECE_STEP));
     p.piece = piece;
     p.pieces = div_up(classes, piece);
-    split(div_up(width, BM) * div_up(rows, BN), piece, p.dh_split, p.dh_k);
-    split(div_up(width, BM) * div_up(piece, BN), rows, p.dw_split, p.dw_k);
+    p.logits = size_of(std::min(piece, classes), rows, width);
     uint64_t at = 0;
-    p.scale = at; at += 256;
-    p.g = at; at += aligned(elem_size(dt) * (uint64_t)rows * piece);
-    p.db = at; at += aligned(4 * (uint64_t)div_up(rows, BN) * classes);
-    p.dh_slab = at;
-    if (p.dh_split > 1 || p.pieces > 1) at += aligned(4 * (uint64_t)p.dh_split * rows * width);
-    p.dw_slab = at;
-    if (p.dw_split > 1) at += aligned(4 * (uint64_t)p.dw_split * piece * width);
-    p.backward_bytes = at;
+    auto take = [&](uint64_t n) { const uint64_t o = at; at += aligned(n); return o; };
+    if (!backward) {
+        p.own = take(4 * rows);
+        p.part = take(12 * (uint64_t)div_up(classes, 128) * rows);
+    } else {
+        p.dh = size_of(width, rows, piece);
+        p.dw = size_of(width, std::max<int64_t>(piece, 128), rows);          // (both operands lie k-major: no tile under 128)
+        if (p.dw == FEW || p.dw == FEWEST) p.dw = MIDDLE;
+        split(div_up(width, bm_of(p.dh)) * div_up(rows, bn_of(p.dh)), piece, p.dh_split, p.dh_k);
+        split(div_up(width, bm_of(p.dw)) * div_up(piece, bn_of(p.dw)), rows, p.dw_split, p.dw_k);
+        p.scale = take(256);
+        p.g = take(2 * (uint64_t)planes_of(dt) * rows * piece);
+        p.db = take(4 * (uint64_t)div_up(rows, bn_of(p.logits)) * classes);
+        p.dh_slab = take(p.dh_split > 1 || p.pieces > 1 ? 4 * (uint64_t)p.dh_split * rows * width : 0);
+        p.dw_slab = take(p.dw_split > 1 ? 4 * (uint64_t)p.dw_split * piece * width : 0);
+    }
+    p.h_laid = take(h_in_place ? 0 : (uint64_t)laid * rows);
+    p.w_laid = take(w_in_place ? 0 : (uint64_t)laid * piece);
+    p.bytes = at;
     return p;
 }
 
-Operand operand(int dt, const void* p, int64_t stride, int64_t extent, const uint8_t* live = nullptr) {
-    const bool vec = ((uintptr_t)p & 15) == 0 && (stride * (int64_t)elem_size(dt)) % 16 == 0;
-    return Operand{p, stride, extent, live, vec ? 1 : 0};
+// what a workspace has to hold whatever the operands' addresses and strides are
+uint64_t workspace_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward) {
+    uint64_t n = plan_of(dt, rows, width, classes, backward, false, false).bytes;
+    if (dt != F32 && width % 8 == 0)                                          // pieces differ: either may need more
+        n = std::max(n, plan_of(dt, rows, width, classes, backward, false, true).bytes);
+    return n;
 }
 
 int check_shape(const char* who, int dtype, int64_t rows, int64_t width, int64_t classes) {
@@ -104,77 +148,147 @@ int guard_device(const char* who, int device) {
     return 0;
 }
 
+template <class C, auto KERNEL, typename... A> int go(hipStream_t stream, int device, int64_t workgroups, A... args) {
+    if (workgroups <= 0 || workgroups > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = 1ull << (device & 63);
+    if (C::LDS_BYTES > 65536 && (device > 63 || !(done.load(std::memory_order_relaxed) & bit))) {        // more than 64 KB of LDS has to be allowed once per kernel and device
+        HIP_TRY(hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES));
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)workgroups), dim3(C::THREADS), C::LDS_BYTES, stream, args...);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+#define Q1_TRY(expr) do { if (int rc_ = (expr)) return rc_; } while (0)
+
+struct Where { hipStream_t stream; int device; };
+
+template <class C, int DT> int statistics(const Where& at, Head hd, float* part, float* own) {
+    hd.tiles_m = (uint32_t)div_up(hd.c1 - hd.c0, C::BM);
+    hd.tiles_n = (uint32_t)div_up(hd.rows, C::BN);
+    return go<C, statistics_kernel<C, DT>>(at.stream, at.device, (int64_t)hd.tiles_m * hd.tiles_n, hd, hd.c0 / C::BM, part, own);
+}
+template <class C, int DT> int gradient(const Where& at, Head hd, const Upstream& up, int64_t piece, const State& st, uint16_t* g, float* db) {
+    hd.tiles_m = (uint32_t)div_up(hd.c1 - hd.c0, C::BM);
+    hd.tiles_n = (uint32_t)div_up(hd.rows, C::BN);
+    return go<C, gradient_kernel<C, DT>>(at.stream, at.device, (int64_t)hd.tiles_m * hd.tiles_n, hd, up, piece, hd.rows * piece, (const float*)st.lse, (const float*)st.entropy, g, db);
+}
+template <class C, int DT, bool BKM> int product(const Where& at, Product pr, int splits) {
+    pr.tiles_m = (uint32_t)div_up(pr.width, C::BM);
+    pr.tiles_n = (uint32_t)div_up(pr.rows, C::BN);
+    return go<C, product_kernel<C, DT, true, BKM>>(at.stream, at.device, (int64_t)pr.tiles_m * pr.tiles_n * splits, pr);
+}
+
+template <int DT> int lay_out(const Where& at, const void* src, int64_t stride, int64_t rows, int64_t width, int64_t padded, const uint8_t* live, void* out) {
+    hipLaunchKernelGGL((lay_out_kernel<DT>), dim3((unsigned)div_up(rows * padded, 2048)), dim3(256), 0, at.stream, (const typename Elem<DT>::type*)src, stride, rows, width, padded, live, (uint16_t*)out);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+// an operand of `rows` rows, as it lies or laid out at `laid` (then the rows have been laid out already)
+Op rows_op(int dt, bool as_it_lies, const void* p, int64_t stride, int64_t rows, int64_t width, int64_t padded, const void* laid) {
+    if (as_it_lies) return Op{(const char*)p, 2 * stride, 0, rows, width, nullptr};
+    return Op{(const char*)laid, 2 * padded, 2 * rows * padded, rows, padded, nullptr};
+}
+// the same memory with the rows as the k of a product
+Op turned(const Op& o, const uint64_t* live) { return Op{o.p, o.stride, o.plane, o.k_extent, o.x_extent, live}; }
+
 template <int DT>
-int forward(hipStream_t stream, const q1env_head& q, const Plan& p, int reduction, float* logp, float* entropy, float* loss) {
+int forward(const Where& at, const q1env_head& q, int reduction, float* logp, float* entropy, float* loss) {
     const int64_t n = q.rows;
     State st(q.state_dev, n);
-    char* ws = (char*)q.ws_dev;
-    const dim3 rows256((unsigned)div_up(n, 256));
     if (n > 0) {
+        const bool hp = in_place(DT, q.hidden_dev, q.hidden_stride, q.width), wp = in_place(DT, q.weight_dev, q.weight_stride, q.width);
+        const Plan p = plan_of(DT, n, q.width, q.classes, false, hp, wp);
+        char* ws = (char*)q.ws_dev;
+        const dim3 rows256((unsigned)div_up(n, 256));
         if (q.target_bits == 64)
-            hipLaunchKernelGGL((prepare_kernel<int64_t>), rows256, dim3(256), 0, stream, (const int64_t*)q.target_dev, n, q.classes, q.ignore_index, st.target, st.live);
+            hipLaunchKernelGGL((prepare_kernel<int64_t>), rows256, dim3(256), 0, at.stream, (const int64_t*)q.target_dev, n, q.classes, q.ignore_index, st.target, st.live, st.bits);
         else
-            hipLaunchKernelGGL((prepare_kernel<int32_t>), rows256, dim3(256), 0, stream, (const int32_t*)q.target_dev, n, q.classes, q.ignore_index, st.target, st.live);
+            hipLaunchKernelGGL((prepare_kernel<int32_t>), rows256, dim3(256), 0, at.stream, (const int32_t*)q.target_dev, n, q.classes, q.ignore_index, st.target, st.live, st.bits);
         HIP_TRY(hipGetLastError());
-        const Head hd{operand(DT, q.weight_dev, q.weight_stride, q.classes), operand(DT, q.hidden_dev, q.hidden_stride, n), q.bias_dev, st.target, n, q.width, q.classes};
-        const int64_t tiles = div_up(q.classes, BM);
-        hipLaunchKernelGGL((statistics_kernel<DT>), dim3((unsigned)tiles, (unsigned)div_up(n, BN)), dim3(256), 0, stream, hd, (float*)(ws + p.part), (float*)(ws + p.own));
-        HIP_TRY(hipGetLastError());
-        hipLaunchKernelGGL(join_kernel, dim3((unsigned)div_up(n, 16)), dim3(256), 0, stream, (const float*)(ws + p.part), (const float*)(ws + p.own), st.target, n, (int)tiles,
-                           logp, entropy, st.entropy, st.lse);
+        if (!hp) Q1_TRY(lay_out<DT>(at, q.hidden_dev, q.hidden_stride, n, q.width, p.padded, nullptr, ws + p.h_laid));
+        const Op h = rows_op(DT, hp, q.hidden_dev, q.hidden_stride, n, q.width, p.padded, ws + p.h_laid);
+        float *part = (float*)(ws + p.part), *own = (float*)(ws + p.own);
+        for (int64_t c0 = 0; c0 < q.classes; c0 += p.piece) {
+            const int64_t c1 = std::min(c0 + p.piece, q.classes);
+            const char* w0 = (const char*)q.weight_dev + elem_size(DT) * c0 * q.weight_stride;
+            if (!wp) Q1_TRY(lay_out<DT>(at, w0, q.weight_stride, c1 - c0, q.width, p.padded, nullptr, ws + p.w_laid));
+            const Head hd{rows_op(DT, wp, w0, q.weight_stride, c1 - c0, q.width, p.padded, ws + p.w_laid), h, q.bias_dev, st.target, n, q.width, q.classes, 0, 0, c0, c1};
+            if (p.logits == LARGE) Q1_TRY((statistics<Large, DT>(at, hd, part, own)));
+            else if (p.logits == MIDDLE) Q1_TRY((statistics<Middle, DT>(at, hd, part, own)));
+            else if (p.logits == FEW) Q1_TRY((statistics<Few, DT>(at, hd, part, own)));
+            else Q1_TRY((statistics<Fewest, DT>(at, hd, part, own)));
+        }
+        hipLaunchKernelGGL(join_kernel, dim3((unsigned)div_up(n, 16)), dim3(256), 0, at.stream, part, own, st.target, n, (int)div_up(q.classes, bm_of(p.logits)), logp, entropy, st.entropy,
+                           st.lse);
         HIP_TRY(hipGetLastError());
     }
     if (loss) {
-        hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, stream, logp, st.live, n, reduction == Q1ENV_REDUCE_MEAN ? 1 : 0, loss, st.each);
+        hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, at.stream, logp, st.live, n, reduction == Q1ENV_REDUCE_MEAN ? 1 : 0, loss, st.each);
         HIP_TRY(hipGetLastError());
     }
     return Q1ENV_OK;
 }
 
 template <int DT>
-int backward(hipStream_t stream, const q1env_head& q, const Plan& p, Upstream up, void* dh, int64_t dh_stride, void* dw, int64_t dw_stride, void* db) {
+int backward(const Where& at, const q1env_head& q, Upstream up, void* dh, int64_t dh_stride, void* dw, int64_t dw_stride, void* db) {
     const int64_t n = q.rows, v = q.classes, d = q.width;
+    const bool hp = in_place(DT, q.hidden_dev, q.hidden_stride, d), wp = in_place(DT, q.weight_dev, q.weight_stride, d);
+    const Plan p = plan_of(DT, n, d, v, true, hp, wp);
     State st(q.state_dev, n);
     char* ws = (char*)q.ws_dev;
-    float* scale = (float*)(ws + p.scale);
+    float *scale = (float*)(ws + p.scale), *db_part = db ? (float*)(ws + p.db) : nullptr;
     up.scale = scale;
     up.each = up.dloss ? st.each : nullptr;
-    hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, stream, up, st.live, n, DT == F16 ? 1 : 0, scale);
+    hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, at.stream, up, st.live, n, DT == F16 ? 1 : 0, scale);
     HIP_TRY(hipGetLastError());
-    const Head hd{operand(DT, q.weight_dev, q.weight_stride, v), operand(DT, q.hidden_dev, q.hidden_stride, n), q.bias_dev, st.target, n, d, v};
-    const unsigned row_tiles = (unsigned)div_up(n, BN), width_tiles = (unsigned)div_up(d, BM);
-    void* g = ws + p.g;
+    if (!hp) Q1_TRY(lay_out<DT>(at, q.hidden_dev, q.hidden_stride, n, d, p.padded, st.live, ws + p.h_laid));
+    const Op h = rows_op(DT, hp, q.hidden_dev, q.hidden_stride, n, d, p.padded, ws + p.h_laid);
+    uint16_t* g = (uint16_t*)(ws + p.g);
     float *dh_slab = p.dh_split > 1 || p.pieces > 1 ? (float*)(ws + p.dh_slab) : nullptr, *dw_slab = p.dw_split > 1 ? (float*)(ws + p.dw_slab) : nullptr;
     const size_t es = elem_size(DT);
+    auto wide = [&](const void* out, int64_t stride, const float* slab) { return slab ? d % 4 == 0 : ((uintptr_t)out & 15) == 0 && stride * es % 16 == 0; };
     for (int64_t c0 = 0; c0 < v; c0 += p.piece) {
-        const int64_t c1 = c0 + p.piece < v ? c0 + p.piece : v, len = c1 - c0;
-        hipLaunchKernelGGL((gradient_kernel<DT>), dim3((unsigned)div_up(len, BM), row_tiles), dim3(256), 0, stream, hd, up, c0, c1, p.piece, st.lse, st.entropy, g,
-                           db ? (float*)(ws + p.db) : nullptr);
-        HIP_TRY(hipGetLastError());
+        const int64_t c1 = std::min(c0 + p.piece, v), len = c1 - c0;
+        const char* w0 = (const char*)q.weight_dev + es * c0 * q.weight_stride;
+        if (!wp) Q1_TRY(lay_out<DT>(at, w0, q.weight_stride, len, d, p.padded, nullptr, ws + p.w_laid));
+        const Op w = rows_op(DT, wp, w0, q.weight_stride, len, d, p.padded, ws + p.w_laid);
+        const Head hd{w, h, q.bias_dev, st.target, n, d, v, 0, 0, c0, c1};
+        if (p.logits == LARGE) Q1_TRY((gradient<Large, DT>(at, hd, up, p.piece, st, g, db_part)));
+        else if (p.logits == MIDDLE) Q1_TRY((gradient<Middle, DT>(at, hd, up, p.piece, st, g, db_part)));
+        else if (p.logits == FEW) Q1_TRY((gradient<Few, DT>(at, hd, up, p.piece, st, g, db_part)));
+        else Q1_TRY((gradient<Fewest, DT>(at, hd, up, p.piece, st, g, db_part)));
+        const Op gr{(const char*)g, 2 * p.piece, 2 * n * p.piece, n, round_up(len, BK), nullptr};         // [row][class of the piece]
         if (dw) {
-            Product pr{operand(DT, q.hidden_dev, q.hidden_stride, d, st.live), operand(DT, g, p.piece, len), n, p.dw_k, len, d, (char*)dw + es * c0 * dw_stride, dw_stride,
-                       dw_slab, 0, scale, nullptr};
-            hipLaunchKernelGGL((product_kernel<DT, true, true>), dim3(width_tiles, (unsigned)div_up(len, BN), (unsigned)p.dw_split), dim3(256), 0, stream, pr);
-            HIP_TRY(hipGetLastError());
+            Op gt = turned(gr, nullptr);
+            gt.x_extent = round_up(len, 8);
+            Product pr{turned(h, hp ? st.bits : nullptr), gt, n, p.dw_k, len, d, 0, 0, (char*)dw + es * c0 * dw_stride, dw_stride, 0, dw_slab, 0, scale, nullptr};
+            pr.vec = wide(pr.out, dw_stride, dw_slab);
+            if (p.dw == LARGE) Q1_TRY((product<Large, DT, true>(at, pr, p.dw_split)));
+            else Q1_TRY((product<Middle, DT, true>(at, pr, p.dw_split)));
             if (dw_slab) {
-                hipLaunchKernelGGL((finish_kernel<DT>), dim3((unsigned)div_up(len * d, 256)), dim3(256), 0, stream, dw_slab, p.dw_split, len, d, scale, (const uint8_t*)nullptr, pr.out,
+                hipLaunchKernelGGL((finish_kernel<DT>), dim3((unsigned)div_up(len * d, 256)), dim3(256), 0, at.stream, dw_slab, p.dw_split, len, d, scale, (const uint8_t*)nullptr, pr.out,
                                    dw_stride);
                 HIP_TRY(hipGetLastError());
             }
         }
         if (dh) {
-            Product pr{operand(DT, (const char*)q.weight_dev + es * c0 * q.weight_stride, q.weight_stride, d), operand(DT, g, p.piece, n), len, p.dh_k, n, d, dh, dh_stride,
-                       dh_slab, c0 > 0 ? 1 : 0, scale, st.live};
-            hipLaunchKernelGGL((product_kernel<DT, true, false>), dim3(width_tiles, row_tiles, (unsigned)p.dh_split), dim3(256), 0, stream, pr);
-            HIP_TRY(hipGetLastError());
+            Product pr{turned(w, nullptr), gr, len, p.dh_k, n, d, 0, 0, dh, dh_stride, 0, dh_slab, c0 > 0 ? 1 : 0, scale, st.live};
+            pr.vec = wide(dh, dh_stride, dh_slab);
+            if (p.dh == LARGE) Q1_TRY((product<Large, DT, false>(at, pr, p.dh_split)));
+            else if (p.dh == MIDDLE) Q1_TRY((product<Middle, DT, false>(at, pr, p.dh_split)));
+            else if (p.dh == FEW) Q1_TRY((product<Few, DT, false>(at, pr, p.dh_split)));
+            else Q1_TRY((product<Fewest, DT, false>(at, pr, p.dh_split)));
         }
     }
     if (dh && dh_slab) {
-        hipLaunchKernelGGL((finish_kernel<DT>), dim3((unsigned)div_up(n * d, 256)), dim3(256), 0, stream, dh_slab, p.dh_split, n, d, scale, st.live, dh, dh_stride);
+        hipLaunchKernelGGL((finish_kernel<DT>), dim3((unsigned)div_up(n * d, 256)), dim3(256), 0, at.stream, dh_slab, p.dh_split, n, d, scale, st.live, dh, dh_stride);
         HIP_TRY(hipGetLastError());
     }
     if (db) {
-        hipLaunchKernelGGL((bias_kernel<DT>), dim3((unsigned)div_up(v, 256)), dim3(256), 0, stream, (const float*)(ws + p.db), v, (int)row_tiles, scale, db);
+        hipLaunchKernelGGL((bias_kernel<DT>), dim3((unsigned)div_up(v, 256)), dim3(256), 0, at.stream, (const float*)db_part, v, (int)div_up(n, bn_of(p.logits)), scale, db);
         HIP_TRY(hipGetLastError());
     }
     return Q1ENV_OK;
@@ -194,8 +308,7 @@ uint64_t q1env_head_state_bytes(int64_t rows) { return rows < 0 || rows > MAX_RO
 uint64_t q1env_head_workspace_bytes(int dtype, int64_t rows, int64_t width, int64_t classes, int backward) {
     if (check_shape("q1env_head_workspace_bytes", dtype, rows, width, classes)) return 0;
     if (rows == 0) return 256;
-    const Plan p = plan_of(dtype, rows, width, classes);
-    return backward ? p.backward_bytes : p.forward_bytes;
+    return workspace_of(dtype, rows, width, classes, backward != 0);
 }
 
 int q1env_head_forward(int device, void* stream, const q1env_head* hd, int reduction, float* logp, float* entropy, float* loss) {
@@ -209,11 +322,11 @@ int q1env_head_forward(int device, void* stream, const q1env_head* hd, int reduc
         return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_forward: workspace smaller than q1env_head_workspace_bytes(..., 0)");
     if (int rc = guard_device(who, device)) return rc;
     DeviceGuard guard(device);
-    const Plan p = hd->rows > 0 ? plan_of(hd->dtype, hd->rows, hd->width, hd->classes) : Plan{};
+    const Where at{(hipStream_t)stream, device};
     switch (hd->dtype) {
-        case Q1ENV_DT_F32: return forward<F32>((hipStream_t)stream, *hd, p, reduction, logp, entropy, loss);
-        case Q1ENV_DT_BF16: return forward<BF16>((hipStream_t)stream, *hd, p, reduction, logp, entropy, loss);
-        default: return forward<F16>((hipStream_t)stream, *hd, p, reduction, logp, entropy, loss);
+        case Q1ENV_DT_F32: return forward<F32>(at, *hd, reduction, logp, entropy, loss);
+        case Q1ENV_DT_BF16: return forward<BF16>(at, *hd, reduction, logp, entropy, loss);
+        default: return forward<F16>(at, *hd, reduction, logp, entropy, loss);
     }
 }
 
@@ -238,12 +351,12 @@ int q1env_head_backward(int device, void* stream, const q1env_head* hd, const fl
         HIP_TRY(hipGetLastError());
         return Q1ENV_OK;
     }
-    const Plan p = plan_of(hd->dtype, hd->rows, hd->width, hd->classes);
+    const Where at{(hipStream_t)stream, device};
     const Upstream up{dlogp, dentropy, dloss, nullptr, nullptr};
     switch (hd->dtype) {
-        case Q1ENV_DT_F32: return backward<F32>((hipStream_t)stream, *hd, p, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
-        case Q1ENV_DT_BF16: return backward<BF16>((hipStream_t)stream, *hd, p, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
-        default: return backward<F16>((hipStream_t)stream, *hd, p, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
+        case Q1ENV_DT_F32: return backward<F32>(at, *hd, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
+        case Q1ENV_DT_BF16: return backward<BF16>(at, *hd, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
+        default: return backward<F16>(at, *hd, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
     }
 }
 

@@ -8,8 +8,8 @@
 //
 // Operand precision: float16 / bfloat16 inputs feed v_mfma_f32_32x32x16 as they are.  A float32 value travels as THREE bfloat16 pieces
 // a = a1 + a2 + a3 (8 + 8 + 8 significant bits: exact) and a product is the six largest of the nine piece products, a1 b1, a1 b2, a2 b1, a1 b3,
-// a3 b1, a2 b2; what is dropped is below 2^-26 of |a b|, under the rounding of the float32 accumulator the products go to.  (The float32
-// matrix instruction runs at 1/16 of the bfloat16 one; six products run at 1/6.)
+// a3 b1, a2 b2; what is dropped is 2^-27 of |a b| typically and 2^-23 at most, under the rounding of the float32 accumulator the products go to.  (The
+// float32 matrix instruction runs at 1/16 of the bfloat16 one; six products run at 1/6.)
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -29,10 +29,19 @@ template <> struct Elem<F32> { typedef float type; static constexpr int planes =
 template <> struct Elem<BF16> { typedef uint16_t type; static constexpr int planes = 1; };
 template <> struct Elem<F16> { typedef uint16_t type; static constexpr int planes = 1; };
 
+// a float32 as three bfloat16 pieces, each the nearest to what the ones before leave (a value that would round to infinity keeps the largest finite first piece)
 __device__ __forceinline__ uint16_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
 __device__ __forceinline__ float bf16_value(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
 __device__ __forceinline__ uint16_t f16_bits(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
 __device__ __forceinline__ float f16_value(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
+
+__device__ __forceinline__ void three_pieces(float a, uint16_t& p1, uint16_t& p2, uint16_t& p3) {
+    p1 = bf16_bits(a);
+    if ((p1 & 0x7fff) == 0x7f80 && fabsf(a) < INFINITY) p1 -= 1;
+    const float r1 = a - bf16_value(p1);
+    p2 = bf16_bits(r1);
+    p3 = bf16_bits(r1 - bf16_value(p2));
+}
 
 template <int DT> __device__ __forceinline__ float to_float(typename Elem<DT>::type v) {
     if constexpr (DT == F32) return v;
@@ -50,229 +59,357 @@ template <int DT> __device__ __forceinline__ f32x16 mfma(const u32x4& a, const u
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// exp(x) for x <= 0 (and -inf, NaN): one hardware exponential, with the rounding error of x log2(e) put back where the result is held in full
-// precision (|x| 2^-24 relative otherwise)
-__device__ __forceinline__ float exp_neg(float x) {
-    const float t = x * 1.4426950408889634f;
-    const float e = __builtin_amdgcn_exp2f(t);
-    const float r = fmaf(x, 1.4426950408889634f, -t) + x * 1.925963033500e-8f;      // log2(e) - float32(log2(e))
-    return t > -150.0f ? fmaf(e, r * 0.6931471805599453f, e) : e;
+// ------------------------------------------------------------------------------------------------------------------------------
+// C[m][n] = sum_k A(m, k) B(n, k) on 16-bit operands, a BM x BN tile per workgroup.
+//
+// An operand lies in memory with k contiguous (KM = false: element (x, k) at p[x stride + k]) or with x contiguous (KM = true: p[k stride + x]).  Both
+// kinds travel from memory to LDS without passing through registers (buffer loads with an LDS destination, 16 bytes per lane, 1 KB per
+// wave instruction; what lies outside the operand reads as zero by the buffer's bounds check), BK = 64 values of k at a time, STAGES tiles in flight:
+// the loads of a tile are issued one (two, three) whole steps before its barrier.  The LDS image is linear in the order of the loading lanes, so bank conflicts are
+// avoided by permuting which 16-byte chunk a lane asks memory for:
+//   KM = false: rows of 128 bytes; chunk c of row x sits at c ^ ((x >> 1) & 7): any 16 lanes of a fragment read (16 rows, one chunk) cover all 64 banks;
+//   KM = true:  rows of 2 BM bytes; the 32-byte unit u of row k sits at u ^ (2 (k & 3)): the transposing read (ds_read_b64_tr_b16: 4 values of k x 16 of x per 16
+//               lanes) touches four rows at four different bank groups.
+// Bound (256 x 256 tile, 8 waves of 128 x 64): per step a wave issues 32 matrix instructions of 32 cycles and reads 24 KB of LDS, 75 % of what the LDS delivers in
+// that time; a 64 x 64 wave tile would need all of it.
+struct Op {
+    const char* p;
+    int64_t stride;             // bytes from row to row
+    int64_t plane;              // bytes from piece to piece (float32 as three bfloat16 pieces)
+    int64_t x_extent;           // valid x (KM: a multiple of 8)
+    int64_t k_extent;           // valid k (not KM: a multiple of 8)
+    const uint64_t* live;       // KM: where set, bit k of the words says whether row k counts (rows that do not are zero whatever memory holds)
+};
+
+constexpr int BK = 64;
+
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_> struct Config {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;             // 32 x 32 tiles per wave
+    static constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;         // load instructions per wave and stage
+    static constexpr int STAGE_BYTES = (BM + BN) * BK * 2, LDS_BYTES = STAGES * STAGE_BYTES;
+    static_assert(LA * WAVES * 8 == BM && LB * WAVES * 8 == BN && TM >= 1 && TN >= 1, "whole load instructions per wave");
+};
+
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) char lds_char;
+constexpr uint32_t OUTSIDE = 0x80000000u;                                   // the resource's size: an offset from here on reads zero
+
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t offset, uint32_t lds) {
+    const uint64_t a = (uint64_t)base;
+    const u32x4 rsrc = {(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, OUTSIDE, 0x00020000u};
+    // (no result registers: what the instruction writes is LDS, waited for with vmcnt before the barrier in front of its use)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_loads() {             // all but the N youngest loads have landed, and this wave's LDS reads are done
+    static_assert(N < 64, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
-// ------------------------------------------------------------------------------------------------------------------------------
-// C[m][n] = sum_k A(m, k) B(n, k), a BM x BN tile per workgroup of 256 lanes (2 x 2 waves of 64 x 64).
-// An operand is (pointer, stride): K-major false: element (x, k) at p[x * stride + k] (k contiguous); true: p[k * stride + x].
-struct Operand {
-    const void* p;
-    int64_t stride;             // elements
-    int64_t extent;             // number of valid x
-    const uint8_t* live;        // K-major only: where set, element (x, k) counts as zero when live[k] == 0 (whatever memory holds there)
-    int vec;                    // 16-byte loads are aligned (pointer and stride)
-};
-
-constexpr int BM = 128, BN = 128, BK = 32, LDS_ROW = BK + 8;      // 80-byte rows: 16-byte aligned, and eight rows cover all 64 banks
-
-template <int DT> struct Stage {                                    // one operand tile, [plane][x][k]
-    uint16_t v[Elem<DT>::planes][BM][LDS_ROW];
-};
-
-template <int DT, bool KMAJOR> struct Loader {
-    typedef typename Elem<DT>::type E;
-    static constexpr int V = 16 / sizeof(E);                        // elements of a 16-byte load
-    static constexpr int CHUNKS = BM * BK / V / 256;                // per lane
-    E r[CHUNKS][V];
-
-    // tile at (x0, k0); k < k_end
-    __device__ __forceinline__ void load(const Operand& o, int64_t x0, int64_t k0, int64_t k_end) {
-        const E* p = (const E*)o.p;
+// the loading side of one operand: XT values of x per tile, COUNT load instructions per wave
+template <int XT, int COUNT, bool KM> struct Feed {
+    uint32_t off[COUNT];        // byte offset of this lane's chunk in the tile, OUTSIDE if its x is
+    int kk[COUNT];              // the chunk's k within the step
+    const char* base;           // of the tile at k = 0
+    __device__ __forceinline__ void init(const Op& o, int64_t x0, int wave, int lane) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int i = c * 256 + (int)threadIdx.x;
-            int64_t x, k;
-            if constexpr (KMAJOR) { x = x0 + (i % (BM / V)) * V; k = k0 + i / (BM / V); }
-            else { x = x0 + i / (BK / V); k = k0 + (i % (BK / V)) * V; }
-            const bool row_ok = KMAJOR ? (k < k_end && (!o.live || o.live[k] != 0)) : x < o.extent;
-            const int64_t left = row_ok ? (KMAJOR ? o.extent - x : k_end - k) : 0;      // valid elements from here on
-            const E* q = KMAJOR ? p + k * o.stride + x : p + x * o.stride + k;
-            if (left >= V && o.vec) {
-                const u32x4 w = *(const u32x4*)q;
-                __builtin_memcpy(r[c], &w, 16);
+        for (int j = 0; j < COUNT; ++j) {
+            const int i = wave * COUNT + j;
+            if constexpr (!KM) {
+                const int x = 8 * i + (lane >> 3), q = (lane & 7) ^ ((x >> 1) & 7);
+                kk[j] = 8 * q;
+                off[j] = x0 + x < o.x_extent ? (uint32_t)(x * o.stride) + 16 * q : OUTSIDE;
             } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) r[c][j] = j < left ? q[j] : (E)0;
+                constexpr int PER = XT / 8;                                  // 16-byte chunks of a row
+                const int at = 64 * i + lane, k = at / PER, c = at % PER, x = 8 * (2 * ((c >> 1) ^ (2 * (k & 3))) + (c & 1));
+                kk[j] = k;
+                off[j] = x0 + x < o.x_extent ? (uint32_t)(k * o.stride) + 2 * x : OUTSIDE;
             }
         }
+        base = o.p + (KM ? 2 * x0 : x0 * o.stride);
     }
-    __device__ __forceinline__ void store(Stage<DT>& s) const {
+    // issues the loads of step k0 (of piece `plane`) into the LDS bytes from `lds` on
+    __device__ __forceinline__ void issue(const Op& o, int plane, int64_t k0, uint32_t lds, int wave, uint64_t live) const {
+        const char* b = base + plane * o.plane + (KM ? k0 * o.stride : 2 * k0);
+        const bool tail = k0 + BK > o.k_extent;
+        const int left = (int)(o.k_extent - k0 < BK ? o.k_extent - k0 : BK);
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int i = c * 256 + (int)threadIdx.x;
-            const int x = KMAJOR ? (i % (BM / V)) * V : i / (BK / V), k = KMAJOR ? i / (BM / V) : (i % (BK / V)) * V;
-            uint16_t piece[Elem<DT>::planes][V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if constexpr (DT == F32) {
-                    const float a = r[c][j];
-                    const uint16_t p1 = bf16_bits(a);
-                    const float r1 = a - bf16_value(p1);
-                    const uint16_t p2 = bf16_bits(r1);
-                    piece[0][j] = p1; piece[1][j] = p2; piece[2][j] = bf16_bits(r1 - bf16_value(p2));
-                } else
-                    piece[0][j] = r[c][j];
-            }
-#pragma unroll
-            for (int q = 0; q < Elem<DT>::planes; ++q) {
-                if constexpr (KMAJOR) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) s.v[q][x + j][k] = piece[q][j];
-                } else
-                    __builtin_memcpy(&s.v[q][x][k], piece[q], 2 * V);
-            }
+        for (int j = 0; j < COUNT; ++j) {
+            uint32_t f = off[j];
+            if (tail && kk[j] >= left) f = OUTSIDE;
+            if (KM && live != ~0ull && !((live >> kk[j]) & 1)) f = OUTSIDE;
+            load_to_lds(b, f, lds + 1024u * (uint32_t)(wave * COUNT + j));
         }
     }
 };
 
-// accumulator layout of v_mfma_f32_32x32x16: lane l holds column n = l % 32, register r holds row m = 8 (r / 4) + 4 (l / 32) + r % 4
-struct Acc { f32x16 t[2][2]; };                                     // [m tile][n tile] of this wave's 64 x 64
+template <class C> struct Acc { f32x16 t[C::TM][C::TN]; };        // lane l: column n = l % 32, register r: row m = 8 (r / 4) + 4 (l / 32) + r % 4
 
-template <int DT, bool AK, bool BK_>
-__device__ __forceinline__ void gemm_tile(const Operand& a, const Operand& b, int64_t m0, int64_t n0, int64_t k_begin, int64_t k_end, Acc& acc,
-                                          Stage<DT>& sa, Stage<DT>& sb) {
-    constexpr int P = Elem<DT>::planes;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+// the steps of the sum: for float32 the six products of the pieces, the smallest first, over all of k each
+template <class C, int DT, bool AK, bool BKM>
+__device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, int64_t n0, int64_t k_begin, int64_t k_end, Acc<C>& acc, char* lds_generic) {
+    constexpr int P = Elem<DT>::planes, SEGS = P == 3 ? 6 : 1;
+    lds_char* lds = (lds_char*)lds_generic;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < C::TN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc.t[i][j][r] = 0.0f;
-    Loader<DT, AK> la;
-    Loader<DT, BK_> lb;
-    la.load(a, m0, k_begin, k_end);
-    lb.load(b, n0, k_begin, k_end);
-    for (int64_t k = k_begin; k < k_end; k += BK) {
-        __syncthreads();                                            // the previous tile has been read
-        la.store(sa);
-        lb.store(sb);
-        __syncthreads();
-        if (k + BK < k_end) {
-            la.load(a, m0, k + BK, k_end);
-            lb.load(b, n0, k + BK, k_end);
+    Feed<C::BM, C::LA, AK> fa;
+    Feed<C::BN, C::LB, BKM> fb;
+    fa.init(a, m0, wave, lane);
+    fb.init(b, n0, wave, lane);
+    const int per_seg = k_end > k_begin ? (int)((k_end - k_begin + BK - 1) / BK) : 0, steps = per_seg * SEGS;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
+
+    int issue_k = 0, issue_seg = 0;                                          // of the next step to be issued
+    auto issue = [&](int slot) {
+        int pa = 0, pb = 0;
+        if constexpr (P == 3) {                                              // (1,1) (0,2) (2,0) (0,1) (1,0) (0,0)
+            pa = (0x010201 >> (4 * issue_seg)) & 15;
+            pb = (0x001021 >> (4 * issue_seg)) & 15;
         }
+        const int64_t k0 = k_begin + (int64_t)issue_k * BK;
+        uint64_t la = ~0ull, lb = ~0ull;
+        if (AK && a.live) la = a.live[k0 / BK];
+        if (BKM && b.live) lb = b.live[k0 / BK];
+        fa.issue(a, pa, k0, lds0 + (uint32_t)slot * C::STAGE_BYTES, wave, la);
+        fb.issue(b, pb, k0, lds0 + (uint32_t)slot * C::STAGE_BYTES + C::BM * BK * 2, wave, lb);
+        if (++issue_k == per_seg) { issue_k = 0; ++issue_seg; }
+    };
+
+    // fragment addresses.  not KM: row x, chunk 2 kt + (lane >> 5) of the step (kt = 0 .. 3); KM: rows 16 kt + 8 (lane >> 5) + 4 h + (s >> 2), unit of x
+    uint32_t ra[AK ? C::TM : 4], rb[BKM ? C::TN : 4];
+    const int s = lane & 15;
+    if constexpr (!AK) {
 #pragma unroll
-        for (int kk = 0; kk < BK; kk += 16) {
-            u32x4 fa[P][2], fb[P][2];
+        for (int kt = 0; kt < 4; ++kt) ra[kt] = (wm + (lane & 31)) * 128 + ((2 * kt + (lane >> 5)) ^ ((lane & 31) >> 1 & 7)) * 16;
+    } else {
 #pragma unroll
-            for (int q = 0; q < P; ++q)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    fa[q][i] = *(const u32x4*)&sa.v[q][wm + 32 * i + (lane & 31)][kk + 8 * (lane >> 5)];
-                    fb[q][i] = *(const u32x4*)&sb.v[q][wn + 32 * i + (lane & 31)][kk + 8 * (lane >> 5)];
-                }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if constexpr (P == 3) {                         // smallest products first
-                        acc.t[i][j] = mfma<DT>(fa[1][i], fb[1][j], acc.t[i][j]);
-                        acc.t[i][j] = mfma<DT>(fa[0][i], fb[2][j], acc.t[i][j]);
-                        acc.t[i][j] = mfma<DT>(fa[2][i], fb[0][j], acc.t[i][j]);
-                        acc.t[i][j] = mfma<DT>(fa[0][i], fb[1][j], acc.t[i][j]);
-                        acc.t[i][j] = mfma<DT>(fa[1][i], fb[0][j], acc.t[i][j]);
-                    }
-                    acc.t[i][j] = mfma<DT>(fa[0][i], fb[0][j], acc.t[i][j]);
-                }
-        }
+        for (int i = 0; i < C::TM; ++i)
+            ra[i] = (8 * (lane >> 5) + (s >> 2)) * (2 * C::BM) + (((wm + 32 * i) / 16 + ((lane >> 4) & 1)) ^ (2 * (s >> 2))) * 32 + (s & 3) * 8;
     }
+    if constexpr (!BKM) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) rb[kt] = C::BM * BK * 2 + (wn + (lane & 31)) * 128 + ((2 * kt + (lane >> 5)) ^ ((lane & 31) >> 1 & 7)) * 16;
+    } else {
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+            rb[j] = C::BM * BK * 2 + (8 * (lane >> 5) + (s >> 2)) * (2 * C::BN) + (((wn + 32 * j) / 16 + ((lane >> 4) & 1)) ^ (2 * (s >> 2))) * 32 + (s & 3) * 8;
+    }
+    auto transposed = [&](uint32_t at, int row_bytes) {
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at + 4 * row_bytes));
+        const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+        return u32x4{l2[0], l2[1], h2[0], h2[1]};
+    };
+
+#pragma unroll
+    for (int g = 0; g < C::STAGES - 1; ++g)
+        if (g < steps) issue(g);
+    int slot = 0;
+    for (int t = 0; t < steps; ++t) {
+        // step t has landed when at most the loads of the steps behind it are outstanding
+        const int behind = steps - 1 - t < C::STAGES - 2 ? steps - 1 - t : C::STAGES - 2;
+        if (C::STAGES == 2 || behind == 0) wait_loads<0>();
+        else if (behind == 1) wait_loads<C::LA + C::LB>();
+        else wait_loads<2 * (C::LA + C::LB)>();
+        barrier();                                                           // ... for every wave, and the slot of step t - 1 has been read
+        if (t + C::STAGES - 1 < steps) issue(slot == 0 ? C::STAGES - 1 : slot - 1);
+        const uint32_t at = (uint32_t)slot * C::STAGE_BYTES;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+            u32x4 x[C::TM], y[C::TN];
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i) {
+                if constexpr (!AK) x[i] = *(__attribute__((address_space(3))) u32x4*)(lds + at + ra[kt] + 4096 * i);
+                else x[i] = transposed(at + ra[i] + kt * 16 * 2 * C::BM, 2 * C::BM);
+            }
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) {
+                if constexpr (!BKM) y[j] = *(__attribute__((address_space(3))) u32x4*)(lds + at + rb[kt] + 4096 * j);
+                else y[j] = transposed(at + rb[j] + kt * 16 * 2 * C::BN, 2 * C::BN);
+            }
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < C::TN; ++j) acc.t[i][j] = mfma<DT>(x[i], y[j], acc.t[i][j]);
+        }
+        slot = slot == C::STAGES - 1 ? 0 : slot + 1;
+    }
+    wait_loads<0>();
+    barrier();                                                               // the LDS is free again
+}
+
+// Workgroup -> tile.  Workgroups are dealt to the eight XCDs in turn, each with an L2 of its own: XCD x takes the x-th eighth of the tiles, and within it tiles go
+// in bands of GROUP tiles of n, so that the workgroups that run at one time on one XCD share their operands' tiles on both sides.
+__device__ __forceinline__ void tile_of(uint32_t id, uint32_t total, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn, uint32_t& z) {
+    constexpr uint32_t GROUP = 8;
+    const uint32_t q = total / 8, r = total % 8, x = id % 8, i = id / 8;
+    uint32_t t = x * q + (x < r ? x : r) + i;
+    const uint32_t plane = tiles_m * tiles_n;
+    z = t / plane;
+    t -= z * plane;
+    const uint32_t band = t / (GROUP * tiles_m), first = band * GROUP, height = tiles_n - first < GROUP ? tiles_n - first : GROUP;
+    t -= band * GROUP * tiles_m;
+    tn = first + t % height;
+    tm = t / height;
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// what a launch over logit tiles knows of the head
-struct Head {
-    Operand w, h;                    // A: weight (m = class), B: hidden (n = row)
-    const void* bias;
-    const int64_t* target;           // classes as the prepare kernel wrote them: -1 = ignored, -2 = out of range
-    int64_t rows, width, classes;
-};
-
-// classes widened to int64 with the two special values, and the liveness bytes
-template <typename T>
-__global__ void __launch_bounds__(256) prepare_kernel(const T* __restrict__ target, int64_t rows, int64_t classes, int64_t ignore, int64_t* __restrict__ out,
-                                                      uint8_t* __restrict__ live) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows) return;
-    const int64_t t = (int64_t)target[i];
-    const bool ign = t == ignore;
-    out[i] = ign ? -1 : (t < 0 || t >= classes ? -2 : t);
-    live[i] = ign ? 0 : 1;
+// Operands that the loads above cannot take as they lie (float32; a width that is not a multiple of 8, addresses or strides that are not multiples of 16 bytes) are laid out
+// first: [piece][row][padded], padded = width rounded up to 64 with zeros; rows that do not count are zero.
+template <int DT>
+__global__ void __launch_bounds__(256) lay_out_kernel(const typename Elem<DT>::type* __restrict__ src, int64_t stride, int64_t rows, int64_t width, int64_t padded,
+                                                      const uint8_t* __restrict__ live, uint16_t* __restrict__ out) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= rows * padded) return;
+    const int64_t r = i / padded, k = i - r * padded;
+    uint16_t q[Elem<DT>::planes][8];
+    const bool on = !live || live[r];
+    const typename Elem<DT>::type* p = src + r * stride + k;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (DT == F32) {
+            three_pieces(on && k + j < width ? p[j] : 0.0f, q[0][j], q[1][j], q[2][j]);
+        } else
+            q[0][j] = on && k + j < width ? p[j] : 0;
+    }
+#pragma unroll
+    for (int z = 0; z < Elem<DT>::planes; ++z) __builtin_memcpy(out + z * rows * padded + i, q[z], 16);
 }
 
-// statistics of a set of classes: maximum m, s = sum exp(l - m), u = sum (l - m) exp(l - m)
+// classes widened to int64 with two special values (-1: ignored, -2: out of range), and the rows that count as bytes and as bits
+template <typename T>
+__global__ void __launch_bounds__(256) prepare_kernel(const T* __restrict__ target, int64_t rows, int64_t classes, int64_t ignore, int64_t* __restrict__ out,
+                                                      uint8_t* __restrict__ live, uint64_t* __restrict__ bits) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = i < rows ? (int64_t)target[i] : ignore;
+    const bool ign = t == ignore;
+    const uint64_t w = __ballot(!ign);
+    if (i >= rows) return;
+    out[i] = ign ? -1 : (t < 0 || t >= classes ? -2 : t);
+    live[i] = ign ? 0 : 1;
+    if ((threadIdx.x & 63) == 0) bits[i / 64] = w;
+}
+
+// what a launch over logit tiles knows of the head
+struct Head {
+    Op w, h;                         // A: weight (m = class), B: hidden (n = row)
+    const void* bias;
+    const int64_t* target;           // as prepare_kernel wrote them
+    int64_t rows, width, classes;
+    uint32_t tiles_m, tiles_n;       // of this launch
+    int64_t c0, c1;                  // the classes of this launch
+};
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// Statistics of a set of classes in units of log2: maximum m of l log2(e), s = sum 2^(l log2(e) - m), u = sum (l log2(e) - m) 2^(l log2(e) - m).  One fused
+// multiply-add and one hardware exponential per logit; the reference m is subtracted inside the fma, so no rounding of l log2(e) itself enters.
 struct Stat { float m, s, u; };
 __device__ __forceinline__ Stat joined(const Stat& a, const Stat& b) {
     const float m = fmaxf(a.m, b.m);
     // a set of classes at -inf has m = -inf, s = u = 0 and counts nothing; a difference is kept where 0 x (difference x s) is still 0 (masks of the type's lowest value)
     const float da = a.m == -INFINITY ? 0.0f : fmaxf(a.m - m, -1.0e30f), db = b.m == -INFINITY ? 0.0f : fmaxf(b.m - m, -1.0e30f);
-    const float fa = a.m == -INFINITY ? 0.0f : exp_neg(da), fb = b.m == -INFINITY ? 0.0f : exp_neg(db);
+    const float fa = a.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(da), fb = b.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(db);
     return Stat{m, fa * a.s + fb * b.s, fa * (a.u + da * a.s) + fb * (b.u + db * b.s)};
 }
 
-// class-tile statistics of each row: max m, s = sum exp(l - m), u = sum (l - m) exp(l - m); and the logit of the row's own class
-template <int DT>
-__global__ void __launch_bounds__(256) statistics_kernel(Head hd, float* __restrict__ part, float* __restrict__ own_logit) {
-    __shared__ Stage<DT> sa, sb;
-    __shared__ float red[2][BN][3];
+// bias of the classes a lane holds: base + 32 i + 8 (r / 4) + r % 4
+template <int DT, class C>
+__device__ __forceinline__ void add_bias(Acc<C>& acc, const void* bias, int64_t base, int64_t c1) {
     typedef typename Elem<DT>::type E;
-    const int64_t m0 = (int64_t)blockIdx.x * BM, n0 = (int64_t)blockIdx.y * BN;
-    Acc acc;
-    gemm_tile<DT, false, false>(hd.w, hd.h, m0, n0, 0, hd.width, acc, sa, sb);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    const E* bias = (const E*)hd.bias;
+    const E* b = (const E*)bias;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int64_t m = base + 32 * i + 8 * (r >> 2) + (r & 3);
+            const float v = to_float<DT>(b[m < c1 ? m : c1 - 1]);           // (what lies past the last class is not used)
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) acc.t[i][j][r] += v;
+        }
+}
+
+// class-tile statistics of each row, and the logit of the row's own class
+template <class C, int DT>
+__global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, int64_t tile0, float* __restrict__ part, float* __restrict__ own_logit) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    uint32_t tm, tn, z;
+    tile_of(blockIdx.x, gridDim.x, hd.tiles_m, hd.tiles_n, tm, tn, z);
+    const int64_t m0 = hd.c0 + (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
+    Acc<C> acc;
+    gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
+    const int64_t base = m0 + wm + 4 * (lane >> 5);                  // class of the lane's register 0
+    if (hd.bias) add_bias<DT>(acc, hd.bias, base, hd.c1);
+    if (m0 + C::BM > hd.c1) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (base + 32 * i + 8 * (r >> 2) + (r & 3) >= hd.c1)
+#pragma unroll
+                    for (int j = 0; j < C::TN; ++j) acc.t[i][j][r] = -INFINITY;
+    }
+    float (*red)[C::BN][3] = (float (*)[C::BN][3])lds;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
         const int nl = wn + 32 * j + (lane & 31);
-        const int64_t n = n0 + nl;
-        const int64_t t = n < hd.rows ? hd.target[n] : -1;
+        const int64_t n = n0 + nl, t = n < hd.rows ? hd.target[n] : -1;
+        const int64_t rel = t - (m0 + wm);
+        if (__any(rel >= 0 && rel < C::TM * 32)) {
+            const int own = t >= base && rel < C::TM * 32 ? (int)(t - base) : -1;
+            float l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) l = own == 32 * i + 8 * (r >> 2) + (r & 3) ? acc.t[i][j][r] : l;
+            if (own >= 0 && (own & 4) == 0) own_logit[n] = l;
+        }
         float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t m = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                float l = acc.t[i][j][r];
-                if (m < hd.classes) {
-                    if (bias) l += to_float<DT>(bias[m]);
-                    if (m == t) own_logit[n] = l;
-                } else
-                    l = -INFINITY;
-                acc.t[i][j][r] = l;
-                mx = fmaxf(mx, l);
-            }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc.t[i][j][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * LOG2E;
         const float ref = mx == -INFINITY ? 0.0f : mx;
         float s = 0.0f, u = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < C::TM; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float d = acc.t[i][j][r] - ref, e = exp_neg(d);
+                const float d = fmaf(acc.t[i][j][r], LOG2E, -ref), e = __builtin_amdgcn_exp2f(d);
                 s += e;
                 u = fmaf(fmaxf(d, -3.0e38f), e, u);                 // a class at -inf adds 0, not 0 x inf
             }
         s += __shfl_xor(s, 32, 64);
         u += __shfl_xor(u, 32, 64);
-        if (lane < 32) { red[wave & 1][nl][0] = mx; red[wave & 1][nl][1] = s; red[wave & 1][nl][2] = u; }
+        if (lane < 32) { red[wave % C::WM][nl][0] = mx; red[wave % C::WM][nl][1] = s; red[wave % C::WM][nl][2] = u; }
     }
     __syncthreads();
-    if (threadIdx.x < BN && n0 + threadIdx.x < hd.rows) {
-        const int nl = threadIdx.x;
-        const Stat t = joined(Stat{red[0][nl][0], red[0][nl][1], red[0][nl][2]}, Stat{red[1][nl][0], red[1][nl][1], red[1][nl][2]});
-        float* o = part + 3 * (size_t)blockIdx.x * hd.rows + n0 + nl;
-        o[0] = t.m; o[hd.rows] = t.s; o[2 * hd.rows] = t.u;
-    }
+    for (int nl = threadIdx.x; nl < C::BN; nl += C::THREADS)
+        if (n0 + nl < hd.rows) {
+            Stat t{red[0][nl][0], red[0][nl][1], red[0][nl][2]};
+#pragma unroll
+            for (int w = 1; w < C::WM; ++w) t = joined(t, Stat{red[w][nl][0], red[w][nl][1], red[w][nl][2]});
+            float* o = part + 3 * (size_t)(tile0 + tm) * hd.rows + n0 + nl;
+            o[0] = t.m; o[hd.rows] = t.s; o[2 * hd.rows] = t.u;
+        }
 }
 
-// joins the tiles' statistics: 16 lanes per row, 16 rows per workgroup
+// joins the tiles' statistics: 16 lanes per row, 16 rows per workgroup.  lse is kept in units of log2
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, const float* __restrict__ own_logit, const int64_t* __restrict__ target,
                                                    int64_t rows, int tiles, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ entropy_kept,
                                                    float* __restrict__ lse) {
@@ -290,9 +427,9 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     if (threadIdx.x < 16 && n < rows) {
         for (int k = 1; k < 16; ++k) a = joined(a, Stat{red[0][k][r], red[1][k][r], red[2][k][r]});
         const int64_t t = target[n];
-        const float ls = logf(a.s);
-        float z = a.m + ls, h = ls - a.u / a.s, lp = 0.0f;
-        if (t >= 0) lp = (own_logit[n] - a.m) - ls;
+        const float ls = __log2f(a.s);
+        float z = a.m + ls, h = LN2 * (ls - a.u / a.s), lp = 0.0f;
+        if (t >= 0) lp = LN2 * (fmaf(own_logit[n], LOG2E, -a.m) - ls);
         else if (t == -1) { h = 0.0f; z = 0.0f; }                  // ignored
         else { lp = h = z = NAN; }                                  // a class that does not exist
         logp[n] = lp;
@@ -362,63 +499,128 @@ __global__ void __launch_bounds__(1024) scale_kernel(Upstream up, const uint8_t*
     }
 }
 
-// a piece [c0, c0 + piece) of the classes: the logits again, and the gradient of each -> g[row][class - c0] (stride `piece`), and the sums over
-// this tile's rows -> db_part[row tile][class]
-template <int DT>
-__global__ void __launch_bounds__(256) gradient_kernel(Head hd, Upstream up, int64_t c0, int64_t c1, int64_t piece, const float* __restrict__ lse, const float* __restrict__ entropy,
-                                                       void* __restrict__ g_out, float* __restrict__ db_part) {
-    __shared__ Stage<DT> sa, sb;
-    typedef typename Elem<DT>::type E;
-    const int64_t m0 = c0 + (int64_t)blockIdx.x * BM, n0 = (int64_t)blockIdx.y * BN;
-    Acc acc;
-    gemm_tile<DT, false, false>(hd.w, hd.h, m0, n0, 0, hd.width, acc, sa, sb);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    const E* bias = (const E*)hd.bias;
-    E* g = (E*)g_out;
+// A lane holds 4 classes of each group of 8 (register quads r4 = 0 .. 3), its partner lane ^ 32 the other 4.  Packed to 16 bits a quad is two words; exchanging the odd quad of
+// the lower half with the even quad of the upper one leaves every lane with 8 neighbours - one 16-byte store: lanes < 32 those of group 2 h, the others those of group 2 h + 1.
+__device__ __forceinline__ u32x4 eight_of(u32x2 even, u32x2 odd) {
+    const auto a = __builtin_amdgcn_permlane32_swap(even[0], odd[0], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(even[1], odd[1], false, false);
+    return u32x4{a[0], b[0], a[1], b[1]};
+}
+template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (DT == F16) {
+        typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+        return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
+    } else {
+        typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+        return __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
+    }
+}
+
+// the sum over the 32 lanes of each half of the wave, in lanes 31 and 63
+__device__ __forceinline__ float half_sum(float v) {
+#define Q1_DPP_ADD(ctrl, mask) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, mask, 0xf, true))
+    Q1_DPP_ADD(0x111, 0xf); Q1_DPP_ADD(0x112, 0xf); Q1_DPP_ADD(0x114, 0xf); Q1_DPP_ADD(0x118, 0xf); Q1_DPP_ADD(0x142, 0xa);
+#undef Q1_DPP_ADD
+    return v;
+}
+
+// a piece [c0, c1) of the classes: the logits again, and the gradient of each -> g[row][class - c0] (stride `piece`; 16 bits, float32 as three pieces g_plane values apart), zero
+// up to the end of the last tile; and the sums over this tile's rows -> db_part[row tile][class]
+template <class C, int DT>
+__global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream up, int64_t piece, int64_t g_plane, const float* __restrict__ lse,
+                                                              const float* __restrict__ entropy, uint16_t* __restrict__ g, float* __restrict__ db_part) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    uint32_t tm, tn, zz;
+    tile_of(blockIdx.x, gridDim.x, hd.tiles_m, hd.tiles_n, tm, tn, zz);
+    const int64_t m0 = hd.c0 + (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
+    Acc<C> acc;
+    gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
+    const int64_t base = m0 + wm + 4 * (lane >> 5);
+    if (hd.bias) add_bias<DT>(acc, hd.bias, base, hd.c1);
     const float sc = up.scale[0];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t n = n0 + wn + 32 * j + (lane & 31);
-        const int64_t t = n < hd.rows ? hd.target[n] : -1;
+    for (int j = 0; j < C::TN; ++j) {
+        const int64_t n = n0 + wn + 32 * j + (lane & 31), t = n < hd.rows ? hd.target[n] : -1;
         const bool on = t != -1;
-        const float z = on ? lse[n] : 0.0f, hrow = on && up.dentropy ? entropy[n] : 0.0f;
-        const float A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) * sc : 0.0f, Ee = on && up.dentropy ? up.dentropy[n] * sc : 0.0f;
+        const float z = on ? lse[n] : 0.0f;
+        const float A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) * sc : 0.0f, E = on && up.dentropy ? up.dentropy[n] * sc : 0.0f;
+        const float hrow = on && up.dentropy ? entropy[n] : 0.0f, El = E * LN2, Ah = A + E * hrow;
+        const bool here = __any(t >= m0 + wm && t < m0 + wm + C::TM * 32);
+        const int own = t >= base && t < base + C::TM * 32 ? (int)(t - base) : -1;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int64_t m = m0 + wm + 32 * i + 8 * r4 + 4 * (lane >> 5);
-                E q[4];
+            for (int r = 0; r < 16; ++r) {
+                const float d = fmaf(acc.t[i][j][r], LOG2E, -z), p = __builtin_amdgcn_exp2f(d);
+                // g = -p (A + E (log p + H)); a class at -inf has p = 0 and a finite factor
+                float v = up.dentropy ? -p * fmaf(El, fmaxf(d, -3.0e38f), Ah) : -p * A;
+                acc.t[i][j][r] = on ? v : 0.0f;
+            }
+        if (here) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = 0.0f;
-                    if (on && m + r < c1) {
-                        float l = acc.t[i][j][4 * r4 + r];
-                        if (bias) l += to_float<DT>(bias[m + r]);
-                        const float d = l - z, p = exp_neg(d);
-                        v = -A * p;
-                        if (up.dentropy) v -= Ee * p * (fmaxf(d, -3.0e38f) + hrow);
-                        if (m + r == t) v += A;
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (own == 32 * i + 8 * (r >> 2) + (r & 3)) acc.t[i][j][r] += A;
+        }
+    }
+    if (m0 + C::BM > hd.c1) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (base + 32 * i + 8 * (r >> 2) + (r & 3) >= hd.c1)
+#pragma unroll
+                    for (int j = 0; j < C::TN; ++j) acc.t[i][j][r] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+        const int64_t n = n0 + wn + 32 * j + (lane & 31);
+        uint16_t* row = g + n * piece + (m0 - hd.c0) + wm + 8 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] = acc.t[i][j][8 * h + r];
+#pragma unroll
+                for (int q = 0; q < Elem<DT>::planes; ++q) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        w[r] = pack2<DT>(v[2 * r], v[2 * r + 1]);
+                        if constexpr (DT == F32) {                  // what this piece leaves for the next
+                            v[2 * r] -= __builtin_bit_cast(float, w[r] << 16);
+                            v[2 * r + 1] -= __builtin_bit_cast(float, w[r] & 0xffff0000u);
+                        }
                     }
-                    acc.t[i][j][4 * r4 + r] = v;
-                    q[r] = from_float<DT>(v);
+                    const u32x4 o = eight_of(u32x2{w[0], w[1]}, u32x2{w[2], w[3]});
+                    if (n < hd.rows) *(u32x4*)(row + q * g_plane + 32 * i + 16 * h) = o;
                 }
-                if (n < hd.rows && m < c0 + piece) __builtin_memcpy(g + n * piece + (m - c0), q, sizeof q);      // piece is a multiple of BM
             }
     }
     if (db_part) {
-        float (*red)[BM] = (float (*)[BM])&sa;                       // [4][BM]: 2 column halves x 2 lane halves never write the same word
-        __syncthreads();
-        for (int i = 0; i < 2; ++i)
+        float (*red)[C::BM] = (float (*)[C::BM])lds;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float v = acc.t[i][0][r] + acc.t[i][1][r];
+                float v = acc.t[i][0][r];
 #pragma unroll
-                for (int off = 16; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-                if ((lane & 31) == 0) red[wave >> 1][wm + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)] = v;
+                for (int j = 1; j < C::TN; ++j) v += acc.t[i][j][r];
+                v = half_sum(v);
+                if ((lane & 31) == 31) red[wave / C::WM][wm + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)] = v;
             }
         __syncthreads();
-        if (threadIdx.x < BM && m0 + threadIdx.x < c1) db_part[(size_t)blockIdx.y * hd.classes + m0 + threadIdx.x] = red[0][threadIdx.x] + red[1][threadIdx.x];
+        for (int m = threadIdx.x; m < C::BM; m += C::THREADS)
+            if (m0 + m < hd.c1) {
+                float v = red[0][m];
+#pragma unroll
+                for (int w = 1; w < C::WN; ++w) v += red[w][m];
+                db_part[(size_t)tn * hd.classes + m0 + m] = v;
+            }
     }
 }
 
@@ -435,44 +637,79 @@ __global__ void __launch_bounds__(256) bias_kernel(const float* __restrict__ par
 // out[n][m] (stride out_stride): m = column of the result (width), n = its row.  slab: the sums stay in float32 [split][rows][width] for
 // finish_kernel (accumulate: added to what is there); without it the scaled result is stored.
 struct Product {
-    Operand a, b;
-    int64_t k, split_k;                // length of the sum; part per z-slice (a multiple of BK)
+    Op a, b;
+    int64_t k, split_k;                // length of the sum; part per split (a multiple of BK)
     int64_t rows, width;               // of the result
+    uint32_t tiles_m, tiles_n;
     void* out;
     int64_t out_stride;
+    int vec;                           // the result takes 16-byte stores: addresses, stride and width
     float* slab;
     int accumulate;
     const float* scale;
     const uint8_t* live;               // result rows that are zero whatever the operands hold
 };
 
-template <int DT, bool AK, bool BK_>
-__global__ void __launch_bounds__(256) product_kernel(Product pr) {
-    __shared__ Stage<DT> sa, sb;
-    const int64_t m0 = (int64_t)blockIdx.x * BM, n0 = (int64_t)blockIdx.y * BN;
-    const int64_t kb = (int64_t)blockIdx.z * pr.split_k, ke = kb + pr.split_k < pr.k ? kb + pr.split_k : pr.k;
-    Acc acc;
-    gemm_tile<DT, AK, BK_>(pr.a, pr.b, m0, n0, kb, ke, acc, sa, sb);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+template <class C, int DT, bool AK, bool BKM>
+__global__ void __launch_bounds__(C::THREADS) product_kernel(Product pr) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef typename Elem<DT>::type E;
+    uint32_t tm, tn, z;
+    tile_of(blockIdx.x, gridDim.x, pr.tiles_m, pr.tiles_n, tm, tn, z);
+    const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
+    const int64_t kb = (int64_t)z * pr.split_k, ke = kb + pr.split_k < pr.k ? kb + pr.split_k : pr.k;
+    Acc<C> acc;
+    gemm_tile<C, DT, AK, BKM>(pr.a, pr.b, m0, n0, kb, ke, acc, lds);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const float sc = pr.slab ? 1.0f : pr.scale[1];
+    float* slab = pr.slab ? pr.slab + (size_t)z * pr.rows * pr.width : nullptr;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < C::TN; ++j) {
         const int64_t n = n0 + wn + 32 * j + (lane & 31);
-        if (n >= pr.rows) continue;
-        const bool on = !pr.live || pr.live[n];
+        const bool row = n < pr.rows, on = row && (!pr.live || pr.live[n]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < C::TM; ++i) {
+            const int64_t m = m0 + wm + 32 * i;
+            if (pr.slab || DT == F32) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t m = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                if (m >= pr.width) continue;
-                if (pr.slab) {
-                    float* o = pr.slab + ((size_t)blockIdx.z * pr.rows + n) * pr.width + m;
-                    *o = pr.accumulate ? *o + acc.t[i][j][r] : acc.t[i][j][r];
-                } else
-                    ((E*)pr.out)[n * pr.out_stride + m] = from_float<DT>(on ? acc.t[i][j][r] * sc : 0.0f);
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const int64_t mm = m + 8 * r4 + 4 * (lane >> 5);
+                    float* o = pr.slab ? slab + n * pr.width + mm : (float*)pr.out + n * pr.out_stride + mm;
+                    f32x4 v;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = pr.slab ? acc.t[i][j][4 * r4 + r] : (on ? acc.t[i][j][4 * r4 + r] * sc : 0.0f);
+                    if (!row) continue;
+                    if (pr.vec && mm + 4 <= pr.width) {
+                        if (pr.slab && pr.accumulate) v += *(const f32x4*)o;
+                        *(f32x4*)o = v;
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (mm + r < pr.width) o[r] = pr.slab && pr.accumulate ? o[r] + v[r] : v[r];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float x = acc.t[i][j][8 * h + 2 * r] * sc, y = acc.t[i][j][8 * h + 2 * r + 1] * sc;
+                        w[r] = on ? pack2<DT>(x, y) : 0u;
+                    }
+                    const u32x4 o8 = eight_of(u32x2{w[0], w[1]}, u32x2{w[2], w[3]});
+                    const int64_t mm = m + 16 * h + 8 * (lane >> 5);
+                    E* o = (E*)pr.out + n * pr.out_stride + mm;
+                    if (!row) continue;
+                    if (pr.vec && mm + 8 <= pr.width) *(u32x4*)o = o8;
+                    else {
+#pragma unroll
+                        for (int r = 0; r < 8; ++r)
+                            if (mm + r < pr.width) o[r] = (E)(o8[r >> 1] >> (16 * (r & 1)));
+                    }
+                }
             }
+        }
     }
 }
 
