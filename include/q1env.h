@@ -615,7 +615,8 @@ uint64_t q1env_head_workspace_bytes(int dtype, int64_t rows, int64_t width, int6
  * rows that are not ignored (Q1ENV_REDUCE_MEAN; 0 when all are). */
 int q1env_head_forward(int device, void* stream, const q1env_head* head, int reduction, float* logp_dev, float* entropy_dev, float* loss_dev);
 /* The gradients of hidden, weight and bias (each may be NULL) for EITHER dlogp / dentropy (float[rows], one may be NULL) OR dloss (one float: the
- * gradient of the loss the forward call wrote).  The head is the one the forward call had, with its state; results are overwritten. */
+ * gradient of the loss the forward call wrote).  The head is the one the forward call had, with its state; results are overwritten.  dentropy needs a
+ * forward call that was asked for the entropy (results are NaN otherwise). */
 int q1env_head_backward(int device, void* stream, const q1env_head* head, const float* dlogp_dev, const float* dentropy_dev, const float* dloss_dev,
                         void* dhidden_dev, int64_t dhidden_stride, void* dweight_dev, int64_t dweight_stride, void* dbias_dev);
 

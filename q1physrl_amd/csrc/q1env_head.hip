@@ -10,7 +10,7 @@ using namespace q1head;
 
 namespace {
 
-constexpr uint64_t PIECE_BYTES = 256ull << 20;     // of the gradient of one piece of the classes
+constexpr uint64_t PIECE_BYTES = 448ull << 20;     // of the gradient of one piece of the classes
 constexpr uint64_t LAID_BYTES = 96ull << 20;       // of the laid-out weights of one piece
 constexpr int64_t MAX_ROWS = 1 << 22, MAX_WIDTH = 1 << 16, MAX_CLASSES = 1 << 22;
 constexpr int64_t PIECE_STEP = 256;                // pieces are whole tiles of every configuration
@@ -44,23 +44,36 @@ struct State {
     }
 };
 
-// which tile a product of m x n results with k terms takes
 enum Size { LARGE, MIDDLE, FEW, FEWEST };
-Size size_of(int64_t m, int64_t n, int64_t k) {
-    if (n <= 32) return FEWEST;
-    if (n <= 64) return FEW;
-    return k >= 512 && div_up(m, 256) * div_up(n, 256) >= 384 ? LARGE : MIDDLE;
-}
 int64_t bm_of(Size s) { return s == LARGE ? 256 : 128; }
 int64_t bn_of(Size s) { return s == LARGE ? 256 : s == MIDDLE ? 128 : s == FEW ? 64 : 32; }
 
-// how the sums of a product are split over workgroups when its result has few tiles
-void split(int64_t tiles, int64_t k, int& n, int64_t& len) {
-    int64_t s = div_up(512, tiles), most = div_up(k, 512);        // two workgroups per CU; a part shorter than 512 costs more in its slab than it gains
-    if (s > most) s = most;
-    if (s < 1) s = 1;
-    len = round_up(div_up(k, s), BK);
-    n = (int)div_up(k, len);
+// The tile of a product of m x n results with k terms, and into how many parts its sum is split, by what it should take in nanoseconds.  One round of Large workgroups (256,
+// one per CU) was measured at 30 ns per term of k, one of Middle (512, two per CU) at 18; `start` is what a round costs besides (prologue and epilogue); the slabs of a split sum are written
+// and read once at 4.5 TB/s.  `split` false: one part only.
+struct Shape { Size size; int parts; int64_t len; };
+Shape shape_of(int64_t m, int64_t n, int64_t k, int products, bool split, double start_large, double start_middle) {
+    if (n <= 64) {                                    // few rows: 512 workgroups (two per CU), parts of 512 terms at least
+        const Size s = n <= 32 ? FEWEST : FEW;
+        const int64_t tiles = div_up(m, bm_of(s));
+        int64_t parts = split ? std::max<int64_t>(1, std::min(div_up(512, tiles), div_up(k, 512))) : 1;
+        const int64_t len = round_up(div_up(k, parts), BK);
+        return Shape{s, (int)div_up(k, len), len};
+    }
+    Shape best{MIDDLE, 1, round_up(k, BK)};
+    double least = 0.0;
+    for (int s = LARGE; s <= MIDDLE; ++s) {
+        const int64_t tiles = div_up(m, bm_of((Size)s)) * div_up(n, bn_of((Size)s)), slots = s == LARGE ? 256 : 512;
+        const int64_t most = split ? std::min<int64_t>(div_up(k, 256), std::max<int64_t>(1, div_up(4 * slots, tiles))) : 1;
+        for (int64_t parts = 1; parts <= most; ++parts) {
+            const int64_t len = round_up(div_up(k, parts), BK), real = div_up(k, len);
+            const double rounds = (double)div_up(tiles * real, slots);
+            double t = rounds * ((double)len * products * (s == LARGE ? 30.0 : 18.0) + (s == LARGE ? start_large : start_middle));
+            if (real > 1) t += 3000.0 + (double)real * (double)m * (double)n * 8.0 / 4500.0;
+            if (least == 0.0 || t < least) { least = t; best = Shape{(Size)s, (int)real, len}; }
+        }
+    }
+    return best;
 }
 
 bool in_place(int dt, const void* p, int64_t stride, int64_t width) {       // whether the loads can take an operand as it lies
@@ -89,18 +102,18 @@ Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward
     if (backward) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(PIECE_BYTES / (2 * planes_of(dt) * rows)) / PIECE_STEP * PIECE_STEP));
     p.piece = piece;
     p.pieces = div_up(classes, piece);
-    p.logits = size_of(std::min(piece, classes), rows, width);
+    const int products = planes_of(dt) == 3 ? 6 : 1;
+    p.logits = shape_of(std::min(piece, classes), rows, width, products, false, 9000.0, 6000.0).size;
     uint64_t at = 0;
     auto take = [&](uint64_t n) { const uint64_t o = at; at += aligned(n); return o; };
     if (!backward) {
         p.own = take(4 * rows);
         p.part = take(12 * (uint64_t)div_up(classes, 128) * rows);
     } else {
-        p.dh = size_of(width, rows, piece);
-        p.dw = size_of(width, std::max<int64_t>(piece, 128), rows);          // (both operands lie k-major: no tile under 128)
-        if (p.dw == FEW || p.dw == FEWEST) p.dw = MIDDLE;
-        split(div_up(width, bm_of(p.dh)) * div_up(rows, bn_of(p.dh)), piece, p.dh_split, p.dh_k);
-        split(div_up(width, bm_of(p.dw)) * div_up(piece, bn_of(p.dw)), rows, p.dw_split, p.dw_k);
+        const Shape dh = shape_of(width, rows, std::min(piece, classes), products, true, 4000.0, 3000.0);
+        const Shape dw = shape_of(width, std::max<int64_t>(std::min(piece, classes), 65), rows, products, true, 4000.0, 3000.0);      // (both operands lie k-major: no tile under 128)
+        p.dh = dh.size; p.dh_split = dh.parts; p.dh_k = dh.len;
+        p.dw = dw.size; p.dw_split = dw.parts; p.dw_k = dw.len;
         p.scale = take(256);
         p.g = take(2 * (uint64_t)planes_of(dt) * rows * piece);
         p.db = take(4 * (uint64_t)div_up(rows, bn_of(p.logits)) * classes);
@@ -164,15 +177,20 @@ template <class C, auto KERNEL, typename... A> int go(hipStream_t stream, int de
 
 struct Where { hipStream_t stream; int device; };
 
-template <class C, int DT> int statistics(const Where& at, Head hd, float* part, float* own) {
+template <class C, int DT> int statistics(const Where& at, Head hd, const Target& target, bool entropy, float* part, float* own) {
     hd.tiles_m = (uint32_t)div_up(hd.c1 - hd.c0, C::BM);
     hd.tiles_n = (uint32_t)div_up(hd.rows, C::BN);
-    return go<C, statistics_kernel<C, DT>>(at.stream, at.device, (int64_t)hd.tiles_m * hd.tiles_n, hd, hd.c0 / C::BM, part, own);
+    const int64_t workgroups = (int64_t)hd.tiles_m * hd.tiles_n;
+    return entropy ? go<C, statistics_kernel<C, DT, true>>(at.stream, at.device, workgroups, hd, target, hd.c0 / C::BM, part, own)
+                   : go<C, statistics_kernel<C, DT, false>>(at.stream, at.device, workgroups, hd, target, hd.c0 / C::BM, part, own);
 }
 template <class C, int DT> int gradient(const Where& at, Head hd, const Upstream& up, int64_t piece, const State& st, uint16_t* g, float* db) {
     hd.tiles_m = (uint32_t)div_up(hd.c1 - hd.c0, C::BM);
     hd.tiles_n = (uint32_t)div_up(hd.rows, C::BN);
-    return go<C, gradient_kernel<C, DT>>(at.stream, at.device, (int64_t)hd.tiles_m * hd.tiles_n, hd, up, piece, hd.rows * piece, (const float*)st.lse, (const float*)st.entropy, g, db);
+    const int64_t workgroups = (int64_t)hd.tiles_m * hd.tiles_n, plane = hd.rows * piece;
+    const float *lse = st.lse, *entropy = st.entropy;
+    return up.dentropy ? go<C, gradient_kernel<C, DT, true>>(at.stream, at.device, workgroups, hd, up, piece, plane, lse, entropy, g, db)
+                       : go<C, gradient_kernel<C, DT, false>>(at.stream, at.device, workgroups, hd, up, piece, plane, lse, entropy, g, db);
 }
 template <class C, int DT, bool BKM> int product(const Where& at, Product pr, int splits) {
     pr.tiles_m = (uint32_t)div_up(pr.width, C::BM);
@@ -202,12 +220,7 @@ int forward(const Where& at, const q1env_head& q, int reduction, float* logp, fl
         const bool hp = in_place(DT, q.hidden_dev, q.hidden_stride, q.width), wp = in_place(DT, q.weight_dev, q.weight_stride, q.width);
         const Plan p = plan_of(DT, n, q.width, q.classes, false, hp, wp);
         char* ws = (char*)q.ws_dev;
-        const dim3 rows256((unsigned)div_up(n, 256));
-        if (q.target_bits == 64)
-            hipLaunchKernelGGL((prepare_kernel<int64_t>), rows256, dim3(256), 0, at.stream, (const int64_t*)q.target_dev, n, q.classes, q.ignore_index, st.target, st.live, st.bits);
-        else
-            hipLaunchKernelGGL((prepare_kernel<int32_t>), rows256, dim3(256), 0, at.stream, (const int32_t*)q.target_dev, n, q.classes, q.ignore_index, st.target, st.live, st.bits);
-        HIP_TRY(hipGetLastError());
+        const Target target{q.target_dev, q.target_bits == 64 ? 1 : 0, q.ignore_index, q.classes};
         if (!hp) Q1_TRY(lay_out<DT>(at, q.hidden_dev, q.hidden_stride, n, q.width, p.padded, nullptr, ws + p.h_laid));
         const Op h = rows_op(DT, hp, q.hidden_dev, q.hidden_stride, n, q.width, p.padded, ws + p.h_laid);
         float *part = (float*)(ws + p.part), *own = (float*)(ws + p.own);
@@ -215,14 +228,14 @@ int forward(const Where& at, const q1env_head& q, int reduction, float* logp, fl
             const int64_t c1 = std::min(c0 + p.piece, q.classes);
             const char* w0 = (const char*)q.weight_dev + elem_size(DT) * c0 * q.weight_stride;
             if (!wp) Q1_TRY(lay_out<DT>(at, w0, q.weight_stride, c1 - c0, q.width, p.padded, nullptr, ws + p.w_laid));
-            const Head hd{rows_op(DT, wp, w0, q.weight_stride, c1 - c0, q.width, p.padded, ws + p.w_laid), h, q.bias_dev, st.target, n, q.width, q.classes, 0, 0, c0, c1};
-            if (p.logits == LARGE) Q1_TRY((statistics<Large, DT>(at, hd, part, own)));
-            else if (p.logits == MIDDLE) Q1_TRY((statistics<Middle, DT>(at, hd, part, own)));
-            else if (p.logits == FEW) Q1_TRY((statistics<Few, DT>(at, hd, part, own)));
-            else Q1_TRY((statistics<Fewest, DT>(at, hd, part, own)));
+            const Head hd{rows_op(DT, wp, w0, q.weight_stride, c1 - c0, q.width, p.padded, ws + p.w_laid), h, q.bias_dev, nullptr, n, q.width, q.classes, 0, 0, c0, c1};
+            if (p.logits == LARGE) Q1_TRY((statistics<Large, DT>(at, hd, target, entropy != nullptr, part, own)));
+            else if (p.logits == MIDDLE) Q1_TRY((statistics<Middle, DT>(at, hd, target, entropy != nullptr, part, own)));
+            else if (p.logits == FEW) Q1_TRY((statistics<Few, DT>(at, hd, target, entropy != nullptr, part, own)));
+            else Q1_TRY((statistics<Fewest, DT>(at, hd, target, entropy != nullptr, part, own)));
         }
-        hipLaunchKernelGGL(join_kernel, dim3((unsigned)div_up(n, 16)), dim3(256), 0, at.stream, part, own, st.target, n, (int)div_up(q.classes, bm_of(p.logits)), logp, entropy, st.entropy,
-                           st.lse);
+        hipLaunchKernelGGL(join_kernel, dim3((unsigned)div_up(n, 64)), dim3(1024), 0, at.stream, part, own, target, n, (int)div_up(q.classes, bm_of(p.logits)), entropy ? 1 : 0, logp,
+                           entropy, st.entropy, st.lse, st.target, st.live, st.bits);
         HIP_TRY(hipGetLastError());
     }
     if (loss) {
@@ -288,7 +301,7 @@ int backward(const Where& at, const q1env_head& q, Upstream up, void* dh, int64_
         HIP_TRY(hipGetLastError());
     }
     if (db) {
-        hipLaunchKernelGGL((bias_kernel<DT>), dim3((unsigned)div_up(v, 256)), dim3(256), 0, at.stream, (const float*)db_part, v, (int)div_up(n, bn_of(p.logits)), scale, db);
+        hipLaunchKernelGGL((bias_kernel<DT>), dim3((unsigned)div_up(v, 64)), dim3(1024), 0, at.stream, (const float*)db_part, v, (int)div_up(n, bn_of(p.logits)), scale, db);
         HIP_TRY(hipGetLastError());
     }
     return Q1ENV_OK;

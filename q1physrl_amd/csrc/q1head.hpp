@@ -152,40 +152,45 @@ template <int XT, int COUNT, bool KM> struct Feed {
 
 template <class C> struct Acc { f32x16 t[C::TM][C::TN]; };        // lane l: column n = l % 32, register r: row m = 8 (r / 4) + 4 (l / 32) + r % 4
 
-// the steps of the sum: for float32 the six products of the pieces, the smallest first, over all of k each
-template <class C, int DT, bool AK, bool BKM>
-__device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, int64_t n0, int64_t k_begin, int64_t k_end, Acc<C>& acc, char* lds_generic) {
-    constexpr int P = Elem<DT>::planes, SEGS = P == 3 ? 6 : 1;
-    lds_char* lds = (lds_char*)lds_generic;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
+template <class C> __device__ __forceinline__ void clear(Acc<C>& acc) {
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc.t[i][j][r] = 0.0f;
+}
+
+// acc += the product.  For float32 the six products of the pieces follow each other within every step of k, so that a piece's tile is still near when it is asked for again.
+// A step's fragments are read one quarter ahead of their use, the last quarter's and the next step's first on either side of the one barrier: the matrix
+// instructions behind it have their operands already.  A slot is free at that barrier (its last fragments are in registers), so STAGES steps are in flight.
+template <class C, int DT, bool AK, bool BKM>
+__device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, int64_t n0, int64_t k_begin, int64_t k_end, Acc<C>& acc, char* lds_generic) {
+    constexpr int P = Elem<DT>::planes, SEGS = P == 3 ? 6 : 1;
+    lds_char* lds = (lds_char*)lds_generic;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     Feed<C::BM, C::LA, AK> fa;
     Feed<C::BN, C::LB, BKM> fb;
     fa.init(a, m0, wave, lane);
     fb.init(b, n0, wave, lane);
-    const int per_seg = k_end > k_begin ? (int)((k_end - k_begin + BK - 1) / BK) : 0, steps = per_seg * SEGS;
+    const int steps = k_end > k_begin ? (int)((k_end - k_begin + BK - 1) / BK) * SEGS : 0;
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
 
-    int issue_k = 0, issue_seg = 0;                                          // of the next step to be issued
+    int64_t issue_k = k_begin;                                               // of the next step to be issued
+    int issue_seg = 0;
     auto issue = [&](int slot) {
         int pa = 0, pb = 0;
         if constexpr (P == 3) {                                              // (1,1) (0,2) (2,0) (0,1) (1,0) (0,0)
             pa = (0x010201 >> (4 * issue_seg)) & 15;
             pb = (0x001021 >> (4 * issue_seg)) & 15;
         }
-        const int64_t k0 = k_begin + (int64_t)issue_k * BK;
         uint64_t la = ~0ull, lb = ~0ull;
-        if (AK && a.live) la = a.live[k0 / BK];
-        if (BKM && b.live) lb = b.live[k0 / BK];
-        fa.issue(a, pa, k0, lds0 + (uint32_t)slot * C::STAGE_BYTES, wave, la);
-        fb.issue(b, pb, k0, lds0 + (uint32_t)slot * C::STAGE_BYTES + C::BM * BK * 2, wave, lb);
-        if (++issue_k == per_seg) { issue_k = 0; ++issue_seg; }
+        if (AK && a.live) la = a.live[issue_k / BK];
+        if (BKM && b.live) lb = b.live[issue_k / BK];
+        fa.issue(a, pa, issue_k, lds0 + (uint32_t)slot * C::STAGE_BYTES, wave, la);
+        fb.issue(b, pb, issue_k, lds0 + (uint32_t)slot * C::STAGE_BYTES + C::BM * BK * 2, wave, lb);
+        if (++issue_seg == SEGS) { issue_seg = 0; issue_k += BK; }
     };
 
     // fragment addresses.  not KM: row x, chunk 2 kt + (lane >> 5) of the step (kt = 0 .. 3); KM: rows 16 kt + 8 (lane >> 5) + 4 h + (s >> 2), unit of x
@@ -213,39 +218,60 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
         const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
         return u32x4{l2[0], l2[1], h2[0], h2[1]};
     };
-
+    u32x4 x[2][C::TM], y[2][C::TN];                                          // fragments: [quarter & 1]
+    auto fetch = [&](uint32_t at, int kt) {
 #pragma unroll
-    for (int g = 0; g < C::STAGES - 1; ++g)
-        if (g < steps) issue(g);
-    int slot = 0;
-    for (int t = 0; t < steps; ++t) {
-        // step t has landed when at most the loads of the steps behind it are outstanding
-        const int behind = steps - 1 - t < C::STAGES - 2 ? steps - 1 - t : C::STAGES - 2;
-        if (C::STAGES == 2 || behind == 0) wait_loads<0>();
-        else if (behind == 1) wait_loads<C::LA + C::LB>();
-        else wait_loads<2 * (C::LA + C::LB)>();
-        barrier();                                                           // ... for every wave, and the slot of step t - 1 has been read
-        if (t + C::STAGES - 1 < steps) issue(slot == 0 ? C::STAGES - 1 : slot - 1);
-        const uint32_t at = (uint32_t)slot * C::STAGE_BYTES;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-            u32x4 x[C::TM], y[C::TN];
-#pragma unroll
-            for (int i = 0; i < C::TM; ++i) {
-                if constexpr (!AK) x[i] = *(__attribute__((address_space(3))) u32x4*)(lds + at + ra[kt] + 4096 * i);
-                else x[i] = transposed(at + ra[i] + kt * 16 * 2 * C::BM, 2 * C::BM);
-            }
-#pragma unroll
-            for (int j = 0; j < C::TN; ++j) {
-                if constexpr (!BKM) y[j] = *(__attribute__((address_space(3))) u32x4*)(lds + at + rb[kt] + 4096 * j);
-                else y[j] = transposed(at + rb[j] + kt * 16 * 2 * C::BN, 2 * C::BN);
-            }
-#pragma unroll
-            for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-                for (int j = 0; j < C::TN; ++j) acc.t[i][j] = mfma<DT>(x[i], y[j], acc.t[i][j]);
+        for (int i = 0; i < C::TM; ++i) {
+            if constexpr (!AK) x[kt & 1][i] = *(__attribute__((address_space(3))) u32x4*)(lds + at + ra[kt] + 4096 * i);
+            else x[kt & 1][i] = transposed(at + ra[i] + kt * 16 * 2 * C::BM, 2 * C::BM);
         }
-        slot = slot == C::STAGES - 1 ? 0 : slot + 1;
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) {
+            if constexpr (!BKM) y[kt & 1][j] = *(__attribute__((address_space(3))) u32x4*)(lds + at + rb[kt] + 4096 * j);
+            else y[kt & 1][j] = transposed(at + rb[j] + kt * 16 * 2 * C::BN, 2 * C::BN);
+        }
+    };
+    auto multiply = [&](int kt) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) acc.t[i][j] = mfma<DT>(x[kt & 1][i], y[kt & 1][j], acc.t[i][j]);
+    };
+    // waits until at most the loads of `behind` steps are outstanding, and for every wave
+    auto landed = [&](int behind) {
+        if (behind <= 0) wait_loads<0>();
+        else if (behind == 1) wait_loads<C::LA + C::LB>();
+        else if (behind == 2) wait_loads<2 * (C::LA + C::LB)>();
+        else wait_loads<3 * (C::LA + C::LB)>();
+        barrier();
+    };
+    static_assert(C::STAGES <= 4, "landed()");
+
+    if (steps > 0) {
+#pragma unroll
+        for (int g = 0; g < C::STAGES; ++g)
+            if (g < steps) issue(g);
+        landed(steps - 1 < C::STAGES - 1 ? steps - 1 : C::STAGES - 1);
+        fetch(0, 0);
+        int slot = 0;
+        for (int t = 0; t < steps; ++t) {
+            const uint32_t at = (uint32_t)slot * C::STAGE_BYTES;
+            const int next = slot == C::STAGES - 1 ? 0 : slot + 1;
+            fetch(at, 1);
+            multiply(0);
+            fetch(at, 2);
+            multiply(1);
+            fetch(at, 3);
+            multiply(2);
+            if (t + 1 < steps) {
+                // behind step t + 1, STAGES - 2 steps have been issued: this step's slot is refilled after the barrier
+                landed(C::STAGES == 2 ? 0 : steps - 2 - t < C::STAGES - 2 ? steps - 2 - t : C::STAGES - 2);
+                if (t + C::STAGES < steps) issue(slot);
+                fetch((uint32_t)next * C::STAGE_BYTES, 0);
+            }
+            multiply(3);
+            slot = next;
+        }
     }
     wait_loads<0>();
     barrier();                                                               // the LDS is free again
@@ -289,25 +315,22 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const typename Elem<DT>::t
     for (int z = 0; z < Elem<DT>::planes; ++z) __builtin_memcpy(out + z * rows * padded + i, q[z], 16);
 }
 
-// classes widened to int64 with two special values (-1: ignored, -2: out of range), and the rows that count as bytes and as bits
-template <typename T>
-__global__ void __launch_bounds__(256) prepare_kernel(const T* __restrict__ target, int64_t rows, int64_t classes, int64_t ignore, int64_t* __restrict__ out,
-                                                      uint8_t* __restrict__ live, uint64_t* __restrict__ bits) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t t = i < rows ? (int64_t)target[i] : ignore;
-    const bool ign = t == ignore;
-    const uint64_t w = __ballot(!ign);
-    if (i >= rows) return;
-    out[i] = ign ? -1 : (t < 0 || t >= classes ? -2 : t);
-    live[i] = ign ? 0 : 1;
-    if ((threadIdx.x & 63) == 0) bits[i / 64] = w;
-}
+// the classes as the caller gave them
+struct Target {
+    const void* p;
+    int wide;                        // int64 (else int32)
+    int64_t ignore, classes;
+    __device__ __forceinline__ int64_t of(int64_t n) const {                // -1: ignored, -2: no such class
+        const int64_t t = wide ? ((const int64_t*)p)[n] : (int64_t)((const int32_t*)p)[n];
+        return t == ignore ? -1 : (t < 0 || t >= classes ? -2 : t);
+    }
+};
 
 // what a launch over logit tiles knows of the head
 struct Head {
     Op w, h;                         // A: weight (m = class), B: hidden (n = row)
     const void* bias;
-    const int64_t* target;           // as prepare_kernel wrote them
+    const int64_t* target;           // as join_kernel wrote them (backward)
     int64_t rows, width, classes;
     uint32_t tiles_m, tiles_n;       // of this launch
     int64_t c0, c1;                  // the classes of this launch
@@ -326,34 +349,41 @@ __device__ __forceinline__ Stat joined(const Stat& a, const Stat& b) {
     return Stat{m, fa * a.s + fb * b.s, fa * (a.u + da * a.s) + fb * (b.u + db * b.s)};
 }
 
-// bias of the classes a lane holds: base + 32 i + 8 (r / 4) + r % 4
+// the sums start from the bias of the classes a lane holds: base + 32 i + 8 r4 + 0 .. 3
 template <int DT, class C>
-__device__ __forceinline__ void add_bias(Acc<C>& acc, const void* bias, int64_t base, int64_t c1) {
+__device__ __forceinline__ void start(Acc<C>& acc, const void* bias, int64_t base, int64_t c1) {
     typedef typename Elem<DT>::type E;
+    if (!bias) return clear(acc);
     const E* b = (const E*)bias;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int64_t m = base + 32 * i + 8 * (r >> 2) + (r & 3);
-            const float v = to_float<DT>(b[m < c1 ? m : c1 - 1]);           // (what lies past the last class is not used)
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int64_t m = base + 32 * i + 8 * r4;
+            E v[4];
+            if (m + 4 <= c1) __builtin_memcpy(v, b + m, sizeof v);
+            else
 #pragma unroll
-            for (int j = 0; j < C::TN; ++j) acc.t[i][j][r] += v;
+                for (int r = 0; r < 4; ++r) v[r] = m + r < c1 ? b[m + r] : (E)0;
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc.t[i][j][4 * r4 + r] = to_float<DT>(v[r]);
         }
 }
 
 // class-tile statistics of each row, and the logit of the row's own class
-template <class C, int DT>
-__global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, int64_t tile0, float* __restrict__ part, float* __restrict__ own_logit) {
+template <class C, int DT, bool ENTROPY>
+__global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target target, int64_t tile0, float* __restrict__ part, float* __restrict__ own_logit) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t tm, tn, z;
     tile_of(blockIdx.x, gridDim.x, hd.tiles_m, hd.tiles_n, tm, tn, z);
     const int64_t m0 = hd.c0 + (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
-    Acc<C> acc;
-    gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const int64_t base = m0 + wm + 4 * (lane >> 5);                  // class of the lane's register 0
-    if (hd.bias) add_bias<DT>(acc, hd.bias, base, hd.c1);
+    Acc<C> acc;
+    start<DT>(acc, hd.bias, base, hd.c1);
+    gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
     if (m0 + C::BM > hd.c1) {
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
@@ -367,7 +397,7 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, int64_t
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
         const int nl = wn + 32 * j + (lane & 31);
-        const int64_t n = n0 + nl, t = n < hd.rows ? hd.target[n] : -1;
+        const int64_t n = n0 + nl, t = n < hd.rows ? target.of(n) : -1;
         const int64_t rel = t - (m0 + wm);
         if (__any(rel >= 0 && rel < C::TM * 32)) {
             const int own = t >= base && rel < C::TM * 32 ? (int)(t - base) : -1;
@@ -392,10 +422,10 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, int64_t
             for (int r = 0; r < 16; ++r) {
                 const float d = fmaf(acc.t[i][j][r], LOG2E, -ref), e = __builtin_amdgcn_exp2f(d);
                 s += e;
-                u = fmaf(fmaxf(d, -3.0e38f), e, u);                 // a class at -inf adds 0, not 0 x inf
+                if constexpr (ENTROPY) u = fmaf(fmaxf(d, -3.0e38f), e, u);      // a class at -inf adds 0, not 0 x inf
             }
         s += __shfl_xor(s, 32, 64);
-        u += __shfl_xor(u, 32, 64);
+        if constexpr (ENTROPY) u += __shfl_xor(u, 32, 64);
         if (lane < 32) { red[wave % C::WM][nl][0] = mx; red[wave % C::WM][nl][1] = s; red[wave % C::WM][nl][2] = u; }
     }
     __syncthreads();
@@ -409,34 +439,45 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, int64_t
         }
 }
 
-// joins the tiles' statistics: 16 lanes per row, 16 rows per workgroup.  lse is kept in units of log2
-__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, const float* __restrict__ own_logit, const int64_t* __restrict__ target,
-                                                   int64_t rows, int tiles, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ entropy_kept,
-                                                   float* __restrict__ lse) {
-    __shared__ float red[3][16][17];
-    const int r = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const int64_t n = (int64_t)blockIdx.x * 16 + r;
+// joins the tiles' statistics: 64 rows per workgroup, wave g takes tiles g, g + 16, ... (four loads of each kind in flight); lse is kept in units of log2.  Also leaves what the
+// backward pass wants of the classes: -1 / -2 / the class, and the rows that count as bytes and as bits.
+__global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ part, const float* __restrict__ own_logit, Target target, int64_t rows, int tiles, int with_entropy,
+                                                    float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ entropy_kept, float* __restrict__ lse,
+                                                    int64_t* __restrict__ classes, uint8_t* __restrict__ live, uint64_t* __restrict__ bits) {
+    __shared__ float red[3][16][64];
+    const int r = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int64_t n = (int64_t)blockIdx.x * 64 + r;
     Stat a{-INFINITY, 0.0f, 0.0f};
     if (n < rows)
-        for (int t = g; t < tiles; t += 16) {
-            const float* o = part + 3 * (size_t)t * rows + n;
-            a = joined(a, Stat{o[0], o[rows], o[2 * rows]});
+        for (int t = g; t < tiles; t += 64) {
+            Stat v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float* o = part + 3 * (size_t)(t + 16 * k) * rows + n;
+                v[k] = t + 16 * k < tiles ? Stat{o[0], o[rows], with_entropy ? o[2 * rows] : 0.0f} : Stat{-INFINITY, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a = joined(a, v[k]);
         }
     red[0][g][r] = a.m; red[1][g][r] = a.s; red[2][g][r] = a.u;
     __syncthreads();
-    if (threadIdx.x < 16 && n < rows) {
-        for (int k = 1; k < 16; ++k) a = joined(a, Stat{red[0][k][r], red[1][k][r], red[2][k][r]});
-        const int64_t t = target[n];
-        const float ls = __log2f(a.s);
-        float z = a.m + ls, h = LN2 * (ls - a.u / a.s), lp = 0.0f;
-        if (t >= 0) lp = LN2 * (fmaf(own_logit[n], LOG2E, -a.m) - ls);
-        else if (t == -1) { h = 0.0f; z = 0.0f; }                  // ignored
-        else { lp = h = z = NAN; }                                  // a class that does not exist
-        logp[n] = lp;
-        if (entropy) entropy[n] = h;
-        entropy_kept[n] = h;
-        lse[n] = z;
-    }
+    if (g != 0) return;
+    const int64_t t = n < rows ? target.of(n) : -1;
+    const uint64_t word = __ballot(t != -1);
+    if (n >= rows) return;
+    for (int k = 1; k < 16; ++k) a = joined(a, Stat{red[0][k][r], red[1][k][r], red[2][k][r]});
+    const float ls = __log2f(a.s);
+    float z = a.m + ls, h = with_entropy ? LN2 * (ls - a.u / a.s) : NAN, lp = 0.0f;
+    if (t >= 0) lp = LN2 * (fmaf(own_logit[n], LOG2E, -a.m) - ls);
+    else if (t == -1) { h = 0.0f; z = 0.0f; }                      // ignored
+    else { lp = h = z = NAN; }                                      // a class that does not exist
+    logp[n] = lp;
+    if (entropy) entropy[n] = h;
+    entropy_kept[n] = h;
+    lse[n] = z;
+    classes[n] = t;
+    live[n] = t == -1 ? 0 : 1;
+    if (r == 0) bits[blockIdx.x] = word;
 }
 
 // loss[0] = -sum logp / max(1, live rows) or -sum logp; loss[1] = what d loss / d(-logp) of a live row is
@@ -526,26 +567,26 @@ __device__ __forceinline__ float half_sum(float v) {
 
 // a piece [c0, c1) of the classes: the logits again, and the gradient of each -> g[row][class - c0] (stride `piece`; 16 bits, float32 as three pieces g_plane values apart), zero
 // up to the end of the last tile; and the sums over this tile's rows -> db_part[row tile][class]
-template <class C, int DT>
+template <class C, int DT, bool ENTROPY>
 __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream up, int64_t piece, int64_t g_plane, const float* __restrict__ lse,
                                                               const float* __restrict__ entropy, uint16_t* __restrict__ g, float* __restrict__ db_part) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t tm, tn, zz;
     tile_of(blockIdx.x, gridDim.x, hd.tiles_m, hd.tiles_n, tm, tn, zz);
     const int64_t m0 = hd.c0 + (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
-    Acc<C> acc;
-    gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const int64_t base = m0 + wm + 4 * (lane >> 5);
-    if (hd.bias) add_bias<DT>(acc, hd.bias, base, hd.c1);
+    Acc<C> acc;
+    start<DT>(acc, hd.bias, base, hd.c1);
+    gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
     const float sc = up.scale[0];
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
         const int64_t n = n0 + wn + 32 * j + (lane & 31), t = n < hd.rows ? hd.target[n] : -1;
         const bool on = t != -1;
         const float z = on ? lse[n] : 0.0f;
-        const float A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) * sc : 0.0f, E = on && up.dentropy ? up.dentropy[n] * sc : 0.0f;
-        const float hrow = on && up.dentropy ? entropy[n] : 0.0f, El = E * LN2, Ah = A + E * hrow;
+        const float A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) * sc : 0.0f, E = ENTROPY && on ? up.dentropy[n] * sc : 0.0f;
+        const float hrow = ENTROPY && on ? entropy[n] : 0.0f, El = E * LN2, Ah = A + E * hrow;
         const bool here = __any(t >= m0 + wm && t < m0 + wm + C::TM * 32);
         const int own = t >= base && t < base + C::TM * 32 ? (int)(t - base) : -1;
 #pragma unroll
@@ -554,7 +595,7 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
             for (int r = 0; r < 16; ++r) {
                 const float d = fmaf(acc.t[i][j][r], LOG2E, -z), p = __builtin_amdgcn_exp2f(d);
                 // g = -p (A + E (log p + H)); a class at -inf has p = 0 and a finite factor
-                float v = up.dentropy ? -p * fmaf(El, fmaxf(d, -3.0e38f), Ah) : -p * A;
+                const float v = ENTROPY ? -p * fmaf(El, fmaxf(d, -3.0e38f), Ah) : -p * A;
                 acc.t[i][j][r] = on ? v : 0.0f;
             }
         if (here) {
@@ -624,13 +665,20 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
     }
 }
 
-// db[class] = scale x sum over row tiles, in the order of the tiles
+// db[class] = scale x sum over row tiles: 64 classes per workgroup, wave g takes tiles g, g + 16, ...; the order is fixed
 template <int DT>
-__global__ void __launch_bounds__(256) bias_kernel(const float* __restrict__ part, int64_t classes, int tiles, const float* __restrict__ scale, void* __restrict__ out) {
-    const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (j >= classes) return;
+__global__ void __launch_bounds__(1024) bias_kernel(const float* __restrict__ part, int64_t classes, int tiles, const float* __restrict__ scale, void* __restrict__ out) {
+    __shared__ float red[16][64];
+    const int r = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int64_t j = (int64_t)blockIdx.x * 64 + r;
     float a = 0.0f;
-    for (int t = 0; t < tiles; ++t) a += part[(size_t)t * classes + j];
+    if (j < classes)
+#pragma unroll 4
+        for (int t = g; t < tiles; t += 16) a += part[(size_t)t * classes + j];
+    red[g][r] = a;
+    __syncthreads();
+    if (g != 0 || j >= classes) return;
+    for (int k = 1; k < 16; ++k) a += red[k][r];
     ((typename Elem<DT>::type*)out)[j] = from_float<DT>(a * scale[1]);
 }
 
@@ -659,6 +707,7 @@ __global__ void __launch_bounds__(C::THREADS) product_kernel(Product pr) {
     const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
     const int64_t kb = (int64_t)z * pr.split_k, ke = kb + pr.split_k < pr.k ? kb + pr.split_k : pr.k;
     Acc<C> acc;
+    clear(acc);
     gemm_tile<C, DT, AK, BKM>(pr.a, pr.b, m0, n0, kb, ke, acc, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const float sc = pr.slab ? 1.0f : pr.scale[1];
