@@ -15,10 +15,10 @@ constexpr uint64_t LAID_BYTES = 96ull << 20;       // of the laid-out weights of
 constexpr int64_t MAX_ROWS = 1 << 22, MAX_WIDTH = 1 << 16, MAX_CLASSES = 1 << 22;
 constexpr int64_t PIECE_STEP = 256;                // pieces are whole tiles of every configuration
 
-typedef Config<256, 256, 2, 4, 2> Large;           // 128 KB of LDS: one workgroup of eight waves per CU
-typedef Config<128, 128, 2, 2, 2> Middle;          // 64 KB: two workgroups of four waves per CU, one computes while the other waits
-typedef Config<128, 64, 4, 1, 3> Few;              // up to 64 rows: 72 KB, two workgroups per CU
-typedef Config<128, 32, 4, 1, 4> Fewest;           // up to 32 rows: 80 KB, two workgroups per CU
+typedef Config<256, 256, 2, 4, 64, 2> Large;           // 128 KB of LDS: one workgroup of eight waves per CU
+typedef Config<128, 128, 2, 2, 64, 2> Middle;          // 64 KB: two workgroups of four waves per CU, one computes while the other waits
+typedef Config<128, 64, 4, 1, 64, 3> Few;              // up to 64 rows: 72 KB, two workgroups per CU
+typedef Config<128, 32, 4, 1, 64, 4> Fewest;           // up to 32 rows: 80 KB, two workgroups per CU
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round_up(int64_t a, int64_t b) { return div_up(a, b) * b; }
@@ -49,26 +49,26 @@ int64_t bm_of(Size s) { return s == LARGE ? 256 : 128; }
 int64_t bn_of(Size s) { return s == LARGE ? 256 : s == MIDDLE ? 128 : s == FEW ? 64 : 32; }
 
 // The tile of a product of m x n results with k terms, and into how many parts its sum is split, by what it should take in nanoseconds.  One round of Large workgroups (256,
-// one per CU) was measured at 30 ns per term of k, one of Middle (512, two per CU) at 18; `start` is what a round costs besides (prologue and epilogue); the slabs of a split sum are written
-// and read once at 4.5 TB/s.  `split` false: one part only.
+// one per CU) was measured at 31 ns per term of k (1075 TFLOP/s), one of Middle (512, two per CU) at 18 (930); `start` is what a round costs besides (prologue and epilogue: 3.3 / 2.5 us for the
+// statistics, 12 / 7 for the gradient, at 50000 x 256 x 4097); the slabs of a split sum are written and read once at 4.5 TB/s.  `split` false: one part only.
 struct Shape { Size size; int parts; int64_t len; };
 Shape shape_of(int64_t m, int64_t n, int64_t k, int products, bool split, double start_large, double start_middle) {
     if (n <= 64) {                                    // few rows: 512 workgroups (two per CU), parts of 512 terms at least
         const Size s = n <= 32 ? FEWEST : FEW;
         const int64_t tiles = div_up(m, bm_of(s));
         int64_t parts = split ? std::max<int64_t>(1, std::min(div_up(512, tiles), div_up(k, 512))) : 1;
-        const int64_t len = round_up(div_up(k, parts), BK);
+        const int64_t len = round_up(div_up(k, parts), PART_STEP);
         return Shape{s, (int)div_up(k, len), len};
     }
-    Shape best{MIDDLE, 1, round_up(k, BK)};
+    Shape best{MIDDLE, 1, round_up(k, PART_STEP)};
     double least = 0.0;
     for (int s = LARGE; s <= MIDDLE; ++s) {
         const int64_t tiles = div_up(m, bm_of((Size)s)) * div_up(n, bn_of((Size)s)), slots = s == LARGE ? 256 : 512;
         const int64_t most = split ? std::min<int64_t>(div_up(k, 256), std::max<int64_t>(1, div_up(4 * slots, tiles))) : 1;
         for (int64_t parts = 1; parts <= most; ++parts) {
-            const int64_t len = round_up(div_up(k, parts), BK), real = div_up(k, len);
+            const int64_t len = round_up(div_up(k, parts), PART_STEP), real = div_up(k, len);
             const double rounds = (double)div_up(tiles * real, slots);
-            double t = rounds * ((double)len * products * (s == LARGE ? 30.0 : 18.0) + (s == LARGE ? start_large : start_middle));
+            double t = rounds * ((double)len * products * (s == LARGE ? 31.0 : 18.0) + (s == LARGE ? start_large : start_middle));
             if (real > 1) t += 3000.0 + (double)real * (double)m * (double)n * 8.0 / 4500.0;
             if (least == 0.0 || t < least) { least = t; best = Shape{(Size)s, (int)real, len}; }
         }
@@ -103,7 +103,7 @@ Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward
     p.piece = piece;
     p.pieces = div_up(classes, piece);
     const int products = planes_of(dt) == 3 ? 6 : 1;
-    p.logits = shape_of(std::min(piece, classes), rows, width, products, false, 9000.0, 6000.0).size;
+    p.logits = shape_of(std::min(piece, classes), rows, width, products, false, backward ? 12000.0 : 3300.0, backward ? 7000.0 : 2500.0).size;
     uint64_t at = 0;
     auto take = [&](uint64_t n) { const uint64_t o = at; at += aligned(n); return o; };
     if (!backward) {
@@ -262,7 +262,8 @@ int backward(const Where& at, const q1env_head& q, Upstream up, void* dh, int64_
     uint16_t* g = (uint16_t*)(ws + p.g);
     float *dh_slab = p.dh_split > 1 || p.pieces > 1 ? (float*)(ws + p.dh_slab) : nullptr, *dw_slab = p.dw_split > 1 ? (float*)(ws + p.dw_slab) : nullptr;
     const size_t es = elem_size(DT);
-    auto wide = [&](const void* out, int64_t stride, const float* slab) { return slab ? d % 4 == 0 : ((uintptr_t)out & 15) == 0 && stride * es % 16 == 0; };
+    // 16-byte stores of a result: address, stride, and for 16-bit types whole chunks of 8 columns
+    auto wide = [&](const void* out, int64_t stride, const float* slab) { return slab ? d % 4 == 0 : ((uintptr_t)out & 15) == 0 && stride * es % 16 == 0 && (es == 4 || d % 8 == 0); };
     for (int64_t c0 = 0; c0 < v; c0 += p.piece) {
         const int64_t c1 = std::min(c0 + p.piece, v), len = c1 - c0;
         const char* w0 = (const char*)q.weight_dev + es * c0 * q.weight_stride;
@@ -273,7 +274,7 @@ int backward(const Where& at, const q1env_head& q, Upstream up, void* dh, int64_
         else if (p.logits == MIDDLE) Q1_TRY((gradient<Middle, DT>(at, hd, up, p.piece, st, g, db_part)));
         else if (p.logits == FEW) Q1_TRY((gradient<Few, DT>(at, hd, up, p.piece, st, g, db_part)));
         else Q1_TRY((gradient<Fewest, DT>(at, hd, up, p.piece, st, g, db_part)));
-        const Op gr{(const char*)g, 2 * p.piece, 2 * n * p.piece, n, round_up(len, BK), nullptr};         // [row][class of the piece]
+        const Op gr{(const char*)g, 2 * p.piece, 2 * n * p.piece, n, round_up(len, PART_STEP), nullptr};         // [row][class of the piece]
         if (dw) {
             Op gt = turned(gr, nullptr);
             gt.x_extent = round_up(len, 8);

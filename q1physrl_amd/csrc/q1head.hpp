@@ -64,10 +64,11 @@ template <int DT> __device__ __forceinline__ f32x16 mfma(const u32x4& a, const u
 //
 // An operand lies in memory with k contiguous (KM = false: element (x, k) at p[x stride + k]) or with x contiguous (KM = true: p[k stride + x]).  Both
 // kinds travel from memory to LDS without passing through registers (buffer loads with an LDS destination, 16 bytes per lane, 1 KB per
-// wave instruction; what lies outside the operand reads as zero by the buffer's bounds check), BK = 64 values of k at a time, STAGES tiles in flight:
+// wave instruction; what lies outside the operand reads as zero by the buffer's bounds check), BK values of k at a time, STAGES tiles in flight:
 // the loads of a tile are issued one (two, three) whole steps before its barrier.  The LDS image is linear in the order of the loading lanes, so bank conflicts are
 // avoided by permuting which 16-byte chunk a lane asks memory for:
-//   KM = false: rows of 128 bytes; chunk c of row x sits at c ^ ((x >> 1) & 7): any 16 lanes of a fragment read (16 rows, one chunk) cover all 64 banks;
+//   KM = false: rows of 2 BK bytes; chunk c of row x sits at c ^ ((x >> 1) & 7) (BK = 64) or c ^ ((x >> 2) & 3) (BK = 32): any 16 lanes of a fragment read (16 rows, one
+//               chunk) cover all 64 banks;
 //   KM = true:  rows of 2 BM bytes; the 32-byte unit u of row k sits at u ^ (2 (k & 3)): the transposing read (ds_read_b64_tr_b16: 4 values of k x 16 of x per 16
 //               lanes) touches four rows at four different bank groups.
 // Bound (256 x 256 tile, 8 waves of 128 x 64): per step a wave issues 32 matrix instructions of 32 cycles and reads 24 KB of LDS, 75 % of what the LDS delivers in
@@ -81,27 +82,30 @@ struct Op {
     const uint64_t* live;       // KM: where set, bit k of the words says whether row k counts (rows that do not are zero whatever memory holds)
 };
 
-constexpr int BK = 64;
-
-template <int BM_, int BN_, int WM_, int WN_, int STAGES_> struct Config {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
+template <int BM_, int BN_, int WM_, int WN_, int BK_, int STAGES_> struct Config {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_;
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;             // 32 x 32 tiles per wave
-    static constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;         // load instructions per wave and stage
-    static constexpr int STAGE_BYTES = (BM + BN) * BK * 2, LDS_BYTES = STAGES * STAGE_BYTES;
-    static_assert(LA * WAVES * 8 == BM && LB * WAVES * 8 == BN && TM >= 1 && TN >= 1, "whole load instructions per wave");
+    static constexpr int LA = BM * BK / 512 / WAVES, LB = BN * BK / 512 / WAVES;         // load instructions per wave and stage
+    static constexpr int A_BYTES = BM * BK * 2, STAGE_BYTES = (BM + BN) * BK * 2, LDS_BYTES = STAGES * STAGE_BYTES;
+    static_assert(BK == 32 || BK == 64, "the LDS image's permutations");
+    static_assert(LA * WAVES * 512 == BM * BK && LB * WAVES * 512 == BN * BK && TM >= 1 && TN >= 1, "whole load instructions per wave");
+    static_assert(STAGES >= 2 && (STAGES - 1) * (LA + LB) < 64 && LDS_BYTES <= 163840, "vmcnt; LDS of a CU");
 };
+constexpr int PART_STEP = 64;               // parts of a split sum are whole steps of every configuration (and whole words of `live`)
 
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((address_space(3))) char lds_char;
 constexpr uint32_t OUTSIDE = 0x80000000u;                                   // the resource's size: an offset from here on reads zero
 
-__device__ __forceinline__ void load_to_lds(const char* base, uint32_t offset, uint32_t lds) {
+// size: the bytes from base on that may be read; an offset from there on reads zero
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t size, uint32_t offset, uint32_t lds) {
     const uint64_t a = (uint64_t)base;
-    const u32x4 rsrc = {(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, OUTSIDE, 0x00020000u};
+    auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };      // (all of it is; the resource has to sit in scalar registers)
+    const u32x4 rsrc = {uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffffu), uniform(size), 0x00020000u};
     // (no result registers: what the instruction writes is LDS, waited for with vmcnt before the barrier in front of its use)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(uniform(lds)), "v"(offset), "s"(rsrc) : "memory");
 }
 template <int N> __device__ __forceinline__ void wait_loads() {             // all but the N youngest loads have landed, and this wave's LDS reads are done
     static_assert(N < 64, "vmcnt");
@@ -113,40 +117,59 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
-// the loading side of one operand: XT values of x per tile, COUNT load instructions per wave
-template <int XT, int COUNT, bool KM> struct Feed {
+// The loading side of one operand: XT values of x per tile, COUNT load instructions per wave, each of ROWS rows of the tile.  What a step costs besides the loads is scalar and little
+// (130 scalar instructions a step took a fifth of the whole product's time): a lane's offsets stay, the step's address moves; rows past the end of k, and steps past it, lie outside
+// the resource and read zero.
+template <int XT, int BK, int COUNT, bool KM, bool LIVE> struct Feed {
+    static constexpr int ROWS = KM ? 512 / XT : 512 / BK;
     uint32_t off[COUNT];        // byte offset of this lane's chunk in the tile, OUTSIDE if its x is
-    int kk[COUNT];              // the chunk's k within the step
-    const char* base;           // of the tile at k = 0
-    __device__ __forceinline__ void init(const Op& o, int64_t x0, int wave, int lane) {
+    int q8[2];                  // not KM: the chunk's k within the step, of even and odd loads
+    const char* at;             // the tile at the next step
+    int left;                   // of k from the next step on
+    uint32_t stride;
+    __device__ __forceinline__ void init(const Op& o, int64_t x0, int64_t k0, int wave, int lane) {
+        constexpr int PER = KM ? XT / 8 : BK / 8;                            // 16-byte chunks of a row
+        const int r = lane / PER, c = lane % PER;
+        stride = (uint32_t)o.stride;
 #pragma unroll
         for (int j = 0; j < COUNT; ++j) {
-            const int i = wave * COUNT + j;
+            const int row = ROWS * (wave * COUNT + j) + r;
             if constexpr (!KM) {
-                const int x = 8 * i + (lane >> 3), q = (lane & 7) ^ ((x >> 1) & 7);
-                kk[j] = 8 * q;
-                off[j] = x0 + x < o.x_extent ? (uint32_t)(x * o.stride) + 16 * q : OUTSIDE;
+                const int q = c ^ (BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
+                off[j] = x0 + row < o.x_extent ? (uint32_t)row * stride + 16 * q : OUTSIDE;
+                if (j < 2) q8[j] = 8 * q;
             } else {
-                constexpr int PER = XT / 8;                                  // 16-byte chunks of a row
-                const int at = 64 * i + lane, k = at / PER, c = at % PER, x = 8 * (2 * ((c >> 1) ^ (2 * (k & 3))) + (c & 1));
-                kk[j] = k;
-                off[j] = x0 + x < o.x_extent ? (uint32_t)(k * o.stride) + 2 * x : OUTSIDE;
+                const int x = 8 * (2 * ((c >> 1) ^ (2 * (row & 3))) + (c & 1));
+                off[j] = x0 + x < o.x_extent ? (uint32_t)row * stride + 2 * x : OUTSIDE;
             }
         }
-        base = o.p + (KM ? 2 * x0 : x0 * o.stride);
+        if constexpr (COUNT == 1) q8[1] = q8[0];
+        at = o.p + (KM ? 2 * x0 + k0 * o.stride : x0 * o.stride + 2 * k0);
+        left = (int)(o.k_extent - k0);
     }
-    // issues the loads of step k0 (of piece `plane`) into the LDS bytes from `lds` on
-    __device__ __forceinline__ void issue(const Op& o, int plane, int64_t k0, uint32_t lds, int wave, uint64_t live) const {
-        const char* b = base + plane * o.plane + (KM ? k0 * o.stride : 2 * k0);
-        const bool tail = k0 + BK > o.k_extent;
-        const int left = (int)(o.k_extent - k0 < BK ? o.k_extent - k0 : BK);
+    // issues the loads of the next step (its piece `plane`) into the LDS bytes from `lds` on; k0: its first k
+    __device__ __forceinline__ void issue(const Op& o, int plane, int64_t k0, uint32_t lds, int wave, int lane) const {
+        const char* b = at + plane * o.plane;
+        const uint32_t size = KM ? (left >= BK ? OUTSIDE : left > 0 ? (uint32_t)left * stride : 0u) : (left > 0 ? OUTSIDE : 0u);
+        uint64_t live = ~0ull;
+        if constexpr (LIVE)
+            if (o.live && left > 0) live = o.live[k0 / 64] >> (k0 % 64);
+        lds += 1024u * (uint32_t)(wave * COUNT);
+        if (!KM && left < BK) {                                              // the step that k ends in
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            uint32_t f = off[j];
-            if (tail && kk[j] >= left) f = OUTSIDE;
-            if (KM && live != ~0ull && !((live >> kk[j]) & 1)) f = OUTSIDE;
-            load_to_lds(b, f, lds + 1024u * (uint32_t)(wave * COUNT + j));
+            for (int j = 0; j < COUNT; ++j) load_to_lds(b, size, q8[j & 1] < left ? off[j] : OUTSIDE, lds + 1024u * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j) {
+                uint32_t f = off[j];
+                if constexpr (LIVE) f = (live >> (ROWS * (wave * COUNT + j) + lane / (XT / 8))) & 1 ? f : OUTSIDE;
+                load_to_lds(b, size, f, lds + 1024u * j);
+            }
         }
+    }
+    __device__ __forceinline__ void advance() {
+        at += KM ? (uint64_t)stride * BK : 2 * BK;
+        left -= BK;
     }
 };
 
@@ -170,10 +193,11 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
     lds_char* lds = (lds_char*)lds_generic;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
-    Feed<C::BM, C::LA, AK> fa;
-    Feed<C::BN, C::LB, BKM> fb;
-    fa.init(a, m0, wave, lane);
-    fb.init(b, n0, wave, lane);
+    constexpr int BK = C::BK, QUARTERS = BK / 16;                            // of a step: 16 values of k each, one matrix instruction deep
+    Feed<C::BM, BK, C::LA, AK, AK && BKM && P == 1> fa;                        // (hidden rows as k: rows that do not count)
+    Feed<C::BN, BK, C::LB, BKM, false> fb;
+    fa.init(a, m0, k_begin, wave, lane);
+    fb.init(b, n0, k_begin, wave, lane);
     const int steps = k_end > k_begin ? (int)((k_end - k_begin + BK - 1) / BK) * SEGS : 0;
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
 
@@ -185,20 +209,22 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
             pa = (0x010201 >> (4 * issue_seg)) & 15;
             pb = (0x001021 >> (4 * issue_seg)) & 15;
         }
-        uint64_t la = ~0ull, lb = ~0ull;
-        if (AK && a.live) la = a.live[issue_k / BK];
-        if (BKM && b.live) lb = b.live[issue_k / BK];
-        fa.issue(a, pa, issue_k, lds0 + (uint32_t)slot * C::STAGE_BYTES, wave, la);
-        fb.issue(b, pb, issue_k, lds0 + (uint32_t)slot * C::STAGE_BYTES + C::BM * BK * 2, wave, lb);
-        if (++issue_seg == SEGS) { issue_seg = 0; issue_k += BK; }
+        fa.issue(a, pa, issue_k, lds0 + (uint32_t)slot * C::STAGE_BYTES, wave, lane);
+        fb.issue(b, pb, issue_k, lds0 + (uint32_t)slot * C::STAGE_BYTES + C::A_BYTES, wave, lane);
+        if (SEGS == 1 || ++issue_seg == SEGS) {
+            issue_seg = 0;
+            issue_k += BK;
+            fa.advance();
+            fb.advance();
+        }
     };
 
-    // fragment addresses.  not KM: row x, chunk 2 kt + (lane >> 5) of the step (kt = 0 .. 3); KM: rows 16 kt + 8 (lane >> 5) + 4 h + (s >> 2), unit of x
-    uint32_t ra[AK ? C::TM : 4], rb[BKM ? C::TN : 4];
-    const int s = lane & 15;
+    // fragment addresses.  not KM: row x, chunk 2 kt + (lane >> 5) of the step; KM: rows 16 kt + 8 (lane >> 5) + 4 h + (s >> 2), unit of x
+    uint32_t ra[AK ? C::TM : QUARTERS], rb[BKM ? C::TN : QUARTERS];
+    const int s = lane & 15, row = lane & 31, permuted = BK == 64 ? row >> 1 & 7 : row >> 2 & 3;
     if constexpr (!AK) {
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) ra[kt] = (wm + (lane & 31)) * 128 + ((2 * kt + (lane >> 5)) ^ ((lane & 31) >> 1 & 7)) * 16;
+        for (int kt = 0; kt < QUARTERS; ++kt) ra[kt] = (wm + row) * (2 * BK) + ((2 * kt + (lane >> 5)) ^ permuted) * 16;
     } else {
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
@@ -206,11 +232,11 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
     }
     if constexpr (!BKM) {
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) rb[kt] = C::BM * BK * 2 + (wn + (lane & 31)) * 128 + ((2 * kt + (lane >> 5)) ^ ((lane & 31) >> 1 & 7)) * 16;
+        for (int kt = 0; kt < QUARTERS; ++kt) rb[kt] = C::A_BYTES + (wn + row) * (2 * BK) + ((2 * kt + (lane >> 5)) ^ permuted) * 16;
     } else {
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
-            rb[j] = C::BM * BK * 2 + (8 * (lane >> 5) + (s >> 2)) * (2 * C::BN) + (((wn + 32 * j) / 16 + ((lane >> 4) & 1)) ^ (2 * (s >> 2))) * 32 + (s & 3) * 8;
+            rb[j] = C::A_BYTES + (8 * (lane >> 5) + (s >> 2)) * (2 * C::BN) + (((wn + 32 * j) / 16 + ((lane >> 4) & 1)) ^ (2 * (s >> 2))) * 32 + (s & 3) * 8;
     }
     auto transposed = [&](uint32_t at, int row_bytes) {
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at));
@@ -222,12 +248,12 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
     auto fetch = [&](uint32_t at, int kt) {
 #pragma unroll
         for (int i = 0; i < C::TM; ++i) {
-            if constexpr (!AK) x[kt & 1][i] = *(__attribute__((address_space(3))) u32x4*)(lds + at + ra[kt] + 4096 * i);
+            if constexpr (!AK) x[kt & 1][i] = *(__attribute__((address_space(3))) u32x4*)(lds + at + ra[kt] + 64 * BK * i);
             else x[kt & 1][i] = transposed(at + ra[i] + kt * 16 * 2 * C::BM, 2 * C::BM);
         }
 #pragma unroll
         for (int j = 0; j < C::TN; ++j) {
-            if constexpr (!BKM) y[kt & 1][j] = *(__attribute__((address_space(3))) u32x4*)(lds + at + rb[kt] + 4096 * j);
+            if constexpr (!BKM) y[kt & 1][j] = *(__attribute__((address_space(3))) u32x4*)(lds + at + rb[kt] + 64 * BK * j);
             else y[kt & 1][j] = transposed(at + rb[j] + kt * 16 * 2 * C::BN, 2 * C::BN);
         }
     };
@@ -237,41 +263,40 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
 #pragma unroll
             for (int j = 0; j < C::TN; ++j) acc.t[i][j] = mfma<DT>(x[kt & 1][i], y[kt & 1][j], acc.t[i][j]);
     };
-    // waits until at most the loads of `behind` steps are outstanding, and for every wave
-    auto landed = [&](int behind) {
-        if (behind <= 0) wait_loads<0>();
-        else if (behind == 1) wait_loads<C::LA + C::LB>();
-        else if (behind == 2) wait_loads<2 * (C::LA + C::LB)>();
-        else wait_loads<3 * (C::LA + C::LB)>();
-        barrier();
-    };
-    static_assert(C::STAGES <= 4, "landed()");
-
-    if (steps > 0) {
+    // the reads of the next quarter go between the matrix instructions of this one, so that neither waits for the other
+    auto interleave = [&]() {
+        constexpr int READS = C::TM * (AK ? 2 : 1) + C::TN * (BKM ? 2 : 1), MM = C::TM * C::TN, PER = (READS + MM - 1) / MM;
 #pragma unroll
-        for (int g = 0; g < C::STAGES; ++g)
-            if (g < steps) issue(g);
-        landed(steps - 1 < C::STAGES - 1 ? steps - 1 : C::STAGES - 1);
-        fetch(0, 0);
-        int slot = 0;
-        for (int t = 0; t < steps; ++t) {
-            const uint32_t at = (uint32_t)slot * C::STAGE_BYTES;
-            const int next = slot == C::STAGES - 1 ? 0 : slot + 1;
-            fetch(at, 1);
-            multiply(0);
-            fetch(at, 2);
-            multiply(1);
-            fetch(at, 3);
-            multiply(2);
-            if (t + 1 < steps) {
-                // behind step t + 1, STAGES - 2 steps have been issued: this step's slot is refilled after the barrier
-                landed(C::STAGES == 2 ? 0 : steps - 2 - t < C::STAGES - 2 ? steps - 2 - t : C::STAGES - 2);
-                if (t + C::STAGES < steps) issue(slot);
-                fetch((uint32_t)next * C::STAGE_BYTES, 0);
-            }
-            multiply(3);
-            slot = next;
+        for (int i = 0; i < MM; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);             // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);               // matrix instructions
         }
+    };
+#pragma unroll
+    for (int g = 0; g < C::STAGES; ++g) issue(g);                            // (steps past the end read zeros: nothing below depends on how many there are)
+    wait_loads<(C::STAGES - 1) * (C::LA + C::LB)>();
+    barrier();
+    fetch(0, 0);
+    int slot = 0;
+    uint32_t at = 0;
+#pragma unroll 1
+    for (int t = 0; t < steps; ++t) {
+#pragma unroll
+        for (int kt = 0; kt + 1 < QUARTERS; ++kt) {
+            if (kt > 0) __builtin_amdgcn_sched_barrier(0);
+            fetch(at, kt + 1);
+            multiply(kt);
+            interleave();
+        }
+        wait_loads<(C::STAGES - 2) * (C::LA + C::LB)>();                      // the next step has landed ...
+        barrier();                                                           // ... for every wave, and this step's slot has been read
+        issue(slot);
+        slot = slot == C::STAGES - 1 ? 0 : slot + 1;
+        at = (uint32_t)slot * C::STAGE_BYTES;
+        fetch(at, 0);
+        multiply(QUARTERS - 1);
+        interleave();
+        __builtin_amdgcn_sched_barrier(0);
     }
     wait_loads<0>();
     barrier();                                                               // the LDS is free again
@@ -280,7 +305,7 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
 // Workgroup -> tile.  Workgroups are dealt to the eight XCDs in turn, each with an L2 of its own: XCD x takes the x-th eighth of the tiles, and within it tiles go
 // in bands of GROUP tiles of n, so that the workgroups that run at one time on one XCD share their operands' tiles on both sides.
 __device__ __forceinline__ void tile_of(uint32_t id, uint32_t total, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn, uint32_t& z) {
-    constexpr uint32_t GROUP = 8;
+    constexpr uint32_t GROUP = 4;
     const uint32_t q = total / 8, r = total % 8, x = id % 8, i = id / 8;
     uint32_t t = x * q + (x < r ? x : r) + i;
     const uint32_t plane = tiles_m * tiles_n;
@@ -404,8 +429,9 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target 
             float l = 0.0f;
 #pragma unroll
             for (int i = 0; i < C::TM; ++i)
+                if (__any(own >= 0 && own >> 5 == i))
 #pragma unroll
-                for (int r = 0; r < 16; ++r) l = own == 32 * i + 8 * (r >> 2) + (r & 3) ? acc.t[i][j][r] : l;
+                    for (int r = 0; r < 16; ++r) l = own == 32 * i + 8 * (r >> 2) + (r & 3) ? acc.t[i][j][r] : l;
             if (own >= 0 && (own & 4) == 0) own_logit[n] = l;
         }
         float mx = -INFINITY;
@@ -557,12 +583,44 @@ template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-// the sum over the 32 lanes of each half of the wave, in lanes 31 and 63
-__device__ __forceinline__ float half_sum(float v) {
-#define Q1_DPP_ADD(ctrl, mask) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, mask, 0xf, true))
-    Q1_DPP_ADD(0x111, 0xf); Q1_DPP_ADD(0x112, 0xf); Q1_DPP_ADD(0x114, 0xf); Q1_DPP_ADD(0x118, 0xf); Q1_DPP_ADD(0x142, 0xa);
-#undef Q1_DPP_ADD
-    return v;
+// A 16-bit result tile goes to memory through the LDS, so that a wave's store covers whole rows of the tile (512 or 256 bytes) and not 32 pieces of 32 rows: 16-byte chunk c of row n
+// sits at c ^ (n & 15), which keeps both the writes (32 rows, one chunk) and the reads (one row) off each other's banks.
+template <class C> __device__ __forceinline__ void put_eight(char* lds, int n, int m, const u32x4& v) {
+    static_assert(C::BN * C::BM * 2 <= C::LDS_BYTES, "the tile fits");
+    *(u32x4*)(lds + n * (2 * C::BM) + ((m >> 3) ^ (n & 15)) * 16) = v;
+}
+template <class C> __device__ __forceinline__ void flush_rows(const char* lds, uint16_t* out, int64_t stride, int rows, int cols) {
+    constexpr int PER = C::BM / 8;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < C::BN * PER; i += C::THREADS) {
+        const int n = i / PER, c = i % PER;
+        const u32x4 v = *(const u32x4*)(lds + n * (2 * C::BM) + (c ^ (n & 15)) * 16);
+        if (n < rows && 8 * c < cols) *(u32x4*)(out + n * stride + 8 * c) = v;
+    }
+}
+
+// Sums of 32 values over the 32 lanes of each half of the wave: every exchange halves what a lane still holds (16 + 8 + 4 + 2 + 1 sums instead of 5 x 32), partners l ^ 16 (a
+// row swap), then l ^ 15, l ^ 7, l ^ 2, l ^ 1.  The lane is left with the sum of value number `which`.
+template <int CTRL> __device__ __forceinline__ float from_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sums_of_32(float (&v)[32], int lane, int& which) {
+    float a[16], b[8], c[4], d[2];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const auto w = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v[k]), __builtin_bit_cast(uint32_t, v[k + 16]), false, false);
+        const uint32_t w0 = w[0], w1 = w[1];
+        a[k] = __builtin_bit_cast(float, w0) + __builtin_bit_cast(float, w1);                   // lanes with bit 4: value k + 16
+    }
+    const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) b[k] = (b3 ? a[k + 8] : a[k]) + from_lane<0x140>(b3 ? a[k] : a[k + 8]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c[k] = (b2 ? b[k + 4] : b[k]) + from_lane<0x141>(b2 ? b[k] : b[k + 4]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) d[k] = (b1 ? c[k + 2] : c[k]) + from_lane<0x4e>(b1 ? c[k] : c[k + 2]);
+    which = lane & 31;
+    return (b0 ? d[1] : d[0]) + from_lane<0xb1>(b0 ? d[0] : d[1]);
 }
 
 // a piece [c0, c1) of the classes: the logits again, and the gradient of each -> g[row][class - c0] (stride `piece`; 16 bits, float32 as three pieces g_plane values apart), zero
@@ -596,15 +654,19 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
                 const float d = fmaf(acc.t[i][j][r], LOG2E, -z), p = __builtin_amdgcn_exp2f(d);
                 // g = -p (A + E (log p + H)); a class at -inf has p = 0 and a finite factor
                 const float v = ENTROPY ? -p * fmaf(El, fmaxf(d, -3.0e38f), Ah) : -p * A;
-                acc.t[i][j][r] = on ? v : 0.0f;
+                acc.t[i][j][r] = v;
             }
-        if (here) {
+        if (!__all(on))                                             // (a row that does not count is zero whatever its hidden row holds)
 #pragma unroll
             for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (own == 32 * i + 8 * (r >> 2) + (r & 3)) acc.t[i][j][r] += A;
-        }
+                for (int r = 0; r < 16; ++r) acc.t[i][j][r] = on ? acc.t[i][j][r] : 0.0f;
+        if (here)
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+                if (__any(own >= 0 && own >> 5 == i))
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc.t[i][j][r] += own == 32 * i + 8 * (r >> 2) + (r & 3) ? A : 0.0f;
     }
     if (m0 + C::BM > hd.c1) {
 #pragma unroll
@@ -615,45 +677,22 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
 #pragma unroll
                     for (int j = 0; j < C::TN; ++j) acc.t[i][j][r] = 0.0f;
     }
-#pragma unroll
-    for (int j = 0; j < C::TN; ++j) {
-        const int64_t n = n0 + wn + 32 * j + (lane & 31);
-        uint16_t* row = g + n * piece + (m0 - hd.c0) + wm + 8 * (lane >> 5);
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float v[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) v[r] = acc.t[i][j][8 * h + r];
-#pragma unroll
-                for (int q = 0; q < Elem<DT>::planes; ++q) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        w[r] = pack2<DT>(v[2 * r], v[2 * r + 1]);
-                        if constexpr (DT == F32) {                  // what this piece leaves for the next
-                            v[2 * r] -= __builtin_bit_cast(float, w[r] << 16);
-                            v[2 * r + 1] -= __builtin_bit_cast(float, w[r] & 0xffff0000u);
-                        }
-                    }
-                    const u32x4 o = eight_of(u32x2{w[0], w[1]}, u32x2{w[2], w[3]});
-                    if (n < hd.rows) *(u32x4*)(row + q * g_plane + 32 * i + 16 * h) = o;
-                }
-            }
-    }
     if (db_part) {
         float (*red)[C::BM] = (float (*)[C::BM])lds;
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
+        for (int i = 0; i < C::TM; i += 2) {
+            float v[32];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float v = acc.t[i][0][r];
+            for (int r = 0; r < 32; ++r) {
+                v[r] = i + r / 16 < C::TM ? acc.t[i + r / 16 < C::TM ? i + r / 16 : i][0][r % 16] : 0.0f;
 #pragma unroll
-                for (int j = 1; j < C::TN; ++j) v += acc.t[i][j][r];
-                v = half_sum(v);
-                if ((lane & 31) == 31) red[wave / C::WM][wm + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)] = v;
+                for (int j = 1; j < C::TN; ++j) v[r] += i + r / 16 < C::TM ? acc.t[i + r / 16 < C::TM ? i + r / 16 : i][j][r % 16] : 0.0f;
             }
+            int r;
+            const float sum = sums_of_32(v, lane, r);
+            const int at = wm + 32 * (i + r / 16) + 8 * (r % 16 >> 2) + 4 * (lane >> 5) + (r & 3);
+            if (i + r / 16 < C::TM) red[wave / C::WM][at] = sum;
+        }
         __syncthreads();
         for (int m = threadIdx.x; m < C::BM; m += C::THREADS)
             if (m0 + m < hd.c1) {
@@ -662,6 +701,32 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
                 for (int w = 1; w < C::WN; ++w) v += red[w][m];
                 db_part[(size_t)tn * hd.classes + m0 + m] = v;
             }
+        __syncthreads();
+    }
+    const int rows = hd.rows - n0 < C::BN ? (int)(hd.rows - n0) : C::BN;
+#pragma unroll
+    for (int q = 0; q < Elem<DT>::planes; ++q) {
+        if (q > 0) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float v0 = acc.t[i][j][8 * h + 2 * r], v1 = acc.t[i][j][8 * h + 2 * r + 1];
+                        w[r] = pack2<DT>(v0, v1);
+                        if (q + 1 < Elem<DT>::planes) {             // what this piece leaves for the next
+                            acc.t[i][j][8 * h + 2 * r] = v0 - __builtin_bit_cast(float, w[r] << 16);
+                            acc.t[i][j][8 * h + 2 * r + 1] = v1 - __builtin_bit_cast(float, w[r] & 0xffff0000u);
+                        }
+                    }
+                    put_eight<C>(lds, wn + 32 * j + (lane & 31), wm + 32 * i + 16 * h + 8 * (lane >> 5), eight_of(u32x2{w[0], w[1]}, u32x2{w[2], w[3]}));
+                }
+        __syncthreads();
+        flush_rows<C>(lds, g + q * g_plane + n0 * piece + (m0 - hd.c0), piece, rows, C::BM);
     }
 }
 
@@ -686,7 +751,7 @@ __global__ void __launch_bounds__(1024) bias_kernel(const float* __restrict__ pa
 // finish_kernel (accumulate: added to what is there); without it the scaled result is stored.
 struct Product {
     Op a, b;
-    int64_t k, split_k;                // length of the sum; part per split (a multiple of BK)
+    int64_t k, split_k;                // length of the sum; part per split (a multiple of PART_STEP)
     int64_t rows, width;               // of the result
     uint32_t tiles_m, tiles_n;
     void* out;
@@ -747,18 +812,22 @@ __global__ void __launch_bounds__(C::THREADS) product_kernel(Product pr) {
                         w[r] = on ? pack2<DT>(x, y) : 0u;
                     }
                     const u32x4 o8 = eight_of(u32x2{w[0], w[1]}, u32x2{w[2], w[3]});
-                    const int64_t mm = m + 16 * h + 8 * (lane >> 5);
-                    E* o = (E*)pr.out + n * pr.out_stride + mm;
-                    if (!row) continue;
-                    if (pr.vec && mm + 8 <= pr.width) *(u32x4*)o = o8;
-                    else {
+                    const int ml = wm + 32 * i + 16 * h + 8 * (lane >> 5);
+                    if (pr.vec) put_eight<C>(lds, wn + 32 * j + (lane & 31), ml, o8);
+                    else if (row) {
+                        E* o = (E*)pr.out + n * pr.out_stride + m0 + ml;
 #pragma unroll
                         for (int r = 0; r < 8; ++r)
-                            if (mm + r < pr.width) o[r] = (E)(o8[r >> 1] >> (16 * (r & 1)));
+                            if (m0 + ml + r < pr.width) o[r] = (E)(o8[r >> 1] >> (16 * (r & 1)));
                     }
                 }
             }
         }
+    }
+    if (DT != F32 && !pr.slab && pr.vec) {
+        __syncthreads();
+        flush_rows<C>(lds, (uint16_t*)pr.out + n0 * pr.out_stride + m0, pr.out_stride, pr.rows - n0 < C::BN ? (int)(pr.rows - n0) : C::BN,
+                      pr.width - m0 < C::BM ? (int)(pr.width - m0) : C::BM);
     }
 }
 
