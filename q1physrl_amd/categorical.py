@@ -16,6 +16,7 @@ are zero whatever the hidden row holds.  A target outside 0 .. V-1 gives NaN.  W
 A captured graph: the forward calls and linear_cross_entropy_grad can be captured; the autograd forms cannot (a capture that meets an eager graph of
 the same leaves ends the process), and say so."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -26,12 +27,24 @@ _DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float
 
 def _rows(x):
     """x (..., D) as (rows, D) with a contiguous last dimension; a copy only where no strided view is one."""
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     x = x.reshape(-1, x.shape[-1])
     return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
 
 
 def _stride(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+@functools.lru_cache(maxsize=256)
+def _state_bytes(n):
+    return _lib.load().q1env_head_state_bytes(n)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(dtype, n, d, v, backward):
+    return _lib.load().q1env_head_workspace_bytes(dtype, n, d, v, backward)
 
 
 def _check(hidden, weight, target, bias, ignore_index):
@@ -58,113 +71,111 @@ def _check(hidden, weight, target, bias, ignore_index):
             raise ValueError("all tensors must be on one device")
 
 
-class _Call:
-    """One head's tensors as the C struct wants them.  Everything it points at stays referenced here until the launches are queued; the caching
-    allocator keeps freed blocks to the stream they were used on."""
+def _head(hidden, weight, target, bias, ignore_index, backward):
+    """The C struct of a head without its state, and the tensors it points at: they are referenced until the launches are queued, and the caching allocator keeps
+    freed blocks to the stream they were used on."""
+    h, w = _rows(hidden), _rows(weight)
+    b = None if bias is None else bias.contiguous()
+    n, d, v, dtype = h.shape[0], h.shape[1], w.shape[0], _DTYPES[h.dtype]
+    nbytes = _workspace_bytes(dtype, n, d, v, backward)
+    if not nbytes:
+        raise ValueError(f"sizes out of range: {n} rows (2^22), width {d} (2^16), {v} classes (2^22)")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
+    s = _lib.Q1Head(dtype, 64 if target is None or target.dtype == torch.int64 else 32, n, d, v, ignore_index, h.data_ptr(), _stride(h), w.data_ptr(), _stride(w),
+                    None if b is None else b.data_ptr(), None if target is None else target.data_ptr(), None, ws.data_ptr(), nbytes)
+    return s, (h, w, b, target, ws)
 
-    def __init__(self, hidden, weight, target, bias, ignore_index, state=None):
-        self.lib = _lib.load()
-        self.hidden, self.weight = _rows(hidden.detach()), _rows(weight.detach())
-        self.bias = None if bias is None else bias.detach().contiguous()
-        self.target = None if target is None else target.reshape(-1).contiguous()
-        self.dtype = _DTYPES[hidden.dtype]
-        self.n, self.d, self.v = self.hidden.shape[0], self.hidden.shape[1], self.weight.shape[0]
-        self.device = hidden.device
-        nstate = self.lib.q1env_head_state_bytes(self.n)
-        if not nstate:
-            raise ValueError(f"{self.n} rows are more than the head takes (2^22)")
-        self.state = torch.empty((nstate,), dtype=torch.uint8, device=self.device) if state is None else state
-        self.ignore_index = ignore_index
 
-    def struct(self, backward):
-        nbytes = self.lib.q1env_head_workspace_bytes(self.dtype, self.n, self.d, self.v, backward)
-        if not nbytes:
-            raise ValueError(f"sizes out of range: {self.n} rows, width {self.d}, {self.v} classes")
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device)
-        return ws, _lib.Q1Head(self.dtype, 64 if self.target is None or self.target.dtype == torch.int64 else 32, self.n, self.d, self.v, self.ignore_index,
-                               self.hidden.data_ptr(), _stride(self.hidden), self.weight.data_ptr(), _stride(self.weight),
-                               0 if self.bias is None else self.bias.data_ptr(), 0 if self.target is None else self.target.data_ptr(),
-                               self.state.data_ptr(), ws.data_ptr(), nbytes)
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
 
-    def _at(self):
-        return self.device.index, torch.cuda.current_stream(self.device).cuda_stream
 
-    def forward(self, entropy, reduction):
-        """logp (n,), entropy (n,) or None, loss () or None"""
-        ws, s = self.struct(0)
-        f32 = dict(dtype=torch.float32, device=self.device)
-        logp = torch.empty((self.n,), **f32)
-        ent = torch.empty((self.n,), **f32) if entropy else None
-        loss = torch.empty((), **f32) if reduction is not None else None
-        dev, stream = self._at()
-        _lib.check(self.lib.q1env_head_forward(dev, stream, C.byref(s), _lib.REDUCE_SUM if reduction == "sum" else _lib.REDUCE_MEAN, logp.data_ptr(),
-                                               ent.data_ptr() if entropy else None, loss.data_ptr() if reduction is not None else None))
-        return logp, ent, loss
+def _forward(hidden, weight, target, bias, ignore_index, reduction):
+    """(logp (n,), entropy (n,), state) without a reduction, (loss (), state) with one"""
+    target = target.reshape(-1).contiguous()
+    s, keep = _head(hidden, weight, target, bias, ignore_index, 0)
+    device, n = hidden.device, s.rows
+    state = torch.empty(_state_bytes(n), dtype=torch.uint8, device=device)
+    s.state_dev = state.data_ptr()
+    logp = torch.empty(n, dtype=torch.float32, device=device)
+    ent = loss = None
+    if reduction is None:
+        ent = torch.empty(n, dtype=torch.float32, device=device)
+    else:
+        loss = torch.empty((), dtype=torch.float32, device=device)
+    _lib.check(_lib.load().q1env_head_forward(device.index, _stream(device), C.byref(s), _lib.REDUCE_SUM if reduction == "sum" else _lib.REDUCE_MEAN, logp.data_ptr(),
+                                              None if ent is None else ent.data_ptr(), None if loss is None else loss.data_ptr()))
+    del keep
+    return (logp, ent, state) if reduction is None else (loss, state)
 
-    def backward(self, dlogp, dentropy, dloss, need):
-        """need: which of (hidden, weight, bias) to differentiate; their gradients ((n, d), (v, d), (v,)) or None"""
-        ws, s = self.struct(1)
-        opt = dict(dtype=self.hidden.dtype, device=self.device)
-        dh = torch.empty((self.n, self.d), **opt) if need[0] else None
-        dw = torch.empty((self.v, self.d), **opt) if need[1] else None
-        db = torch.empty((self.v,), **opt) if need[2] and self.bias is not None else None
-        if dh is None and dw is None and db is None or (dlogp is None and dentropy is None and dloss is None):
-            return dh, dw, db
-        f = [None if g is None else g.to(torch.float32).reshape(-1).contiguous() for g in (dlogp, dentropy, dloss)]
-        dev, stream = self._at()
-        _lib.check(self.lib.q1env_head_backward(dev, stream, C.byref(s), *[None if g is None else g.data_ptr() for g in f],
-                                                None if dh is None else dh.data_ptr(), self.d, None if dw is None else dw.data_ptr(), self.d,
-                                                None if db is None else db.data_ptr()))
+
+def _upstream(g):
+    return g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
+
+
+def _backward(hidden, weight, bias, state, dlogp, dentropy, dloss, need):
+    """need: which of (hidden, weight, bias) to differentiate; their gradients or None"""
+    s, keep = _head(hidden, weight, None, bias, 0, 1)
+    s.state_dev = state.data_ptr()
+    dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need[0] else None
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need[1] else None
+    db = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device) if need[2] and bias is not None else None
+    if dh is None and dw is None and db is None:
         return dh, dw, db
-
-
-def _refuse_capture(tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("the differentiable forms cannot be captured into a graph: capture linear_cross_entropy_grad, or the forward under torch.no_grad()")
+    up = _upstream(dlogp), _upstream(dentropy), _upstream(dloss)
+    _lib.check(_lib.load().q1env_head_backward(hidden.device.index, _stream(hidden.device), C.byref(s), *[None if g is None else g.data_ptr() for g in up],
+                                               None if dh is None else dh.data_ptr(), s.width, None if dw is None else dw.data_ptr(), s.width,
+                                               None if db is None else db.data_ptr()))
+    del keep
+    return dh, dw, db
 
 
 class _Categorical(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, bias, ignore_index, reduction):
-        call = _Call(hidden, weight, target, bias, ignore_index)
-        logp, ent, loss = call.forward(reduction is None, reduction)
-        ctx.save_for_backward(hidden, weight, bias, call.state)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        *out, state = _forward(hidden, weight, target, bias, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, bias, state)
+        ctx.reduction = reduction
         ctx.set_materialize_grads(False)
-        return (logp, ent) if reduction is None else loss
+        return tuple(out) if reduction is None else out[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        hidden, weight, bias, state = ctx.saved_tensors
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the backward pass of the wide categorical head cannot be captured into a graph: capture linear_cross_entropy_grad")
-        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
         if all(g is None for g in grads):
             return None, None, None, None, None, None
-        call = _Call(hidden, weight, None, bias, ctx.ignore_index, state)
+        hidden, weight, bias, state = ctx.saved_tensors
         up = (grads[0], grads[1], None) if ctx.reduction is None else (None, None, grads[0])
-        dh, dw, db = call.backward(*up, need)
-        return (None if dh is None else dh.view(hidden.shape)), dw, None, db, None, None
+        need = ctx.needs_input_grad
+        dh, dw, db = _backward(hidden, weight, bias, state, *up, (need[0], need[1], need[3]))
+        return dh, dw, None, db, None, None
+
+
+def _apply(hidden, weight, target, bias, ignore_index, reduction):
+    _check(hidden, weight, target, bias, ignore_index)
+    if not (torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))):
+        return _forward(hidden, weight, target, bias, ignore_index, reduction)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the differentiable forms cannot be captured into a graph: capture linear_cross_entropy_grad, or the forward under torch.no_grad()")
+    out = _Categorical.apply(hidden, weight, target, bias, ignore_index, reduction)
+    return out if reduction is None else (out,)
 
 
 def linear_categorical(hidden, weight, actions, bias=None, *, ignore_index=-100):
     """(log-probability, entropy) of the given actions, float32, in actions' shape."""
-    _check(hidden, weight, actions, bias, ignore_index)
-    _refuse_capture((hidden, weight, bias))
-    logp, ent = _Categorical.apply(hidden, weight, actions, bias, ignore_index, None)
-    return logp.view(actions.shape), ent.view(actions.shape)
+    logp, ent = _apply(hidden, weight, actions, bias, ignore_index, None)[:2]
+    return (logp, ent) if actions.dim() == 1 else (logp.view(actions.shape), ent.view(actions.shape))
 
 
 def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100, reduction="mean"):
     """Minus the log-probability of the targets: its mean over the rows that are not ignored (0 when all are), "sum", or "none" (per row)."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-    _check(hidden, weight, target, bias, ignore_index)
-    _refuse_capture((hidden, weight, bias))
     if reduction == "none":
-        return -_Categorical.apply(hidden, weight, target, bias, ignore_index, None)[0].view(target.shape)
-    return _Categorical.apply(hidden, weight, target, bias, ignore_index, reduction)
+        return -_apply(hidden, weight, target, bias, ignore_index, None)[0].view(target.shape)
+    return _apply(hidden, weight, target, bias, ignore_index, reduction)[0]
 
 
 @torch.no_grad()
@@ -175,8 +186,6 @@ def linear_cross_entropy_grad(hidden, weight, target, bias=None, *, ignore_index
     _check(hidden, weight, target, bias, ignore_index)
     if grad_scale is not None and not (torch.is_tensor(grad_scale) and grad_scale.numel() == 1 and grad_scale.dtype == torch.float32 and grad_scale.device == hidden.device):
         raise ValueError("grad_scale must be one float32 on hidden's device")
-    call = _Call(hidden, weight, target, bias, ignore_index)
-    _, _, loss = call.forward(False, reduction)
-    one = torch.ones((), dtype=torch.float32, device=call.device) if grad_scale is None else grad_scale
-    dh, dw, db = call.backward(None, None, one, (True, True, True))
-    return loss, dh.view(hidden.shape), dw, db
+    loss, state = _forward(hidden, weight, target, bias, ignore_index, reduction)
+    one = torch.ones((), dtype=torch.float32, device=hidden.device) if grad_scale is None else grad_scale
+    return loss, *_backward(hidden, weight, bias, state, None, None, one, (True, True, True))

@@ -69,8 +69,8 @@ template <int DT> __device__ __forceinline__ f32x16 mfma(const u32x4& a, const u
 // avoided by permuting which 16-byte chunk a lane asks memory for:
 //   KM = false: rows of 2 BK bytes; chunk c of row x sits at c ^ ((x >> 1) & 7) (BK = 64) or c ^ ((x >> 2) & 3) (BK = 32): any 16 lanes of a fragment read (16 rows, one
 //               chunk) cover all 64 banks;
-//   KM = true:  rows of 2 BM bytes; the 32-byte unit u of row k sits at u ^ (2 (k & 3)): the transposing read (ds_read_b64_tr_b16: 4 values of k x 16 of x per 16
-//               lanes) touches four rows at four different bank groups.
+//   KM = true:  rows of 2 BM bytes; the 32-byte unit u of row k sits at u ^ (2 (k & 3)) (u ^ (k & 2) in rows of 128 bytes): the transposing read (ds_read_b64_tr_b16: 4 values
+//               of k x 16 of x per 16 lanes) touches four rows at four different bank groups.
 // Bound (256 x 256 tile, 8 waves of 128 x 64): per step a wave issues 32 matrix instructions of 32 cycles and reads 24 KB of LDS, 75 % of what the LDS delivers in
 // that time; a 64 x 64 wave tile would need all of it.
 struct Op {
@@ -117,6 +117,8 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
+template <int XT> __device__ __forceinline__ int unit_flip(int k) { return XT >= 128 ? 2 * (k & 3) : k & 2; }
+
 // The loading side of one operand: XT values of x per tile, COUNT load instructions per wave, each of ROWS rows of the tile.  What a step costs besides the loads is scalar and little
 // (130 scalar instructions a step took a fifth of the whole product's time): a lane's offsets stay, the step's address moves; rows past the end of k, and steps past it, lie outside
 // the resource and read zero.
@@ -139,7 +141,7 @@ template <int XT, int BK, int COUNT, bool KM, bool LIVE> struct Feed {
                 off[j] = x0 + row < o.x_extent ? (uint32_t)row * stride + 16 * q : OUTSIDE;
                 if (j < 2) q8[j] = 8 * q;
             } else {
-                const int x = 8 * (2 * ((c >> 1) ^ (2 * (row & 3))) + (c & 1));
+                const int x = 8 * (2 * ((c >> 1) ^ unit_flip<XT>(row)) + (c & 1));
                 off[j] = x0 + x < o.x_extent ? (uint32_t)row * stride + 2 * x : OUTSIDE;
             }
         }
@@ -228,7 +230,7 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
     } else {
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
-            ra[i] = (8 * (lane >> 5) + (s >> 2)) * (2 * C::BM) + (((wm + 32 * i) / 16 + ((lane >> 4) & 1)) ^ (2 * (s >> 2))) * 32 + (s & 3) * 8;
+            ra[i] = (8 * (lane >> 5) + (s >> 2)) * (2 * C::BM) + (((wm + 32 * i) / 16 + ((lane >> 4) & 1)) ^ unit_flip<C::BM>(s >> 2)) * 32 + (s & 3) * 8;
     }
     if constexpr (!BKM) {
 #pragma unroll
@@ -236,7 +238,7 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
     } else {
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
-            rb[j] = C::A_BYTES + (8 * (lane >> 5) + (s >> 2)) * (2 * C::BN) + (((wn + 32 * j) / 16 + ((lane >> 4) & 1)) ^ (2 * (s >> 2))) * 32 + (s & 3) * 8;
+            rb[j] = C::A_BYTES + (8 * (lane >> 5) + (s >> 2)) * (2 * C::BN) + (((wn + 32 * j) / 16 + ((lane >> 4) & 1)) ^ unit_flip<C::BN>(s >> 2)) * 32 + (s & 3) * 8;
     }
     auto transposed = [&](uint32_t at, int row_bytes) {
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at));
@@ -320,24 +322,35 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t total, uint32_t ti
 // ------------------------------------------------------------------------------------------------------------------------------
 // Operands that the loads above cannot take as they lie (float32; a width that is not a multiple of 8, addresses or strides that are not multiples of 16 bytes) are laid out
 // first: [piece][row][padded], padded = width rounded up to 64 with zeros; rows that do not count are zero.
+struct Lay {
+    const void* src;
+    int64_t stride, rows;             // elements
+    const uint8_t* live;
+    uint16_t* out;
+    uint32_t groups;                  // workgroups of 2048 values
+};
 template <int DT>
-__global__ void __launch_bounds__(256) lay_out_kernel(const typename Elem<DT>::type* __restrict__ src, int64_t stride, int64_t rows, int64_t width, int64_t padded,
-                                                      const uint8_t* __restrict__ live, uint16_t* __restrict__ out) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-    if (i >= rows * padded) return;
+__global__ void __launch_bounds__(256) lay_out_kernel(Lay first, Lay second, int64_t width, int64_t padded) {
+    const bool one = blockIdx.x < first.groups;
+    const Lay& l = one ? first : second;
+    const int64_t i = ((int64_t)(one ? blockIdx.x : blockIdx.x - first.groups) * 256 + threadIdx.x) * 8;
+    if (i >= l.rows * padded) return;
     const int64_t r = i / padded, k = i - r * padded;
     uint16_t q[Elem<DT>::planes][8];
-    const bool on = !live || live[r];
-    const typename Elem<DT>::type* p = src + r * stride + k;
+    const bool on = !l.live || l.live[r];
+    const typename Elem<DT>::type* p = (const typename Elem<DT>::type*)l.src + r * l.stride + k;
+    typename Elem<DT>::type v[8];
+    if (on && k + 8 <= width) __builtin_memcpy(v, p, sizeof v);
+    else
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = on && k + j < width ? p[j] : (typename Elem<DT>::type)0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        if constexpr (DT == F32) {
-            three_pieces(on && k + j < width ? p[j] : 0.0f, q[0][j], q[1][j], q[2][j]);
-        } else
-            q[0][j] = on && k + j < width ? p[j] : 0;
+        if constexpr (DT == F32) three_pieces(v[j], q[0][j], q[1][j], q[2][j]);
+        else q[0][j] = v[j];
     }
 #pragma unroll
-    for (int z = 0; z < Elem<DT>::planes; ++z) __builtin_memcpy(out + z * rows * padded + i, q[z], 16);
+    for (int z = 0; z < Elem<DT>::planes; ++z) __builtin_memcpy(l.out + z * l.rows * padded + i, q[z], 16);
 }
 
 // the classes as the caller gave them
@@ -469,7 +482,8 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target 
 // backward pass wants of the classes: -1 / -2 / the class, and the rows that count as bytes and as bits.
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ part, const float* __restrict__ own_logit, Target target, int64_t rows, int tiles, int with_entropy,
                                                     float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ entropy_kept, float* __restrict__ lse,
-                                                    int64_t* __restrict__ classes, uint8_t* __restrict__ live, uint64_t* __restrict__ bits) {
+                                                    int64_t* __restrict__ classes, uint8_t* __restrict__ live, uint64_t* __restrict__ bits, int mean,
+                                                    float* __restrict__ loss, float* __restrict__ each) {
     __shared__ float red[3][16][64];
     const int r = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int64_t n = (int64_t)blockIdx.x * 64 + r;
@@ -490,20 +504,33 @@ __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ pa
     if (g != 0) return;
     const int64_t t = n < rows ? target.of(n) : -1;
     const uint64_t word = __ballot(t != -1);
-    if (n >= rows) return;
-    for (int k = 1; k < 16; ++k) a = joined(a, Stat{red[0][k][r], red[1][k][r], red[2][k][r]});
-    const float ls = __log2f(a.s);
-    float z = a.m + ls, h = with_entropy ? LN2 * (ls - a.u / a.s) : NAN, lp = 0.0f;
-    if (t >= 0) lp = LN2 * (fmaf(own_logit[n], LOG2E, -a.m) - ls);
-    else if (t == -1) { h = 0.0f; z = 0.0f; }                      // ignored
-    else { lp = h = z = NAN; }                                      // a class that does not exist
-    logp[n] = lp;
-    if (entropy) entropy[n] = h;
-    entropy_kept[n] = h;
-    lse[n] = z;
-    classes[n] = t;
-    live[n] = t == -1 ? 0 : 1;
-    if (r == 0) bits[blockIdx.x] = word;
+    float lp = 0.0f;
+    if (n < rows) {
+        for (int k = 1; k < 16; ++k) a = joined(a, Stat{red[0][k][r], red[1][k][r], red[2][k][r]});
+        const float ls = __log2f(a.s);
+        float z = a.m + ls, h = with_entropy ? LN2 * (ls - a.u / a.s) : NAN;
+        if (t >= 0) lp = LN2 * (fmaf(own_logit[n], LOG2E, -a.m) - ls);
+        else if (t == -1) { h = 0.0f; z = 0.0f; }                  // ignored
+        else { lp = h = z = NAN; }                                  // a class that does not exist
+        logp[n] = lp;
+        if (entropy) entropy[n] = h;
+        entropy_kept[n] = h;
+        lse[n] = z;
+        classes[n] = t;
+        live[n] = t == -1 ? 0 : 1;
+        if (r == 0) bits[blockIdx.x] = word;
+    }
+    if (loss) {                                                     // (given where these are all the rows: at most 64)
+        double sum = (double)lp;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        if (r == 0) {
+            const int c = __popcll(word);
+            const double d = mean ? (double)(c > 0 ? c : 1) : 1.0;
+            *loss = (float)(0.0 - sum / d);
+            *each = (float)(1.0 / d);
+        }
+    }
 }
 
 // loss[0] = -sum logp / max(1, live rows) or -sum logp; loss[1] = what d loss / d(-logp) of a live row is
@@ -528,27 +555,23 @@ __global__ void __launch_bounds__(1024) loss_kernel(const float* __restrict__ lo
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// The gradient's scale.  g is stored as it is in float32 and bfloat16.  Float16 loses what lies below 2^-24, so there the stored values are
-// g / scale with a power of two `scale` that brings the largest possible |g| to 2^14, and the products' results are multiplied by it.
+// The gradient's scale.  For one upstream value of all rows (dloss) the stored values are p - [j = t] and the factor is applied to the results.  For one per row g is stored as it
+// is in float32 and bfloat16.  Float16 loses what lies below 2^-24, so there the stored values are g / table with a power of two that brings the largest possible |g| to
+// 2^14, and the results are multiplied by it.
 struct Upstream {
     const float* dlogp;              // per row, or null
     const float* dentropy;           // per row, or null
     const float* dloss;              // one value (with each): A_i = -dloss each for every live row
     const float* each;
-    const float* scale;              // written by scale_kernel
+    const float* table;              // scale_kernel's, or null
+    int f16;
+    __device__ __forceinline__ float stored() const { return dloss ? (f16 ? 16384.0f : 1.0f) : table ? table[0] : 1.0f; }
+    __device__ __forceinline__ float result() const { return dloss ? *dloss * *each * (f16 ? 0x1p-14f : 1.0f) : table ? table[1] : 1.0f; }
 };
 
-// scale[0]: what stored values are multiplied by, scale[1]: what results are multiplied by
-__global__ void __launch_bounds__(1024) scale_kernel(Upstream up, const uint8_t* __restrict__ live, int64_t rows, int f16, float* __restrict__ scale) {
+// table[0]: what stored values are multiplied by, table[1]: what results are multiplied by (float16, per-row upstream values)
+__global__ void __launch_bounds__(1024) scale_kernel(Upstream up, const uint8_t* __restrict__ live, int64_t rows, float* __restrict__ table) {
     __shared__ float red[16];
-    if (up.dloss) {                  // one factor for all rows: the stored values are p - [j = t], which need no further scale but float16's
-        if (threadIdx.x == 0) { scale[0] = f16 ? 16384.0f : 1.0f; scale[1] = *up.dloss * *up.each * (f16 ? 0x1p-14f : 1.0f); }
-        return;
-    }
-    if (!f16) {
-        if (threadIdx.x == 0) { scale[0] = 1.0f; scale[1] = 1.0f; }
-        return;
-    }
     float mx = 0.0f;
     for (int64_t i = threadIdx.x; i < rows; i += 1024)
         if (live[i]) mx = fmaxf(mx, (up.dlogp ? fabsf(up.dlogp[i]) : 0.0f) + (up.dentropy ? 16.0f * fabsf(up.dentropy[i]) : 0.0f));   // |p (log p + H)| < 16 up to 2^22 classes
@@ -561,8 +584,8 @@ __global__ void __launch_bounds__(1024) scale_kernel(Upstream up, const uint8_t*
         int e = 0;
         if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &e);       // mx in [2^(e-1), 2^e)
         e = e < -110 ? -110 : (e > 126 ? 126 : e);
-        scale[0] = ldexpf(1.0f, 14 - e);
-        scale[1] = ldexpf(1.0f, e - 14);
+        table[0] = ldexpf(1.0f, 14 - e);
+        table[1] = ldexpf(1.0f, e - 14);
     }
 }
 
@@ -584,17 +607,18 @@ template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // A 16-bit result tile goes to memory through the LDS, so that a wave's store covers whole rows of the tile (512 or 256 bytes) and not 32 pieces of 32 rows: 16-byte chunk c of row n
-// sits at c ^ (n & 15), which keeps both the writes (32 rows, one chunk) and the reads (one row) off each other's banks.
+// sits at c ^ (n & 15) (& 7 in rows of 8 chunks), which keeps both the writes (32 rows, one chunk) and the reads (one row) off each other's banks.
+template <class C> __device__ __forceinline__ int chunk_at(int n, int c) { return n * (2 * C::BM) + (c ^ (n & (C::BM / 8 < 16 ? C::BM / 8 - 1 : 15))) * 16; }
 template <class C> __device__ __forceinline__ void put_eight(char* lds, int n, int m, const u32x4& v) {
     static_assert(C::BN * C::BM * 2 <= C::LDS_BYTES, "the tile fits");
-    *(u32x4*)(lds + n * (2 * C::BM) + ((m >> 3) ^ (n & 15)) * 16) = v;
+    *(u32x4*)(lds + chunk_at<C>(n, m >> 3)) = v;
 }
 template <class C> __device__ __forceinline__ void flush_rows(const char* lds, uint16_t* out, int64_t stride, int rows, int cols) {
     constexpr int PER = C::BM / 8;
 #pragma unroll 4
     for (int i = threadIdx.x; i < C::BN * PER; i += C::THREADS) {
         const int n = i / PER, c = i % PER;
-        const u32x4 v = *(const u32x4*)(lds + n * (2 * C::BM) + (c ^ (n & 15)) * 16);
+        const u32x4 v = *(const u32x4*)(lds + chunk_at<C>(n, c));
         if (n < rows && 8 * c < cols) *(u32x4*)(out + n * stride + 8 * c) = v;
     }
 }
@@ -637,7 +661,7 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
     Acc<C> acc;
     start<DT>(acc, hd.bias, base, hd.c1);
     gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
-    const float sc = up.scale[0];
+    const float sc = up.stored();
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
         const int64_t n = n0 + wn + 32 * j + (lane & 31), t = n < hd.rows ? hd.target[n] : -1;
@@ -730,23 +754,6 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
     }
 }
 
-// db[class] = scale x sum over row tiles: 64 classes per workgroup, wave g takes tiles g, g + 16, ...; the order is fixed
-template <int DT>
-__global__ void __launch_bounds__(1024) bias_kernel(const float* __restrict__ part, int64_t classes, int tiles, const float* __restrict__ scale, void* __restrict__ out) {
-    __shared__ float red[16][64];
-    const int r = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t j = (int64_t)blockIdx.x * 64 + r;
-    float a = 0.0f;
-    if (j < classes)
-#pragma unroll 4
-        for (int t = g; t < tiles; t += 16) a += part[(size_t)t * classes + j];
-    red[g][r] = a;
-    __syncthreads();
-    if (g != 0 || j >= classes) return;
-    for (int k = 1; k < 16; ++k) a += red[k][r];
-    ((typename Elem<DT>::type*)out)[j] = from_float<DT>(a * scale[1]);
-}
-
 // out[n][m] (stride out_stride): m = column of the result (width), n = its row.  slab: the sums stay in float32 [split][rows][width] for
 // finish_kernel (accumulate: added to what is there); without it the scaled result is stored.
 struct Product {
@@ -759,23 +766,21 @@ struct Product {
     int vec;                           // the result takes 16-byte stores: addresses, stride and width
     float* slab;
     int accumulate;
-    const float* scale;
     const uint8_t* live;               // result rows that are zero whatever the operands hold
 };
 
 template <class C, int DT, bool AK, bool BKM>
-__global__ void __launch_bounds__(C::THREADS) product_kernel(Product pr) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+__device__ __forceinline__ void product_tile(const Product& pr, const Upstream& up, uint32_t id, uint32_t total, char* lds) {
     typedef typename Elem<DT>::type E;
     uint32_t tm, tn, z;
-    tile_of(blockIdx.x, gridDim.x, pr.tiles_m, pr.tiles_n, tm, tn, z);
+    tile_of(id, total, pr.tiles_m, pr.tiles_n, tm, tn, z);
     const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
     const int64_t kb = (int64_t)z * pr.split_k, ke = kb + pr.split_k < pr.k ? kb + pr.split_k : pr.k;
     Acc<C> acc;
     clear(acc);
     gemm_tile<C, DT, AK, BKM>(pr.a, pr.b, m0, n0, kb, ke, acc, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
-    const float sc = pr.slab ? 1.0f : pr.scale[1];
+    const float sc = pr.slab ? 1.0f : up.result();
     float* slab = pr.slab ? pr.slab + (size_t)z * pr.rows * pr.width : nullptr;
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
@@ -831,19 +836,85 @@ __global__ void __launch_bounds__(C::THREADS) product_kernel(Product pr) {
     }
 }
 
-// result = scale x sum of the slabs, in their order
-template <int DT>
-__global__ void __launch_bounds__(256) finish_kernel(const float* __restrict__ slab, int splits, int64_t rows, int64_t width, const float* __restrict__ scale,
-                                                     const uint8_t* __restrict__ live, void* __restrict__ out, int64_t out_stride) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * width) return;
-    const int64_t n = i / width, m = i - n * width;
-    float a = 0.0f;
-    if (!live || live[n]) {
-        for (int s = 0; s < splits; ++s) a += slab[(size_t)s * rows * width + i];
-        a *= scale[1];
+// The weights' gradient (both operands with the rows as k) and the hidden rows' (the weights with the classes as k) of one piece, in one launch: neither fills the device's last
+// round alone.  groups: workgroups of the first, a multiple of 8 (the XCDs' turn) unless it is the only one.
+template <class C, int DT>
+__global__ void __launch_bounds__(C::THREADS) products_kernel(Product dw, Product dh, Upstream up, uint32_t dw_tiles, uint32_t dw_groups) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if (blockIdx.x < dw_groups) {
+        if (blockIdx.x < dw_tiles) product_tile<C, DT, true, true>(dw, up, blockIdx.x, dw_tiles, lds);
+    } else
+        product_tile<C, DT, true, false>(dh, up, blockIdx.x - dw_groups, gridDim.x - dw_groups, lds);
+}
+template <class C, int DT>
+__global__ void __launch_bounds__(C::THREADS) rows_product_kernel(Product dh, Upstream up) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    product_tile<C, DT, true, false>(dh, up, blockIdx.x, gridDim.x, lds);
+}
+
+// result = scale x sum of the slabs, in their order; and db[class] = scale x sum over the row tiles: 64 classes per workgroup, wave g takes tiles g, g + 4, ...
+struct Finish {
+    const float* slab;
+    int64_t splits, rows, width;
+    const uint8_t* live;
+    void* out;
+    int64_t out_stride;
+    int vec;                          // width, stride and address take four values at a time
+    uint32_t groups;                  // workgroups of 1024 values
+};
+struct FinishBias {
+    const float* part;
+    int64_t classes;
+    int tiles;
+    void* out;
+    uint32_t groups;
+};
+template <int DT> __device__ __forceinline__ void finish(const Finish& f, float scale, uint32_t group) {
+    typedef typename Elem<DT>::type E;
+    const int64_t total = f.rows * f.width, i0 = ((int64_t)group * 256 + threadIdx.x) * 4;
+    if (i0 >= total) return;
+    if (f.vec) {
+        const int64_t n = i0 / f.width, m = i0 - n * f.width;
+        f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (!f.live || f.live[n]) {
+#pragma unroll 4
+            for (int64_t s = 0; s < f.splits; ++s) a += *(const f32x4*)(f.slab + s * total + i0);
+            a *= scale;
+        }
+        E v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = from_float<DT>(a[k]);
+        __builtin_memcpy((E*)f.out + n * f.out_stride + m, v, sizeof v);
+        return;
     }
-    ((typename Elem<DT>::type*)out)[n * out_stride + m] = from_float<DT>(a);
+    for (int64_t i = i0; i < i0 + 4 && i < total; ++i) {
+        const int64_t n = i / f.width, m = i - n * f.width;
+        float a = 0.0f;
+        if (!f.live || f.live[n]) {
+            for (int64_t s = 0; s < f.splits; ++s) a += f.slab[s * total + i];
+            a *= scale;
+        }
+        ((E*)f.out)[n * f.out_stride + m] = from_float<DT>(a);
+    }
+}
+template <int DT>
+__global__ void __launch_bounds__(256) finish_kernel(Finish dw, Finish dh, FinishBias db, Upstream up) {
+    __shared__ float red[4][64];
+    const float scale = up.result();
+    uint32_t b = blockIdx.x;
+    if (b < dw.groups) return finish<DT>(dw, scale, b);
+    b -= dw.groups;
+    if (b < dh.groups) return finish<DT>(dh, scale, b);
+    b -= dh.groups;
+    const int r = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int64_t j = (int64_t)b * 64 + r;
+    float a = 0.0f;
+    if (j < db.classes)
+#pragma unroll 8
+        for (int t = g; t < db.tiles; t += 4) a += db.part[(size_t)t * db.classes + j];
+    red[g][r] = a;
+    __syncthreads();
+    if (g == 0 && j < db.classes) ((typename Elem<DT>::type*)db.out)[j] = from_float<DT>((red[0][r] + red[1][r] + red[2][r] + red[3][r]) * scale);
 }
 
 }  // namespace q1head
