@@ -6,15 +6,27 @@ policies apply with tf.clip_by_global_norm; the reference's trainer config leave
 
 Tensors: CUDA, one device, float32 / bfloat16 / float16 (mixed as they come), any shape; dense ones in any order of dimensions, or rows of contiguous
 values at a pitch (a column slice).  Squares are summed in float64 in an order that the sizes alone fix: the same bits every time."""
+import functools
 import operator
+from array import array
 
-import numpy as np
 import torch
 
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 _T = torch.Tensor
+_PLAIN = {torch.Tensor, torch.nn.Parameter}
+_dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
+
+
+@functools.lru_cache(maxsize=64)
+def _workspace_bytes(count):
+    return _lib.load().q1env_grad_norm_workspace_bytes(count)
+
+
+def _address(a):
+    return None if a is None else a.buffer_info()[0]
 
 
 def _pitched(t):
@@ -40,10 +52,8 @@ def _order(t):
 
 
 def _layouts(tensors, out):
-    """The cols / src_pitch / dst_pitch arrays, or three Nones where every tensor is contiguous."""
-    if all(map(_T.is_contiguous, tensors)) and (out is None or all(map(_T.is_contiguous, out))):
-        return None, None, None
-    cols, sp, dp = (np.zeros(len(tensors), np.int64) for _ in range(3))
+    """The cols / src_pitch / dst_pitch arrays of tensors that are not all contiguous."""
+    cols, sp, dp = (array("q", bytes(8 * len(tensors))) for _ in range(3))
     for i, t in enumerate(tensors):
         o = t if out is None else out[i]
         if t.numel() == 0:
@@ -59,8 +69,8 @@ def _layouts(tensors, out):
 
 
 def _tensors(tensors, what):
-    tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    if not all(map(torch.is_tensor, tensors)):
+    tensors = [tensors] if isinstance(tensors, _T) else list(tensors)
+    if not _PLAIN.issuperset(map(type, tensors)) and not all(map(torch.is_tensor, tensors)):
         raise TypeError(f"{what}: tensors only")
     return tensors
 
@@ -72,58 +82,64 @@ def _run(tensors, out, max_norm, scale):
         raise ValueError("scale must be positive and finite")
     if max_norm is not None and not float(max_norm) >= 0.0:
         raise ValueError("max_norm must not be negative or NaN")
-    if not tensors:
+    n = len(tensors)
+    if n == 0:
         raise ValueError("no tensors: there is no device to put the norm on")
-    kinds = list(map(operator.attrgetter("dtype"), tensors))
-    if not all(map(_DTYPES.__contains__, set(kinds))):
-        raise TypeError(f"gradients must be float32, bfloat16 or float16, got {set(kinds) - set(_DTYPES)}")
-    if len(tensors) > 65536:
+    if n > 65536:
         raise ValueError("more than 65536 tensors")
+    kinds = list(map(_dtype, tensors))
+    if not _DTYPES.keys() >= set(kinds):
+        raise TypeError(f"gradients must be float32, bfloat16 or float16, got {set(kinds) - set(_DTYPES)}")
+    values = list(map(_T.numel, tensors))
+    devices = set(map(_T.get_device, tensors))
+    plain = all(map(_T.is_contiguous, tensors))
     if out is not None:
         out = _tensors(out, "out")
-        if len(out) != len(tensors):
-            raise ValueError(f"{len(out)} tensors in out for {len(tensors)} gradients")
-        if list(map(operator.attrgetter("dtype"), out)) != kinds:
+        if len(out) != n:
+            raise ValueError(f"{len(out)} tensors in out for {n} gradients")
+        if list(map(_dtype, out)) != kinds:
             raise TypeError("out must have the gradients' dtypes")
-        if list(map(operator.attrgetter("shape"), out)) != list(map(operator.attrgetter("shape"), tensors)):
-            raise ValueError("out must have the gradients' shapes")
-    devices = set(map(_T.get_device, tensors)) | (set(map(_T.get_device, out)) if out is not None else set())
+        plain = plain and all(map(_T.is_contiguous, out))
+        if list(map(_T.numel, out)) != values or (not plain and list(map(_shape, out)) != list(map(_shape, tensors))):
+            raise ValueError("out must have the gradients' shapes (their numbers of values where all are contiguous)")
+        devices |= set(map(_T.get_device, out))
     if min(devices) < 0:
         raise _lib.Q1EnvError("gradient clipping runs on an MI355X only: there is no CPU fallback")
     if len(devices) != 1:
         raise ValueError("all tensors must be on one device")
+    cols = sp = dp = None
+    if not plain:
+        if out is not None or max_norm is None:          # only read: a broadcast gradient (stride 0) counts as the values it stands for
+            tensors = [t if t.is_contiguous() or _pitched(t) is not None else t.contiguous() for t in tensors]
+        cols, sp, dp = _layouts(tensors, out)
+    src = array("Q", map(_T.data_ptr, tensors))
+    sizes = array("q", values)
+    dtype = array("i", map(_DTYPES.__getitem__, kinds))
     dev = devices.pop()
-    if out is not None or max_norm is None:              # only read: a broadcast gradient (stride 0) counts as the values it stands for
-        tensors = [t if t.is_contiguous() or _pitched(t) is not None else t.contiguous() for t in tensors]
-    cols, sp, dp = _layouts(tensors, out)
-    lib, n = _lib.load(), len(tensors)
-    src = np.array(list(map(_T.data_ptr, tensors)), np.uint64)
-    values = np.array(list(map(_T.numel, tensors)), np.int64)
-    dtype = np.full(n, _DTYPES[kinds[0]], np.int32) if len(set(kinds)) == 1 else np.array([_DTYPES[k] for k in kinds], np.int32)
-    device = torch.device("cuda", dev)
-    nbytes = lib.q1env_grad_norm_workspace_bytes(n)
-    buf = torch.empty((nbytes // 8 + 1,), dtype=torch.float64, device=device)            # the partial sums
+    device = tensors[0].device
+    lib = _lib.load()
+    nbytes = _workspace_bytes(n)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=device)                          # the partial sums, and a long list's table
     norm = torch.empty((), dtype=torch.float32, device=device)
     stream = torch.cuda.current_stream(device).cuda_stream
-    p = _lib.ptr
+    p = _address
     if max_norm is None:
-        _lib.check(lib.q1env_grad_norm(dev, stream, n, p(src), p(values), p(dtype), p(cols), p(sp), scale, norm.data_ptr(), buf.data_ptr(), nbytes))
+        _lib.check(lib.q1env_grad_norm(dev, stream, n, p(src), p(sizes), p(dtype), p(cols), p(sp), scale, norm.data_ptr(), buf.data_ptr(), nbytes))
     else:
-        dst = src if out is None else np.array(list(map(_T.data_ptr, out)), np.uint64)
-        _lib.check(lib.q1env_grad_clip(dev, stream, n, p(src), p(dst), p(values), p(dtype), p(cols), p(sp), p(dp), scale, float(max_norm), norm.data_ptr(),
+        dst = src if out is None else array("Q", map(_T.data_ptr, out))
+        _lib.check(lib.q1env_grad_clip(dev, stream, n, p(src), p(dst), p(sizes), p(dtype), p(cols), p(sp), p(dp), scale, float(max_norm), norm.data_ptr(),
                                        buf.data_ptr(), nbytes))
+        torch.autograd.graph.increment_version(tensors if out is None else out)          # autograd has to know what was written
     return norm
 
 
-@torch.no_grad()
 def grad_norm(grads, *, scale=1.0):
     """|scale| x the 2-norm over all tensors: float32 () on their device."""
     return _run(grads, None, None, scale)
 
 
-@torch.no_grad()
 def clip_grad_norm_(grads, max_norm, *, scale=1.0, out=None):
     """grads <- grads x scale x min(1, max_norm / norm), norm = grad_norm(grads, scale=scale); returns the norm.  out: where the results go instead
-    (tensors of the same shapes and dtypes that overlap nothing but, each, its own source); the gradients stay as they are.  A NaN norm makes every result
+    (tensors of the same shapes - or, where all are contiguous, sizes - and dtypes that overlap nothing but, each, its own source); the gradients stay as they are.  A NaN norm makes every result
     NaN; an infinite one turns finite values to zero."""
     return _run(grads, out, max_norm, scale)

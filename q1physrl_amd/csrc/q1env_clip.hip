@@ -4,32 +4,32 @@
 //
 // Two passes: squares summed in float64 (no overflow or underflow of a float32 gradient's square, and an order fixed by the sizes alone: the
 // same bits every time), one partial per workgroup; then every workgroup adds the partials up in the same order - cheaper than a third
-// launch - and writes its share.  The tensors travel in the kernel arguments, so nothing is uploaded, nothing is kept between calls and a captured launch holds
-// its own table.
+// launch - and writes its share, last values first: those the device's last-level cache still holds from the first pass.  Up to SLOTS table slots travel in the kernel
+// arguments; longer lists are first written to the workspace by small launches that carry SLOTS each.  Nothing is uploaded or kept between calls, and a captured
+// launch holds its own table.
+// Bound: memory.  536 870 913 float32 values (2.1 GB read, read again, written): 395 us for the first pass (5.4 TB/s), 794 for the second (5.4 TB/s; a plain copy makes 4.8).
 #include "q1env_host.hpp"
 
 #include <algorithm>
 
 namespace {
 
-constexpr int TENSORS = 96;                       // per launch: 96 x 40 bytes, under 4 KB of kernel arguments
+constexpr int SLOTS = 120;                        // 32 bytes each: under 4 KB of kernel arguments
 constexpr int THREADS = 256;
-constexpr int MAX_BLOCKS = 2048;                  // eight workgroups per CU
+constexpr int MAX_BLOCKS = 2048, MAX_CLIP_BLOCKS = 1024;      // eight workgroups per CU for the pass that reads, four for the one that reads and writes (794 us against 909)
 constexpr int64_t UNIT_MIN = 1024, UNIT_MAX = 8192;      // values a workgroup takes at a time
 
-struct __attribute__((packed, aligned(4))) Tensor {
-    const void* src;
-    void* dst;
-    int64_t count;
-    int32_t cols;                                 // 0 = contiguous, else values per row of the pitched form
-    int32_t src_pitch, dst_pitch;                 // values from row to row
+constexpr uint32_t PITCHED = 16, LAYOUT = 32;     // kinds of slot besides the dtype
+struct Slot {
+    const void* src;                              // LAYOUT (the slot behind a pitched tensor's): values per row
+    void* dst;                                    // LAYOUT: values from row to row of src
+    int64_t count;                                // LAYOUT: of dst
+    uint32_t first;                               // first unit of the tensor
+    uint32_t kind;
 };
-
 struct Table {
-    Tensor t[TENSORS];
-    uint32_t first[TENSORS];                      // first unit of each tensor
-    uint32_t n, units, unit;
-    uint32_t dtype;
+    Slot t[SLOTS];
+    uint32_t n, units, unit, pad;
 };
 static_assert(sizeof(Table) <= 4000, "the table has to fit the kernel arguments");
 
@@ -55,50 +55,79 @@ __device__ __forceinline__ double block_sum(double a, double* red) {
     return red[0] + red[1] + red[2] + red[3];
 }
 
-// runs f(tensor, first value, end) over the units of workgroup blockIdx.x: an even share, in the order of the table
-template <typename F> __device__ __forceinline__ void each_unit(const Table& tb, F f) {
-    const uint32_t per = (tb.units + gridDim.x - 1) / gridDim.x;
-    uint32_t u = blockIdx.x * per;
-    const uint32_t end = u + per < tb.units ? u + per : tb.units;
-    if (u >= end) return;
-    uint32_t lo = 0, hi = tb.n;                   // the last tensor whose first unit is <= u
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (tb.first[mid] <= u) lo = mid;
-        else hi = mid;
-    }
-    for (; u < end; ++u) {
-        while (lo + 1 < tb.n && tb.first[lo + 1] <= u) ++lo;
-        const int64_t a = (int64_t)(u - tb.first[lo]) * tb.unit;
-        const int64_t b = a + tb.unit < tb.t[lo].count ? a + tb.unit : tb.t[lo].count;
-        f(tb.t[lo], a, b);
+// runs f(slot, first value, end) over units blockIdx.x, blockIdx.x + gridDim.x, ... (neighbouring workgroups stream neighbouring memory), forwards or backwards
+template <bool BACK, typename F> __device__ __forceinline__ void each_unit(const Slot* __restrict__ t, uint32_t n, uint32_t units, uint32_t unit, F f) {
+    const uint32_t mine = blockIdx.x < units ? (units - 1 - blockIdx.x) / gridDim.x + 1 : 0;
+    uint32_t lo = 0, hi = n;                      // where the slot is looked for
+    for (uint32_t i = 0; i < mine; ++i) {
+        const uint32_t u = blockIdx.x + (BACK ? mine - 1 - i : i) * gridDim.x;
+        if (BACK) lo = 0;
+        else hi = n;
+        while (hi - lo > 1) {                     // the last slot whose first unit is <= u
+            const uint32_t mid = (lo + hi) >> 1;
+            if (t[mid].first <= u) lo = mid;
+            else hi = mid;
+        }
+        const uint32_t at = t[lo].kind & LAYOUT ? lo - 1 : lo;
+        const int64_t a = (int64_t)(u - t[at].first) * unit, count = t[at].count;
+        f(t + at, a, a + unit < count ? a + unit : count);
     }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(THREADS) squares_kernel(Table tb, double* __restrict__ partial) {
+template <int DT> __device__ __forceinline__ double squares(const Slot* t, int64_t a, int64_t b, double acc) {
     typedef typename El<DT>::type E;
     constexpr int V = 16 / sizeof(E);
-    __shared__ double red[4];
-    double acc = 0.0;
-    each_unit(tb, [&](const Tensor& t, int64_t a, int64_t b) {
-        const E* p = (const E*)t.src;
-        if (t.cols) {
-            for (int64_t i = a + threadIdx.x; i < b; i += THREADS) {
-                const int64_t r = i / t.cols;
-                const double x = (double)value<DT>(p[r * t.src_pitch + (i - r * t.cols)]);
-                acc = fma(x, x, acc);
-            }
-            return;
+    const E* p = (const E*)t->src;
+    if (t->kind & PITCHED) {
+        const int64_t cols = (int64_t)t[1].src, pitch = (int64_t)t[1].dst;
+        for (int64_t i = a + threadIdx.x; i < b; i += THREADS) {
+            const int64_t r = i / cols;
+            const double x = (double)value<DT>(p[r * pitch + (i - r * cols)]);
+            acc = fma(x, x, acc);
         }
-        int64_t i = a + (int64_t)threadIdx.x * V;
-        for (; i + V <= b; i += THREADS * V) {
-            E v[V];
-            __builtin_memcpy(v, p + i, 16);
+        return acc;
+    }
+    int64_t i = a + (int64_t)threadIdx.x * V;
+    for (; i + V <= b; i += THREADS * V) {
+        E v[V];
+        __builtin_memcpy(v, p + i, 16);
 #pragma unroll
-            for (int j = 0; j < V; ++j) { const double x = (double)value<DT>(v[j]); acc = fma(x, x, acc); }
+        for (int j = 0; j < V; ++j) { const double x = (double)value<DT>(v[j]); acc = fma(x, x, acc); }
+    }
+    for (; i < b; ++i) { const double x = (double)value<DT>(p[i]); acc = fma(x, x, acc); }
+    return acc;
+}
+
+template <int DT> __device__ __forceinline__ void scaled(const Slot* t, int64_t a, int64_t b, float c) {
+    typedef typename El<DT>::type E;
+    constexpr int V = 16 / sizeof(E);
+    const E* p = (const E*)t->src;
+    E* q = (E*)t->dst;
+    if (c == 1.0f && (const E*)q == p) return;                                   // in place and nothing to clip
+    if (t->kind & PITCHED) {
+        const int64_t cols = (int64_t)t[1].src, ps = (int64_t)t[1].dst, pd = t[1].count;
+        for (int64_t i = a + threadIdx.x; i < b; i += THREADS) {
+            const int64_t r = i / cols, k = i - r * cols;
+            q[r * pd + k] = rounded<DT>(value<DT>(p[r * ps + k]) * c);
         }
-        for (; i < b; ++i) { const double x = (double)value<DT>(p[i]); acc = fma(x, x, acc); }
+        return;
+    }
+    int64_t i = a + (int64_t)threadIdx.x * V;
+    for (; i + V <= b; i += THREADS * V) {
+        E w[V];
+        __builtin_memcpy(w, p + i, 16);
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[j] = rounded<DT>(value<DT>(w[j]) * c);
+        __builtin_memcpy(q + i, w, 16);
+    }
+    for (; i < b; ++i) q[i] = rounded<DT>(value<DT>(p[i]) * c);
+}
+
+__device__ __forceinline__ void squares_of(const Slot* t, uint32_t n, uint32_t units, uint32_t unit, double* __restrict__ partial, double* red) {
+    double acc = 0.0;
+    each_unit<false>(t, n, units, unit, [&](const Slot* s, int64_t a, int64_t b) {
+        const uint32_t dt = s->kind & 15;
+        acc = dt == Q1ENV_DT_F32 ? squares<Q1ENV_DT_F32>(s, a, b, acc) : dt == Q1ENV_DT_BF16 ? squares<Q1ENV_DT_BF16>(s, a, b, acc) : squares<Q1ENV_DT_F16>(s, a, b, acc);
     });
     acc = block_sum(acc, red);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
@@ -117,35 +146,39 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const double* __restrict_
     if (threadIdx.x == 0) *norm = (float)v;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(THREADS) clip_kernel(Table tb, const double* __restrict__ partial, int n, double scale, double max_norm, float* __restrict__ norm) {
-    typedef typename El<DT>::type E;
-    constexpr int V = 16 / sizeof(E);
-    __shared__ double red[4];
-    const double v = norm_of(partial, n, scale, red);
-    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+__device__ __forceinline__ void clip_of(const Slot* t, uint32_t n, uint32_t units, uint32_t unit, const double* __restrict__ partial, int parts, double scale, double max_norm,
+                                        float* __restrict__ norm, double* red) {
+    const double v = norm_of(partial, parts, scale, red);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
     const float c = (float)(scale * (v <= max_norm ? 1.0 : max_norm / v));       // a NaN norm makes every value NaN
-    each_unit(tb, [&](const Tensor& t, int64_t a, int64_t b) {
-        const E* p = (const E*)t.src;
-        E* q = (E*)t.dst;
-        if (c == 1.0f && (const E*)q == p) return;                               // in place and nothing to clip
-        if (t.cols) {
-            for (int64_t i = a + threadIdx.x; i < b; i += THREADS) {
-                const int64_t r = i / t.cols, k = i - r * t.cols;
-                q[r * t.dst_pitch + k] = rounded<DT>(value<DT>(p[r * t.src_pitch + k]) * c);
-            }
-            return;
-        }
-        int64_t i = a + (int64_t)threadIdx.x * V;
-        for (; i + V <= b; i += THREADS * V) {
-            E w[V];
-            __builtin_memcpy(w, p + i, 16);
-#pragma unroll
-            for (int j = 0; j < V; ++j) w[j] = rounded<DT>(value<DT>(w[j]) * c);
-            __builtin_memcpy(q + i, w, 16);
-        }
-        for (; i < b; ++i) q[i] = rounded<DT>(value<DT>(p[i]) * c);
+    each_unit<true>(t, n, units, unit, [&](const Slot* s, int64_t a, int64_t b) {
+        const uint32_t dt = s->kind & 15;
+        if (dt == Q1ENV_DT_F32) scaled<Q1ENV_DT_F32>(s, a, b, c);
+        else if (dt == Q1ENV_DT_BF16) scaled<Q1ENV_DT_BF16>(s, a, b, c);
+        else scaled<Q1ENV_DT_F16>(s, a, b, c);
     });
+}
+
+// the table in the kernel arguments, or in the workspace
+__global__ void __launch_bounds__(THREADS) squares_kernel(Table tb, double* __restrict__ partial) {
+    __shared__ double red[4];
+    squares_of(tb.t, tb.n, tb.units, tb.unit, partial, red);
+}
+__global__ void __launch_bounds__(THREADS) squares_long_kernel(const Slot* __restrict__ t, uint32_t n, uint32_t units, uint32_t unit, double* __restrict__ partial) {
+    __shared__ double red[4];
+    squares_of(t, n, units, unit, partial, red);
+}
+__global__ void __launch_bounds__(THREADS) clip_kernel(Table tb, const double* __restrict__ partial, int parts, double scale, double max_norm, float* __restrict__ norm) {
+    __shared__ double red[4];
+    clip_of(tb.t, tb.n, tb.units, tb.unit, partial, parts, scale, max_norm, norm, red);
+}
+__global__ void __launch_bounds__(THREADS) clip_long_kernel(const Slot* __restrict__ t, uint32_t n, uint32_t units, uint32_t unit, const double* __restrict__ partial, int parts,
+                                                            double scale, double max_norm, float* __restrict__ norm) {
+    __shared__ double red[4];
+    clip_of(t, n, units, unit, partial, parts, scale, max_norm, norm, red);
+}
+__global__ void __launch_bounds__(THREADS) table_kernel(Table tb, Slot* __restrict__ out) {
+    for (uint32_t i = threadIdx.x; i < tb.n; i += THREADS) out[i] = tb.t[i];
 }
 
 size_t elem_size(int dt) { return dt == Q1ENV_DT_F32 ? 4 : 2; }
@@ -204,7 +237,8 @@ int check_job(const char* who, const Job& j, bool write) {
         s.push_back({da, da + (rows - 1) * dp + c * es, i, dp, c * es});
         if (sa != da || sp != dp) s.push_back({sa, sa + (rows - 1) * sp + c * es, ~i, sp, c * es});      // ~i: a source
     }
-    std::sort(s.begin(), s.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
+    const auto before = [](const Span& x, const Span& y) { return x.a < y.a; };
+    if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
     std::vector<size_t> open;
     for (size_t k = 0; k < s.size(); ++k) {
         size_t kept = 0;
@@ -216,39 +250,6 @@ int check_job(const char* who, const Job& j, bool write) {
         }
         open.resize(kept);
         open.push_back(k);
-    }
-    return 0;
-}
-
-// cuts the tensors into tables of one dtype and at most TENSORS entries and launches go(table, blocks, first block) for each
-template <typename F> int each_table(const Job& j, int64_t unit, int max_blocks, F go) {
-    int at = 0, block0 = 0;
-    int64_t all_units = 0;
-    for (int i = 0; i < j.count; ++i) all_units += (j.values[i] + unit - 1) / unit;
-    Table tb;
-    while (at < j.count) {
-        tb.n = 0;
-        tb.unit = (uint32_t)unit;
-        tb.dtype = (uint32_t)j.dtype[at];
-        uint64_t units = 0;
-        for (; at < j.count && tb.n < TENSORS && (uint32_t)j.dtype[at] == tb.dtype; ++at) {
-            if (j.values[at] == 0) continue;
-            Tensor& t = tb.t[tb.n];
-            t.src = j.src[at];
-            t.dst = j.dst ? j.dst[at] : nullptr;
-            t.count = j.values[at];
-            t.cols = j.cols ? (int32_t)j.cols[at] : 0;
-            t.src_pitch = t.cols ? (int32_t)j.src_pitch[at] : 0;
-            t.dst_pitch = t.cols && j.dst ? (int32_t)j.dst_pitch[at] : 0;
-            tb.first[tb.n++] = (uint32_t)units;
-            units += (uint64_t)((j.values[at] + unit - 1) / unit);
-        }
-        if (tb.n == 0) continue;
-        tb.units = (uint32_t)units;
-        int64_t blocks = (int64_t)((double)max_blocks * (double)units / (double)all_units);      // this table's share
-        blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)units));
-        if (int rc = go(tb, (unsigned)blocks, block0)) return rc;
-        block0 += (int)blocks;
     }
     return 0;
 }
@@ -275,29 +276,46 @@ int run(const char* who, int device, hipStream_t stream, const Job& j, bool writ
     if (device < 0 || device >= n) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": no such device");
     DeviceGuard guard(device);
     double* partial = (double*)ws;
-    int parts = 0;
-    int rc = each_table(j, unit, MAX_BLOCKS, [&](const Table& tb, unsigned blocks, int block0) -> int {
-        parts = block0 + (int)blocks;
-        if (tb.dtype == Q1ENV_DT_F32) hipLaunchKernelGGL((squares_kernel<Q1ENV_DT_F32>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial + block0);
-        else if (tb.dtype == Q1ENV_DT_BF16) hipLaunchKernelGGL((squares_kernel<Q1ENV_DT_BF16>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial + block0);
-        else hipLaunchKernelGGL((squares_kernel<Q1ENV_DT_F16>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial + block0);
+    // the slots, straight into the table that a launch takes
+    Table tb;
+    tb.n = 0;
+    tb.unit = (uint32_t)unit;
+    tb.pad = 0;
+    Slot* const far = (Slot*)((char*)ws + 8 * MAX_BLOCKS);
+    uint64_t units = 0;
+    uint32_t slots = 0;                           // in the workspace already
+    auto spill = [&]() -> int {
+        hipLaunchKernelGGL(table_kernel, dim3(1), dim3(THREADS), 0, stream, tb, far + slots);
         HIP_TRY(hipGetLastError());
+        slots += tb.n;
+        tb.n = 0;
         return 0;
-    });
-    if (rc) return rc;
-    if (!write || parts == 0) {
-        hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(THREADS), 0, stream, partial, parts, scale, norm);
-        HIP_TRY(hipGetLastError());
-        return Q1ENV_OK;
+    };
+    for (int i = 0; i < j.count; ++i) {
+        if (j.values[i] == 0) continue;
+        const bool pitched = j.cols && j.cols[i] != 0;
+        if (tb.n + (pitched ? 2 : 1) > SLOTS)
+            if (int rc = spill()) return rc;
+        tb.t[tb.n++] = Slot{j.src[i], j.dst ? j.dst[i] : nullptr, j.values[i], (uint32_t)units, (uint32_t)j.dtype[i] | (pitched ? PITCHED : 0)};
+        if (pitched) tb.t[tb.n++] = Slot{(const void*)j.cols[i], (void*)j.src_pitch[i], j.dst_pitch ? j.dst_pitch[i] : 0, (uint32_t)units, LAYOUT};
+        units += (uint64_t)((j.values[i] + unit - 1) / unit);
     }
-    return each_table(j, unit, MAX_BLOCKS, [&](const Table& tb, unsigned blocks, int block0) -> int {
-        float* out = block0 == 0 ? norm : nullptr;
-        if (tb.dtype == Q1ENV_DT_F32) hipLaunchKernelGGL((clip_kernel<Q1ENV_DT_F32>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial, parts, scale, max_norm, out);
-        else if (tb.dtype == Q1ENV_DT_BF16) hipLaunchKernelGGL((clip_kernel<Q1ENV_DT_BF16>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial, parts, scale, max_norm, out);
-        else hipLaunchKernelGGL((clip_kernel<Q1ENV_DT_F16>), dim3(blocks), dim3(THREADS), 0, stream, tb, partial, parts, scale, max_norm, out);
+    const bool lng = slots > 0;
+    if (lng && tb.n > 0)
+        if (int rc = spill()) return rc;
+    tb.units = (uint32_t)units;
+    const unsigned blocks = (unsigned)std::min<uint64_t>(units, MAX_BLOCKS);
+    if (blocks > 0) {
+        if (lng) hipLaunchKernelGGL(squares_long_kernel, dim3(blocks), dim3(THREADS), 0, stream, far, slots, tb.units, tb.unit, partial);
+        else hipLaunchKernelGGL(squares_kernel, dim3(blocks), dim3(THREADS), 0, stream, tb, partial);
         HIP_TRY(hipGetLastError());
-        return 0;
-    });
+    }
+    const unsigned clip_blocks = std::min<unsigned>(blocks, MAX_CLIP_BLOCKS);
+    if (!write || blocks == 0) hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(THREADS), 0, stream, partial, (int)blocks, scale, norm);
+    else if (lng) hipLaunchKernelGGL(clip_long_kernel, dim3(clip_blocks), dim3(THREADS), 0, stream, far, slots, tb.units, tb.unit, partial, (int)blocks, scale, max_norm, norm);
+    else hipLaunchKernelGGL(clip_kernel, dim3(clip_blocks), dim3(THREADS), 0, stream, tb, partial, (int)blocks, scale, max_norm, norm);
+    HIP_TRY(hipGetLastError());
+    return Q1ENV_OK;
 }
 
 }  // namespace
@@ -305,8 +323,8 @@ int run(const char* who, int device, hipStream_t stream, const Job& j, bool writ
 extern "C" {
 
 uint64_t q1env_grad_norm_workspace_bytes(int count) {
-    // one partial per workgroup: MAX_BLOCKS shares, and one more for each table that is too small for a share (a table per TENSORS tensors or change of dtype)
-    return count < 0 || count > 65536 ? 0 : 8ull * (MAX_BLOCKS + (uint64_t)count + 1);
+    // a partial per workgroup, and a long list's table (two slots for a pitched tensor)
+    return count < 0 || count > 65536 ? 0 : 8ull * MAX_BLOCKS + (2 * count > SLOTS ? 2 * sizeof(Slot) * (uint64_t)count : 0);
 }
 
 int q1env_grad_norm(int device, void* stream, int count, const void* const* src, const int64_t* values, const int32_t* dtype, const int64_t* cols, const int64_t* pitch, double scale,
