@@ -90,6 +90,8 @@ struct Plan {
     Size logits, dh, dw;
     int dh_split, dw_split;
     int64_t dh_k, dw_k;                // classes / rows per split
+    bool few;                          // the forward pass of up to 32 float32 rows (few_rows_kernel)
+    int64_t tiles;                     // partial statistics per row
     uint64_t part, own, scale, g, db, dh_slab, dw_slab, h_laid, w_laid;        // byte offsets in the workspace
     uint64_t bytes;
 };
@@ -97,6 +99,8 @@ struct Plan {
 // w_in_place / h_in_place: the workspace has to suffice for any address, so its size is asked for with both false
 Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward, bool h_in_place, bool w_in_place) {
     Plan p{};
+    p.few = !backward && dt == F32 && rows <= 32;
+    if (p.few) h_in_place = w_in_place = true;
     p.padded = round_up(width, 64);
     const int64_t all = round_up(classes, PIECE_STEP);
     int64_t piece = all;
@@ -111,7 +115,8 @@ Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward
     auto take = [&](uint64_t n) { const uint64_t o = at; at += aligned(n); return o; };
     if (!backward) {
         p.own = take(4 * rows);
-        p.part = take(12 * (uint64_t)div_up(classes, bm_of(p.logits)) * rows);
+        p.tiles = p.few ? std::min<int64_t>(div_up(classes, 32), 2048) : div_up(classes, bm_of(p.logits));
+        p.part = take(12 * (uint64_t)p.tiles * rows);
     } else {
         const Shape dh = shape_of(width, rows, std::min(piece, classes), products, true, 4000.0, 3000.0, false);
         const Shape dw = shape_of(width, std::min(piece, classes), rows, products, true, 4000.0, 3000.0, true);
@@ -244,7 +249,16 @@ int forward(const Where& at, const q1env_head& q, int reduction, float* logp, fl
         const Target target{q.target_dev, q.target_bits == 64 ? 1 : 0, q.ignore_index, q.classes};
         const Op h = rows_op(DT, hp, q.hidden_dev, q.hidden_stride, n, q.width, p.padded, ws + p.h_laid);
         float *part = (float*)(ws + p.part), *own = (float*)(ws + p.own);
-        for (int64_t c0 = 0; c0 < q.classes; c0 += p.piece) {
+        if (p.few) {
+            auto vec = [](const void* x, int64_t stride) { return ((uintptr_t)x & 15) == 0 && stride % 4 == 0 ? 1 : 0; };
+            const float *w = (const float*)q.weight_dev, *x = (const float*)q.hidden_dev;
+            if (entropy) hipLaunchKernelGGL((few_rows_kernel<true>), dim3((unsigned)p.tiles), dim3(256), 0, at.stream, w, q.weight_stride, vec(w, q.weight_stride), x, q.hidden_stride,
+                                            vec(x, q.hidden_stride), (const float*)q.bias_dev, target, (int)n, q.width, part, own);
+            else hipLaunchKernelGGL((few_rows_kernel<false>), dim3((unsigned)p.tiles), dim3(256), 0, at.stream, w, q.weight_stride, vec(w, q.weight_stride), x, q.hidden_stride,
+                                    vec(x, q.hidden_stride), (const float*)q.bias_dev, target, (int)n, q.width, part, own);
+            HIP_TRY(hipGetLastError());
+        }
+        for (int64_t c0 = 0; c0 < q.classes && !p.few; c0 += p.piece) {
             const int64_t c1 = std::min(c0 + p.piece, q.classes);
             const char* w0 = (const char*)q.weight_dev + elem_size(DT) * c0 * q.weight_stride;
             Q1_TRY(lay_out<DT>(at, Lay{q.hidden_dev, q.hidden_stride, hp || c0 > 0 ? 0 : n, nullptr, (uint16_t*)(ws + p.h_laid), 0},
@@ -257,9 +271,14 @@ int forward(const Where& at, const q1env_head& q, int reduction, float* logp, fl
             else if (p.logits == FEW) Q1_TRY((statistics<Few, DT>(at, hd, target, e, part, own)));
             else Q1_TRY((statistics<Fewest, DT>(at, hd, target, e, part, own)));
         }
-        float* here = n <= 64 ? loss : nullptr;                               // one workgroup joins all the rows: it has the loss too
-        hipLaunchKernelGGL(join_kernel, dim3((unsigned)div_up(n, 64)), dim3(1024), 0, at.stream, part, own, target, n, (int)div_up(q.classes, bm_of(p.logits)), entropy ? 1 : 0, logp,
-                           entropy, st.entropy, st.lse, st.target, st.live, st.bits, mean, here, st.each);
+        const bool tall = p.tiles > 64 && n <= 4096;                          // many tiles of few rows
+        float* here = n <= (tall ? 16 : 64) ? loss : nullptr;                 // one workgroup joins all the rows: it has the loss too
+        if (tall)
+            hipLaunchKernelGGL((join_kernel<16>), dim3((unsigned)div_up(n, 16)), dim3(1024), 0, at.stream, part, own, target, n, (int)p.tiles, entropy ? 1 : 0, logp, entropy, st.entropy,
+                               st.lse, st.target, st.live, st.bits, mean, here, st.each);
+        else
+            hipLaunchKernelGGL((join_kernel<64>), dim3((unsigned)div_up(n, 64)), dim3(1024), 0, at.stream, part, own, target, n, (int)p.tiles, entropy ? 1 : 0, logp, entropy, st.entropy,
+                               st.lse, st.target, st.live, st.bits, mean, here, st.each);
         HIP_TRY(hipGetLastError());
         if (here) return Q1ENV_OK;
     }

@@ -478,30 +478,114 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target 
         }
 }
 
-// joins the tiles' statistics: 64 rows per workgroup, wave g takes tiles g, g + 16, ... (four loads of each kind in flight); lse is kept in units of log2.  Also leaves what the
-// backward pass wants of the classes: -1 / -2 / the class, and the rows that count as bytes and as bits.
+// Up to 32 rows of float32: no laying out, no LDS on the way.  A workgroup takes 32 classes at a time, its four waves a quarter of the width each; a lane loads 16 bytes of its class (or row)
+// at k = 8 q + 4 (lane >> 5) and feeds them to four float32 matrix instructions - which value of k a lane holds does not matter as long as both operands hold the same.  At 16 FLOP per weight
+// the instruction's rate is no bound.  One row against 721 classes of 256: latency, 5 us (13 + 3 with pieces laid out first).
+template <bool ENTROPY>
+__global__ void __launch_bounds__(256) few_rows_kernel(const float* __restrict__ w, int64_t w_stride, int w_vec, const float* __restrict__ h, int64_t h_stride, int h_vec,
+                                                       const float* __restrict__ bias, Target target, int rows, int64_t width, float* __restrict__ part, float* __restrict__ own_logit) {
+    __shared__ float sums[4][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 31;
+    const int64_t quarter = (width + 31) / 32 * 8, k_first = wave * quarter + 4 * (lane >> 5);
+    const int steps = (int)(quarter / 8);
+    const int64_t classes = target.classes, t = x < rows ? target.of(x) : -1;
+    const float* hr = h + x * h_stride;
+    Stat all{-INFINITY, 0.0f, 0.0f};
+    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < classes; c0 += (int64_t)gridDim.x * 32) {
+        const float* wr = w + (c0 + x) * w_stride;
+        const bool w_ok = c0 + x < classes;
+        f32x16 acc = {};
+        auto four = [&](const float* p, bool ok, int vec, int64_t k) {
+            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (ok && vec && k + 4 <= width) v = *(const f32x4*)(p + k);
+            else if (ok)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (k + j < width) v[j] = p[k + j];
+            return v;
+        };
+        constexpr int AHEAD = 8;                                             // steps whose loads are in flight together
+        for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+            f32x4 a[AHEAD], b[AHEAD];
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s) {
+                const int64_t k = s0 + s < steps ? k_first + 8 * (int64_t)(s0 + s) : width;
+                a[s] = four(wr, w_ok, w_vec, k);
+                b[s] = four(hr, x < rows, h_vec, k);
+            }
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s][j], b[s][j], acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[wave][r][lane] = acc[r];
+        __syncthreads();
+        if (wave == 0) {
+            const int64_t base = c0 + 4 * (lane >> 5);
+            float l[16], mx = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t m = base + 8 * (r >> 2) + (r & 3);
+                l[r] = -INFINITY;
+                if (m < classes) {
+                    l[r] = (sums[0][r][lane] + sums[1][r][lane]) + (sums[2][r][lane] + sums[3][r][lane]);
+                    if (bias) l[r] += bias[m];
+                    if (m == t) own_logit[x] = l[r];
+                }
+                mx = fmaxf(mx, l[r]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * LOG2E;
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+            Stat st{mx, 0.0f, 0.0f};
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float d = fmaf(l[r], LOG2E, -ref), e = __builtin_amdgcn_exp2f(d);
+                st.s += e;
+                if constexpr (ENTROPY) st.u = fmaf(fmaxf(d, -3.0e38f), e, st.u);
+            }
+            st.s += __shfl_xor(st.s, 32, 64);
+            if constexpr (ENTROPY) st.u += __shfl_xor(st.u, 32, 64);
+            all = joined(all, st);
+        }
+        __syncthreads();
+    }
+    if (wave == 0 && lane < rows) {
+        float* o = part + 3 * (size_t)blockIdx.x * rows + lane;
+        o[0] = all.m; o[rows] = all.s; o[2 * rows] = all.u;
+    }
+}
+
+// Joins the tiles' statistics: R rows per workgroup, 1024 / R lanes take the tiles of a row in turn (four loads of each kind in flight); lse is kept in units of log2.  Also leaves what the
+// backward pass wants of the classes: -1 / -2 / the class, and the rows that count as bytes and as bits.  R = 64 where there are many rows, 16 where there are many tiles (64 rows
+// of 1025 tiles: 21 us with R = 64).
+template <int R>
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ part, const float* __restrict__ own_logit, Target target, int64_t rows, int tiles, int with_entropy,
                                                     float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ entropy_kept, float* __restrict__ lse,
                                                     int64_t* __restrict__ classes, uint8_t* __restrict__ live, uint64_t* __restrict__ bits, int mean,
                                                     float* __restrict__ loss, float* __restrict__ each) {
-    __shared__ float red[3][16][64];
-    const int r = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t n = (int64_t)blockIdx.x * 64 + r;
+    static_assert(R == 64 || R == 16, "the words of bits");
+    constexpr int G = 1024 / R;
+    __shared__ float red[3][16][R];
+    const int r = threadIdx.x % R, g = threadIdx.x / R, wave = threadIdx.x >> 6;
+    const int64_t n = (int64_t)blockIdx.x * R + r;
     Stat a{-INFINITY, 0.0f, 0.0f};
     if (n < rows)
-        for (int t = g; t < tiles; t += 64) {
+        for (int t = g; t < tiles; t += 4 * G) {
             Stat v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float* o = part + 3 * (size_t)(t + 16 * k) * rows + n;
-                v[k] = t + 16 * k < tiles ? Stat{o[0], o[rows], with_entropy ? o[2 * rows] : 0.0f} : Stat{-INFINITY, 0.0f, 0.0f};
+                const float* o = part + 3 * (size_t)(t + G * k) * rows + n;
+                v[k] = t + G * k < tiles ? Stat{o[0], o[rows], with_entropy ? o[2 * rows] : 0.0f} : Stat{-INFINITY, 0.0f, 0.0f};
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) a = joined(a, v[k]);
         }
-    red[0][g][r] = a.m; red[1][g][r] = a.s; red[2][g][r] = a.u;
+#pragma unroll
+    for (int off = R; off < 64; off *= 2) a = joined(a, Stat{__shfl_xor(a.m, off, 64), __shfl_xor(a.s, off, 64), __shfl_xor(a.u, off, 64)});
+    if ((threadIdx.x & 63) < R) { red[0][wave][r] = a.m; red[1][wave][r] = a.s; red[2][wave][r] = a.u; }
     __syncthreads();
-    if (g != 0) return;
+    if (threadIdx.x >= R) return;
     const int64_t t = n < rows ? target.of(n) : -1;
     const uint64_t word = __ballot(t != -1);
     float lp = 0.0f;
@@ -518,12 +602,15 @@ __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ pa
         lse[n] = z;
         classes[n] = t;
         live[n] = t == -1 ? 0 : 1;
-        if (r == 0) bits[blockIdx.x] = word;
+        if (r == 0) {
+            if (R == 64) bits[blockIdx.x] = word;
+            else ((uint16_t*)bits)[blockIdx.x] = (uint16_t)word;
+        }
     }
-    if (loss) {                                                     // (given where these are all the rows: at most 64)
+    if (loss) {                                                     // (given where these are all the rows)
         double sum = (double)lp;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        for (int off = R / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
         if (r == 0) {
             const int c = __popcll(word);
             const double d = mean ? (double)(c > 0 ? c : 1) : 1.0;
