@@ -129,7 +129,12 @@ def _run(tensors, out, max_norm, scale):
         dst = src if out is None else array("Q", map(_T.data_ptr, out))
         _lib.check(lib.q1env_grad_clip(dev, stream, n, p(src), p(dst), p(sizes), p(dtype), p(cols), p(sp), p(dp), scale, float(max_norm), norm.data_ptr(),
                                        buf.data_ptr(), nbytes))
-        torch.autograd.graph.increment_version(tensors if out is None else out)          # autograd has to know what was written
+        written = tensors if out is None else out
+        try:
+            torch.autograd.graph.increment_version(written)                              # autograd has to know what was written
+        except RuntimeError:
+            if not any(map(_T.is_inference, written)):                                   # (tensors made in inference mode have no version)
+                raise
     return norm
 
 

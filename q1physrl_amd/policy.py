@@ -189,6 +189,23 @@ class Q1Policy(nn.Module):
     def forward(self, obs):
         return self.pi(obs), self.vf(obs).squeeze(-1)
 
+    def evaluate_actions(self, obs, keys, mouse):
+        """(log-probability, entropy, value) of given actions (keys (B, K) 0/1, mouse (B,) step indices) of a policy with a discrete mouse, float32 (B,), without
+        the 2S+1 mouse logits of any sample being stored (q1physrl_amd.categorical): what Q1PhysActionDist(logits).logp / .entropy give, for heads
+        that are too wide to keep.  GPU only."""
+        if not self.allow_yaw or self.discrete_yaw_steps == -1:
+            raise ValueError("evaluate_actions is for a discrete mouse (discrete_yaw_steps != -1): the other action structures have a handful of logits")
+        from .categorical import linear_categorical
+        k2 = 2 * self.num_keys
+        hidden = self.pi[:-1](obs)
+        weight, bias = self.pi[-1].weight.to(hidden.dtype), self.pi[-1].bias.to(hidden.dtype)
+        key_logits = nn.functional.linear(hidden, weight[:k2], bias[:k2]).float()
+        logp, entropy = linear_categorical(hidden, weight[k2:], mouse.reshape(-1).long(), bias[k2:])
+        for k in range(self.num_keys):
+            c = Categorical2(key_logits[:, 2 * k:2 * k + 2])
+            logp, entropy = logp + c.logp(keys[:, k]), entropy + c.entropy()
+        return logp, entropy, self.vf(obs).squeeze(-1).float()
+
     def num_parameters(self):
         return sum(p.numel() for p in self.parameters())
 

@@ -44,19 +44,56 @@ def ppo_loss(policy, batch, action_range, clip_param, vf_clip_param, vf_loss_coe
     return total, stats
 
 
+def ppo_loss_logits_free(policy, batch, clip_param, vf_clip_param, vf_loss_coeff, entropy_coeff, kl_coeff, autocast_dtype=None):
+    """ppo_loss for a discrete mouse whose logits are never stored, neither the old policy's nor the new one's (Q1Policy.evaluate_actions).  The KL term, which
+    ppo_loss takes from both rows of logits, is estimated from the sampled actions instead: with r = pi_new(a) / pi_old(a), E_old[r - 1 - log r] = KL(old || new), every term
+    of it non-negative, and the same expected gradient."""
+    with torch.autocast("cuda", dtype=autocast_dtype, enabled=autocast_dtype is not None):
+        logp, entropy, value = policy.evaluate_actions(batch["obs"], batch["keys"], batch["mouse"])
+    log_ratio = logp - batch["logp"]
+    ratio = torch.exp(log_ratio)
+    adv = batch["adv"]
+    surrogate = torch.minimum(adv * ratio, adv * torch.clamp(ratio, 1.0 - clip_param, 1.0 + clip_param))
+    v_clipped = batch["value"] + torch.clamp(value - batch["value"], -vf_clip_param, vf_clip_param)
+    vf_loss = torch.maximum((value - batch["vtarg"]) ** 2, (v_clipped - batch["vtarg"]) ** 2)
+    kl = ratio - 1.0 - log_ratio
+    total = torch.mean(-surrogate + kl_coeff * kl + vf_loss_coeff * vf_loss - entropy_coeff * entropy)
+    stats = {"total_loss": total.detach(), "policy_loss": -surrogate.mean().detach(), "vf_loss": vf_loss.mean().detach(),
+             "kl": kl.mean().detach(), "entropy": entropy.mean().detach()}
+    return total, stats
+
+
 STAT_KEYS = ("entropy", "kl", "policy_loss", "total_loss", "vf_loss")      # sorted: the order of the stats vector
 
 
-def allreduce_grads_(params, world):
-    """Average gradients over ranks with ONE collective on a flat bucket."""
+def allreduce_grads_(params, world, grad_clip=None):
+    """Average gradients over ranks with ONE collective on a flat bucket; with grad_clip the averages are clipped by their global norm on the way back from
+    the bucket.  Returns the norm of the averaged gradients (before clipping) where grad_clip is given."""
     grads = [p.grad for p in params if p.grad is not None]
     flat = torch.cat([g.reshape(-1) for g in grads])
     dist.all_reduce(flat, op=dist.ReduceOp.SUM)
+    if grad_clip is not None and flat.is_cuda:
+        from .clip import clip_grad_norm_
+        return clip_grad_norm_([v.view(g.shape) for v, g in zip(flat.split([g.numel() for g in grads]), grads)], grad_clip, scale=1.0 / world, out=grads)
     flat /= world
     off = 0
     for g in grads:
         g.copy_(flat[off:off + g.numel()].view_as(g))
         off += g.numel()
+    return None if grad_clip is None else clip_grads_(params, grad_clip)
+
+
+def clip_grads_(params, grad_clip):
+    """RLlib's grad_clip (tf.clip_by_global_norm): gradients scaled in place by min(1, grad_clip / global norm); returns the norm as a device scalar.  On the GPU one
+    kernel per pass over all of them (q1physrl_amd.clip); parameters on the CPU, where the learner runs in tests, take the formula as it stands."""
+    grads = [p.grad for p in params if p.grad is not None]
+    if grads[0].is_cuda:
+        from .clip import clip_grad_norm_
+        return clip_grad_norm_(grads, grad_clip)
+    norm = torch.sqrt(sum((g.double() ** 2).sum() for g in grads)).float()
+    for g in grads:
+        g.mul_(grad_clip / torch.clamp(norm, min=grad_clip))
+    return norm
 
 
 class NativeStep:
@@ -201,6 +238,12 @@ class PPOLearner:
     fused_loss:  the loss and its gradient w.r.t. (logits, value) come from ONE HIP kernel (q1env_ppo_loss_grad, closed-form
                  derivatives) instead of ~100 elementwise torch launches and their autograd twins; torch autograd only runs the
                  two MLPs.  Needs `env` (a TensorVectorEnv: its handle supplies num_keys / action_range and the stream).
+    grad_clip:   RLlib's option of that name (unset in the reference's trainer config): the gradients of a step are clipped by their global norm before the
+                 optimizer; self.grad_norm holds the last step's norm (a device scalar).  With native=True the optimizer is then torch's, as with several
+                 processes (the library's own step goes from gradient sums to new weights in one kernel).
+    logits_free: for a discrete mouse with many steps: the loss takes log-probability and entropy of the sampled actions from the network's hidden layer and
+                 last weights (Q1Policy.evaluate_actions) and estimates the KL from them, so that no (samples x 2S+1) array exists; GPU only, not with
+                 native / fused_loss (their kernels walk stored logits) or use_graph (the head's differentiable form cannot be captured).
     native:      the WHOLE step up to the gradients - minibatch gather, both MLPs forward and backward, the loss gradient, the weight
                  gradients - is the library's own gfx950 kernels (NativeStep / q1env_learner_step: float16 matrix-core operands,
                  float32 accumulation and master weights); torch only runs the (fused) Adam.  Needs `env`; implies the fused loss.
@@ -210,7 +253,7 @@ class PPOLearner:
                  vf_loss_coeff=1.0, entropy_coeff=0.01, kl_coeff=0.2, kl_target=0.0036, num_sgd_iter=30,
                  minibatch_size=128, num_keys=4, seed=0, use_graph=False, fused_loss=False, env=None, discrete_yaw_steps=-1,
                  allow_yaw=True, autocast_dtype=None, fused_adam=False, native=False, native_splits=32, native_adam=True, persistent=None,
-                 dynamic_loss_scale=False, precision="f16"):
+                 dynamic_loss_scale=False, precision="f16", grad_clip=None, logits_free=False):
         self.policy = policy
         self.action_range = float(action_range)
         self.gamma, self.lam = gamma, lam
@@ -222,7 +265,15 @@ class PPOLearner:
         self.world = dist.get_world_size() if dist.is_available() and dist.is_initialized() else 1
         self.use_graph = bool(use_graph) and self.world == 1
         self.fused_loss, self.env = bool(fused_loss), env
-        self.native, self.native_splits, self.native_adam = bool(native), int(native_splits), bool(native_adam)
+        if grad_clip is not None and not float(grad_clip) > 0.0:
+            raise ValueError("grad_clip must be positive")
+        self.grad_clip, self.grad_norm = None if grad_clip is None else float(grad_clip), None
+        self.logits_free = bool(logits_free)
+        if self.logits_free and (not allow_yaw or discrete_yaw_steps == -1):
+            raise ValueError("logits_free=True is for a discrete mouse (discrete_yaw_steps != -1)")
+        if self.logits_free and (native or fused_loss or use_graph):
+            raise ValueError("logits_free=True cannot be combined with native, fused_loss or use_graph")
+        self.native, self.native_splits, self.native_adam = bool(native), int(native_splits), bool(native_adam) and grad_clip is None
         # persistent: the whole update (num_sgd_iter epochs of 128-sample minibatches) as ONE dispatch (NativeStep.epochs); None = whenever
         # the shape allows it (native, own Adam, single process, minibatch 128, the reference's action structure)
         self.persistent = persistent
@@ -285,7 +336,7 @@ class PPOLearner:
         keys = ((traj["keys"].reshape(-1, 1).long() >> torch.arange(self.num_keys, device=adv.device)) & 1)
         return {"obs": traj["obs"][:t].reshape(t * n, 6), "keys": keys, "keys_packed": traj["keys"].reshape(-1),
                 "mouse": traj["mouse"].reshape(-1, 1), "logp": traj["logp"].reshape(-1), "value": traj["value"][:t].reshape(-1),
-                "adv": adv.reshape(-1), "vtarg": vtarg.reshape(-1), "old_logits": old_logits}
+                "adv": adv.reshape(-1), "vtarg": vtarg.reshape(-1), **({} if old_logits is None else {"old_logits": old_logits})}
 
     def _sgd_step(self, mb):
         """One minibatch: forward, loss, backward, (gradient all-reduce,) Adam.  Returns the stats vector (STAT_KEYS order).
@@ -300,8 +351,7 @@ class PPOLearner:
                                   skip_reduce=True, use_cursor=True, adam=(g["lr"], g["betas"], g["eps"]))
                 return None
             stats = self._native.step(self._full, self._idx, self.clip_param, self.vf_clip_param, self.vf_loss_coeff, self.entropy_coeff, self._klc)
-            if self.world > 1:
-                allreduce_grads_([p for p in self.policy.parameters()], self.world)
+            self._reduce_and_clip()
             self.opt.step()
             self._native.images()
             return stats
@@ -327,6 +377,12 @@ class PPOLearner:
             self.opt.zero_grad(set_to_none=True)
             torch.autograd.backward([logits, value], [dlogits, dvalue])
             stats = partials.sum(dim=0) / bsz
+        elif self.logits_free:
+            loss, st = ppo_loss_logits_free(self.policy, mb, self.clip_param, self.vf_clip_param, self.vf_loss_coeff, self.entropy_coeff, self._klc,
+                                            autocast_dtype=self.autocast_dtype)
+            self.opt.zero_grad(set_to_none=True)
+            loss.backward()
+            stats = torch.stack([st[k].float() for k in STAT_KEYS])
         else:
             loss, st = ppo_loss(self.policy, mb, self.action_range, self.clip_param, self.vf_clip_param, self.vf_loss_coeff,
                                 self.entropy_coeff, self._klc, self.num_keys, self.discrete_yaw_steps, self.allow_yaw,
@@ -334,10 +390,16 @@ class PPOLearner:
             self.opt.zero_grad(set_to_none=True)
             loss.backward()
             stats = torch.stack([st[k].float() for k in STAT_KEYS])
-        if self.world > 1:
-            allreduce_grads_([p for p in self.policy.parameters()], self.world)
+        self._reduce_and_clip()
         self.opt.step()
         return stats
+
+    def _reduce_and_clip(self):
+        params = list(self.policy.parameters())
+        if self.world > 1:
+            self.grad_norm = allreduce_grads_(params, self.world, self.grad_clip)
+        elif self.grad_clip is not None:
+            self.grad_norm = clip_grads_(params, self.grad_clip)
 
     def _capture(self, b, mb, dev):
         """Capture one SGD step on static minibatch buffers into a hipGraph (warm-up on a side stream first; the warm-up and
@@ -468,7 +530,9 @@ class PPOLearner:
         """SGD epochs over one trajectory batch; adv/vtarg from q1env_gae.  Returns averaged stats (python floats)."""
         dev = adv.device
         t, n = traj["reward"].shape
-        if "logits" in traj:                    # the behaviour policy's own outputs (exact even when sampling ran in bf16)
+        if self.logits_free:
+            old_logits = None
+        elif "logits" in traj:                  # the behaviour policy's own outputs (exact even when sampling ran in bf16)
             old_logits = traj["logits"].reshape(t * n, -1)
         else:
             with torch.no_grad():
@@ -504,7 +568,7 @@ class PPOLearner:
         own_adam = self.native and self.world == 1 and self.native_adam
         use_persistent = bool(own_adam and self.persistent is not False and self._native.persistent_ok() and total >= mb)
         if (self.persistent is True or self.precision == "f32") and not use_persistent:
-            raise ValueError("PPOLearner(persistent=True / precision='f32') needs native=True, native_adam=True, one process, minibatch_size 128 and the reference's action structure")
+            raise ValueError("PPOLearner(persistent=True / precision='f32') needs native=True, native_adam=True, one process, minibatch_size 128, the reference's action structure and no grad_clip")
         # lr / betas / eps are kernel ARGUMENTS of the native Adam, baked into a captured graph: a changed param_group re-captures
         if self.native:
             self.env._dev.learner_set_loss_scale(self.pi_upscale, self.value_downscale)

@@ -156,6 +156,19 @@ def test_captured_and_replayed_and_side_streams():
 
 
 @gpu
+def test_autograd_learns_of_the_write_and_inference_tensors_are_taken():
+    x = torch.randn(10, device="cuda", requires_grad=True)
+    y = x * 2
+    z = y.exp()                                                     # saves its result
+    clip.clip_grad_norm_([z.detach()], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        z.sum().backward()
+    with torch.inference_mode():
+        g = torch.full((16,), 2.0, device="cuda")
+        assert float(clip.clip_grad_norm_([g], 4.0)) == 8.0 and bool((g == 1.0).all())
+
+
+@gpu
 def test_the_same_tensor_twice_and_overlaps_are_refused():
     g = torch.randn(100, device="cuda")
     with pytest.raises(_lib.Q1EnvError, match="overlap"):

@@ -43,6 +43,8 @@ ap.add_argument("--native", action="store_true", help="native learner step: gath
 ap.add_argument("--native-splits", type=int, default=32, help="workgroups per network of the split-K weight-gradient kernel")
 ap.add_argument("--save", default="", help="write the final policy weights (npz, RLlib fcnet naming) here")
 ap.add_argument("--discrete-yaw-steps", type=int, default=-1, help="Config.discrete_yaw_steps: the mouse becomes Discrete(2S+1) (a Categorical policy head)")
+ap.add_argument("--grad-clip", type=float, default=0.0, help="clip the gradients by their global norm (RLlib's grad_clip; 0 = off, as in the reference's config)")
+ap.add_argument("--logits-free", action="store_true", help="with --discrete-yaw-steps: the loss without stored mouse logits (PPOLearner(logits_free=True)); the learner then runs without a graph")
 ap.add_argument("--refcfg", action="store_true",
                 help="the REFERENCE's training configuration (VERDICT r3 item 5): data/params.yml trainer_config (lr 5e-6, train_batch_size 50 000, "
                      "kl_target 0.0036, entropy 0.01, gamma 0.99, lambda 0.95, vf_clip 100) and env_config (params.yml:16-33), RLlib 0.8.4 PPO defaults "
@@ -92,10 +94,11 @@ fused = P.FusedPolicyForward(pol, env) if args.fused_policy else None
 smp = GpuSampler(env, fused if fused is not None else pol, horizon=args.horizon, use_graph=not args.no_graph, resident=args.resident)
 env._dev.learner_set_step_mode(args.step_mode)
 lrn = ppo.PPOLearner(pol, float(cfg.action_range), lr=args.lr, num_sgd_iter=args.epochs, minibatch_size=args.minibatch,
-                     entropy_coeff=args.entropy, kl_target=args.kl_target, seed=args.seed + rank, use_graph=not args.no_graph, fused_loss=args.fused_loss, env=env,
+                     entropy_coeff=args.entropy, kl_target=args.kl_target, seed=args.seed + rank, use_graph=not args.no_graph and not args.logits_free, fused_loss=args.fused_loss, env=env,
                      discrete_yaw_steps=args.discrete_yaw_steps, autocast_dtype=torch.bfloat16 if args.learner_bf16 else None, fused_adam=not args.no_fused_adam,
                      native=args.native, native_splits=args.native_splits, persistent=False if args.no_persistent else None,
-                     dynamic_loss_scale=args.dynamic_loss_scale, precision="f32" if args.learner_fp32 else "f16")
+                     dynamic_loss_scale=args.dynamic_loss_scale, precision="f32" if args.learner_fp32 else "f16",
+                     grad_clip=args.grad_clip or None, logits_free=args.logits_free)
 log = []
 start_iter, best_metric, best_file = 0, float("-inf"), None
 
