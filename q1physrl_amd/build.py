@@ -41,8 +41,7 @@ TU_FLAGS = {"q1env_learner.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
             # optimizer: that pass rewrites a uniform-address atomic into a wave reduction + s_waitcnt vmcnt(0) + readfirstlane, i.e. it
             # makes the barrier poll that is requested early and looked at late (q1learner_persist.hpp, barrier 3) synchronous again
             # the training operators: without the packed float32 instructions, which the compiler otherwise forms from ordinary float code
-            "q1env_head.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
-            "q1env_clip.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
+            **{"q1env_%s.hip" % u: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for u in ("head", "head_f32", "head_bf16", "head_f16", "clip")},
             "q1env_plearner.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]}
 LINK_FLAGS = ["--offload-arch=gfx950", "-shared", "-fPIC"]
 HIPCC_FLAGS = COMPILE_FLAGS + ["-shared"]     # (kept for tools that compile a single file the old way, e.g. tools/asan_check.sh)

@@ -1,146 +1,10 @@
 // q1env_head.hip - the wide categorical head of libq1env.so (include/q1env.h q1env_head_*): log-probability, entropy and cross entropy of given
-// classes from hidden rows and the head's weights without the logits ever being kept, and the gradients (kernels: q1head.hpp).
-#include "q1env_host.hpp"
-#include "q1head.hpp"
-
-#include <algorithm>
-#include <atomic>
+// classes from hidden rows and the head's weights without the logits ever being kept, and the gradients (kernels: q1head.hpp, what runs when: q1head_calls.hpp).
+#include "q1head_calls.hpp"
 
 using namespace q1head;
 
 namespace {
-
-constexpr uint64_t PIECE_BYTES = 448ull << 20;     // of the gradient of one piece of the classes
-constexpr uint64_t LAID_BYTES = 96ull << 20;       // of the laid-out weights of one piece
-constexpr int64_t MAX_ROWS = 1 << 22, MAX_WIDTH = 1 << 16, MAX_CLASSES = 1 << 22;
-constexpr int64_t PIECE_STEP = 256;                // pieces are whole tiles of every configuration
-
-typedef Config<256, 256, 2, 4, 64, 2> Large;           // 128 KB of LDS: one workgroup of eight waves per CU
-typedef Config<128, 128, 2, 2, 64, 2> Middle;          // 64 KB: two workgroups of four waves per CU, one computes while the other waits
-typedef Config<64, 64, 2, 2, 64, 4> Small;         // where Middle's tiles would leave most CUs idle: 64 KB, four steps in flight
-typedef Config<128, 64, 4, 1, 64, 3> Few;              // up to 64 rows: 72 KB, two workgroups per CU
-typedef Config<128, 32, 4, 1, 64, 4> Fewest;           // up to 32 rows: 80 KB, two workgroups per CU
-
-int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int64_t round_up(int64_t a, int64_t b) { return div_up(a, b) * b; }
-uint64_t aligned(uint64_t x) { return (x + 255) & ~255ull; }
-size_t elem_size(int dt) { return dt == F32 ? 4 : 2; }
-int planes_of(int dt) { return dt == F32 ? 3 : 1; }
-
-// the forward pass's results as the backward pass reads them (q1env_head_state_bytes)
-struct State {
-    float *lse, *entropy, *each;
-    int64_t* target;
-    uint8_t* live;
-    uint64_t* bits;
-    static uint64_t bytes(int64_t n) { return 2 * aligned(4 * n) + aligned(8 * n) + aligned(n) + aligned(8 * div_up(n, 64)) + 256; }
-    State(void* p, int64_t n) {
-        char* c = (char*)p;
-        lse = (float*)c; c += aligned(4 * n);
-        entropy = (float*)c; c += aligned(4 * n);
-        target = (int64_t*)c; c += aligned(8 * n);
-        live = (uint8_t*)c; c += aligned(n);
-        bits = (uint64_t*)c; c += aligned(8 * div_up(n, 64));
-        each = (float*)c;
-    }
-};
-
-enum Size { LARGE, MIDDLE, SMALL, FEW, FEWEST };
-int64_t bm_of(Size s) { return s == LARGE ? 256 : s == SMALL ? 64 : 128; }
-int64_t bn_of(Size s) { return s == LARGE ? 256 : s == MIDDLE ? 128 : s == FEWEST ? 32 : 64; }
-
-// The tile of a product of m x n results with k terms, and into how many parts its sum is split, by what it should take in nanoseconds.  One round of Large workgroups (256,
-// one per CU) was measured at 31 ns per term of k (1075 TFLOP/s), one of Middle (512, two per CU) at 18 (930); `start` is what a round costs besides (prologue and epilogue: 3.3 / 2.5 us for the
-// statistics, 12 / 7 for the gradient, at 50000 x 256 x 4097); the slabs of a split sum are written and read once at 4.5 TB/s.  `split` false: one part only.
-struct Shape { Size size; int parts; int64_t len; };
-Shape shape_of(int64_t m, int64_t n, int64_t k, int products, bool split, double start_large, double start_middle, bool k_major) {
-    if (n <= 64 && !k_major) {                        // few rows: 512 workgroups (two per CU), parts of 512 terms at least
-        const Size s = n <= 32 ? FEWEST : FEW;
-        const int64_t tiles = div_up(m, bm_of(s));
-        int64_t parts = split ? std::max<int64_t>(1, std::min(div_up(512, tiles), div_up(k, 512))) : 1;
-        const int64_t len = round_up(div_up(k, parts), PART_STEP);
-        return Shape{s, (int)div_up(k, len), len};
-    }
-    Shape best{MIDDLE, 1, round_up(k, PART_STEP)};
-    double least = 0.0;
-    for (int s = LARGE; s <= SMALL; ++s) {
-        const int64_t tiles = div_up(m, bm_of((Size)s)) * div_up(n, bn_of((Size)s)), slots = s == LARGE ? 256 : 512;
-        const double start = s == LARGE ? start_large : s == MIDDLE ? start_middle : start_middle / 2;
-        const int64_t most = split ? std::min<int64_t>(div_up(k, 256), std::max<int64_t>(1, div_up(4 * slots, tiles))) : 1;
-        for (int64_t parts = 1; parts <= most; ++parts) {
-            const int64_t len = round_up(div_up(k, parts), PART_STEP), real = div_up(k, len), groups = tiles * real;
-            // a term of k of one round; of a round that leaves every workgroup a CU to itself
-            const double full = s == LARGE ? 31.0 : s == MIDDLE ? 18.0 : 9.5, alone = s == LARGE ? 31.0 : s == MIDDLE ? 11.0 : 5.0;
-            double t = (double)div_up(groups, slots) * ((double)len * products * (groups <= 256 ? alone : full) + start);
-            if (real > 1) t += 3000.0 + (double)real * (double)m * (double)n * 8.0 / 4500.0;
-            if (least == 0.0 || t < least) { least = t; best = Shape{(Size)s, (int)real, len}; }
-        }
-    }
-    return best;
-}
-
-bool in_place(int dt, const void* p, int64_t stride, int64_t width) {       // whether the loads can take an operand as it lies
-    return dt != F32 && ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && width % 8 == 0 && stride < (1 << 21);
-}
-
-struct Plan {
-    int64_t padded;                    // width of laid-out rows
-    int64_t piece;                     // classes per piece
-    int64_t pieces;
-    Size logits, dh, dw;
-    int dh_split, dw_split;
-    int64_t dh_k, dw_k;                // classes / rows per split
-    bool few;                          // the forward pass of up to 32 float32 rows (few_rows_kernel)
-    int64_t tiles;                     // partial statistics per row
-    uint64_t part, own, scale, g, db, dh_slab, dw_slab, h_laid, w_laid;        // byte offsets in the workspace
-    uint64_t bytes;
-};
-
-// w_in_place / h_in_place: the workspace has to suffice for any address, so its size is asked for with both false
-Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward, bool h_in_place, bool w_in_place) {
-    Plan p{};
-    p.few = !backward && dt == F32 && rows <= 32;
-    if (p.few) h_in_place = w_in_place = true;
-    p.padded = round_up(width, 64);
-    const int64_t all = round_up(classes, PIECE_STEP);
-    int64_t piece = all;
-    const int64_t laid = planes_of(dt) * 2 * p.padded;                        // bytes of a laid-out row
-    if (!w_in_place) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(LAID_BYTES / laid) / PIECE_STEP * PIECE_STEP));
-    if (backward) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(PIECE_BYTES / (2 * planes_of(dt) * rows)) / PIECE_STEP * PIECE_STEP));
-    p.piece = piece;
-    p.pieces = div_up(classes, piece);
-    const int products = planes_of(dt) == 3 ? 6 : 1;
-    p.logits = shape_of(std::min(piece, classes), rows, width, products, false, backward ? 12000.0 : 3300.0, backward ? 7000.0 : 2500.0, false).size;
-    uint64_t at = 0;
-    auto take = [&](uint64_t n) { const uint64_t o = at; at += aligned(n); return o; };
-    if (!backward) {
-        p.own = take(4 * rows);
-        p.tiles = p.few ? std::min<int64_t>(div_up(classes, 32), 2048) : div_up(classes, bm_of(p.logits));
-        p.part = take(12 * (uint64_t)p.tiles * rows);
-    } else {
-        const Shape dh = shape_of(width, rows, std::min(piece, classes), products, true, 4000.0, 3000.0, false);
-        const Shape dw = shape_of(width, std::min(piece, classes), rows, products, true, 4000.0, 3000.0, true);
-        p.dh = dh.size; p.dh_split = dh.parts; p.dh_k = dh.len;
-        p.dw = dw.size; p.dw_split = dw.parts; p.dw_k = dw.len;
-        p.scale = take(256);
-        p.g = take(2 * (uint64_t)planes_of(dt) * rows * piece);
-        p.db = take(4 * (uint64_t)div_up(rows, bn_of(p.logits)) * classes);
-        p.dh_slab = take(p.dh_split > 1 || p.pieces > 1 ? 4 * (uint64_t)p.dh_split * rows * width : 0);
-        p.dw_slab = take(p.dw_split > 1 ? 4 * (uint64_t)p.dw_split * piece * width : 0);
-    }
-    p.h_laid = take(h_in_place ? 0 : (uint64_t)laid * rows);
-    p.w_laid = take(w_in_place ? 0 : (uint64_t)laid * piece);
-    p.bytes = at;
-    return p;
-}
-
-// what a workspace has to hold whatever the operands' addresses and strides are
-uint64_t workspace_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward) {
-    uint64_t n = plan_of(dt, rows, width, classes, backward, false, false).bytes;
-    if (dt != F32 && width % 8 == 0)                                          // pieces differ: either may need more
-        n = std::max(n, plan_of(dt, rows, width, classes, backward, false, true).bytes);
-    return n;
-}
 
 int check_shape(const char* who, int dtype, int64_t rows, int64_t width, int64_t classes) {
     if (dtype != Q1ENV_DT_F32 && dtype != Q1ENV_DT_BF16 && dtype != Q1ENV_DT_F16) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": unknown dtype");
@@ -167,194 +31,6 @@ int guard_device(const char* who, int device) {
     if (hipGetDeviceCount(&n) != hipSuccess || n == 0) return fail(Q1ENV_ERR_NO_DEVICE, std::string(who) + ": no HIP device (there is no CPU fallback)");
     if (device < 0 || device >= n) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": no such device");
     return 0;
-}
-
-template <class C, auto KERNEL, typename... A> int go(hipStream_t stream, int device, int64_t workgroups, A... args) {
-    if (workgroups <= 0 || workgroups > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
-    static std::atomic<uint64_t> done{0};
-    const uint64_t bit = 1ull << (device & 63);
-    if (C::LDS_BYTES > 65536 && (device > 63 || !(done.load(std::memory_order_relaxed) & bit))) {        // more than 64 KB of LDS has to be allowed once per kernel and device
-        HIP_TRY(hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES));
-        done.fetch_or(bit, std::memory_order_relaxed);
-    }
-    hipLaunchKernelGGL(KERNEL, dim3((unsigned)workgroups), dim3(C::THREADS), C::LDS_BYTES, stream, args...);
-    HIP_TRY(hipGetLastError());
-    return 0;
-}
-#define Q1_TRY(expr) do { if (int rc_ = (expr)) return rc_; } while (0)
-
-struct Where { hipStream_t stream; int device; };
-
-template <class C, int DT> int statistics(const Where& at, Head hd, const Target& target, bool entropy, float* part, float* own) {
-    hd.tiles_m = (uint32_t)div_up(hd.c1 - hd.c0, C::BM);
-    hd.tiles_n = (uint32_t)div_up(hd.rows, C::BN);
-    const int64_t workgroups = (int64_t)hd.tiles_m * hd.tiles_n;
-    return entropy ? go<C, statistics_kernel<C, DT, true>>(at.stream, at.device, workgroups, hd, target, hd.c0 / C::BM, part, own)
-                   : go<C, statistics_kernel<C, DT, false>>(at.stream, at.device, workgroups, hd, target, hd.c0 / C::BM, part, own);
-}
-template <class C, int DT> int gradient(const Where& at, Head hd, const Upstream& up, int64_t piece, const State& st, uint16_t* g, float* db) {
-    hd.tiles_m = (uint32_t)div_up(hd.c1 - hd.c0, C::BM);
-    hd.tiles_n = (uint32_t)div_up(hd.rows, C::BN);
-    const int64_t workgroups = (int64_t)hd.tiles_m * hd.tiles_n, plane = hd.rows * piece;
-    const float *lse = st.lse, *entropy = st.entropy;
-    return up.dentropy ? go<C, gradient_kernel<C, DT, true>>(at.stream, at.device, workgroups, hd, up, piece, plane, lse, entropy, g, db)
-                       : go<C, gradient_kernel<C, DT, false>>(at.stream, at.device, workgroups, hd, up, piece, plane, lse, entropy, g, db);
-}
-// workgroups of a product in C's tiles
-template <class C> int64_t tiles_of(Product& pr, int splits) {
-    pr.tiles_m = (uint32_t)div_up(pr.width, C::BM);
-    pr.tiles_n = (uint32_t)div_up(pr.rows, C::BN);
-    return (int64_t)pr.tiles_m * pr.tiles_n * splits;
-}
-// dw and dh may each be absent (null out)
-template <class C, int DT> int products(const Where& at, Product dw, int dw_split, Product dh, int dh_split, const Upstream& up) {
-    const int64_t a = dw.out ? tiles_of<C>(dw, dw_split) : 0, b = dh.out ? tiles_of<C>(dh, dh_split) : 0, padded = b > 0 ? round_up(a, 8) : a;
-    if (a > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
-    return a + b == 0 ? 0 : go<C, products_kernel<C, DT>>(at.stream, at.device, padded + b, dw, dh, up, (uint32_t)a, (uint32_t)padded);
-}
-template <class C, int DT> int rows_product(const Where& at, Product dh, int dh_split, const Upstream& up) {
-    const int64_t groups = tiles_of<C>(dh, dh_split);
-    return go<C, rows_product_kernel<C, DT>>(at.stream, at.device, groups, dh, up);
-}
-
-// lays out what has rows, in one launch
-template <int DT> int lay_out(const Where& at, Lay a, Lay b, int64_t width, int64_t padded) {
-    const int64_t ga = div_up(a.rows * padded, 2048), gb = div_up(b.rows * padded, 2048);
-    if (ga + gb == 0) return 0;
-    if (ga + gb > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many values");
-    a.groups = (uint32_t)ga;
-    b.groups = (uint32_t)gb;
-    hipLaunchKernelGGL((lay_out_kernel<DT>), dim3((unsigned)(ga + gb)), dim3(256), 0, at.stream, a, b, width, padded);
-    HIP_TRY(hipGetLastError());
-    return 0;
-}
-
-// an operand of `rows` rows, as it lies or laid out at `laid` (then the rows have been laid out already)
-Op rows_op(int dt, bool as_it_lies, const void* p, int64_t stride, int64_t rows, int64_t width, int64_t padded, const void* laid) {
-    if (as_it_lies) return Op{(const char*)p, 2 * stride, 0, rows, width, nullptr};
-    return Op{(const char*)laid, 2 * padded, 2 * rows * padded, rows, padded, nullptr};
-}
-// the same memory with the rows as the k of a product
-Op turned(const Op& o, const uint64_t* live) { return Op{o.p, o.stride, o.plane, o.k_extent, o.x_extent, live}; }
-
-template <int DT>
-int forward(const Where& at, const q1env_head& q, int reduction, float* logp, float* entropy, float* loss) {
-    const int64_t n = q.rows;
-    const int mean = reduction == Q1ENV_REDUCE_MEAN ? 1 : 0;
-    State st(q.state_dev, n);
-    if (n > 0) {
-        const bool hp = in_place(DT, q.hidden_dev, q.hidden_stride, q.width), wp = in_place(DT, q.weight_dev, q.weight_stride, q.width);
-        const Plan p = plan_of(DT, n, q.width, q.classes, false, hp, wp);
-        char* ws = (char*)q.ws_dev;
-        const Target target{q.target_dev, q.target_bits == 64 ? 1 : 0, q.ignore_index, q.classes};
-        const Op h = rows_op(DT, hp, q.hidden_dev, q.hidden_stride, n, q.width, p.padded, ws + p.h_laid);
-        float *part = (float*)(ws + p.part), *own = (float*)(ws + p.own);
-        if (p.few) {
-            auto vec = [](const void* x, int64_t stride) { return ((uintptr_t)x & 15) == 0 && stride % 4 == 0 ? 1 : 0; };
-            const float *w = (const float*)q.weight_dev, *x = (const float*)q.hidden_dev;
-            if (entropy) hipLaunchKernelGGL((few_rows_kernel<true>), dim3((unsigned)p.tiles), dim3(256), 0, at.stream, w, q.weight_stride, vec(w, q.weight_stride), x, q.hidden_stride,
-                                            vec(x, q.hidden_stride), (const float*)q.bias_dev, target, (int)n, q.width, part, own);
-            else hipLaunchKernelGGL((few_rows_kernel<false>), dim3((unsigned)p.tiles), dim3(256), 0, at.stream, w, q.weight_stride, vec(w, q.weight_stride), x, q.hidden_stride,
-                                    vec(x, q.hidden_stride), (const float*)q.bias_dev, target, (int)n, q.width, part, own);
-            HIP_TRY(hipGetLastError());
-        }
-        for (int64_t c0 = 0; c0 < q.classes && !p.few; c0 += p.piece) {
-            const int64_t c1 = std::min(c0 + p.piece, q.classes);
-            const char* w0 = (const char*)q.weight_dev + elem_size(DT) * c0 * q.weight_stride;
-            Q1_TRY(lay_out<DT>(at, Lay{q.hidden_dev, q.hidden_stride, hp || c0 > 0 ? 0 : n, nullptr, (uint16_t*)(ws + p.h_laid), 0},
-                               Lay{w0, q.weight_stride, wp ? 0 : c1 - c0, nullptr, (uint16_t*)(ws + p.w_laid), 0}, q.width, p.padded));
-            const Head hd{rows_op(DT, wp, w0, q.weight_stride, c1 - c0, q.width, p.padded, ws + p.w_laid), h, q.bias_dev, nullptr, n, q.width, q.classes, 0, 0, c0, c1};
-            const bool e = entropy != nullptr;
-            if (p.logits == LARGE) Q1_TRY((statistics<Large, DT>(at, hd, target, e, part, own)));
-            else if (p.logits == MIDDLE) Q1_TRY((statistics<Middle, DT>(at, hd, target, e, part, own)));
-            else if (p.logits == SMALL) Q1_TRY((statistics<Small, DT>(at, hd, target, e, part, own)));
-            else if (p.logits == FEW) Q1_TRY((statistics<Few, DT>(at, hd, target, e, part, own)));
-            else Q1_TRY((statistics<Fewest, DT>(at, hd, target, e, part, own)));
-        }
-        const bool tall = p.tiles > 64 && n <= 4096;                          // many tiles of few rows
-        float* here = n <= (tall ? 16 : 64) ? loss : nullptr;                 // one workgroup joins all the rows: it has the loss too
-        if (tall)
-            hipLaunchKernelGGL((join_kernel<16>), dim3((unsigned)div_up(n, 16)), dim3(1024), 0, at.stream, part, own, target, n, (int)p.tiles, entropy ? 1 : 0, logp, entropy, st.entropy,
-                               st.lse, st.target, st.live, st.bits, mean, here, st.each);
-        else
-            hipLaunchKernelGGL((join_kernel<64>), dim3((unsigned)div_up(n, 64)), dim3(1024), 0, at.stream, part, own, target, n, (int)p.tiles, entropy ? 1 : 0, logp, entropy, st.entropy,
-                               st.lse, st.target, st.live, st.bits, mean, here, st.each);
-        HIP_TRY(hipGetLastError());
-        if (here) return Q1ENV_OK;
-    }
-    if (loss) {
-        hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, at.stream, logp, st.live, n, mean, loss, st.each);
-        HIP_TRY(hipGetLastError());
-    }
-    return Q1ENV_OK;
-}
-
-template <int DT>
-int backward(const Where& at, const q1env_head& q, Upstream up, void* dh, int64_t dh_stride, void* dw, int64_t dw_stride, void* db) {
-    const int64_t n = q.rows, v = q.classes, d = q.width;
-    const bool hp = in_place(DT, q.hidden_dev, q.hidden_stride, d), wp = in_place(DT, q.weight_dev, q.weight_stride, d);
-    const Plan p = plan_of(DT, n, d, v, true, hp, wp);
-    State st(q.state_dev, n);
-    char* ws = (char*)q.ws_dev;
-    float* db_part = db ? (float*)(ws + p.db) : nullptr;
-    up.each = up.dloss ? st.each : nullptr;
-    up.f16 = DT == F16;
-    if (DT == F16 && !up.dloss) {
-        hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, at.stream, up, st.live, n, (float*)(ws + p.scale));
-        HIP_TRY(hipGetLastError());
-        up.table = (const float*)(ws + p.scale);
-    }
-    const Op h = rows_op(DT, hp, q.hidden_dev, q.hidden_stride, n, d, p.padded, ws + p.h_laid);
-    uint16_t* g = (uint16_t*)(ws + p.g);
-    float *dh_slab = p.dh_split > 1 || p.pieces > 1 ? (float*)(ws + p.dh_slab) : nullptr, *dw_slab = p.dw_split > 1 ? (float*)(ws + p.dw_slab) : nullptr;
-    const int64_t es = (int64_t)elem_size(DT);
-    // 16-byte stores of a result: address, stride, and for 16-bit types whole chunks of 8 columns; four values at a time from a slab
-    auto wide = [&](const void* out, int64_t stride, const float* slab) { return slab ? d % 4 == 0 : ((uintptr_t)out & 15) == 0 && stride * es % 16 == 0 && (es == 4 || d % 8 == 0); };
-    auto four = [&](const void* out, int64_t stride) { return d % 4 == 0 && stride % 4 == 0 && (uintptr_t)out % (4 * es) == 0; };
-    for (int64_t c0 = 0; c0 < v; c0 += p.piece) {
-        const int64_t c1 = std::min(c0 + p.piece, v), len = c1 - c0;
-        const bool last = c1 == v;
-        const char* w0 = (const char*)q.weight_dev + es * c0 * q.weight_stride;
-        Q1_TRY(lay_out<DT>(at, Lay{q.hidden_dev, q.hidden_stride, hp || c0 > 0 ? 0 : n, st.live, (uint16_t*)(ws + p.h_laid), 0},
-                           Lay{w0, q.weight_stride, wp ? 0 : len, nullptr, (uint16_t*)(ws + p.w_laid), 0}, d, p.padded));
-        const Op w = rows_op(DT, wp, w0, q.weight_stride, len, d, p.padded, ws + p.w_laid);
-        const Head hd{w, h, q.bias_dev, st.target, n, d, v, 0, 0, c0, c1};
-        if (p.logits == LARGE) Q1_TRY((gradient<Large, DT>(at, hd, up, p.piece, st, g, db_part)));
-        else if (p.logits == MIDDLE) Q1_TRY((gradient<Middle, DT>(at, hd, up, p.piece, st, g, db_part)));
-        else if (p.logits == SMALL) Q1_TRY((gradient<Small, DT>(at, hd, up, p.piece, st, g, db_part)));
-        else if (p.logits == FEW) Q1_TRY((gradient<Few, DT>(at, hd, up, p.piece, st, g, db_part)));
-        else Q1_TRY((gradient<Fewest, DT>(at, hd, up, p.piece, st, g, db_part)));
-        const Op gr{(const char*)g, 2 * p.piece, 2 * n * p.piece, n, round_up(len, PART_STEP), nullptr};         // [row][class of the piece]
-        Op gt = turned(gr, nullptr);
-        gt.x_extent = round_up(len, 8);
-        Product pw{turned(h, hp ? st.bits : nullptr), gt, n, p.dw_k, len, d, 0, 0, dw ? (char*)dw + es * c0 * dw_stride : nullptr, dw_stride, 0, dw_slab, 0, nullptr};
-        Product ph{turned(w, nullptr), gr, len, p.dh_k, n, d, 0, 0, dh, dh_stride, 0, dh_slab, c0 > 0 ? 1 : 0, st.live};
-        pw.vec = wide(pw.out, dw_stride, dw_slab);
-        ph.vec = wide(dh, dh_stride, dh_slab);
-        const Product none{};
-        const bool together = p.dw == p.dh && dw && dh;
-        if (dw) {
-            const Product& with = together ? ph : none;
-            if (p.dw == LARGE) Q1_TRY((products<Large, DT>(at, pw, p.dw_split, with, p.dh_split, up)));
-            else if (p.dw == MIDDLE) Q1_TRY((products<Middle, DT>(at, pw, p.dw_split, with, p.dh_split, up)));
-            else Q1_TRY((products<Small, DT>(at, pw, p.dw_split, with, p.dh_split, up)));
-        }
-        if (dh && !together) {
-            if (p.dh == LARGE) Q1_TRY((products<Large, DT>(at, none, 0, ph, p.dh_split, up)));
-            else if (p.dh == MIDDLE) Q1_TRY((products<Middle, DT>(at, none, 0, ph, p.dh_split, up)));
-            else if (p.dh == SMALL) Q1_TRY((products<Small, DT>(at, none, 0, ph, p.dh_split, up)));
-            else if (p.dh == FEW) Q1_TRY((rows_product<Few, DT>(at, ph, p.dh_split, up)));
-            else Q1_TRY((rows_product<Fewest, DT>(at, ph, p.dh_split, up)));
-        }
-        Finish fw{dw_slab, p.dw_split, len, d, nullptr, pw.out, dw_stride, four(pw.out, dw_stride) ? 1 : 0, dw && dw_slab ? (uint32_t)div_up(len * d, 1024) : 0};
-        Finish fh{dh_slab, p.dh_split, n, d, st.live, dh, dh_stride, four(dh, dh_stride) ? 1 : 0, dh && dh_slab && last ? (uint32_t)div_up(n * d, 1024) : 0};
-        FinishBias fb{db_part, v, (int)div_up(n, bn_of(p.logits)), db, db && last ? (uint32_t)div_up(v, 64) : 0};
-        if (const uint64_t groups = (uint64_t)fw.groups + fh.groups + fb.groups) {
-            hipLaunchKernelGGL((finish_kernel<DT>), dim3((unsigned)groups), dim3(256), 0, at.stream, fw, fh, fb, up);
-            HIP_TRY(hipGetLastError());
-        }
-    }
-    return Q1ENV_OK;
 }
 
 }  // namespace
@@ -385,11 +61,10 @@ int q1env_head_forward(int device, void* stream, const q1env_head* hd, int reduc
         return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_forward: workspace smaller than q1env_head_workspace_bytes(..., 0)");
     if (int rc = guard_device(who, device)) return rc;
     DeviceGuard guard(device);
-    const Where at{(hipStream_t)stream, device};
     switch (hd->dtype) {
-        case Q1ENV_DT_F32: return forward<F32>(at, *hd, reduction, logp, entropy, loss);
-        case Q1ENV_DT_BF16: return forward<BF16>(at, *hd, reduction, logp, entropy, loss);
-        default: return forward<F16>(at, *hd, reduction, logp, entropy, loss);
+        case Q1ENV_DT_F32: return q1_head_forward_f32(device, (hipStream_t)stream, *hd, reduction, logp, entropy, loss);
+        case Q1ENV_DT_BF16: return q1_head_forward_bf16(device, (hipStream_t)stream, *hd, reduction, logp, entropy, loss);
+        default: return q1_head_forward_f16(device, (hipStream_t)stream, *hd, reduction, logp, entropy, loss);
     }
 }
 
@@ -414,12 +89,10 @@ int q1env_head_backward(int device, void* stream, const q1env_head* hd, const fl
         HIP_TRY(hipGetLastError());
         return Q1ENV_OK;
     }
-    const Where at{(hipStream_t)stream, device};
-    const Upstream up{dlogp, dentropy, dloss, nullptr, nullptr, 0};
     switch (hd->dtype) {
-        case Q1ENV_DT_F32: return backward<F32>(at, *hd, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
-        case Q1ENV_DT_BF16: return backward<BF16>(at, *hd, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
-        default: return backward<F16>(at, *hd, up, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
+        case Q1ENV_DT_F32: return q1_head_backward_f32(device, (hipStream_t)stream, *hd, dlogp, dentropy, dloss, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
+        case Q1ENV_DT_BF16: return q1_head_backward_bf16(device, (hipStream_t)stream, *hd, dlogp, dentropy, dloss, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
+        default: return q1_head_backward_f16(device, (hipStream_t)stream, *hd, dlogp, dentropy, dloss, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
     }
 }
 

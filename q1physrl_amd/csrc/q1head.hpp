@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 namespace q1head {
+namespace {                                // every translation unit carries the kernels it launches
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -186,17 +187,19 @@ template <class C> __device__ __forceinline__ void clear(Acc<C>& acc) {
             for (int r = 0; r < 16; ++r) acc.t[i][j][r] = 0.0f;
 }
 
-// acc += the product.  For float32 the six products of the pieces follow each other within every step of k, so that a piece's tile is still near when it is asked for again.
+// acc += the product of operands in AP and BP pieces.  The products of the pieces (six for float32; two where only the gradient has a second piece) follow each other within every step
+// of k, so that a piece's tile is still near when it is asked for again.
 // A step's fragments are read one quarter ahead of their use, the last quarter's and the next step's first on either side of the one barrier: the matrix
 // instructions behind it have their operands already.  A slot is free at that barrier (its last fragments are in registers), so STAGES steps are in flight.
-template <class C, int DT, bool AK, bool BKM>
+template <class C, int DT, int AP, int BP, bool AK, bool BKM>
 __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, int64_t n0, int64_t k_begin, int64_t k_end, Acc<C>& acc, char* lds_generic) {
-    constexpr int P = Elem<DT>::planes, SEGS = P == 3 ? 6 : 1;
+    static_assert((AP == 1 && (BP == 1 || BP == 2)) || (AP == 3 && BP == 3), "pieces of the operands");
+    constexpr int SEGS = AP == 3 ? 6 : BP;
     lds_char* lds = (lds_char*)lds_generic;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     constexpr int BK = C::BK, QUARTERS = BK / 16;                            // of a step: 16 values of k each, one matrix instruction deep
-    Feed<C::BM, BK, C::LA, AK, AK && BKM && P == 1> fa;                        // (hidden rows as k: rows that do not count)
+    Feed<C::BM, BK, C::LA, AK, AK && BKM && AP == 1> fa;                        // (hidden rows as k: rows that do not count)
     Feed<C::BN, BK, C::LB, BKM, false> fb;
     fa.init(a, m0, k_begin, wave, lane);
     fb.init(b, n0, k_begin, wave, lane);
@@ -207,10 +210,11 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
     int issue_seg = 0;
     auto issue = [&](int slot) {
         int pa = 0, pb = 0;
-        if constexpr (P == 3) {                                              // (1,1) (0,2) (2,0) (0,1) (1,0) (0,0)
+        if constexpr (AP == 3) {                                             // (1,1) (0,2) (2,0) (0,1) (1,0) (0,0)
             pa = (0x010201 >> (4 * issue_seg)) & 15;
             pb = (0x001021 >> (4 * issue_seg)) & 15;
-        }
+        } else if constexpr (BP == 2)
+            pb = 1 - issue_seg;
         fa.issue(a, pa, issue_k, lds0 + (uint32_t)slot * C::STAGE_BYTES, wave, lane);
         fb.issue(b, pb, issue_k, lds0 + (uint32_t)slot * C::STAGE_BYTES + C::A_BYTES, wave, lane);
         if (SEGS == 1 || ++issue_seg == SEGS) {
@@ -421,7 +425,7 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target 
     const int64_t base = m0 + wm + 4 * (lane >> 5);                  // class of the lane's register 0
     Acc<C> acc;
     start<DT>(acc, hd.bias, base, hd.c1);
-    gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
+    gemm_tile<C, DT, Elem<DT>::planes, Elem<DT>::planes, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
     if (m0 + C::BM > hd.c1) {
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
@@ -476,84 +480,6 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target 
             float* o = part + 3 * (size_t)(tile0 + tm) * hd.rows + n0 + nl;
             o[0] = t.m; o[hd.rows] = t.s; o[2 * hd.rows] = t.u;
         }
-}
-
-// Up to 32 rows of float32: no laying out, no LDS on the way.  A workgroup takes 32 classes at a time, its four waves a quarter of the width each; a lane loads 16 bytes of its class (or row)
-// at k = 8 q + 4 (lane >> 5) and feeds them to four float32 matrix instructions - which value of k a lane holds does not matter as long as both operands hold the same.  At 16 FLOP per weight
-// the instruction's rate is no bound.  One row against 721 classes of 256: latency, 5 us (13 + 3 with pieces laid out first).
-template <bool ENTROPY>
-__global__ void __launch_bounds__(256) few_rows_kernel(const float* __restrict__ w, int64_t w_stride, int w_vec, const float* __restrict__ h, int64_t h_stride, int h_vec,
-                                                       const float* __restrict__ bias, Target target, int rows, int64_t width, float* __restrict__ part, float* __restrict__ own_logit) {
-    __shared__ float sums[4][16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 31;
-    const int64_t quarter = (width + 31) / 32 * 8, k_first = wave * quarter + 4 * (lane >> 5);
-    const int steps = (int)(quarter / 8);
-    const int64_t classes = target.classes, t = x < rows ? target.of(x) : -1;
-    const float* hr = h + x * h_stride;
-    Stat all{-INFINITY, 0.0f, 0.0f};
-    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < classes; c0 += (int64_t)gridDim.x * 32) {
-        const float* wr = w + (c0 + x) * w_stride;
-        const bool w_ok = c0 + x < classes;
-        f32x16 acc = {};
-        auto four = [&](const float* p, bool ok, int vec, int64_t k) {
-            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (ok && vec && k + 4 <= width) v = *(const f32x4*)(p + k);
-            else if (ok)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (k + j < width) v[j] = p[k + j];
-            return v;
-        };
-        constexpr int AHEAD = 8;                                             // steps whose loads are in flight together
-        for (int s0 = 0; s0 < steps; s0 += AHEAD) {
-            f32x4 a[AHEAD], b[AHEAD];
-#pragma unroll
-            for (int s = 0; s < AHEAD; ++s) {
-                const int64_t k = s0 + s < steps ? k_first + 8 * (int64_t)(s0 + s) : width;
-                a[s] = four(wr, w_ok, w_vec, k);
-                b[s] = four(hr, x < rows, h_vec, k);
-            }
-#pragma unroll
-            for (int s = 0; s < AHEAD; ++s)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s][j], b[s][j], acc, 0, 0, 0);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sums[wave][r][lane] = acc[r];
-        __syncthreads();
-        if (wave == 0) {
-            const int64_t base = c0 + 4 * (lane >> 5);
-            float l[16], mx = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t m = base + 8 * (r >> 2) + (r & 3);
-                l[r] = -INFINITY;
-                if (m < classes) {
-                    l[r] = (sums[0][r][lane] + sums[1][r][lane]) + (sums[2][r][lane] + sums[3][r][lane]);
-                    if (bias) l[r] += bias[m];
-                    if (m == t) own_logit[x] = l[r];
-                }
-                mx = fmaxf(mx, l[r]);
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * LOG2E;
-            const float ref = mx == -INFINITY ? 0.0f : mx;
-            Stat st{mx, 0.0f, 0.0f};
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float d = fmaf(l[r], LOG2E, -ref), e = __builtin_amdgcn_exp2f(d);
-                st.s += e;
-                if constexpr (ENTROPY) st.u = fmaf(fmaxf(d, -3.0e38f), e, st.u);
-            }
-            st.s += __shfl_xor(st.s, 32, 64);
-            if constexpr (ENTROPY) st.u += __shfl_xor(st.u, 32, 64);
-            all = joined(all, st);
-        }
-        __syncthreads();
-    }
-    if (wave == 0 && lane < rows) {
-        float* o = part + 3 * (size_t)blockIdx.x * rows + lane;
-        o[0] = all.m; o[rows] = all.s; o[2 * rows] = all.u;
-    }
 }
 
 // Joins the tiles' statistics: R rows per workgroup, 1024 / R lanes take the tiles of a row in turn (four loads of each kind in flight); lse is kept in units of log2.  Also leaves what the
@@ -627,6 +553,7 @@ __global__ void __launch_bounds__(1024) loss_kernel(const float* __restrict__ lo
     __shared__ int64_t cnt[16];
     double a = 0.0;
     int64_t c = 0;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < rows; i += 1024) { a += (double)logp[i]; c += live[i]; }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) { a += __shfl_down(a, off, 64); c += __shfl_down((long long)c, off, 64); }
@@ -693,6 +620,11 @@ template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
+template <int DT> __device__ __forceinline__ float low_of(uint32_t w) {       // the value in the low 16 bits of a packed pair
+    if constexpr (DT == F16) return f16_value((uint16_t)w);
+    else return __builtin_bit_cast(float, w << 16);
+}
+
 // A 16-bit result tile goes to memory through the LDS, so that a wave's store covers whole rows of the tile (512 or 256 bytes) and not 32 pieces of 32 rows: 16-byte chunk c of row n
 // sits at c ^ (n & 15) (& 7 in rows of 8 chunks), which keeps both the writes (32 rows, one chunk) and the reads (one row) off each other's banks.
 template <class C> __device__ __forceinline__ int chunk_at(int n, int c) { return n * (2 * C::BM) + (c ^ (n & (C::BM / 8 < 16 ? C::BM / 8 - 1 : 15))) * 16; }
@@ -736,7 +668,10 @@ __device__ __forceinline__ float sums_of_32(float (&v)[32], int lane, int& which
 
 // a piece [c0, c1) of the classes: the logits again, and the gradient of each -> g[row][class - c0] (stride `piece`; 16 bits, float32 as three pieces g_plane values apart), zero
 // up to the end of the last tile; and the sums over this tile's rows -> db_part[row tile][class]
-template <class C, int DT, bool ENTROPY>
+// GP: pieces the gradient is stored in.  One in 16-bit types: its rounding leaves an error of the size that the result's own rounding leaves anyway (bfloat16, random upstream, 50176 rows:
+// 0.0024 of the results' norm instead of 0.0017), and a second piece would double the products.  Two up to 256 rows, where the few roundings need not even out (2 rows of 2 classes: 0.004 with
+// one, 0.0017 with two) and the products are bound by memory; three for float32.
+template <class C, int DT, int GP, bool ENTROPY>
 __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream up, int64_t piece, int64_t g_plane, const float* __restrict__ lse,
                                                               const float* __restrict__ entropy, uint16_t* __restrict__ g, float* __restrict__ db_part) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -747,7 +682,7 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
     const int64_t base = m0 + wm + 4 * (lane >> 5);
     Acc<C> acc;
     start<DT>(acc, hd.bias, base, hd.c1);
-    gemm_tile<C, DT, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
+    gemm_tile<C, DT, Elem<DT>::planes, Elem<DT>::planes, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
     const float sc = up.stored();
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
@@ -816,7 +751,7 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
     }
     const int rows = hd.rows - n0 < C::BN ? (int)(hd.rows - n0) : C::BN;
 #pragma unroll
-    for (int q = 0; q < Elem<DT>::planes; ++q) {
+    for (int q = 0; q < GP; ++q) {
         if (q > 0) __syncthreads();
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
@@ -829,15 +764,162 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
                     for (int r = 0; r < 4; ++r) {
                         const float v0 = acc.t[i][j][8 * h + 2 * r], v1 = acc.t[i][j][8 * h + 2 * r + 1];
                         w[r] = pack2<DT>(v0, v1);
-                        if (q + 1 < Elem<DT>::planes) {             // what this piece leaves for the next
-                            acc.t[i][j][8 * h + 2 * r] = v0 - __builtin_bit_cast(float, w[r] << 16);
-                            acc.t[i][j][8 * h + 2 * r + 1] = v1 - __builtin_bit_cast(float, w[r] & 0xffff0000u);
+                        if (q + 1 < GP) {                           // what this piece leaves for the next
+                            acc.t[i][j][8 * h + 2 * r] = v0 - low_of<DT>(w[r]);
+                            acc.t[i][j][8 * h + 2 * r + 1] = v1 - low_of<DT>(w[r] >> 16);
                         }
                     }
                     put_eight<C>(lds, wn + 32 * j + (lane & 31), wm + 32 * i + 16 * h + 8 * (lane >> 5), eight_of(u32x2{w[0], w[1]}, u32x2{w[2], w[3]}));
                 }
         __syncthreads();
         flush_rows<C>(lds, g + q * g_plane + n0 * piece + (m0 - hd.c0), piece, rows, C::BM);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------
+// float32 with few rows or few classes (32 at most): memory decides, the float32 matrix instruction (16 FLOP per byte at 32) is fast enough, and laying pieces out
+// would cost several times the reading: 100000 x 256 x 32 takes 57 us forward and 250 with gradients, 33 classes laid out take 105 and 385; 32 x 4096 x 4096 54 and 166, 33 rows 152 and 363.  No LDS on the way in: a lane loads 16 bytes at k = 8 q + 4 (lane >> 5) of its class, row or column and feeds them to four instructions - which
+// value of k a lane holds does not matter as long as both operands hold the same.
+// What lies outside is loaded from `safe` (any address that may be read) and replaced by zero, without a branch.  Loads of 16 bytes may start at any float.
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+struct Skinny {
+    const float *w, *h, *bias;
+    int64_t w_stride, h_stride;
+    int64_t rows, width, classes;
+};
+__device__ __forceinline__ float one_of(const float* p, const float* safe, bool in) {
+    const float v = *(in ? p : safe);
+    return in ? v : 0.0f;
+}
+__device__ __forceinline__ f32x4 four_of(const float* p, const float* safe, bool in) {          // `safe`: four values
+    const f32x4 v = *(const f32x4_any*)(in ? p : safe);
+    return f32x4{in ? v[0] : 0.0f, in ? v[1] : 0.0f, in ? v[2] : 0.0f, in ? v[3] : 0.0f};
+}
+__device__ __forceinline__ f32x4 up_to_three_of(const float* p, const float* safe, int count) {
+    return f32x4{one_of(p, safe, count > 0), one_of(p + 1, safe, count > 1), one_of(p + 2, safe, count > 2), 0.0f};
+}
+// the logits of classes c0 .. c0 + 31 and rows r0 .. r0 + 31, a quarter of the width per wave; complete in `l` of wave 0 (register r: class c0 + 4 (lane >> 5) + 8 (r / 4) + r % 4, row r0 + lane % 32)
+__device__ __forceinline__ void skinny_logits(const Skinny& q, int64_t c0, int64_t r0, float (*sums)[16][64], float (&l)[16]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 31, half = lane >> 5;
+    const int whole = (int)(q.width & ~3), quarter = (whole + 31) / 32 * 8, k_first = wave * quarter + 4 * half, steps = quarter / 8;
+    const bool w_ok = c0 + x < q.classes, h_ok = r0 + x < q.rows;
+    const float *wr = w_ok ? q.w + (c0 + x) * q.w_stride : q.w, *hr = h_ok ? q.h + (r0 + x) * q.h_stride : q.h;
+    f32x16 acc = {};
+    auto multiply = [&](const f32x4& a, const f32x4& b) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc, 0, 0, 0);
+    };
+    constexpr int AHEAD = 8;                                                 // steps whose loads are in flight together (two sets of four in turn measured the same or slower: fewer waves fit)
+    for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+        f32x4 a[AHEAD], b[AHEAD];
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) {
+            const int k = k_first + 8 * (s0 + s);
+            const bool in = s0 + s < steps && k < whole;
+            a[s] = four_of(wr + k, wr, w_ok && in);
+            b[s] = four_of(hr + k, hr, h_ok && in);
+        }
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) multiply(a[s], b[s]);
+    }
+    if (wave == 3 && whole < q.width) {                                      // the last one to three values
+        const int left = half == 0 ? (int)q.width - whole : 0;
+        multiply(up_to_three_of(wr + whole, wr, w_ok ? left : 0), up_to_three_of(hr + whole, hr, h_ok ? left : 0));
+    }
+    __syncthreads();                                                         // (what was there has been read)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sums[wave][r][lane] = acc[r];
+    __syncthreads();
+    if (wave != 0) return;
+    const int64_t base = c0 + 4 * (lane >> 5);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int64_t m = base + 8 * (r >> 2) + (r & 3);
+        l[r] = -INFINITY;
+        if (m < q.classes) {
+            l[r] = (sums[0][r][lane] + sums[1][r][lane]) + (sums[2][r][lane] + sums[3][r][lane]);
+            if (q.bias) l[r] += q.bias[m];
+        }
+    }
+}
+
+// statistics of 32 rows (workgroup / groups) over every groups-th 32 classes
+template <bool ENTROPY>
+__global__ void __launch_bounds__(256) skinny_statistics_kernel(Skinny q, Target target, uint32_t groups, float* __restrict__ part, float* __restrict__ own_logit) {
+    __shared__ float sums[4][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t group = blockIdx.x % groups;
+    const int64_t r0 = (int64_t)(blockIdx.x / groups) * 32, n = r0 + (lane & 31), t = n < q.rows ? target.of(n) : -1;
+    Stat all{-INFINITY, 0.0f, 0.0f};
+    for (int64_t c0 = (int64_t)group * 32; c0 < q.classes; c0 += (int64_t)groups * 32) {
+        float l[16];
+        skinny_logits(q, c0, r0, sums, l);
+        if (wave != 0) continue;
+        const int64_t base = c0 + 4 * (lane >> 5);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (t >= 0 && base + 8 * (r >> 2) + (r & 3) == t) own_logit[n] = l[r];
+            mx = fmaxf(mx, l[r]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * LOG2E;
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        Stat st{mx, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float d = fmaf(l[r], LOG2E, -ref), e = __builtin_amdgcn_exp2f(d);
+            st.s += e;
+            if constexpr (ENTROPY) st.u = fmaf(fmaxf(d, -3.0e38f), e, st.u);
+        }
+        st.s += __shfl_xor(st.s, 32, 64);
+        if constexpr (ENTROPY) st.u += __shfl_xor(st.u, 32, 64);
+        all = joined(all, st);
+    }
+    if (wave == 0 && lane < 32 && n < q.rows) {
+        float* o = part + 3 * (size_t)group * q.rows + n;
+        o[0] = all.m; o[q.rows] = all.s; o[2 * q.rows] = all.u;
+    }
+}
+
+// g[row][class] in float32, rows of `stride` values (whole 32s, zero past the last class).  A workgroup takes 32 classes (workgroup % groups) and every teams-th 32 rows, and leaves the sums
+// over its rows in db_part[team][class].
+template <bool ENTROPY>
+__global__ void __launch_bounds__(256) skinny_gradient_kernel(Skinny q, Upstream up, const int64_t* __restrict__ target, uint32_t groups, uint32_t teams, const float* __restrict__ lse,
+                                                              const float* __restrict__ entropy, float* __restrict__ g, int64_t stride, float* __restrict__ db_part) {
+    __shared__ float sums[4][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t team = blockIdx.x / groups;
+    const int64_t c0 = (int64_t)(blockIdx.x % groups) * 32, base = c0 + 4 * (lane >> 5);
+    float db[32] = {};
+    for (int64_t r0 = (int64_t)team * 32; r0 < q.rows; r0 += (int64_t)teams * 32) {
+        float l[16];
+        skinny_logits(q, c0, r0, sums, l);
+        if (wave != 0) continue;
+        const int64_t n = r0 + (lane & 31), t = n < q.rows ? target[n] : -1;
+        const bool on = t != -1;
+        const float z = on ? lse[n] : 0.0f, hrow = ENTROPY && on ? entropy[n] : 0.0f;
+        const float A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) : 0.0f, E = ENTROPY && on ? up.dentropy[n] : 0.0f, El = E * LN2, Ah = A + E * hrow;
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            f32x4 o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t m = base + 8 * r4 + r;
+                const float d = fmaf(l[4 * r4 + r], LOG2E, -z), p = __builtin_amdgcn_exp2f(d);
+                float v = ENTROPY ? -p * fmaf(El, fmaxf(d, -3.0e38f), Ah) : -p * A;
+                if (m == t) v += A;
+                v = on && m < q.classes ? v : 0.0f;
+                o[r] = v;
+                db[4 * r4 + r] += v;
+            }
+            if (n < q.rows) *(f32x4*)(g + n * stride + base + 8 * r4) = o;
+        }
+    }
+    if (db_part && wave == 0) {
+        int r;
+        const float sum = sums_of_32(db, lane, r);                           // (values 16 .. 31 are zero)
+        const int64_t m = base + 8 * (r >> 2) + (r & 3);
+        if (r < 16 && m < q.classes) db_part[(size_t)team * q.classes + m] = sum;
     }
 }
 
@@ -856,7 +938,7 @@ struct Product {
     const uint8_t* live;               // result rows that are zero whatever the operands hold
 };
 
-template <class C, int DT, bool AK, bool BKM>
+template <class C, int DT, int GP, bool AK, bool BKM>
 __device__ __forceinline__ void product_tile(const Product& pr, const Upstream& up, uint32_t id, uint32_t total, char* lds) {
     typedef typename Elem<DT>::type E;
     uint32_t tm, tn, z;
@@ -865,7 +947,7 @@ __device__ __forceinline__ void product_tile(const Product& pr, const Upstream& 
     const int64_t kb = (int64_t)z * pr.split_k, ke = kb + pr.split_k < pr.k ? kb + pr.split_k : pr.k;
     Acc<C> acc;
     clear(acc);
-    gemm_tile<C, DT, AK, BKM>(pr.a, pr.b, m0, n0, kb, ke, acc, lds);
+    gemm_tile<C, DT, Elem<DT>::planes, GP, AK, BKM>(pr.a, pr.b, m0, n0, kb, ke, acc, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const float sc = pr.slab ? 1.0f : up.result();
     float* slab = pr.slab ? pr.slab + (size_t)z * pr.rows * pr.width : nullptr;
@@ -925,18 +1007,98 @@ __device__ __forceinline__ void product_tile(const Product& pr, const Upstream& 
 
 // The weights' gradient (both operands with the rows as k) and the hidden rows' (the weights with the classes as k) of one piece, in one launch: neither fills the device's last
 // round alone.  groups: workgroups of the first, a multiple of 8 (the XCDs' turn) unless it is the only one.
-template <class C, int DT>
+template <class C, int DT, int GP>
 __global__ void __launch_bounds__(C::THREADS) products_kernel(Product dw, Product dh, Upstream up, uint32_t dw_tiles, uint32_t dw_groups) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     if (blockIdx.x < dw_groups) {
-        if (blockIdx.x < dw_tiles) product_tile<C, DT, true, true>(dw, up, blockIdx.x, dw_tiles, lds);
+        if (blockIdx.x < dw_tiles) product_tile<C, DT, GP, true, true>(dw, up, blockIdx.x, dw_tiles, lds);
     } else
-        product_tile<C, DT, true, false>(dh, up, blockIdx.x - dw_groups, gridDim.x - dw_groups, lds);
+        product_tile<C, DT, GP, true, false>(dh, up, blockIdx.x - dw_groups, gridDim.x - dw_groups, lds);
 }
-template <class C, int DT>
+template <class C, int DT, int GP>
 __global__ void __launch_bounds__(C::THREADS) rows_product_kernel(Product dh, Upstream up) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    product_tile<C, DT, true, false>(dh, up, blockIdx.x, gridDim.x, lds);
+    product_tile<C, DT, GP, true, false>(dh, up, blockIdx.x, gridDim.x, lds);
+}
+
+// out[n][m] = sum_k a[k][m] b(k, n) for the products around a skinny gradient (m >= 4), 128 x 32 results per unit of work: b[k stride + n] (BKM) or b[n stride + k].  Lane x of a half holds columns
+// m0 + 4 x .. 4 x + 3, one for each of four accumulators, so that a result's four neighbours end in one lane.  SHARED: the four waves of a workgroup take k in turns and add
+// up through the LDS (long sums); else each wave has a unit of its own.
+struct SkinnyProduct {
+    const float *a, *b;
+    int64_t a_stride, b_stride;
+    const uint8_t* live;               // rows k of a that count, or null
+    int64_t m, n, k, part;             // part: k per split, a multiple of 32
+    uint32_t tiles_m, tiles_n, splits;
+    float* out;                        // [split][n][m] slabs, or the result at out_stride
+    int64_t out_stride;
+    int slab;
+    const uint8_t* out_live;           // result rows that are zero whatever the operands hold
+};
+template <bool BKM, bool SHARED>
+__global__ void __launch_bounds__(256) skinny_product_kernel(SkinnyProduct q, Upstream up) {
+    __shared__ float sums[SHARED ? 4 : 1][SHARED ? 64 : 1][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 31, half = lane >> 5;
+    const uint32_t unit = SHARED ? blockIdx.x : blockIdx.x * 4 + wave;
+    if (!SHARED && unit >= q.tiles_m * q.tiles_n * q.splits) return;
+    const uint32_t tm = unit % q.tiles_m, tn = unit / q.tiles_m % q.tiles_n, z = unit / q.tiles_m / q.tiles_n;
+    const int64_t m0 = (int64_t)tm * 128, n0 = (int64_t)tn * 32, kb = z * q.part, ke = kb + q.part < q.k ? kb + q.part : q.k;
+    const bool n_ok = n0 + x < q.n;
+    auto columns = [&](int i) { return m0 + 4 * i + 4 <= q.m ? m0 + 4 * i : q.m - 4; };          // of lane i; those past the last column take the last four once more
+    f32x16 acc[4] = {};
+    constexpr int STEP = SHARED ? 32 : 8;
+    f32x4 a[2][4], b[2];                                                     // one step is loaded while the one before it is multiplied
+    auto load = [&](int set, int64_t k0) {
+        const int64_t k = k0 + 4 * half;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bool in = k + j < ke;
+            if (q.live) in = q.live[in ? k + j : 0] != 0 && in;
+            a[set][j] = four_of(q.a + (k + j) * q.a_stride + columns(x), q.a, in);
+        }
+        if constexpr (BKM) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[set][j] = one_of(q.b + (k + j) * q.b_stride + n0 + x, q.b, n_ok && k + j < ke);
+        } else
+            b[set] = four_of(q.b + (n0 + x) * q.b_stride + k, q.b, n_ok && k < ke);          // (a gradient's rows: zero from the last class to the next 32)
+    };
+    auto use = [&](int set) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[set][j][c], b[set][j], acc[c], 0, 0, 0);
+    };
+    int64_t k0 = kb + (SHARED ? 8 * wave : 0);
+    load(0, k0);
+    for (; k0 < ke; k0 += 2 * STEP) {
+        load(1, k0 + STEP);
+        use(0);
+        load(0, k0 + 2 * STEP);
+        use(1);
+    }
+    if constexpr (SHARED) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sums[wave][16 * c + r][lane] = acc[c][r];
+        __syncthreads();
+    }
+    if (!n_ok) return;
+    float* row = q.out + (q.slab ? ((int64_t)z * q.n + n0 + x) * q.m : (n0 + x) * q.out_stride);
+    const float sc = q.slab ? 1.0f : up.result();
+    const bool on = q.slab || !q.out_live || q.out_live[n0 + x];
+#pragma unroll
+    for (int i = 0; i < (SHARED ? 4 : 16); ++i) {                            // (of four waves each finishes a quarter of the registers)
+        const int r = SHARED ? 4 * wave + i : i;
+        f32x4 o;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if constexpr (SHARED) o[c] = (sums[0][16 * c + r][lane] + sums[1][16 * c + r][lane]) + (sums[2][16 * c + r][lane] + sums[3][16 * c + r][lane]);
+            else o[c] = acc[c][i];
+            o[c] = on ? o[c] * sc : 0.0f;
+        }
+        *(f32x4_any*)(row + columns(8 * (r >> 2) + 4 * half + (r & 3))) = o;
+    }
 }
 
 // result = scale x sum of the slabs, in their order; and db[class] = scale x sum over the row tiles: 64 classes per workgroup, wave g takes tiles g, g + 4, ...
@@ -964,7 +1126,7 @@ template <int DT> __device__ __forceinline__ void finish(const Finish& f, float 
         const int64_t n = i0 / f.width, m = i0 - n * f.width;
         f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
         if (!f.live || f.live[n]) {
-#pragma unroll 4
+#pragma unroll 8
             for (int64_t s = 0; s < f.splits; ++s) a += *(const f32x4*)(f.slab + s * total + i0);
             a *= scale;
         }
@@ -997,11 +1159,12 @@ __global__ void __launch_bounds__(256) finish_kernel(Finish dw, Finish dh, Finis
     const int64_t j = (int64_t)b * 64 + r;
     float a = 0.0f;
     if (j < db.classes)
-#pragma unroll 8
+#pragma unroll 32
         for (int t = g; t < db.tiles; t += 4) a += db.part[(size_t)t * db.classes + j];
     red[g][r] = a;
     __syncthreads();
     if (g == 0 && j < db.classes) ((typename Elem<DT>::type*)db.out)[j] = from_float<DT>((red[0][r] + red[1][r] + red[2][r] + red[3][r]) * scale);
 }
 
+}  // namespace
 }  // namespace q1head

@@ -210,6 +210,65 @@ def test_masked_classes(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("n,d,v", [(2, 73, 2), (1, 64, 40), (31, 48, 70), (60, 200, 130), (100, 64, 300), (256, 136, 257)])
+def test_few_rows_of_16_bits_keep_the_gradient_finer_than_their_type(n, d, v, dtype):
+    """Few rows do not average the roundings of a stored gradient, so it is held in two pieces: ut^2 of it is lost, not ut (ut the type's half step), and the results are off by their
+    own rounding and what float32 leaves: the bounds of the other tests with ut^2 for the stored gradient."""
+    h, w, b, t = make(n, d, v, dtype, seed=n, ignored=0.0)
+    leaves = [x.requires_grad_() for x in (h, w, b)]
+    got = torch.autograd.grad(categorical.linear_categorical(h, w, t, b), leaves, (torch.ones(n, device="cuda"), torch.full((n,), 0.25, device="cuda")))
+    T = Truth(h, w, b, t)
+    A, E = torch.ones(n, device="cuda", dtype=torch.float64), torch.full((n,), 0.25, device="cuda", dtype=torch.float64)
+    g = -T.p * (A[:, None] + E[:, None] * (T.lp + T.entropy[:, None]))
+    g.scatter_add_(1, T.t[:, None], A[:, None])
+    size = T.p * (1 + 0.25 * (T.lp.abs() + T.entropy[:, None] + 1))
+    ut = HALF[dtype]
+    # the second piece's smallest step in float16: half of 2^-24 at a scale that brings the largest possible value to 2^13 at least
+    off = size * T.e[:, None] + g.abs() * ut * ut + 4 * U * (size + g.abs()) + (2.0 ** -38 * 5 if dtype == torch.float16 else 0.0)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for name, x, ref, err, part, k in (("dh", got[0], g @ T.w, off @ T.w.abs(), g.abs() @ T.w.abs(), 2 * v), ("dw", got[1], g.T @ T.h, off.T @ T.h.abs(), g.abs().T @ T.h.abs(), 2 * n)):
+        near(x, ref, err * 1.01 + (k + 8) * 2 * U * (part + err) + ut * ref.abs() * 1.01 + tiny, name)
+
+
+SKINNY = [(1, 1, 1), (5, 3, 2), (9, 4, 3), (1, 7, 33), (2, 300, 31), (31, 130, 1000), (32, 64, 32), (32, 1000, 4099), (33, 61, 32), (500, 8, 1), (1000, 257, 15), (3001, 128, 32), (700, 2171, 5), (33, 70, 33)]
+
+
+@gpu
+@pytest.mark.parametrize("n,d,v", SKINNY)
+@pytest.mark.parametrize("how", ["whole", "views", "odd"])
+def test_few_rows_or_classes_of_float32(n, d, v, how):
+    """At most 32 rows or classes of float32 are read straight from memory: whole rows, rows with a pitch (in and out), and rows that start at any 4 bytes."""
+    h, w, b, t = make(n, d, v, torch.float32, seed=n + d + v)
+    if how != "whole":
+        pad = 4 if how == "views" else 3
+
+        def laid(x):
+            wide = torch.full((x.shape[0], x.shape[1] + 2 * pad), float("nan"), device="cuda")
+            wide[:, pad:pad + x.shape[1]] = x
+            return wide[:, pad:pad + x.shape[1]]
+        h, w = laid(h), laid(w)
+    if n > 1 and bool((t != IGN).any()):
+        dead = (t == IGN).nonzero()[:, 0]
+        h[dead] = float("nan")                                                 # what ignored rows hold
+    leaves = [x.requires_grad_() for x in (h, w, b)]
+    logp, ent = categorical.linear_categorical(h, w, t, b)
+    T = Truth(h, w, b, t)
+    near(logp, T.logp, T.elogp, "logp")
+    near(ent, T.entropy, T.eent, "entropy")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    A, E = torch.randn(n, device="cuda", generator=g), torch.randn(n, device="cuda", generator=g)
+    for entropy in (True, False):
+        if entropy:
+            got = torch.autograd.grad((logp, ent), leaves, (A, E), retain_graph=True)
+        else:
+            got = torch.autograd.grad(logp, leaves, A)
+        for name, x, (r, tol) in zip(("dh", "dw", "db"), got, T.grads(A, E if entropy else torch.zeros_like(E))):
+            near(x, r, tol, name)
+        assert bool((got[0][t == IGN] == 0).all())
+
+
+@gpu
 @pytest.mark.parametrize("bad", [-1, 700, 2 ** 40])
 def test_classes_that_do_not_exist_are_nan(bad):
     h, w, b, t = make(20, 64, 700, torch.float32, ignored=0.0)
