@@ -7,6 +7,8 @@
 //   q1env_server.hip    the resident tick server (q1server.hpp)
 //   q1env_resident.hip  the resident sampler (q1resident.hpp)
 //   q1env_learner.hip   the native PPO learner step (q1learner.hpp, q1ppo_loss.hpp)
+//   q1env_head.hip      the wide categorical head's entry points; its kernels (q1head.hpp) per element type in q1env_head_f32 / _bf16 / _f16.hip (q1head_calls.hpp)
+//   q1env_clip.hip      gradient norm and clipping over many tensors
 //   q1env_diag.hip      timers, PMC traffic calibration, division self-test
 //
 // Kernels live in the translation unit that launches them (no relocatable device code: each TU carries its own code object).
