@@ -40,9 +40,11 @@ TU_FLAGS = {"q1env_learner.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
             # the persistent learner: the same register form (its step loop read 220 accumulator registers back per step), and NO atomic
             # optimizer: that pass rewrites a uniform-address atomic into a wave reduction + s_waitcnt vmcnt(0) + readfirstlane, i.e. it
             # makes the barrier poll that is requested early and looked at late (q1learner_persist.hpp, barrier 3) synchronous again
-            # the training operators: without the packed float32 instructions, which the compiler otherwise forms from ordinary float code
-            **{"q1env_%s.hip" % u: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for u in ("head", "head_f32", "head_bf16", "head_f16", "clip")},
             "q1env_plearner.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]}
+# No packed float32 instructions, which the compiler otherwise forms from ordinary float code: some of their forms have given wrong results now and then.  The env core keeps them:
+# its rollout is one wave per SIMD and pays for every instruction (237 a tick with them, 242 without: 90.4e9 and 89.3e9 env steps/s), and every tick is held to the oracle.
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+TU_FLAGS = {src: NO_PACKED + TU_FLAGS.get(src, []) for src in map(os.path.basename, SOURCES) if src != "q1env_core.hip"}
 LINK_FLAGS = ["--offload-arch=gfx950", "-shared", "-fPIC"]
 HIPCC_FLAGS = COMPILE_FLAGS + ["-shared"]     # (kept for tools that compile a single file the old way, e.g. tools/asan_check.sh)
 
