@@ -89,9 +89,12 @@ template <int BM_, int BN_, int WM_, int WN_, int BK_, int STAGES_> struct Confi
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;             // 32 x 32 tiles per wave
     static constexpr int LA = BM * BK / 512 / WAVES, LB = BN * BK / 512 / WAVES;         // load instructions per wave and stage
     static constexpr int A_BYTES = BM * BK * 2, STAGE_BYTES = (BM + BN) * BK * 2, LDS_BYTES = STAGES * STAGE_BYTES;
+    // what the epilogue over logits wants of every row, behind the stages; not where two workgroups fill the CU's LDS already (they hide each other's loads)
+    static constexpr bool KEEPS_ROWS = 2 * LDS_BYTES != 163840;
+    static constexpr int ALL_BYTES = LDS_BYTES + (KEEPS_ROWS ? 20 * BN : 0);
     static_assert(BK == 32 || BK == 64, "the LDS image's permutations");
     static_assert(LA * WAVES * 512 == BM * BK && LB * WAVES * 512 == BN * BK && TM >= 1 && TN >= 1, "whole load instructions per wave");
-    static_assert(STAGES >= 2 && (STAGES - 1) * (LA + LB) < 64 && LDS_BYTES <= 163840, "vmcnt; LDS of a CU");
+    static_assert(STAGES >= 2 && (STAGES - 1) * (LA + LB) < 64 && ALL_BYTES <= 163840, "vmcnt; LDS of a CU");
 };
 constexpr int PART_STEP = 64;               // parts of a split sum are whole steps of every configuration (and whole words of `live`)
 
@@ -191,8 +194,9 @@ template <class C> __device__ __forceinline__ void clear(Acc<C>& acc) {
 // of k, so that a piece's tile is still near when it is asked for again.
 // A step's fragments are read one quarter ahead of their use, the last quarter's and the next step's first on either side of the one barrier: the matrix
 // instructions behind it have their operands already.  A slot is free at that barrier (its last fragments are in registers), so STAGES steps are in flight.
-template <class C, int DT, int AP, int BP, bool AK, bool BKM>
-__device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, int64_t n0, int64_t k_begin, int64_t k_end, Acc<C>& acc, char* lds_generic) {
+// `meanwhile` runs when the first steps' loads are under way: it gives acc its first values, and what it loads arrives with them.
+template <class C, int DT, int AP, int BP, bool AK, bool BKM, typename F>
+__device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, int64_t n0, int64_t k_begin, int64_t k_end, Acc<C>& acc, char* lds_generic, F&& meanwhile) {
     static_assert((AP == 1 && (BP == 1 || BP == 2)) || (AP == 3 && BP == 3), "pieces of the operands");
     constexpr int SEGS = AP == 3 ? 6 : BP;
     lds_char* lds = (lds_char*)lds_generic;
@@ -280,6 +284,7 @@ __device__ __forceinline__ void gemm_tile(const Op& a, const Op& b, int64_t m0, 
     };
 #pragma unroll
     for (int g = 0; g < C::STAGES; ++g) issue(g);                            // (steps past the end read zeros: nothing below depends on how many there are)
+    meanwhile();
     wait_loads<(C::STAGES - 1) * (C::LA + C::LB)>();
     barrier();
     fetch(0, 0);
@@ -424,8 +429,16 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const int64_t base = m0 + wm + 4 * (lane >> 5);                  // class of the lane's register 0
     Acc<C> acc;
-    start<DT>(acc, hd.bias, base, hd.c1);
-    gemm_tile<C, DT, Elem<DT>::planes, Elem<DT>::planes, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
+    int* own_of = (int*)(lds + C::LDS_BYTES);                         // the row's own class within the tile, negative: none
+    auto own_class = [&](int64_t n) {
+        const int64_t t = n < hd.rows ? target.of(n) - m0 : -1;
+        return t >= 0 && t < C::BM ? (int)t : -1;
+    };
+    gemm_tile<C, DT, Elem<DT>::planes, Elem<DT>::planes, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds, [&] {
+        start<DT>(acc, hd.bias, base, hd.c1);
+        if constexpr (C::KEEPS_ROWS)
+            if (threadIdx.x < C::BN) own_of[threadIdx.x] = own_class(n0 + threadIdx.x);
+    });
     if (m0 + C::BM > hd.c1) {
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
@@ -439,17 +452,16 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target 
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
         const int nl = wn + 32 * j + (lane & 31);
-        const int64_t n = n0 + nl, t = n < hd.rows ? target.of(n) : -1;
-        const int64_t rel = t - (m0 + wm);
+        const int rel = (C::KEEPS_ROWS ? own_of[nl] : own_class(n0 + nl)) - wm;
         if (__any(rel >= 0 && rel < C::TM * 32)) {
-            const int own = t >= base && rel < C::TM * 32 ? (int)(t - base) : -1;
+            const int own = rel >= 4 * (lane >> 5) && rel < C::TM * 32 ? rel - 4 * (lane >> 5) : -1;
             float l = 0.0f;
 #pragma unroll
             for (int i = 0; i < C::TM; ++i)
                 if (__any(own >= 0 && own >> 5 == i))
 #pragma unroll
                     for (int r = 0; r < 16; ++r) l = own == 32 * i + 8 * (r >> 2) + (r & 3) ? acc.t[i][j][r] : l;
-            if (own >= 0 && (own & 4) == 0) own_logit[n] = l;
+            if (own >= 0 && (own & 4) == 0) own_logit[n0 + nl] = l;
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -681,18 +693,41 @@ __global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const int64_t base = m0 + wm + 4 * (lane >> 5);
     Acc<C> acc;
-    start<DT>(acc, hd.bias, base, hd.c1);
-    gemm_tile<C, DT, Elem<DT>::planes, Elem<DT>::planes, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds);
-    const float sc = up.stored();
+    struct Row { int own; float z, A, E, h; };                       // own class within the tile, -1: none, -2: the row does not count; log-sum-exp, upstream values, entropy
+    int* own_of = (int*)(lds + C::LDS_BYTES);
+    float* row_of = (float*)(own_of + C::BN);
+    auto row = [&](int64_t n) {
+        const int64_t t = n < hd.rows ? hd.target[n] : -1;
+        const bool on = t != -1;
+        const float sc = up.stored();
+        Row r;
+        r.own = !on ? -2 : t >= m0 && t < m0 + C::BM ? (int)(t - m0) : -1;
+        r.z = on ? lse[n] : 0.0f;
+        r.A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) * sc : 0.0f;
+        r.E = ENTROPY && on ? up.dentropy[n] * sc : 0.0f;
+        r.h = ENTROPY && on ? entropy[n] : 0.0f;
+        return r;
+    };
+    gemm_tile<C, DT, Elem<DT>::planes, Elem<DT>::planes, false, false>(hd.w, hd.h, m0 - hd.c0, n0, 0, hd.width, acc, lds, [&] {
+        start<DT>(acc, hd.bias, base, hd.c1);
+        if constexpr (C::KEEPS_ROWS)
+            if (const int x = threadIdx.x; x < C::BN) {
+                const Row r = row(n0 + x);
+                own_of[x] = r.own; row_of[x] = r.z; row_of[C::BN + x] = r.A;
+                if constexpr (ENTROPY) { row_of[2 * C::BN + x] = r.E; row_of[3 * C::BN + x] = r.h; }
+            }
+    });
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
-        const int64_t n = n0 + wn + 32 * j + (lane & 31), t = n < hd.rows ? hd.target[n] : -1;
-        const bool on = t != -1;
-        const float z = on ? lse[n] : 0.0f;
-        const float A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) * sc : 0.0f, E = ENTROPY && on ? up.dentropy[n] * sc : 0.0f;
-        const float hrow = ENTROPY && on ? entropy[n] : 0.0f, El = E * LN2, Ah = A + E * hrow;
-        const bool here = __any(t >= m0 + wm && t < m0 + wm + C::TM * 32);
-        const int own = t >= base && t < base + C::TM * 32 ? (int)(t - base) : -1;
+        const int nl = wn + 32 * j + (lane & 31);
+        Row q;
+        if constexpr (C::KEEPS_ROWS) q = Row{own_of[nl], row_of[nl], row_of[C::BN + nl], ENTROPY ? row_of[2 * C::BN + nl] : 0.0f, ENTROPY ? row_of[3 * C::BN + nl] : 0.0f};
+        else q = row(n0 + nl);
+        const bool on = q.own != -2;
+        const float z = q.z, A = q.A, El = q.E * LN2, Ah = A + q.E * q.h;
+        const int rel = q.own - wm;
+        const bool here = __any(rel >= 0 && rel < C::TM * 32);
+        const int own = rel >= 4 * (lane >> 5) && rel < C::TM * 32 ? rel - 4 * (lane >> 5) : -1;
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
@@ -946,8 +981,7 @@ __device__ __forceinline__ void product_tile(const Product& pr, const Upstream& 
     const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
     const int64_t kb = (int64_t)z * pr.split_k, ke = kb + pr.split_k < pr.k ? kb + pr.split_k : pr.k;
     Acc<C> acc;
-    clear(acc);
-    gemm_tile<C, DT, Elem<DT>::planes, GP, AK, BKM>(pr.a, pr.b, m0, n0, kb, ke, acc, lds);
+    gemm_tile<C, DT, Elem<DT>::planes, GP, AK, BKM>(pr.a, pr.b, m0, n0, kb, ke, acc, lds, [&] { clear(acc); });
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const float sc = pr.slab ? 1.0f : up.result();
     float* slab = pr.slab ? pr.slab + (size_t)z * pr.rows * pr.width : nullptr;

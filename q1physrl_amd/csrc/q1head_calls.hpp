@@ -171,11 +171,11 @@ template <class C, auto KERNEL, typename... A> int go(hipStream_t stream, int de
     if (workgroups <= 0 || workgroups > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
     static std::atomic<uint64_t> done{0};
     const uint64_t bit = 1ull << (device & 63);
-    if (C::LDS_BYTES > 65536 && (device > 63 || !(done.load(std::memory_order_relaxed) & bit))) {        // more than 64 KB of LDS has to be allowed once per kernel and device
-        HIP_TRY(hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES));
+    if (C::ALL_BYTES > 65536 && (device > 63 || !(done.load(std::memory_order_relaxed) & bit))) {        // more than 64 KB of LDS has to be allowed once per kernel and device
+        HIP_TRY(hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, C::ALL_BYTES));
         done.fetch_or(bit, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL(KERNEL, dim3((unsigned)workgroups), dim3(C::THREADS), C::LDS_BYTES, stream, args...);
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)workgroups), dim3(C::THREADS), C::ALL_BYTES, stream, args...);
     HIP_TRY(hipGetLastError());
     return 0;
 }
