@@ -583,7 +583,7 @@ int q1env_sample_resident(q1env_t* env, const q1env_resident_args* args);
 
 /* ---- (ABI v7) wide categorical head and gradient clipping: training operators without an environment handle ---------------------
  * These calls take a device index and a hipStream_t (NULL = the device's default stream) instead of a handle, are asynchronous on that stream,
- * keep nothing between calls, allocate nothing and may be captured into a graph.  Two calls may run at the same time if they share no workspace
+ * keep nothing between calls, allocate nothing on the device and may be captured into a graph.  Two calls may run at the same time if they share no workspace
  * or state.  Element types: */
 enum { Q1ENV_DT_F32 = 0, Q1ENV_DT_BF16 = 1, Q1ENV_DT_F16 = 2 };
 enum { Q1ENV_REDUCE_MEAN = 0, Q1ENV_REDUCE_SUM = 1 };
@@ -615,7 +615,8 @@ uint64_t q1env_head_workspace_bytes(int dtype, int64_t rows, int64_t width, int6
  * rows that are not ignored (Q1ENV_REDUCE_MEAN; 0 when all are). */
 int q1env_head_forward(int device, void* stream, const q1env_head* head, int reduction, float* logp_dev, float* entropy_dev, float* loss_dev);
 /* The gradients of hidden, weight and bias (each may be NULL) for EITHER dlogp / dentropy (float[rows], one may be NULL) OR dloss (one float: the
- * gradient of the loss the forward call wrote).  The head is the one the forward call had, with its state; results are overwritten.  dentropy needs a
+ * gradient of the loss the forward call wrote).  The head is the one the forward call had, with its state; results are overwritten.  A result (of either call) may not
+ * overlap what the call reads, the workspace or another result (rows of one pitch may interleave); state and workspace are aligned to 16 bytes.  dentropy needs a
  * forward call that was asked for the entropy (results are NaN otherwise). */
 int q1env_head_backward(int device, void* stream, const q1env_head* head, const float* dlogp_dev, const float* dentropy_dev, const float* dloss_dev,
                         void* dhidden_dev, int64_t dhidden_stride, void* dweight_dev, int64_t dweight_stride, void* dbias_dev);

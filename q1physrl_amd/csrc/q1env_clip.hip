@@ -193,15 +193,8 @@ struct Job {
     const int64_t *cols, *src_pitch, *dst_pitch;
 };
 
-struct Span { uintptr_t a, b; int i; uintptr_t pitch, row; };        // bytes
-
-// two pitched tensors of the same pitch may interleave: column slices of one matrix
-bool apart(const Span& x, const Span& y) {
-    if (x.b <= y.a || y.b <= x.a) return true;
-    if (!x.pitch || x.pitch != y.pitch) return false;
-    const uintptr_t off = y.a >= x.a ? (y.a - x.a) % x.pitch : (x.pitch - (x.a - y.a) % x.pitch) % x.pitch;      // y's columns within x's rows
-    return off >= x.row && off + y.row <= x.pitch;
-}
+struct Span { Extent x; int i; };
+uintptr_t end_of(const Extent& x) { return x.at + (uintptr_t)(x.rows - 1) * x.pitch + x.row; }
 
 int check_job(const char* who, const Job& j, bool write) {
     if (j.count < 0 || j.count > 65536) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": tensor count out of range (0 .. 65536)");
@@ -234,18 +227,18 @@ int check_job(const char* who, const Job& j, bool write) {
         const int64_t c = j.cols && j.cols[i] ? j.cols[i] : j.values[i], rows = j.values[i] / c;
         const uintptr_t sp = j.cols && j.cols[i] ? (uintptr_t)j.src_pitch[i] * es : 0, dp = j.cols && j.cols[i] ? (uintptr_t)j.dst_pitch[i] * es : 0;
         const uintptr_t sa = (uintptr_t)j.src[i], da = (uintptr_t)j.dst[i];
-        s.push_back({da, da + (rows - 1) * dp + c * es, i, dp, c * es});
-        if (sa != da || sp != dp) s.push_back({sa, sa + (rows - 1) * sp + c * es, ~i, sp, c * es});      // ~i: a source
+        s.push_back({{da, rows, c * es, dp}, i});
+        if (sa != da || sp != dp) s.push_back({{sa, rows, c * es, sp}, ~i});      // ~i: a source
     }
-    const auto before = [](const Span& x, const Span& y) { return x.a < y.a; };
+    const auto before = [](const Span& x, const Span& y) { return x.x.at < y.x.at; };
     if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
     std::vector<size_t> open;
     for (size_t k = 0; k < s.size(); ++k) {
         size_t kept = 0;
         for (size_t o : open) {
-            if (s[o].b <= s[k].a) continue;
+            if (end_of(s[o].x) <= s[k].x.at) continue;
             open[kept++] = o;
-            if ((s[o].i >= 0 || s[k].i >= 0) && !apart(s[o], s[k]))
+            if ((s[o].i >= 0 || s[k].i >= 0) && !apart(s[o].x, s[k].x))
                 return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": a result overlaps another tensor (the same tensor twice, or a destination that is not its own source)");
         }
         open.resize(kept);
@@ -267,6 +260,7 @@ int run(const char* who, int device, hipStream_t stream, const Job& j, bool writ
     if (!norm) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": norm is NULL");
     if (!(scale > 0.0) || std::isinf(scale)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": scale must be positive and finite");
     if (write && !(max_norm >= 0.0)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": max_norm must not be negative or NaN");
+    if ((uintptr_t)ws % 8 || (uintptr_t)norm % 4) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": workspace / norm is not aligned (8 / 4 bytes)");
     if (!ws || ws_bytes < q1env_grad_norm_workspace_bytes(j.count)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": workspace smaller than q1env_grad_norm_workspace_bytes");
     const int64_t unit = unit_of(j);
     for (int i = 0; i < j.count; ++i)
@@ -330,13 +324,13 @@ uint64_t q1env_grad_norm_workspace_bytes(int count) {
 int q1env_grad_norm(int device, void* stream, int count, const void* const* src, const int64_t* values, const int32_t* dtype, const int64_t* cols, const int64_t* pitch, double scale,
                     float* norm, void* ws, uint64_t ws_bytes) {
     const Job j{count, src, nullptr, values, dtype, cols, pitch, nullptr};
-    return run("q1env_grad_norm", device, (hipStream_t)stream, j, false, scale, 0.0, norm, ws, ws_bytes);
+    return no_throw("q1env_grad_norm", [&] { return run("q1env_grad_norm", device, (hipStream_t)stream, j, false, scale, 0.0, norm, ws, ws_bytes); });
 }
 
 int q1env_grad_clip(int device, void* stream, int count, const void* const* src, void* const* dst, const int64_t* values, const int32_t* dtype, const int64_t* cols,
                     const int64_t* src_pitch, const int64_t* dst_pitch, double scale, double max_norm, float* norm, void* ws, uint64_t ws_bytes) {
     const Job j{count, src, dst, values, dtype, cols, src_pitch, dst_pitch};
-    return run("q1env_grad_clip", device, (hipStream_t)stream, j, true, scale, max_norm, norm, ws, ws_bytes);
+    return no_throw("q1env_grad_clip", [&] { return run("q1env_grad_clip", device, (hipStream_t)stream, j, true, scale, max_norm, norm, ws, ws_bytes); });
 }
 
 }  // extern "C"

@@ -22,8 +22,27 @@ int check_head(const char* who, const q1env_head* hd) {
     const uintptr_t size = elem_size(hd->dtype);
     if ((uintptr_t)hd->hidden_dev % size || (uintptr_t)hd->weight_dev % size || (uintptr_t)hd->bias_dev % size)
         return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": a pointer is not aligned to its element size");
+    if ((uintptr_t)hd->state_dev % 16 || (uintptr_t)hd->ws_dev % 16) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": state / workspace is not aligned to 16 bytes");
     if (hd->rows > 0 && !hd->state_dev) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": state is NULL");
     return 0;
+}
+
+// results against everything that is read, the workspace and each other
+int check_apart(const char* who, const Extent* results, int n, const q1env_head& hd, uint64_t ws_bytes, bool backward) {
+    const uintptr_t es = elem_size(hd.dtype);
+    const Extent others[] = {{(uintptr_t)hd.hidden_dev, hd.rows, (uintptr_t)hd.width * es, (uintptr_t)hd.hidden_stride * es},
+                             {(uintptr_t)hd.weight_dev, hd.classes, (uintptr_t)hd.width * es, (uintptr_t)hd.weight_stride * es},
+                             {(uintptr_t)hd.bias_dev, 1, (uintptr_t)hd.classes * es, 0},
+                             {backward ? 0 : (uintptr_t)hd.target_dev, 1, (uintptr_t)hd.rows * hd.target_bits / 8, 0},
+                             {(uintptr_t)hd.state_dev, 1, q1env_head_state_bytes(hd.rows), 0},
+                             {(uintptr_t)hd.ws_dev, 1, ws_bytes, 0}};
+    for (int i = 0; i < n; ++i) {
+        for (const Extent& o : others)
+            if (!apart(results[i], o)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": a result overlaps an operand, the state or the workspace");
+        for (int k = 0; k < i; ++k)
+            if (!apart(results[i], results[k])) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": two results overlap");
+    }
+    return apart(others[4], others[5]) ? 0 : fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": the state overlaps the workspace");
 }
 
 int guard_device(const char* who, int device) {
@@ -50,15 +69,21 @@ uint64_t q1env_head_workspace_bytes(int dtype, int64_t rows, int64_t width, int6
     return workspace_of(dtype, rows, width, classes, backward != 0);
 }
 
-int q1env_head_forward(int device, void* stream, const q1env_head* hd, int reduction, float* logp, float* entropy, float* loss) {
+}  // extern "C"
+
+static int head_forward(int device, void* stream, const q1env_head* hd, int reduction, float* logp, float* entropy, float* loss) {
     const char* who = "q1env_head_forward";
     if (int rc = check_head(who, hd)) return rc;
     if (hd->target_bits != 32 && hd->target_bits != 64) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_forward: target_bits must be 32 or 64");
     if (hd->rows > 0 && (!hd->target_dev || !logp)) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_forward: target / logp is NULL");
     if (loss && !hd->state_dev) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_forward: state is NULL");
     if (reduction != Q1ENV_REDUCE_MEAN && reduction != Q1ENV_REDUCE_SUM) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_forward: unknown reduction");
-    if (hd->rows > 0 && (!hd->ws_dev || hd->ws_bytes < q1env_head_workspace_bytes(hd->dtype, hd->rows, hd->width, hd->classes, 0)))
+    const uint64_t need = hd->rows > 0 ? q1env_head_workspace_bytes(hd->dtype, hd->rows, hd->width, hd->classes, 0) : 0;
+    if (need && (!hd->ws_dev || hd->ws_bytes < need))
         return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_forward: workspace smaller than q1env_head_workspace_bytes(..., 0)");
+    if ((uintptr_t)logp % 4 || (uintptr_t)entropy % 4 || (uintptr_t)loss % 4 || (uintptr_t)hd->target_dev % (hd->target_bits / 8)) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_forward: a pointer is not aligned to its element size");
+    const Extent results[] = {{(uintptr_t)logp, 1, 4 * (uintptr_t)hd->rows, 0}, {(uintptr_t)entropy, 1, 4 * (uintptr_t)hd->rows, 0}, {(uintptr_t)loss, 1, 4, 0}};
+    if (int rc = check_apart(who, results, 3, *hd, need, false)) return rc;
     if (int rc = guard_device(who, device)) return rc;
     DeviceGuard guard(device);
     switch (hd->dtype) {
@@ -68,8 +93,8 @@ int q1env_head_forward(int device, void* stream, const q1env_head* hd, int reduc
     }
 }
 
-int q1env_head_backward(int device, void* stream, const q1env_head* hd, const float* dlogp, const float* dentropy, const float* dloss, void* dhidden, int64_t dhidden_stride,
-                        void* dweight, int64_t dweight_stride, void* dbias) {
+static int head_backward(int device, void* stream, const q1env_head* hd, const float* dlogp, const float* dentropy, const float* dloss, void* dhidden, int64_t dhidden_stride, void* dweight,
+                         int64_t dweight_stride, void* dbias) {
     const char* who = "q1env_head_backward";
     if (int rc = check_head(who, hd)) return rc;
     if (dloss && (dlogp || dentropy)) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_backward: either dloss or the per-row gradients");
@@ -78,8 +103,17 @@ int q1env_head_backward(int device, void* stream, const q1env_head* hd, const fl
     if ((dhidden && dhidden_stride < hd->width) || (dweight && dweight_stride < hd->width)) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_backward: a row stride is smaller than the width");
     const uintptr_t size = elem_size(hd->dtype);
     if ((uintptr_t)dhidden % size || (uintptr_t)dweight % size || (uintptr_t)dbias % size) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_backward: a pointer is not aligned to its element size");
-    if (hd->rows > 0 && (!hd->ws_dev || hd->ws_bytes < q1env_head_workspace_bytes(hd->dtype, hd->rows, hd->width, hd->classes, 1)))
+    const uint64_t need = hd->rows > 0 ? q1env_head_workspace_bytes(hd->dtype, hd->rows, hd->width, hd->classes, 1) : 0;
+    if (need && (!hd->ws_dev || hd->ws_bytes < need))
         return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_backward: workspace smaller than q1env_head_workspace_bytes(..., 1)");
+    if ((uintptr_t)dlogp % 4 || (uintptr_t)dentropy % 4 || (uintptr_t)dloss % 4) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_backward: a pointer is not aligned to its element size");
+    const Extent results[] = {{(uintptr_t)dhidden, hd->rows, hd->width * size, dhidden_stride * size}, {(uintptr_t)dweight, hd->classes, hd->width * size, dweight_stride * size},
+                              {(uintptr_t)dbias, 1, hd->classes * size, 0}};
+    if (int rc = check_apart(who, results, 3, *hd, need, true)) return rc;
+    const Extent upstream[] = {{(uintptr_t)dlogp, 1, 4 * (uintptr_t)hd->rows, 0}, {(uintptr_t)dentropy, 1, 4 * (uintptr_t)hd->rows, 0}, {(uintptr_t)dloss, 1, 4, 0}};
+    for (const Extent& r : results)
+        for (const Extent& u : upstream)
+            if (!apart(r, u)) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_backward: a result overlaps an upstream gradient");
     if (int rc = guard_device(who, device)) return rc;
     DeviceGuard guard(device);
     if (hd->rows == 0) {                             // no sample: the weights' gradients are zero
@@ -94,6 +128,17 @@ int q1env_head_backward(int device, void* stream, const q1env_head* hd, const fl
         case Q1ENV_DT_BF16: return q1_head_backward_bf16(device, (hipStream_t)stream, *hd, dlogp, dentropy, dloss, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
         default: return q1_head_backward_f16(device, (hipStream_t)stream, *hd, dlogp, dentropy, dloss, dhidden, dhidden_stride, dweight, dweight_stride, dbias);
     }
+}
+
+extern "C" {
+
+int q1env_head_forward(int device, void* stream, const q1env_head* hd, int reduction, float* logp, float* entropy, float* loss) {
+    return no_throw("q1env_head_forward", [&] { return head_forward(device, stream, hd, reduction, logp, entropy, loss); });
+}
+
+int q1env_head_backward(int device, void* stream, const q1env_head* hd, const float* dlogp, const float* dentropy, const float* dloss, void* dhidden, int64_t dhidden_stride,
+                        void* dweight, int64_t dweight_stride, void* dbias) {
+    return no_throw("q1env_head_backward", [&] { return head_backward(device, stream, hd, dlogp, dentropy, dloss, dhidden, dhidden_stride, dweight, dweight_stride, dbias); });
 }
 
 }  // extern "C"

@@ -31,6 +31,30 @@
 Q1_HIDDEN int q1_fail(int code, const std::string& msg);
 Q1_HIDDEN const char* q1_last_error_cstr();
 static inline int fail(int code, const std::string& msg) { return q1_fail(code, msg); }
+// runs the body of an entry point that may allocate on the host: no exception leaves the library
+template <typename F> static inline int no_throw(const char* who, F&& f) {
+    try {
+        return f();
+    } catch (...) {                                      // (only the host's memory can run out)
+        try {
+            return fail(Q1ENV_ERR_ALLOC, std::string(who) + ": out of host memory");
+        } catch (...) {
+            return Q1ENV_ERR_ALLOC;
+        }
+    }
+}
+
+// what one operand or result of a call occupies: `rows` rows of `row` bytes, `pitch` bytes apart
+struct Extent { uintptr_t at; int64_t rows; uintptr_t row, pitch; };
+// rows of one pitch may interleave: column slices of one matrix
+static inline bool apart(const Extent& x, const Extent& y) {
+    if (!x.at || !y.at || x.rows <= 0 || y.rows <= 0 || !x.row || !y.row) return true;
+    const uintptr_t xe = x.at + (uintptr_t)(x.rows - 1) * x.pitch + x.row, ye = y.at + (uintptr_t)(y.rows - 1) * y.pitch + y.row;
+    if (xe <= y.at || ye <= x.at) return true;
+    if (!x.pitch || x.pitch != y.pitch) return false;
+    const uintptr_t off = y.at >= x.at ? (y.at - x.at) % x.pitch : (x.pitch - (x.at - y.at) % x.pitch) % x.pitch;      // y's columns within x's rows
+    return off >= x.row && off + y.row <= x.pitch;
+}
 
 #define HIP_TRY(expr)                                                                         \
     do {                                                                                      \

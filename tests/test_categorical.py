@@ -213,8 +213,8 @@ def test_masked_classes(dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("n,d,v", [(2, 73, 2), (1, 64, 40), (31, 48, 70), (60, 200, 130), (100, 64, 300), (256, 136, 257)])
 def test_few_rows_of_16_bits_keep_the_gradient_finer_than_their_type(n, d, v, dtype):
-    """Few rows do not average the roundings of a stored gradient, so it is held in two pieces: ut^2 of it is lost, not ut (ut the type's half step), and the results are off by their
-    own rounding and what float32 leaves: the bounds of the other tests with ut^2 for the stored gradient."""
+    """The few roundings of a gradient of few rows need not even out, so it is held in two pieces: ut^2 of it is lost, not ut (ut the type's half step), and the results are off by
+    their own rounding and what float32 leaves: the bounds of the other tests with ut^2 for the stored gradient."""
     h, w, b, t = make(n, d, v, dtype, seed=n, ignored=0.0)
     leaves = [x.requires_grad_() for x in (h, w, b)]
     got = torch.autograd.grad(categorical.linear_categorical(h, w, t, b), leaves, (torch.ones(n, device="cuda"), torch.full((n,), 0.25, device="cuda")))
@@ -266,6 +266,30 @@ def test_few_rows_or_classes_of_float32(n, d, v, how):
         for name, x, (r, tol) in zip(("dh", "dw", "db"), got, T.grads(A, E if entropy else torch.zeros_like(E))):
             near(x, r, tol, name)
         assert bool((got[0][t == IGN] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("n,d,v", [(20, 64, 700), (300, 64, 31), (1, 36, 90)])
+def test_masked_classes_of_few_rows_or_classes(n, d, v):
+    h, w, b, t = make(n, d, v, torch.float32, seed=4, ignored=0.0)
+    off = torch.zeros(v, dtype=torch.bool, device="cuda")
+    off[3:v // 2] = True
+    off[v - 1] = True
+    t = torch.where(off[t], 1, t)
+    for low in (-float("inf"), torch.finfo(torch.float32).min):
+        bias = torch.where(off, low, b)
+        T = Truth(h, w, torch.where(off, -float("inf"), b), t)
+        logp, ent = categorical.linear_categorical(h, w, t, bias)
+        near(logp, T.logp, T.elogp, "logp")
+        near(ent, T.entropy, T.eent, "entropy")
+        leaves = [x.clone().requires_grad_() for x in (h, w, bias)]
+        A, E = torch.linspace(-1, 1, n, device="cuda"), torch.linspace(0.5, 0.1, n, device="cuda")
+        got = torch.autograd.grad(categorical.linear_categorical(leaves[0], leaves[1], t, leaves[2]), leaves, (A, E))
+        for name, x, (r, tol) in zip(("dh", "dw", "db"), got, T.grads(A, E)):
+            near(x, r, tol, name)
+        assert not bool(got[1][off].any()) and not bool(got[2][off].any())
+    nothing = torch.full_like(b, -float("inf"))
+    assert bool(torch.isnan(categorical.linear_categorical(h, w, t, nothing)[0]).all())
 
 
 @gpu
@@ -459,3 +483,31 @@ def test_the_library_refuses_results():
     assert b(0, None, C.byref(h), 4096, None, None, None, 8, 4096, 7, None) == -1
     assert b(0, None, C.byref(h), 4096, None, None, 4098, 8, None, 8, None) == -1
     assert b"alignment" in lib.q1env_last_error() or b"aligned" in lib.q1env_last_error()
+
+
+def test_the_library_refuses_overlaps_and_odd_addresses():
+    """what a call writes may not overlap what it reads, its workspace or another result; rows of one pitch may interleave (that call goes on to the device)"""
+    lib = _lib.load()
+    rows, width, classes, base = 64, 8, 5, 1 << 24
+    at = dict(hidden_dev=base, weight_dev=base + (1 << 16), bias_dev=base + (2 << 16), target_dev=base + (3 << 16), state_dev=base + (4 << 16), ws_dev=base + (1 << 20))
+    free = base + (8 << 16)
+    f, b = lib.q1env_head_forward, lib.q1env_head_backward
+
+    def refused(rc, what):
+        assert rc == -1 and what in lib.q1env_last_error(), (rc, lib.q1env_last_error())
+    ok = head(rows=rows, width=width, classes=classes, **at)
+    for p in (at["hidden_dev"], at["weight_dev"] + 4, at["bias_dev"], at["target_dev"] + 8, at["state_dev"] + 64, at["ws_dev"] + 16):
+        refused(f(0, None, C.byref(ok), 0, p, None, None), b"overlaps")
+        if p != at["target_dev"] + 8:
+            refused(b(0, None, C.byref(ok), free, None, None, p, width, None, width, None), b"overlap")
+    refused(f(0, None, C.byref(ok), 0, free, free + 4, None), b"overlap")
+    refused(b(0, None, C.byref(ok), free, None, None, free, width, None, width, None), b"upstream")
+    refused(b(0, None, C.byref(ok), free, None, None, free + 4096, width, free + 4096 + 4, width, None), b"two results")
+    refused(f(0, None, C.byref(ok), 0, free + 2, None, None), b"aligned")
+    refused(f(0, None, C.byref(head(rows=rows, width=width, classes=classes, **{**at, "ws_dev": at["ws_dev"] + 8})), 0, free, None, None), b"aligned")
+    refused(f(0, None, C.byref(head(rows=rows, width=width, classes=classes, **{**at, "state_dev": at["ws_dev"] + 256})), 0, free, None, None), b"overlaps the workspace")
+    refused(b(0, None, C.byref(ok), free + 1, None, None, free + 4096, width, None, width, None), b"aligned")
+    pitched = head(rows=rows, width=width, classes=classes, **{**at, "hidden_stride": 2 * width})
+    rc = b(99, None, C.byref(pitched), free, None, None, at["hidden_dev"] + 4 * width, 2 * width, None, width, None)
+    assert rc != 0 and b"overlap" not in lib.q1env_last_error()                # (no such device)
+    refused(b(0, None, C.byref(pitched), free, None, None, at["hidden_dev"] + 4 * width - 4, 2 * width, None, width, None), b"overlap")
