@@ -72,7 +72,7 @@ def allreduce_grads_(params, world, grad_clip=None):
     grads = [p.grad for p in params if p.grad is not None]
     flat = torch.cat([g.reshape(-1) for g in grads])
     dist.all_reduce(flat, op=dist.ReduceOp.SUM)
-    if grad_clip is not None and flat.is_cuda:
+    if grad_clip is not None and flat.is_cuda and all(g.dtype == flat.dtype and g.is_contiguous() for g in grads):
         from .clip import clip_grad_norm_
         return clip_grad_norm_([v.view(g.shape) for v, g in zip(flat.split([g.numel() for g in grads]), grads)], grad_clip, scale=1.0 / world, out=grads)
     flat /= world

@@ -228,3 +228,24 @@ def test_two_ranks_clip_the_average(tmp_path):
     for x, y, m in zip(a[0], b[0], mean):
         assert torch.equal(x, y) and torch.allclose(x, m * (0.25 / norm), rtol=1e-6, atol=1e-12)
     assert abs(float(a[1]) - norm) <= 1e-6 * norm
+
+
+@gpu
+def test_averaged_and_clipped_gradients_of_mixed_types_and_layouts(monkeypatch):
+    """allreduce_grads_(grad_clip=...) where the bucket's views do not have the gradients' types or layouts: the same values as averaging and then clipping."""
+    monkeypatch.setattr(ppo.dist, "all_reduce", lambda t, op=None: t.mul_(2))          # two ranks with the same gradients
+    torch.manual_seed(0)
+    for mixed in (False, True):
+        params = [torch.nn.Parameter(torch.zeros(n, device="cuda")) for n in (300, 40)] + [torch.nn.Parameter(torch.zeros(30, 20, device="cuda"))]
+        if mixed:
+            params[1] = torch.nn.Parameter(torch.zeros(40, device="cuda", dtype=torch.bfloat16))
+        for p in params:
+            p.grad = torch.randn(p.shape, device="cuda").to(p.dtype)
+        params[2].grad = torch.randn(20, 30, device="cuda").t()
+        want = [p.grad.clone() for p in params]
+        norm = torch.sqrt(sum((g.double() ** 2).sum() for g in want))
+        got = ppo.allreduce_grads_(params, 2, 0.5)
+        assert abs(float(got) - float(norm)) <= 1e-6 * float(norm)                     # a double sum rounded once: half a step of float32
+        for p, w in zip(params, want):
+            ref = w.double() * (0.5 / norm)
+            assert bool(((p.grad.double() - ref).abs() <= ref.abs() * (2 ** -8 + 2 ** -22 if p.dtype == torch.bfloat16 else 2 ** -22)).all())
