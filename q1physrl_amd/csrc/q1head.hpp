@@ -331,6 +331,7 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t total, uint32_t ti
 // ------------------------------------------------------------------------------------------------------------------------------
 // Operands that the loads above cannot take as they lie (float32; a width that is not a multiple of 8, addresses or strides that are not multiples of 16 bytes) are laid out
 // first: [piece][row][padded], padded = width rounded up to 64 with zeros; rows that do not count are zero.
+// Bound: memory (32768 + 1441 float32 rows of 256: 16 us for 35 MB read and 53 written, 5.4 TB/s).
 struct Lay {
     const void* src;
     int64_t stride, rows;             // elements
@@ -419,7 +420,10 @@ __device__ __forceinline__ void start(Acc<C>& acc, const void* bias, int64_t bas
         }
 }
 
-// class-tile statistics of each row, and the logit of the row's own class
+// class-tile statistics of each row, and the logit of the row's own class.  The accumulators never leave the registers: one fused multiply-add, one exponential, an addition (and two more
+// instructions for the entropy) per logit, then three floats per row and tile.
+// Bound: the matrix pipe where k is long (8192 x 2048 x 131072 bfloat16: 3.40 ms, 1290 TFLOP/s, the pipe 67 % busy, no bank conflict; a large library product makes 1225 to 1481); the weights
+// where there are few rows (64 x 4096 x 131073: 194 us, 5.5 TB/s); start and epilogue of a tile where k is short (50000 x 256 x 4097: 165 us, 640 TFLOP/s, four steps of k in a tile).
 template <class C, int DT, bool ENTROPY>
 __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target target, int64_t tile0, float* __restrict__ part, float* __restrict__ own_logit) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -496,7 +500,7 @@ __global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target 
 
 // Joins the tiles' statistics: R rows per workgroup, 1024 / R lanes take the tiles of a row in turn (four loads of each kind in flight); lse is kept in units of log2.  Also leaves what the
 // backward pass wants of the classes: -1 / -2 / the class, and the rows that count as bytes and as bits.  R = 64 where there are many rows, 16 where there are many tiles (64 rows
-// of 1025 tiles: 21 us with R = 64).
+// of 1025 tiles: 21 us with R = 64, 12 with 16).  Bound: latency (8192 rows of 512 tiles: 14 us for 50 MB).
 template <int R>
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ part, const float* __restrict__ own_logit, Target target, int64_t rows, int tiles, int with_entropy,
                                                     float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ entropy_kept, float* __restrict__ lse,
@@ -680,6 +684,8 @@ __device__ __forceinline__ float sums_of_32(float (&v)[32], int lane, int& which
 
 // a piece [c0, c1) of the classes: the logits again, and the gradient of each -> g[row][class - c0] (stride `piece`; 16 bits, float32 as three pieces g_plane values apart), zero
 // up to the end of the last tile; and the sums over this tile's rows -> db_part[row tile][class]
+// Bound: as statistics_kernel, and 16 bits per logit written (8192 x 2048 x 28672: 844 us, 1140 TFLOP/s, 470 MB; 50000 x 256 x 4097: 255 us, 410 MB).  Storing g costs less than a third
+// computation of the logits, which both products would otherwise need.
 // GP: pieces the gradient is stored in.  One in 16-bit types: its rounding leaves an error of the size that the result's own rounding leaves anyway (bfloat16, random upstream, 50176 rows:
 // 0.0024 of the results' norm instead of 0.0017), and a second piece would double the products.  Two up to 256 rows, where the few roundings need not even out (2 rows of 2 classes: 0.004 with
 // one, 0.0017 with two) and the products are bound by memory; three for float32.
@@ -958,6 +964,9 @@ __global__ void __launch_bounds__(256) skinny_gradient_kernel(Skinny q, Upstream
     }
 }
 
+// dW = g^T h and dh = g W from the stored gradient, both in one launch where they take the same tiles.  The operands lie with k outermost (h, W, and g for dW): ds_read_tr turns them on the
+// way from the LDS.  A sum is split over workgroups where its tiles would leave CUs idle; the parts are added in order (same bits every time), no atomics.
+// Bound: the matrix pipe (8192 x 2048 x 28672, both: 1.65 ms, 1165 TFLOP/s, 58 % busy; 50000 x 256 x 4097: 250 us, 840 TFLOP/s: 451 units of work on 256 CUs).
 // out[n][m] (stride out_stride): m = column of the result (width), n = its row.  slab: the sums stay in float32 [split][rows][width] for
 // finish_kernel (accumulate: added to what is there); without it the scaled result is stored.
 struct Product {
@@ -1135,7 +1144,7 @@ __global__ void __launch_bounds__(256) skinny_product_kernel(SkinnyProduct q, Up
     }
 }
 
-// result = scale x sum of the slabs, in their order; and db[class] = scale x sum over the row tiles: 64 classes per workgroup, wave g takes tiles g, g + 4, ...
+// result = scale x sum of the slabs, in their order (22 us for 15 slabs of 4097 x 256 and the bias at 50000 rows); and db[class] = scale x sum over the row tiles: 64 classes per workgroup, wave g takes tiles g, g + 4, ...
 struct Finish {
     const float* slab;
     int64_t splits, rows, width;
