@@ -83,9 +83,9 @@ struct Op {
     const uint64_t* live;       // KM: where set, bit k of the words says whether row k counts (rows that do not are zero whatever memory holds)
 };
 
-template <int BM_, int BN_, int WM_, int WN_, int BK_, int STAGES_> struct Config {
+template <int BM_, int BN_, int WM_, int WN_, int BK_, int STAGES_, int PER_SIMD_ = 1> struct Config {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_;
-    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, PER_SIMD = PER_SIMD_;          // PER_SIMD: waves the registers have to suffice for
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;             // 32 x 32 tiles per wave
     static constexpr int LA = BM * BK / 512 / WAVES, LB = BN * BK / 512 / WAVES;         // load instructions per wave and stage
     static constexpr int A_BYTES = BM * BK * 2, STAGE_BYTES = (BM + BN) * BK * 2, LDS_BYTES = STAGES * STAGE_BYTES;
@@ -423,9 +423,10 @@ __device__ __forceinline__ void start(Acc<C>& acc, const void* bias, int64_t bas
 // class-tile statistics of each row, and the logit of the row's own class.  The accumulators never leave the registers: one fused multiply-add, one exponential, an addition (and two more
 // instructions for the entropy) per logit, then three floats per row and tile.
 // Bound: the matrix pipe where k is long (8192 x 2048 x 131072 bfloat16: 3.40 ms, 1290 TFLOP/s, the pipe 67 % busy, no bank conflict; a large library product makes 1225 to 1481); the weights
-// where there are few rows (64 x 4096 x 131073: 194 us, 5.5 TB/s); start and epilogue of a tile where k is short (50000 x 256 x 4097: 165 us, 640 TFLOP/s, four steps of k in a tile).
+// where there are few rows (64 x 4096 x 131073: 194 us, 5.5 TB/s); start and epilogue of a tile where k is short (50176 x 256 x 4352: 151 us, 739 TFLOP/s, two workgroups per CU in different phases; 164 with one of
+// 256 x 256).
 template <class C, int DT, bool ENTROPY>
-__global__ void __launch_bounds__(C::THREADS) statistics_kernel(Head hd, Target target, int64_t tile0, float* __restrict__ part, float* __restrict__ own_logit) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) statistics_kernel(Head hd, Target target, int64_t tile0, float* __restrict__ part, float* __restrict__ own_logit) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t tm, tn, z;
     tile_of(blockIdx.x, gridDim.x, hd.tiles_m, hd.tiles_n, tm, tn, z);
@@ -684,13 +685,13 @@ __device__ __forceinline__ float sums_of_32(float (&v)[32], int lane, int& which
 
 // a piece [c0, c1) of the classes: the logits again, and the gradient of each -> g[row][class - c0] (stride `piece`; 16 bits, float32 as three pieces g_plane values apart), zero
 // up to the end of the last tile; and the sums over this tile's rows -> db_part[row tile][class]
-// Bound: as statistics_kernel, and 16 bits per logit written (8192 x 2048 x 28672: 844 us, 1140 TFLOP/s, 470 MB; 50000 x 256 x 4097: 255 us, 410 MB).  Storing g costs less than a third
+// Bound: as statistics_kernel, and 16 bits per logit written (8192 x 2048 x 28672: 844 us, 1140 TFLOP/s, 470 MB; 50176 x 256 x 4352: 219 us, 437 MB).  Storing g costs less than a third
 // computation of the logits, which both products would otherwise need.
 // GP: pieces the gradient is stored in.  One in 16-bit types: its rounding leaves an error of the size that the result's own rounding leaves anyway (bfloat16, random upstream, 50176 rows:
 // 0.0024 of the results' norm instead of 0.0017), and a second piece would double the products.  Two up to 256 rows, where the few roundings need not even out (2 rows of 2 classes: 0.004 with
 // one, 0.0017 with two) and the products are bound by memory; three for float32.
 template <class C, int DT, int GP, bool ENTROPY>
-__global__ void __launch_bounds__(C::THREADS) gradient_kernel(Head hd, Upstream up, int64_t piece, int64_t g_plane, const float* __restrict__ lse,
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) gradient_kernel(Head hd, Upstream up, int64_t piece, int64_t g_plane, const float* __restrict__ lse,
                                                               const float* __restrict__ entropy, uint16_t* __restrict__ g, float* __restrict__ db_part) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t tm, tn, zz;
@@ -1051,7 +1052,7 @@ __device__ __forceinline__ void product_tile(const Product& pr, const Upstream& 
 // The weights' gradient (both operands with the rows as k) and the hidden rows' (the weights with the classes as k) of one piece, in one launch: neither fills the device's last
 // round alone.  groups: workgroups of the first, a multiple of 8 (the XCDs' turn) unless it is the only one.
 template <class C, int DT, int GP>
-__global__ void __launch_bounds__(C::THREADS) products_kernel(Product dw, Product dh, Upstream up, uint32_t dw_tiles, uint32_t dw_groups) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) products_kernel(Product dw, Product dh, Upstream up, uint32_t dw_tiles, uint32_t dw_groups) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     if (blockIdx.x < dw_groups) {
         if (blockIdx.x < dw_tiles) product_tile<C, DT, GP, true, true>(dw, up, blockIdx.x, dw_tiles, lds);
@@ -1059,7 +1060,7 @@ __global__ void __launch_bounds__(C::THREADS) products_kernel(Product dw, Produc
         product_tile<C, DT, GP, true, false>(dh, up, blockIdx.x - dw_groups, gridDim.x - dw_groups, lds);
 }
 template <class C, int DT, int GP>
-__global__ void __launch_bounds__(C::THREADS) rows_product_kernel(Product dh, Upstream up) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) rows_product_kernel(Product dh, Upstream up) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     product_tile<C, DT, GP, true, false>(dh, up, blockIdx.x, gridDim.x, lds);
 }

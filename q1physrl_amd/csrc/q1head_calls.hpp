@@ -11,13 +11,14 @@
 namespace q1head {
 namespace {
 
-constexpr uint64_t PIECE_BYTES = 448ull << 20;     // of the gradient of one piece of the classes
+constexpr uint64_t PIECE_BYTES = 448ull << 20;     // of the gradient of one piece of the classes (half of it: 15 % slower at 50000 x 256 x 4097 and 4096 x 1024 x 32768, 1 % at 8192 x 2048 x 131072)
 constexpr uint64_t LAID_BYTES = 96ull << 20;       // of the laid-out weights of one piece
 constexpr int64_t MAX_ROWS = 1 << 22, MAX_WIDTH = 1 << 16, MAX_CLASSES = 1 << 22;
 constexpr int64_t PIECE_STEP = 256;                // pieces are whole tiles of every configuration
 
 typedef Config<256, 256, 2, 4, 64, 2> Large;           // 128 KB of LDS: one workgroup of eight waves per CU
 typedef Config<128, 128, 2, 2, 64, 2> Middle;          // 64 KB: two workgroups of four waves per CU, one computes while the other waits
+typedef Config<128, 256, 2, 4, 32, 3, 4> Pair;         // 77 KB: two workgroups of eight waves per CU, one's epilogue beside the other's products; for logits of 16-bit types with a short k
 typedef Config<64, 64, 2, 2, 64, 4> Small;         // where Middle's tiles would leave most CUs idle: 64 KB, four steps in flight
 typedef Config<128, 64, 4, 1, 64, 3> Few;              // up to 64 rows: 72 KB, two workgroups per CU
 typedef Config<128, 32, 4, 1, 64, 4> Fewest;           // up to 32 rows: 80 KB, two workgroups per CU
@@ -46,15 +47,19 @@ struct State {
     }
 };
 
-enum Size { LARGE, MIDDLE, SMALL, FEW, FEWEST };
+enum Size { LARGE, MIDDLE, SMALL, PAIR, FEW, FEWEST };
 int64_t bm_of(Size s) { return s == LARGE ? 256 : s == SMALL ? 64 : 128; }
-int64_t bn_of(Size s) { return s == LARGE ? 256 : s == MIDDLE ? 128 : s == FEWEST ? 32 : 64; }
+int64_t bn_of(Size s) { return s == LARGE || s == PAIR ? 256 : s == MIDDLE ? 128 : s == FEWEST ? 32 : 64; }
 
 // The tile of a product of m x n results with k terms, and into how many parts its sum is split, by what it should take in nanoseconds.  One round of Large workgroups (256,
-// one per CU) was measured at 31 ns per term of k (1075 TFLOP/s), one of Middle (512, two per CU) at 18 (930); `start` is what a round costs besides (prologue and epilogue: 3.3 / 2.5 us for the
-// statistics, 12 / 7 for the gradient, at 50000 x 256 x 4097); the slabs of a split sum are written and read once at 4.5 TB/s.  `split` false: one part only.
+// one per CU) was measured at 31 ns per term of k (1075 TFLOP/s), one of Middle (512, two per CU) at 18 (930), of Pair (512) at 36; Start is what a round costs besides, prologue and epilogue:
+// 50176 x 256 x 4352 takes 164 / 189 / 151 us of statistics and 250 / 294 / 219 of gradients in Large / Middle / Pair, 4096 x 1024 x 32768 282 / 356 / 331 of statistics.  The slabs of a split sum
+// are written and read once at 4.5 TB/s.
+struct Start { double large, middle, pair; };          // nanoseconds; pair 0: not for this product
+constexpr Start STATISTICS{4500.0, 2600.0, 2400.0}, GRADIENT{11500.0, 6800.0, 7600.0}, PRODUCT{4000.0, 3000.0, 0.0};
+// `split` false: one part only
 struct Shape { Size size; int parts; int64_t len; };
-Shape shape_of(int64_t m, int64_t n, int64_t k, int products, bool split, double start_large, double start_middle, bool k_major) {
+Shape shape_of(int64_t m, int64_t n, int64_t k, int products, bool split, const Start& starts, bool k_major) {
     if (n <= 64 && !k_major) {                        // few rows: 512 workgroups (two per CU), parts of 512 terms at least
         const Size s = n <= 32 ? FEWEST : FEW;
         const int64_t tiles = div_up(m, bm_of(s));
@@ -64,14 +69,15 @@ Shape shape_of(int64_t m, int64_t n, int64_t k, int products, bool split, double
     }
     Shape best{MIDDLE, 1, round_up(k, PART_STEP)};
     double least = 0.0;
-    for (int s = LARGE; s <= SMALL; ++s) {
+    for (int s = LARGE; s <= PAIR; ++s) {
+        if (s == PAIR && (starts.pair == 0.0 || products > 1)) continue;
         const int64_t tiles = div_up(m, bm_of((Size)s)) * div_up(n, bn_of((Size)s)), slots = s == LARGE ? 256 : 512;
-        const double start = s == LARGE ? start_large : s == MIDDLE ? start_middle : start_middle / 2;
+        const double start = s == LARGE ? starts.large : s == MIDDLE ? starts.middle : s == PAIR ? starts.pair : starts.middle / 2;
         const int64_t most = split ? std::min<int64_t>(div_up(k, 256), std::max<int64_t>(1, div_up(4 * slots, tiles))) : 1;
         for (int64_t parts = 1; parts <= most; ++parts) {
             const int64_t len = round_up(div_up(k, parts), PART_STEP), real = div_up(k, len), groups = tiles * real;
             // a term of k of one round; of a round that leaves every workgroup a CU to itself
-            const double full = s == LARGE ? 31.0 : s == MIDDLE ? 18.0 : 9.5, alone = s == LARGE ? 31.0 : s == MIDDLE ? 11.0 : 5.0;
+            const double full = s == LARGE ? 31.0 : s == MIDDLE ? 18.0 : s == PAIR ? 36.0 : 9.5, alone = s == LARGE ? 31.0 : s == MIDDLE ? 11.0 : s == PAIR ? 20.0 : 5.0;
             double t = (double)div_up(groups, slots) * ((double)len * products * (groups <= 256 ? alone : full) + start);
             if (real > 1) t += 3000.0 + (double)real * (double)m * (double)n * 8.0 / 4500.0;
             if (least == 0.0 || t < least) { least = t; best = Shape{(Size)s, (int)real, len}; }
@@ -99,7 +105,7 @@ void split_together(Shape& dw, int64_t dw_m, int64_t dw_n, int64_t dw_k, Shape& 
     if (dw.size != dh.size || dw.size > SMALL) return;
     const Size s = dw.size;
     const int64_t slots = s == LARGE ? 256 : 512, ta = div_up(dw_m, bm_of(s)) * div_up(dw_n, bn_of(s)), tb = div_up(dh_m, bm_of(s)) * div_up(dh_n, bn_of(s));
-    const double step = (s == LARGE ? 31.0 : s == MIDDLE ? 18.0 : 9.5) * products, start = s == LARGE ? 4000.0 : s == MIDDLE ? 3000.0 : 1500.0;
+    const double step = (s == LARGE ? 31.0 : s == MIDDLE ? 18.0 : 9.5) * products, start = s == LARGE ? PRODUCT.large : s == MIDDLE ? PRODUCT.middle : PRODUCT.middle / 2;
     auto slabs = [](int64_t parts, int64_t m, int64_t n) { return parts > 1 ? (double)parts * (double)m * (double)n * 8.0 / 4500.0 : 0.0; };
     if ((double)(ta * dw_k + tb * dh_k) * step / (double)slots < 50000.0) return;                       // not worth the search
     double least = 0.0;
@@ -162,8 +168,8 @@ Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward
     p.piece = piece;
     p.pieces = div_up(classes, piece);
     const int products = planes_of(dt) == 3 ? 6 : 1;
-    p.logits = shape_of(std::min(piece, classes), rows, width, products, false, backward ? 12000.0 : 3300.0, backward ? 7000.0 : 2500.0, false).size;
-    if (backward && p.two && p.logits == LARGE) p.logits = MIDDLE;            // (the registers of a Large tile do not last for the second piece)
+    p.logits = shape_of(std::min(piece, classes), rows, width, products, false, backward ? GRADIENT : STATISTICS, false).size;
+    if (backward && p.two && (p.logits == LARGE || p.logits == PAIR)) p.logits = MIDDLE;          // (the others' registers do not last for the second piece)
     uint64_t at = 0;
     auto take = [&](uint64_t n) { const uint64_t o = at; at += aligned(n); return o; };
     if (!backward) {
@@ -183,8 +189,8 @@ Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward
         p.dh_slab = take(p.dh_split > 1 ? 4 * (uint64_t)p.dh_split * rows * width : 0);
         p.dw_slab = take(p.dw_split > 1 ? 4 * (uint64_t)p.dw_split * classes * width : 0);
     } else {
-        Shape dh = shape_of(width, rows, std::min(piece, classes), products * (p.two ? 2 : 1), true, 4000.0, 3000.0, false);
-        Shape dw = shape_of(width, std::min(piece, classes), rows, products * (p.two ? 2 : 1), true, 4000.0, 3000.0, true);
+        Shape dh = shape_of(width, rows, std::min(piece, classes), products * (p.two ? 2 : 1), true, PRODUCT, false);
+        Shape dw = shape_of(width, std::min(piece, classes), rows, products * (p.two ? 2 : 1), true, PRODUCT, true);
         split_together(dw, width, std::min(piece, classes), rows, dh, width, rows, std::min(piece, classes), products * (p.two ? 2 : 1));
         p.dh = dh.size; p.dh_split = dh.parts; p.dh_k = dh.len;
         p.dw = dw.size; p.dw_split = dw.parts; p.dw_k = dw.len;
@@ -340,6 +346,7 @@ int forward(const Where& at, const q1env_head& q, int reduction, float* logp, fl
             const bool e = entropy != nullptr;
             if (p.logits == LARGE) Q1_TRY((statistics<Large, DT>(at, hd, target, e, part, own)));
             else if (p.logits == MIDDLE) Q1_TRY((statistics<Middle, DT>(at, hd, target, e, part, own)));
+            else if (p.logits == PAIR) Q1_TRY((statistics<std::conditional_t<DT == F32, Middle, Pair>, DT>(at, hd, target, e, part, own)));          // (never float32)
             else if (p.logits == SMALL) Q1_TRY((statistics<Small, DT>(at, hd, target, e, part, own)));
             else if (p.logits == FEW) Q1_TRY((statistics<Few, DT>(at, hd, target, e, part, own)));
             else Q1_TRY((statistics<Fewest, DT>(at, hd, target, e, part, own)));
@@ -413,6 +420,7 @@ int backward(const Where& at, const q1env_head& q, const Plan& p, bool hp, bool 
         const Head hd{w, h, q.bias_dev, st.target, n, d, v, 0, 0, c0, c1};
         if (p.logits == LARGE) Q1_TRY((gradient<std::conditional_t<GP == 2, Middle, Large>, DT, GP>(at, hd, up, p.piece, st, g, db_part)));          // (two pieces: never LARGE)
         else if (p.logits == MIDDLE) Q1_TRY((gradient<Middle, DT, GP>(at, hd, up, p.piece, st, g, db_part)));
+        else if (p.logits == PAIR) Q1_TRY((gradient<std::conditional_t<GP == 1, Pair, Middle>, DT, GP>(at, hd, up, p.piece, st, g, db_part)));          // (one piece: never float32)
         else if (p.logits == SMALL) Q1_TRY((gradient<Small, DT, GP>(at, hd, up, p.piece, st, g, db_part)));
         else if (p.logits == FEW) Q1_TRY((gradient<Few, DT, GP>(at, hd, up, p.piece, st, g, db_part)));
         else Q1_TRY((gradient<Fewest, DT, GP>(at, hd, up, p.piece, st, g, db_part)));
