@@ -111,6 +111,29 @@ def test_rows_and_gradients(n, d, v, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(20001, 72, 2049), (3000, 136, 2100), (1500, 300, 9000), (5000, 520, 3000), (2047, 1001, 8200), (4100, 1024, 5000), (8200, 1040, 8300)])
+def test_sizes_of_every_tile(n, d, v, dtype):
+    """sizes at which every tile, whole and split sums, and both backward products together and apart take their turn, with partial tiles on every side"""
+    h, w, b, t = make(n, d, v, dtype, seed=v, ignored=0.2)
+    h = torch.where((t == IGN)[:, None], float("nan"), h)
+    leaves = [x.requires_grad_() for x in (h, w, b)]
+    logp, ent = categorical.linear_categorical(h, w, t, b)
+    T = Truth(h, w, b, t)
+    near(logp, T.logp, T.elogp, "logp")
+    near(ent, T.entropy, T.eent, "entropy")
+    g = torch.Generator(device="cuda").manual_seed(9)
+    A, E = torch.randn(n, device="cuda", generator=g), torch.randn(n, device="cuda", generator=g) * 0.1
+    for name, x, (r, tol) in zip(("dh", "dw", "db"), torch.autograd.grad((logp, ent), leaves, (A, E)), T.grads(A, E)):
+        near(x, r, tol, name)
+    loss, *got = categorical.linear_cross_entropy_grad(h, w, t, b)
+    k = T.ok.double().sum()
+    near(loss, -T.logp.sum() / k, (T.elogp * T.ok).sum() / k + 2 * U * T.logp.abs().sum() / k, "loss")
+    for name, x, (r, tol) in zip(("dh", "dw", "db"), got, T.grads((-1.0 / k).expand(n), torch.zeros(n, device="cuda"))):
+        near(x, r, tol, name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("n,d,v", [(1, 16, 3), (200, 256, 361), (129, 100, 1025)])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_cross_entropy(n, d, v, dtype, reduction):
@@ -328,6 +351,46 @@ def test_strides_and_alignment(dtype, d):
     assert got[1].shape == (7, 11, d) and torch.equal(got[1].view(n, d), ref[1]) and torch.equal(got[2], ref[2])
     logp, ent = categorical.linear_categorical(h.view(7, 11, d), w, t.view(7, 11), b)
     assert logp.shape == ent.shape == (7, 11)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_offsets_past_32_bits(dtype):
+    """a weight of more than 2^32 bytes, and rows of hidden further apart than the loads into the LDS reach (they are laid out first)"""
+    n, d, v = (40, 32776, 66001) if dtype == torch.bfloat16 else (33, 16392, 66001)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = (torch.randn(v, d, device="cuda", generator=g, dtype=torch.float32) * (2.0 / math.sqrt(d))).to(dtype)
+    h = torch.randn(n, d, device="cuda", generator=g).to(dtype)
+    t = torch.randint(0, v, (n,), device="cuda", generator=g)
+    t[:4] = torch.tensor([v - 1, v - 2, 0, IGN], device="cuda")
+    z = torch.cat([h.double() @ c.double().T for c in w.split(4096)], 1)
+    absz = torch.cat([h.double().abs() @ c.double().abs().T for c in w.split(4096)], 1)
+    ok = t != IGN
+    lse = torch.logsumexp(z, 1)
+    el = ((d + 8) * 2 * U * absz).amax(1)
+    logp = torch.where(ok, z.gather(1, t.clamp(min=0)[:, None])[:, 0] - lse, 0.0)
+    e = 2 * (2 * el + (256 + v / 2048 + 16) * 2 * U + 8 * U * (lse.abs() + logp.abs() + 1))
+    loss, dh, dw, _ = categorical.linear_cross_entropy_grad(h, w, t)
+    k = ok.double().sum()
+    near(loss, -logp.sum() / k, (e / 2 * ok).sum() / k + 2 * U * logp.abs().sum() / k, "loss")
+    p = torch.exp(z - lse[:, None])
+    q = p.clone()
+    q[ok.nonzero()[:, 0], t[ok]] -= 1.0
+    q = torch.where(ok[:, None], q / k, 0.0)
+    off = torch.where(ok[:, None], p * (e[:, None] + 4 * U) / k, 0.0) + (HALF[dtype] + 4 * U) * q.abs()
+    for part in (slice(0, 64), slice(v - 64, v)):
+        ref = q[:, part].T @ h.double()
+        near(dw[part], ref, off[:, part].T @ h.double().abs() * 1.01 + (n + 8) * 2 * U * (q[:, part].abs().T @ h.double().abs()) + HALF[dtype] * ref.abs() * 1.01 + 1e-30, "dw")
+    ref = sum(q[:, c0:c0 + 4096] @ w[c0:c0 + 4096].double() for c0 in range(0, v, 4096))
+    size = sum(off[:, c0:c0 + 4096] @ w[c0:c0 + 4096].double().abs() for c0 in range(0, v, 4096))
+    total = sum(q[:, c0:c0 + 4096].abs() @ w[c0:c0 + 4096].double().abs() for c0 in range(0, v, 4096))
+    near(dh, ref, size * 1.01 + (v + 8) * 2 * U * total + HALF[dtype] * ref.abs() * 1.01 + 1e-30, "dh")
+    del w, dw
+    wide = torch.zeros(n, 2 ** 21 + 16, dtype=dtype, device="cuda")
+    wide[:, 8:8 + 512] = h[:, :512]
+    w2, b2 = torch.randn(300, 512, device="cuda", generator=g).to(dtype), None
+    got, want = categorical.linear_cross_entropy_grad(wide[:, 8:520], w2, t % 300, b2), categorical.linear_cross_entropy_grad(h[:, :512].contiguous(), w2, t % 300, b2)
+    assert all(torch.equal(x, y) for x, y in zip(got, want) if x is not None)
 
 
 @gpu

@@ -117,6 +117,25 @@ def test_what_is_not_finite_is_not_hidden():
 
 
 @gpu
+def test_more_than_32_bits_of_values():
+    """a tensor of more than 2^31 values (2^32 bytes), and rows of one further apart than that in all"""
+    n = 2 ** 31 + 77
+    g = torch.full((n,), 0.25, device="cuda", dtype=torch.bfloat16)
+    g[-1] = 3.0
+    norm = clip.clip_grad_norm_([g], 1.0)
+    true = math.sqrt((n - 1) * 0.0625 + 9.0)
+    assert abs(float(norm) - true) <= 2.0 ** -23 * true
+    want = torch.tensor([0.25 / true, 3.0 / true], dtype=torch.float64)
+    got = torch.stack([g[0], g[-1]]).double().cpu()
+    assert bool(((got - want).abs() <= want * (2.0 ** -8 + 2.0 ** -22)).all()) and bool((g[:-1] == g[0]).all())
+    rows = g[:2 ** 31].view(2 ** 11, 2 ** 20)[:, 5:9]
+    rows.fill_(2.0)
+    assert abs(float(clip.grad_norm([rows])) - math.sqrt(4.0 * 4 * 2 ** 11)) <= 2.0 ** -23 * 200
+    clip.clip_grad_norm_([rows], 0.0)
+    assert not bool(rows.any()) and float(g[4]) == float(g[0]) and float(g[9]) == float(g[0])
+
+
+@gpu
 def test_zero_gradients_and_a_zero_bound():
     z = [torch.zeros(100, device="cuda"), torch.zeros(0, device="cuda")]
     assert float(clip.clip_grad_norm_(z, 0.0)) == 0.0 and not bool(z[0].any())
