@@ -12,7 +12,9 @@ namespace q1head {
 namespace {
 
 constexpr uint64_t PIECE_BYTES = 448ull << 20;     // of the gradient of one piece of the classes (half of it: 15 % slower at 50000 x 256 x 4097 and 4096 x 1024 x 32768, 1 % at 8192 x 2048 x 131072)
-constexpr uint64_t LAID_BYTES = 96ull << 20;       // of the laid-out weights of one piece
+// of the laid-out weights of one piece.  float32 always needs them: a piece of 96 MiB costs 10 to 20 % (1578 x 1344 x 16658: 2115 us against 1726, 64 x 1024 x 50000 forward 238 against 180); 16-bit
+// weights only where they are not aligned
+constexpr uint64_t laid_bytes(int dt) { return dt == 0 ? 448ull << 20 : 160ull << 20; }
 constexpr int64_t MAX_ROWS = 1 << 22, MAX_WIDTH = 1 << 16, MAX_CLASSES = 1 << 22;
 constexpr int64_t PIECE_STEP = 256;                // pieces are whole tiles of every configuration
 
@@ -152,6 +154,19 @@ void skinny_split(int64_t tiles, int64_t k, int& n, int64_t& len) {
     n = (int)div_up(k, len);
 }
 
+// of the pieces of at most `most` classes that come to `pieces` of them, the size whose 256 x 256 tiles take the fewest rounds over the CUs (4096 x 1024 x 32768 float32: two of 16384 instead of
+// 18944 and 13824 take 5200 us instead of 5880; 8192 x 2048 x 131072: four of 28672 and one of 16384 14470, five of 26368 15000)
+int64_t even_piece(int64_t most, int64_t pieces, int64_t classes, int64_t rows) {
+    if (pieces == 1) return most;
+    const int64_t r = div_up(rows, 256), all = div_up(classes, PIECE_STEP), last = most / PIECE_STEP, first = std::min(last, div_up(all, pieces)), step = std::max<int64_t>(1, (last - first) / 64);
+    int64_t best = first, least = INT64_MAX;
+    for (int64_t c = first; c <= last; c += step) {
+        const int64_t whole = all / c, rounds = whole * div_up(c * r, 256) + div_up((all - whole * c) * r, 256);
+        if (rounds <= least) { least = rounds; best = c; }                    // (the largest of equals: longer sums in dh)
+    }
+    return best * PIECE_STEP;
+}
+
 // w_in_place / h_in_place: the workspace has to suffice for any address, so its size is asked for with both false
 Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward, bool h_in_place, bool w_in_place) {
     Plan p{};
@@ -163,9 +178,10 @@ Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward
     int64_t piece = all;
     const int64_t g_pieces = p.two ? 2 : planes_of(dt);                        // of the stored gradient
     const int64_t laid = planes_of(dt) * 2 * p.padded;                        // bytes of a laid-out row
-    if (!w_in_place) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(LAID_BYTES / laid) / PIECE_STEP * PIECE_STEP));
+    if (!w_in_place) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(laid_bytes(dt) / laid) / PIECE_STEP * PIECE_STEP));
     if (backward) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(PIECE_BYTES / (2 * g_pieces * rows)) / PIECE_STEP * PIECE_STEP));
-    p.piece = piece;
+    p.pieces = div_up(classes, piece);
+    p.piece = piece = even_piece(piece, p.pieces, classes, rows);
     p.pieces = div_up(classes, piece);
     const int products = planes_of(dt) == 3 ? 6 : 1;
     p.logits = shape_of(std::min(piece, classes), rows, width, products, false, backward ? GRADIENT : STATISTICS, false).size;
