@@ -111,9 +111,10 @@ def test_rows_and_gradients(n, d, v, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("n,d,v", [(20001, 72, 2049), (3000, 136, 2100), (1500, 300, 9000), (5000, 520, 3000), (2047, 1001, 8200), (4100, 1024, 5000), (8200, 1040, 8300)])
+@pytest.mark.parametrize("n,d,v", [(20001, 72, 2049), (3000, 136, 2100), (1500, 300, 9000), (5000, 520, 3000), (2047, 1001, 8200), (4100, 1024, 5000), (8200, 1040, 8300), (70, 4095, 60000), (400, 4094, 45000)])
 def test_sizes_of_every_tile(n, d, v, dtype):
-    """sizes at which every tile, whole and split sums, and both backward products together and apart take their turn, with partial tiles on every side"""
+    """sizes at which every tile, whole and split sums, and both backward products together and apart take their turn, with partial tiles on every side; and laid-out
+    weights of every type in several pieces"""
     h, w, b, t = make(n, d, v, dtype, seed=v, ignored=0.2)
     h = torch.where((t == IGN)[:, None], float("nan"), h)
     leaves = [x.requires_grad_() for x in (h, w, b)]
