@@ -385,6 +385,9 @@ struct Head {
 };
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// A probability below 2^NOTHING is zero in float32 (the smallest value is 2^-149).  Its logarithm is held to that in the entropy's gradient, where it is multiplied by an upstream value before the
+// probability: a class at -inf, or at the type's lowest value, gives 0 x a finite factor.
+constexpr float NOTHING = -160.0f;
 
 // Statistics of a set of classes in units of log2: maximum m of l log2(e), s = sum 2^(l log2(e) - m), u = sum (l log2(e) - m) 2^(l log2(e) - m).  One fused
 // multiply-add and one hardware exponential per logit; the reference m is subtracted inside the fma, so no rounding of l log2(e) itself enters.
@@ -740,8 +743,7 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) gradient_kernel(Head 
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float d = fmaf(acc.t[i][j][r], LOG2E, -z), p = __builtin_amdgcn_exp2f(d);
-                // g = -p (A + E (log p + H)); a class at -inf has p = 0 and a finite factor
-                const float v = ENTROPY ? -p * fmaf(El, fmaxf(d, -3.0e38f), Ah) : -p * A;
+                const float v = ENTROPY ? -p * fmaf(El, fmaxf(d, NOTHING), Ah) : -p * A;      // g = -p (A + E (log p + H))
                 acc.t[i][j][r] = v;
             }
         if (!__all(on))                                             // (a row that does not count is zero whatever its hidden row holds)
@@ -948,7 +950,7 @@ __global__ void __launch_bounds__(256) skinny_gradient_kernel(Skinny q, Upstream
             for (int r = 0; r < 4; ++r) {
                 const int64_t m = base + 8 * r4 + r;
                 const float d = fmaf(l[4 * r4 + r], LOG2E, -z), p = __builtin_amdgcn_exp2f(d);
-                float v = ENTROPY ? -p * fmaf(El, fmaxf(d, -3.0e38f), Ah) : -p * A;
+                float v = ENTROPY ? -p * fmaf(El, fmaxf(d, NOTHING), Ah) : -p * A;
                 if (m == t) v += A;
                 v = on && m < q.classes ? v : 0.0f;
                 o[r] = v;

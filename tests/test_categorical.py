@@ -575,3 +575,32 @@ def test_the_library_refuses_overlaps_and_odd_addresses():
     rc = b(99, None, C.byref(pitched), free, None, None, at["hidden_dev"] + 4 * width, 2 * width, None, width, None)
     assert rc != 0 and b"overlap" not in lib.q1env_last_error()                # (no such device)
     refused(b(0, None, C.byref(pitched), free, None, None, at["hidden_dev"] + 4 * width - 4, 2 * width, None, width, None), b"overlap")
+
+
+# ---- masked classes under an entropy gradient, rows far from zero
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(20, 64, 700), (60, 64, 700), (300, 72, 31), (400, 64, 700), (3000, 256, 700)])
+@pytest.mark.parametrize("bonus", [2.0 ** -15, 0.5, 4.0])
+def test_entropy_gradients_of_masked_classes(n, d, v, dtype, bonus):
+    """A class at -inf, or at the type's lowest value, has probability zero and no gradient whatever the upstream of the entropy is (its log-probability times that
+    upstream must not run past float32): every kernel of every type, from an entropy bonus of a mean over many rows to upstream values above 1."""
+    h, w, b, t = make(n, d, v, dtype, seed=n + v)
+    off = torch.zeros(v, dtype=torch.bool, device="cuda")
+    off[3:v // 2] = True
+    off[v - 1] = True
+    t = torch.where((t != IGN) & off[t.clamp(min=0)], 1, t)
+    T = Truth(h, w, torch.where(off, -float("inf"), b.float()).to(dtype), t)
+    A, E = torch.linspace(-1, 1, n, device="cuda") * bonus, torch.linspace(0.5, 1, n, device="cuda") * bonus
+    ref = T.grads(A, E)
+    for low in (-float("inf"), torch.finfo(dtype).min):
+        bias = torch.where(off, torch.full_like(b, low), b)
+        leaves = [x.clone().requires_grad_() for x in (h, w, bias)]
+        logp, ent = categorical.linear_categorical(leaves[0], leaves[1], t, leaves[2])
+        near(logp, T.logp, T.elogp, "logp")
+        near(ent, T.entropy, T.eent, "entropy")
+        got = torch.autograd.grad((logp, ent), leaves, (A, E))
+        for name, x, (r, tol) in zip(("dh", "dw", "db"), got, ref):
+            near(x, r, tol, f"{name}, masked by {low}")
+        assert not bool(got[1][off].any()) and not bool(got[2][off].any())
