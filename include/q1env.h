@@ -592,8 +592,9 @@ enum { Q1ENV_REDUCE_MEAN = 0, Q1ENV_REDUCE_SUM = 1 };
  * mouse's child distribution of Q1PhysActionDist (q1physrl/action_dist.py:221-222; Discrete(2S+1), env.py:216-219) is over logits that exist.
  *   lse_i = log sum_j exp l_ij    logp_i = l_i,target(i) - lse_i    H_i = lse_i - sum_j p_ij l_ij
  * hidden, weight, bias have one element type; products are accumulated and all statistics are held in float32.  float32 operands keep their
- * 24 bits (three bfloat16 pieces, six matrix products; the float32 matrix instruction with at most 32 rows or classes).  A class whose bias is -inf takes no part; a row without any class left is NaN, as is a
- * row whose target lies outside 0 .. classes - 1 (and its gradients).  Rows with target == ignore_index are padding: logp = H = 0, no
+ * 24 bits (three bfloat16 pieces, six matrix products; the float32 matrix instruction with at most 32 rows or classes).  Only differences of logits count, whatever their size: a row whose
+ * classes all sit at the type's lowest value is uniform (a log-probability below float32's range is its lowest value).  A class whose bias is -inf takes no part; a row without any class left
+ * is NaN, as is a row whose target lies outside 0 .. classes - 1 (and its gradients).  Rows with target == ignore_index are padding: logp = H = 0, no
  * gradient, not counted by the mean, whatever their hidden row holds (NaN included).  Results do not depend on how the device is occupied:
  * the same call gives the same bits. */
 typedef struct q1env_head {

@@ -12,7 +12,9 @@
 // float32 matrix instruction runs at 1/16 of the bfloat16 one; six products run at 1/6.)
 #pragma once
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <stdint.h>
+#include <type_traits>
 
 namespace q1head {
 namespace {                                // every translation unit carries the kernels it launches
@@ -388,14 +390,16 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // A probability below 2^NOTHING is zero in float32 (the smallest value is 2^-149).  Its logarithm is held to that in the entropy's gradient, where it is multiplied by an upstream value before the
 // probability: a class at -inf, or at the type's lowest value, gives 0 x a finite factor.
 constexpr float NOTHING = -160.0f;
+// Rows whose largest logit lies within this of zero take l log2(e) - m log2(e) as one fma on the rounded m log2(e) (and on the rounded log-sum-exp in the gradient: 2^-17 at most, 5e-6 of a
+// probability).  Farther out (masks of the type's lowest value, -1e9, rows that have nothing else) that rounding would be all that is left: there m is subtracted first.
+constexpr float NEAR = 128.0f;
 
-// Statistics of a set of classes in units of log2: maximum m of l log2(e), s = sum 2^(l log2(e) - m), u = sum (l log2(e) - m) 2^(l log2(e) - m).  One fused
-// multiply-add and one hardware exponential per logit; the reference m is subtracted inside the fma, so no rounding of l log2(e) itself enters.
+// Statistics of a set of classes: the largest logit m, s = sum 2^x and u = sum x 2^x over x = (l - m) log2(e).  One fused multiply-add and one hardware exponential per logit.
 struct Stat { float m, s, u; };
 __device__ __forceinline__ Stat joined(const Stat& a, const Stat& b) {
     const float m = fmaxf(a.m, b.m);
     // a set of classes at -inf has m = -inf, s = u = 0 and counts nothing; a difference is kept where 0 x (difference x s) is still 0 (masks of the type's lowest value)
-    const float da = a.m == -INFINITY ? 0.0f : fmaxf(a.m - m, -1.0e30f), db = b.m == -INFINITY ? 0.0f : fmaxf(b.m - m, -1.0e30f);
+    const float da = a.m == -INFINITY ? 0.0f : fmaxf((a.m - m) * LOG2E, -1.0e30f), db = b.m == -INFINITY ? 0.0f : fmaxf((b.m - m) * LOG2E, -1.0e30f);
     const float fa = a.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(da), fb = b.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(db);
     return Stat{m, fa * a.s + fb * b.s, fa * (a.u + da * a.s) + fb * (b.u + db * b.s)};
 }
@@ -476,17 +480,26 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) statistics_kernel(Hea
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc.t[i][j][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * LOG2E;
-        const float ref = mx == -INFINITY ? 0.0f : mx;
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m = mx == -INFINITY ? 0.0f : mx, ref = m * LOG2E;
         float s = 0.0f, u = 0.0f;
+        auto add_up = [&](auto near) {
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
+            for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float d = fmaf(acc.t[i][j][r], LOG2E, -ref), e = __builtin_amdgcn_exp2f(d);
-                s += e;
-                if constexpr (ENTROPY) u = fmaf(fmaxf(d, -3.0e38f), e, u);      // a class at -inf adds 0, not 0 x inf
-            }
+                for (int r = 0; r < 16; ++r) {
+                    const float d = near ? fmaf(acc.t[i][j][r], LOG2E, -ref) : (acc.t[i][j][r] - m) * LOG2E, e = __builtin_amdgcn_exp2f(d);
+                    s += e;
+                    if constexpr (ENTROPY) u = fmaf(fmaxf(d, -3.0e38f), e, u);      // a class at -inf adds 0, not 0 x inf
+                }
+        };
+        if (__all(fabsf(m) <= NEAR)) {
+            add_up(std::true_type{});
+            const float off = fmaf(m, LOG2E, -ref), f = __builtin_amdgcn_exp2f(-off);      // from ref, which was rounded, to m log2(e)
+            if constexpr (ENTROPY) u = f * fmaf(-off, s, u);
+            s *= f;
+        } else
+            add_up(std::false_type{});
         s += __shfl_xor(s, 32, 64);
         if constexpr (ENTROPY) u += __shfl_xor(u, 32, 64);
         if (lane < 32) { red[wave % C::WM][nl][0] = mx; red[wave % C::WM][nl][1] = s; red[wave % C::WM][nl][2] = u; }
@@ -502,13 +515,14 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) statistics_kernel(Hea
         }
 }
 
-// Joins the tiles' statistics: R rows per workgroup, 1024 / R lanes take the tiles of a row in turn (four loads of each kind in flight); lse is kept in units of log2.  Also leaves what the
+// Joins the tiles' statistics: R rows per workgroup, 1024 / R lanes take the tiles of a row in turn (four loads of each kind in flight).  The log-sum-exp is kept in its two parts, m and
+// log2 s: where m is far from zero their sum would lose the second.  Also leaves what the
 // backward pass wants of the classes: -1 / -2 / the class, and the rows that count as bytes and as bits.  R = 64 where there are many rows, 16 where there are many tiles (64 rows
 // of 1025 tiles: 21 us with R = 64, 12 with 16).  Bound: latency (8192 rows of 512 tiles: 14 us for 50 MB).
 template <int R>
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ part, const float* __restrict__ own_logit, Target target, int64_t rows, int tiles, int with_entropy,
-                                                    float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ entropy_kept, float* __restrict__ lse,
-                                                    int64_t* __restrict__ classes, uint8_t* __restrict__ live, uint64_t* __restrict__ bits, int mean,
+                                                    float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ entropy_kept, float* __restrict__ top,
+                                                    float* __restrict__ rest, int64_t* __restrict__ classes, uint8_t* __restrict__ live, uint64_t* __restrict__ bits, int mean,
                                                     float* __restrict__ loss, float* __restrict__ each) {
     static_assert(R == 64 || R == 16, "the words of bits");
     constexpr int G = 1024 / R;
@@ -537,15 +551,17 @@ __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ pa
     float lp = 0.0f;
     if (n < rows) {
         for (int k = 1; k < 16; ++k) a = joined(a, Stat{red[0][k][r], red[1][k][r], red[2][k][r]});
-        const float ls = __log2f(a.s);
-        float z = a.m + ls, h = with_entropy ? LN2 * (ls - a.u / a.s) : NAN;
-        if (t >= 0) lp = LN2 * (fmaf(own_logit[n], LOG2E, -a.m) - ls);
-        else if (t == -1) { h = 0.0f; z = 0.0f; }                  // ignored
-        else { lp = h = z = NAN; }                                  // a class that does not exist
+        float ls = __log2f(a.s), m = a.m, h = with_entropy ? LN2 * (ls - a.u / a.s) : NAN;
+        if (t >= 0) {
+            lp = fmaf(-LN2, ls, own_logit[n] - m);
+            if (lp == -INFINITY && own_logit[n] != -INFINITY) lp = -FLT_MAX;      // (finite logits further apart than float32 reaches)
+        } else if (t == -1) h = m = ls = 0.0f;                      // ignored
+        else { lp = h = ls = NAN; m = 0.0f; }                       // a class that does not exist
         logp[n] = lp;
         if (entropy) entropy[n] = h;
         entropy_kept[n] = h;
-        lse[n] = z;
+        top[n] = m;
+        rest[n] = ls;
         classes[n] = t;
         live[n] = t == -1 ? 0 : 1;
         if (r == 0) {
@@ -694,8 +710,8 @@ __device__ __forceinline__ float sums_of_32(float (&v)[32], int lane, int& which
 // 0.0024 of the results' norm instead of 0.0017), and a second piece would double the products.  Two up to 256 rows, where the few roundings need not even out (2 rows of 2 classes: 0.004 with
 // one, 0.0017 with two) and the products are bound by memory; three for float32.
 template <class C, int DT, int GP, bool ENTROPY>
-__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) gradient_kernel(Head hd, Upstream up, int64_t piece, int64_t g_plane, const float* __restrict__ lse,
-                                                              const float* __restrict__ entropy, uint16_t* __restrict__ g, float* __restrict__ db_part) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) gradient_kernel(Head hd, Upstream up, int64_t piece, int64_t g_plane, const float* __restrict__ top,
+                                                              const float* __restrict__ rest, const float* __restrict__ entropy, uint16_t* __restrict__ g, float* __restrict__ db_part) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t tm, tn, zz;
     tile_of(blockIdx.x, gridDim.x, hd.tiles_m, hd.tiles_n, tm, tn, zz);
@@ -703,7 +719,7 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) gradient_kernel(Head 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave % C::WM) * (C::TM * 32), wn = (wave / C::WM) * (C::TN * 32);
     const int64_t base = m0 + wm + 4 * (lane >> 5);
     Acc<C> acc;
-    struct Row { int own; float z, A, E, h; };                       // own class within the tile, -1: none, -2: the row does not count; log-sum-exp, upstream values, entropy
+    struct Row { int own; float z, A, E, h; };                       // own class within the tile, -1: none, -2: the row does not count; log-sum-exp in units of log2, upstream values, entropy
     int* own_of = (int*)(lds + C::LDS_BYTES);
     float* row_of = (float*)(own_of + C::BN);
     auto row = [&](int64_t n) {
@@ -712,7 +728,7 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) gradient_kernel(Head 
         const float sc = up.stored();
         Row r;
         r.own = !on ? -2 : t >= m0 && t < m0 + C::BM ? (int)(t - m0) : -1;
-        r.z = on ? lse[n] : 0.0f;
+        r.z = on ? fmaf(top[n], LOG2E, rest[n]) : 0.0f;
         r.A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) * sc : 0.0f;
         r.E = ENTROPY && on ? up.dentropy[n] * sc : 0.0f;
         r.h = ENTROPY && on ? entropy[n] : 0.0f;
@@ -738,14 +754,21 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) gradient_kernel(Head 
         const int rel = q.own - wm;
         const bool here = __any(rel >= 0 && rel < C::TM * 32);
         const int own = rel >= 4 * (lane >> 5) && rel < C::TM * 32 ? rel - 4 * (lane >> 5) : -1;
+        float m = 0.0f, ls = 0.0f;
+        auto weigh = [&](auto near) {
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
+            for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float d = fmaf(acc.t[i][j][r], LOG2E, -z), p = __builtin_amdgcn_exp2f(d);
-                const float v = ENTROPY ? -p * fmaf(El, fmaxf(d, NOTHING), Ah) : -p * A;      // g = -p (A + E (log p + H))
-                acc.t[i][j][r] = v;
-            }
+                for (int r = 0; r < 16; ++r) {
+                    const float d = near ? fmaf(acc.t[i][j][r], LOG2E, -z) : fmaf(acc.t[i][j][r] - m, LOG2E, -ls), p = __builtin_amdgcn_exp2f(d);
+                    acc.t[i][j][r] = ENTROPY ? -p * fmaf(El, fmaxf(d, NOTHING), Ah) : -p * A;      // g = -p (A + E (log p + H))
+                }
+        };
+        if (__all(fabsf(z) <= NEAR * LOG2E)) weigh(std::true_type{});
+        else {                                                       // one more instruction per logit
+            if (on && n0 + nl < hd.rows) { m = top[n0 + nl]; ls = rest[n0 + nl]; }
+            weigh(std::false_type{});
+        }
         if (!__all(on))                                             // (a row that does not count is zero whatever its hidden row holds)
 #pragma unroll
             for (int i = 0; i < C::TM; ++i)
@@ -906,12 +929,12 @@ __global__ void __launch_bounds__(256) skinny_statistics_kernel(Skinny q, Target
             if (t >= 0 && base + 8 * (r >> 2) + (r & 3) == t) own_logit[n] = l[r];
             mx = fmaxf(mx, l[r]);
         }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * LOG2E;
-        const float ref = mx == -INFINITY ? 0.0f : mx;
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m = mx == -INFINITY ? 0.0f : mx;
         Stat st{mx, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float d = fmaf(l[r], LOG2E, -ref), e = __builtin_amdgcn_exp2f(d);
+            const float d = (l[r] - m) * LOG2E, e = __builtin_amdgcn_exp2f(d);
             st.s += e;
             if constexpr (ENTROPY) st.u = fmaf(fmaxf(d, -3.0e38f), e, st.u);
         }
@@ -928,8 +951,8 @@ __global__ void __launch_bounds__(256) skinny_statistics_kernel(Skinny q, Target
 // g[row][class] in float32, rows of `stride` values (whole 32s, zero past the last class).  A workgroup takes 32 classes (workgroup % groups) and every teams-th 32 rows, and leaves the sums
 // over its rows in db_part[team][class].
 template <bool ENTROPY>
-__global__ void __launch_bounds__(256) skinny_gradient_kernel(Skinny q, Upstream up, const int64_t* __restrict__ target, uint32_t groups, uint32_t teams, const float* __restrict__ lse,
-                                                              const float* __restrict__ entropy, float* __restrict__ g, int64_t stride, float* __restrict__ db_part) {
+__global__ void __launch_bounds__(256) skinny_gradient_kernel(Skinny q, Upstream up, const int64_t* __restrict__ target, uint32_t groups, uint32_t teams, const float* __restrict__ top,
+                                                              const float* __restrict__ rest, const float* __restrict__ entropy, float* __restrict__ g, int64_t stride, float* __restrict__ db_part) {
     __shared__ float sums[4][16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t team = blockIdx.x / groups;
@@ -941,7 +964,7 @@ __global__ void __launch_bounds__(256) skinny_gradient_kernel(Skinny q, Upstream
         if (wave != 0) continue;
         const int64_t n = r0 + (lane & 31), t = n < q.rows ? target[n] : -1;
         const bool on = t != -1;
-        const float z = on ? lse[n] : 0.0f, hrow = ENTROPY && on ? entropy[n] : 0.0f;
+        const float mrow = on ? top[n] : 0.0f, ls = on ? rest[n] : 0.0f, hrow = ENTROPY && on ? entropy[n] : 0.0f;
         const float A = on ? (up.dloss ? -1.0f : (up.dlogp ? up.dlogp[n] : 0.0f)) : 0.0f, E = ENTROPY && on ? up.dentropy[n] : 0.0f, El = E * LN2, Ah = A + E * hrow;
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
@@ -949,7 +972,7 @@ __global__ void __launch_bounds__(256) skinny_gradient_kernel(Skinny q, Upstream
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int64_t m = base + 8 * r4 + r;
-                const float d = fmaf(l[4 * r4 + r], LOG2E, -z), p = __builtin_amdgcn_exp2f(d);
+                const float d = fmaf(l[4 * r4 + r] - mrow, LOG2E, -ls), p = __builtin_amdgcn_exp2f(d);
                 float v = ENTROPY ? -p * fmaf(El, fmaxf(d, NOTHING), Ah) : -p * A;
                 if (m == t) v += A;
                 v = on && m < q.classes ? v : 0.0f;

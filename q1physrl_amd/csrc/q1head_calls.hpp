@@ -33,14 +33,15 @@ int planes_of(int dt) { return dt == F32 ? 3 : 1; }
 
 // the forward pass's results as the backward pass reads them (q1env_head_state_bytes)
 struct State {
-    float *lse, *entropy, *each;
+    float *top, *rest, *entropy, *each;
     int64_t* target;
     uint8_t* live;
     uint64_t* bits;
-    static uint64_t bytes(int64_t n) { return 2 * aligned(4 * n) + aligned(8 * n) + aligned(n) + aligned(8 * div_up(n, 64)) + 256; }
+    static uint64_t bytes(int64_t n) { return 3 * aligned(4 * n) + aligned(8 * n) + aligned(n) + aligned(8 * div_up(n, 64)) + 256; }
     State(void* p, int64_t n) {
         char* c = (char*)p;
-        lse = (float*)c; c += aligned(4 * n);
+        top = (float*)c; c += aligned(4 * n);
+        rest = (float*)c; c += aligned(4 * n);
         entropy = (float*)c; c += aligned(4 * n);
         target = (int64_t*)c; c += aligned(8 * n);
         live = (uint8_t*)c; c += aligned(n);
@@ -257,9 +258,9 @@ template <class C, int DT, int GP> int gradient(const Where& at, Head hd, const 
     hd.tiles_m = (uint32_t)div_up(hd.c1 - hd.c0, C::BM);
     hd.tiles_n = (uint32_t)div_up(hd.rows, C::BN);
     const int64_t workgroups = (int64_t)hd.tiles_m * hd.tiles_n, plane = hd.rows * piece;
-    const float *lse = st.lse, *entropy = st.entropy;
-    return up.dentropy ? go<C, gradient_kernel<C, DT, GP, true>>(at.stream, at.device, workgroups, hd, up, piece, plane, lse, entropy, g, db)
-                       : go<C, gradient_kernel<C, DT, GP, false>>(at.stream, at.device, workgroups, hd, up, piece, plane, lse, entropy, g, db);
+    const float *top = st.top, *rest = st.rest, *entropy = st.entropy;
+    return up.dentropy ? go<C, gradient_kernel<C, DT, GP, true>>(at.stream, at.device, workgroups, hd, up, piece, plane, top, rest, entropy, g, db)
+                       : go<C, gradient_kernel<C, DT, GP, false>>(at.stream, at.device, workgroups, hd, up, piece, plane, top, rest, entropy, g, db);
 }
 // workgroups of a product in C's tiles
 template <class C> int64_t tiles_of(Product& pr, int splits) {
@@ -312,9 +313,9 @@ int skinny_gradient(const Where& at, const Skinny& q, const Upstream& up, const 
     const uint32_t groups = (uint32_t)div_up(q.classes, 32);
     const dim3 grid(groups * teams);
     const int64_t* t = st.target;
-    const float *lse = st.lse, *entropy = st.entropy;
-    if (up.dentropy) hipLaunchKernelGGL((skinny_gradient_kernel<true>), grid, dim3(256), 0, at.stream, q, up, t, groups, teams, lse, entropy, g, stride, db);
-    else hipLaunchKernelGGL((skinny_gradient_kernel<false>), grid, dim3(256), 0, at.stream, q, up, t, groups, teams, lse, entropy, g, stride, db);
+    const float *top = st.top, *rest = st.rest, *entropy = st.entropy;
+    if (up.dentropy) hipLaunchKernelGGL((skinny_gradient_kernel<true>), grid, dim3(256), 0, at.stream, q, up, t, groups, teams, top, rest, entropy, g, stride, db);
+    else hipLaunchKernelGGL((skinny_gradient_kernel<false>), grid, dim3(256), 0, at.stream, q, up, t, groups, teams, top, rest, entropy, g, stride, db);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -371,10 +372,10 @@ int forward(const Where& at, const q1env_head& q, int reduction, float* logp, fl
         float* here = n <= (tall ? 16 : 64) ? loss : nullptr;                 // one workgroup joins all the rows: it has the loss too
         if (tall)
             hipLaunchKernelGGL((join_kernel<16>), dim3((unsigned)div_up(n, 16)), dim3(1024), 0, at.stream, part, own, target, n, (int)p.tiles, entropy ? 1 : 0, logp, entropy, st.entropy,
-                               st.lse, st.target, st.live, st.bits, mean, here, st.each);
+                               st.top, st.rest, st.target, st.live, st.bits, mean, here, st.each);
         else
             hipLaunchKernelGGL((join_kernel<64>), dim3((unsigned)div_up(n, 64)), dim3(1024), 0, at.stream, part, own, target, n, (int)p.tiles, entropy ? 1 : 0, logp, entropy, st.entropy,
-                               st.lse, st.target, st.live, st.bits, mean, here, st.each);
+                               st.top, st.rest, st.target, st.live, st.bits, mean, here, st.each);
         HIP_TRY(hipGetLastError());
         if (here) return Q1ENV_OK;
     }

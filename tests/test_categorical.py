@@ -604,3 +604,58 @@ def test_entropy_gradients_of_masked_classes(n, d, v, dtype, bonus):
         for name, x, (r, tol) in zip(("dh", "dw", "db"), got, ref):
             near(x, r, tol, f"{name}, masked by {low}")
         assert not bool(got[1][off].any()) and not bool(got[2][off].any())
+
+
+def _far_biases(dtype, v):
+    """biases that put a row far from zero: (name, bias); logits are the biases themselves where the hidden row is zero"""
+    info = torch.finfo(dtype)
+    g = torch.Generator(device="cuda").manual_seed(v)
+    r = torch.randn(v, device="cuda", generator=g)
+    low = torch.full((v,), info.min, device="cuda", dtype=dtype)
+    out = [("all at the lowest value", low)]
+    some = low.clone()
+    some[::3] = r[::3].to(dtype)
+    out.append(("two thirds at the lowest value", some))
+    top = r.to(dtype, copy=True)
+    top[v // 2] = info.max
+    out.append(("one at the largest value", top))
+    if dtype == torch.float16:
+        out.append(("around -6e4", (-60000.0 + 32.0 * torch.round(r)).to(dtype)))
+    else:
+        out.append(("all at -1e9", torch.full((v,), -1e9, device="cuda", dtype=dtype)))
+        out.append(("around -1e9", (-1e9 + 64.0 * torch.round(r)).to(dtype)))
+        out.append(("between 1e38 and 3e38", (torch.linspace(1e38, 3e38, v, device="cuda")).to(dtype)))
+        out.append(("between -3e38 and -1e38", (torch.linspace(-1e38, -3e38, v, device="cuda")).to(dtype)))
+        out.append(("from -3e38 to 3e38", (3e38 * torch.linspace(-1, 1, v, device="cuda")).to(dtype)))
+    out.append(("around 1000", (1000.0 + r).to(dtype)))
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,v", [(1, 700), (20, 700), (300, 31), (40, 700), (100, 300), (300, 700), (2500, 600)])
+def test_rows_far_from_zero(n, v, dtype):
+    """Rows whose logits are all very small, or of any size: the distribution depends on the differences alone.  With zero hidden rows the logits are the biases, exactly, so that only the
+    sums, the exponentials and the final roundings are off; no term of the log-sum-exp's own magnitude is allowed.  (Differences past float32's range are held to its largest value.)"""
+    d = 64
+    h, w, _, t = make(n, d, v, dtype, seed=n)
+    h = torch.zeros_like(h)
+    for name, b in _far_biases(dtype, v):
+        bd = b.double()
+        T = Truth(h, w, bd - bd.max(), t)                                      # only differences count: the shift is exact enough in float64, and keeps log V
+        T.logp = T.logp.clamp(min=-float(torch.finfo(torch.float32).max))
+        T.el = torch.zeros_like(T.el)
+        T.elogp = (256 + v / 2048 + 16) * 2 * U + 8 * U * (T.lse.abs() + T.logp.abs() + 1)
+        few = (256 + v / 2048 + 16) * 2 * U + 8 * U * (T.lse.abs() + 30)       # of a probability that is not zero: its logarithm is above -105
+        T.e = 2 * few
+        T.eent = T.e * (T.p * (T.lp.abs() + 1)).sum(1) + few
+        leaves = [x.clone().requires_grad_() for x in (h, w, b)]
+        logp, ent = categorical.linear_categorical(leaves[0], leaves[1], t, leaves[2])
+        near(logp, T.logp, T.elogp, f"logp, {name}")
+        near(ent, T.entropy, T.eent, f"entropy, {name}")
+        A, E = torch.linspace(-1, 1, n, device="cuda"), torch.linspace(0.5, 0.1, n, device="cuda")
+        for what, x, (r, tol) in zip(("dh", "dw", "db"), torch.autograd.grad((logp, ent), leaves, (A, E)), T.grads(A, E)):
+            near(x, r, tol, f"{what}, {name}")
+    loss, dh, dw, db = categorical.linear_cross_entropy_grad(h, w, t, torch.full((v,), torch.finfo(dtype).min, device="cuda", dtype=dtype), reduction="sum")
+    live = int((t != IGN).sum())
+    assert abs(float(loss) - live * math.log(v)) <= live * math.log(v) * 2.0 ** -12 and all(bool(torch.isfinite(x).all()) for x in (dh, dw, db))
