@@ -145,6 +145,6 @@ def grad_norm(grads, *, scale=1.0):
 
 def clip_grad_norm_(grads, max_norm, *, scale=1.0, out=None):
     """grads <- grads x scale x min(1, max_norm / norm), norm = grad_norm(grads, scale=scale); returns the norm.  out: where the results go instead
-    (tensors of the same shapes - or, where all are contiguous, sizes - and dtypes that overlap nothing but, each, its own source); the gradients stay as they are.  A NaN norm makes every result
-    NaN; an infinite one turns finite values to zero."""
+    (tensors of the same shapes - or, where all are contiguous, sizes - and dtypes that overlap nothing but, each, its own source); the gradients stay as they are.  A NaN gradient makes the norm and every
+    result NaN, an infinite one turns finite values to zero.  A norm past float32's range is returned as inf; the gradients are clipped by its float64 value."""
     return _run(grads, out, max_norm, scale)

@@ -10,6 +10,8 @@
 // Bound: memory.  536 870 913 float32 values (2.1 GB read, read again, written): 395 us for the first pass (5.4 TB/s), 794 for the second (5.4 TB/s; a plain copy makes 4.8).
 #include "q1env_host.hpp"
 
+#include <float.h>
+
 #include <algorithm>
 
 namespace {
@@ -98,17 +100,20 @@ template <int DT> __device__ __forceinline__ double squares(const Slot* t, int64
     return acc;
 }
 
-template <int DT> __device__ __forceinline__ void scaled(const Slot* t, int64_t a, int64_t b, float c) {
+// FAR: a factor outside float32's normal range (a norm or a scale beyond it) would lose its bits, or all of it: the product is a float64's
+template <int DT, bool FAR> __device__ __forceinline__ void scaled(const Slot* t, int64_t a, int64_t b, double factor) {
     typedef typename El<DT>::type E;
     constexpr int V = 16 / sizeof(E);
     const E* p = (const E*)t->src;
     E* q = (E*)t->dst;
-    if (c == 1.0f && (const E*)q == p) return;                                   // in place and nothing to clip
+    const float c = (float)factor;
+    auto times = [&](E x) { return rounded<DT>(FAR ? (float)((double)value<DT>(x) * factor) : value<DT>(x) * c); };
+    if (!FAR && c == 1.0f && (const E*)q == p) return;                                   // in place and nothing to clip
     if (t->kind & PITCHED) {
         const int64_t cols = (int64_t)t[1].src, ps = (int64_t)t[1].dst, pd = t[1].count;
         for (int64_t i = a + threadIdx.x; i < b; i += THREADS) {
             const int64_t r = i / cols, k = i - r * cols;
-            q[r * pd + k] = rounded<DT>(value<DT>(p[r * ps + k]) * c);
+            q[r * pd + k] = times(p[r * ps + k]);
         }
         return;
     }
@@ -117,10 +122,10 @@ template <int DT> __device__ __forceinline__ void scaled(const Slot* t, int64_t 
         E w[V];
         __builtin_memcpy(w, p + i, 16);
 #pragma unroll
-        for (int j = 0; j < V; ++j) w[j] = rounded<DT>(value<DT>(w[j]) * c);
+        for (int j = 0; j < V; ++j) w[j] = times(w[j]);
         __builtin_memcpy(q + i, w, 16);
     }
-    for (; i < b; ++i) q[i] = rounded<DT>(value<DT>(p[i]) * c);
+    for (; i < b; ++i) q[i] = times(p[i]);
 }
 
 __device__ __forceinline__ void squares_of(const Slot* t, uint32_t n, uint32_t units, uint32_t unit, double* __restrict__ partial, double* red) {
@@ -133,29 +138,36 @@ __device__ __forceinline__ void squares_of(const Slot* t, uint32_t n, uint32_t u
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
-// the norm from the partials, the same in every workgroup
-__device__ __forceinline__ double norm_of(const double* __restrict__ partial, int n, double scale, double* red) {
+// the norm (before the scale) from the partials, the same in every workgroup
+__device__ __forceinline__ double norm_of(const double* __restrict__ partial, int n, double* red) {
     double a = 0.0;
     for (int i = threadIdx.x; i < n; i += THREADS) a += partial[i];
-    return sqrt(block_sum(a, red)) * fabs(scale);
+    return sqrt(block_sum(a, red));
 }
 
 __global__ void __launch_bounds__(THREADS) norm_kernel(const double* __restrict__ partial, int n, double scale, float* __restrict__ norm) {
     __shared__ double red[4];
-    const double v = norm_of(partial, n, scale, red);
-    if (threadIdx.x == 0) *norm = (float)v;
+    const double v = norm_of(partial, n, red);
+    if (threadIdx.x == 0) *norm = (float)(v * scale);
 }
 
 __device__ __forceinline__ void clip_of(const Slot* t, uint32_t n, uint32_t units, uint32_t unit, const double* __restrict__ partial, int parts, double scale, double max_norm,
                                         float* __restrict__ norm, double* red) {
-    const double v = norm_of(partial, parts, scale, red);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
-    const float c = (float)(scale * (v <= max_norm ? 1.0 : max_norm / v));       // a NaN norm makes every value NaN
+    const double v = norm_of(partial, parts, red);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)(v * scale);
+    const double c = v * scale <= max_norm ? scale : max_norm / v;               // a NaN norm makes every value NaN
+    const bool far = c > 0.0 && (c < (double)FLT_MIN || c > (double)FLT_MAX);
     each_unit<true>(t, n, units, unit, [&](const Slot* s, int64_t a, int64_t b) {
         const uint32_t dt = s->kind & 15;
-        if (dt == Q1ENV_DT_F32) scaled<Q1ENV_DT_F32>(s, a, b, c);
-        else if (dt == Q1ENV_DT_BF16) scaled<Q1ENV_DT_BF16>(s, a, b, c);
-        else scaled<Q1ENV_DT_F16>(s, a, b, c);
+        if (far) {
+            if (dt == Q1ENV_DT_F32) scaled<Q1ENV_DT_F32, true>(s, a, b, c);
+            else if (dt == Q1ENV_DT_BF16) scaled<Q1ENV_DT_BF16, true>(s, a, b, c);
+            else scaled<Q1ENV_DT_F16, true>(s, a, b, c);
+        } else {
+            if (dt == Q1ENV_DT_F32) scaled<Q1ENV_DT_F32, false>(s, a, b, c);
+            else if (dt == Q1ENV_DT_BF16) scaled<Q1ENV_DT_BF16, false>(s, a, b, c);
+            else scaled<Q1ENV_DT_F16, false>(s, a, b, c);
+        }
     });
 }
 

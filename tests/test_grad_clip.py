@@ -257,3 +257,22 @@ def test_the_library_refuses():
     assert call(lib, src=[4096, 4096 + 12], dst=[4096, 4096 + 12], values=[20, 20], cols=[4, 4], sp=[10, 10], dp=[10, 10]) == -1
     assert b"overlap" in lib.q1env_last_error()
     assert lib.q1env_grad_norm_workspace_bytes(-1) == 0 and lib.q1env_grad_norm_workspace_bytes(12) > 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_factors_outside_float32s_range(dtype):
+    """A norm past float32's largest value is reported as inf, but the gradients are clipped by it as by any other: the factor, below float32's normal range here (and above it for
+    the tiny gradients), keeps its bits.  A value is one float64 product, a rounding to float32 and one to the type."""
+    tol = 2.0 ** -24 + HALF[dtype] + 2.0 ** -40
+    for n, amp, scale, bound in ((1_000_003, 3e38, 1.0, 0.5), (5, 2.5e38, 1.0, 1e-6), (3001, 1e-30, 1e40, 1e300), (3001, 1e-35, 1e42, 1e5)):
+        g = torch.full((n,), amp, device="cuda").to(dtype)
+        a = float(g[0])
+        norm = math.sqrt(n) * a * scale
+        want = a * scale * min(1.0, bound / norm)
+        for pitched in (False, True):
+            src = torch.zeros(n, 3, device="cuda", dtype=dtype)[:, 1:2] if pitched else torch.empty(n, 1, device="cuda", dtype=dtype)
+            src.copy_(g[:, None])
+            got = clip.clip_grad_norm_([src], bound, scale=scale)
+            assert (math.isinf(float(got)) if norm > 3.5e38 else abs(float(got) / norm - 1) <= 2.0 ** -23)
+            assert bool(((src.double() - want).abs() <= want * tol).all()), (n, amp, float(src[0, 0]), want)
