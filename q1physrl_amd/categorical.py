@@ -11,7 +11,7 @@ exponential and the gradient of each alive there; here a float or two per sample
 
 hidden (..., D), weight (V, D) and bias (V,) are float32, bfloat16 or float16 CUDA tensors of one type; actions / target (...) int32 or int64.  Rows may be
 strided; a last dimension that is not contiguous is copied.  Rows whose target is ignore_index are padding: log-probability, entropy and gradients
-are zero whatever the hidden row holds.  A target outside 0 .. V-1 gives NaN.  Work runs on the tensors' device, on its current stream.
+are zero whatever the hidden row holds.  A target outside 0 .. V-1 gives NaN.  There is no forward-mode derivative and no second one: both raise.  Work runs on the tensors' device, on its current stream.
 
 A captured graph: the forward calls and linear_cross_entropy_grad can be captured; the autograd forms cannot (a capture that meets an eager graph of
 the same leaves ends the process), and say so."""
@@ -21,6 +21,7 @@ import functools
 import torch
 
 from . import _lib
+from .clip import refuse_tangents
 
 _DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
@@ -64,6 +65,7 @@ def _check(hidden, weight, target, bias, ignore_index):
         raise ValueError(f"bias must be ({weight.shape[0]},), got {tuple(bias.shape)}")
     if not isinstance(ignore_index, int) or not -2 ** 63 <= ignore_index < 2 ** 63:
         raise ValueError("ignore_index must be an int of 64 bits")
+    refuse_tangents([t for t in (hidden, weight, bias) if t is not None], "the wide categorical head")
     if not hidden.is_cuda:
         raise _lib.Q1EnvError("the wide categorical head runs on an MI355X only: there is no CPU fallback")
     for t in (weight, target, bias):

@@ -5,12 +5,13 @@ policies apply with tf.clip_by_global_norm; the reference's trainer config leave
     norm = clip_grad_norm_(bucket_views, 0.5, scale=1 / world, out=[p.grad for p in params])
 
 Tensors: CUDA, one device, float32 / bfloat16 / float16 (mixed as they come), any shape; dense ones in any order of dimensions, or rows of contiguous
-values at a pitch (a column slice).  Squares are summed in float64 in an order that the sizes alone fix: the same bits every time."""
+values at a pitch (a column slice).  Results carry no graph, as those of torch's own clipping do not: a norm is no loss term, and forward-mode tangents are refused.  Squares are summed in float64 in an order that the sizes alone fix: the same bits every time."""
 import functools
 import operator
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -23,6 +24,12 @@ _dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
 @functools.lru_cache(maxsize=64)
 def _workspace_bytes(count):
     return _lib.load().q1env_grad_norm_workspace_bytes(count)
+
+
+def refuse_tangents(tensors, what):
+    """Raises where a tensor carries a forward-mode tangent: the kernels would drop it without a word."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _address(a):
@@ -87,6 +94,7 @@ def _run(tensors, out, max_norm, scale):
         raise ValueError("no tensors: there is no device to put the norm on")
     if n > 65536:
         raise ValueError("more than 65536 tensors")
+    refuse_tangents(tensors, "the gradient norm")
     kinds = list(map(_dtype, tensors))
     if not _DTYPES.keys() >= set(kinds):
         raise TypeError(f"gradients must be float32, bfloat16 or float16, got {set(kinds) - set(_DTYPES)}")

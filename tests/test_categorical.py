@@ -659,3 +659,22 @@ def test_rows_far_from_zero(n, v, dtype):
     loss, dh, dw, db = categorical.linear_cross_entropy_grad(h, w, t, torch.full((v,), torch.finfo(dtype).min, device="cuda", dtype=dtype), reduction="sum")
     live = int((t != IGN).sum())
     assert abs(float(loss) - live * math.log(v)) <= live * math.log(v) * 2.0 ** -12 and all(bool(torch.isfinite(x).all()) for x in (dh, dw, db))
+
+
+def test_refuses_forward_mode_tangents():
+    """a dual tensor does not require grad: without a check it would go past the autograd function and come back without its tangent"""
+    import torch.autograd.forward_ad as fwad
+    h, w, b, t = torch.zeros(4, 8), torch.zeros(5, 8), torch.zeros(5), torch.zeros(4, dtype=torch.int64)
+    calls = (categorical.linear_categorical, categorical.linear_cross_entropy, categorical.linear_cross_entropy_grad)
+    with fwad.dual_level():
+        for f in calls:
+            for k in (0, 1, 3):
+                args = [h, w, t, b]
+                args[k] = fwad.make_dual(args[k], torch.ones_like(args[k]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(*args)
+            with pytest.raises(_lib.Q1EnvError):                               # (no tangent: on to the next check)
+                f(h, w, t, b)
+    for f in calls[:2]:
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda x: f(x, w, t, b), (h,), (torch.ones_like(h),))

@@ -276,3 +276,20 @@ def test_factors_outside_float32s_range(dtype):
             got = clip.clip_grad_norm_([src], bound, scale=scale)
             assert (math.isinf(float(got)) if norm > 3.5e38 else abs(float(got) / norm - 1) <= 2.0 ** -23)
             assert bool(((src.double() - want).abs() <= want * tol).all()), (n, amp, float(src[0, 0]), want)
+
+
+def test_refuses_forward_mode_tangents():
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level():
+        x = fwad.make_dual(torch.ones(3), torch.ones(3))
+        for f in (lambda: clip.grad_norm([torch.ones(2), x]), lambda: clip.clip_grad_norm_([x], 1.0), lambda: clip.clip_grad_norm_([x], 1.0, out=[torch.zeros(3)])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+
+
+@gpu
+def test_results_carry_no_graph():
+    x = torch.randn(50, device="cuda", requires_grad=True)
+    g = x * 3.0
+    out = [torch.zeros(50, device="cuda")]
+    assert not clip.grad_norm([g]).requires_grad and not clip.clip_grad_norm_([g], 1.0, out=out).requires_grad and not out[0].requires_grad
