@@ -339,13 +339,14 @@ struct Lay {
     int64_t stride, rows;             // elements
     const uint8_t* live;
     uint16_t* out;
-    uint32_t groups;                  // workgroups of 2048 values
+    int64_t groups;                   // workgroups of 2048 values
 };
 template <int DT>
-__global__ void __launch_bounds__(256) lay_out_kernel(Lay first, Lay second, int64_t width, int64_t padded) {
-    const bool one = blockIdx.x < first.groups;
+__global__ void __launch_bounds__(256) lay_out_kernel(Lay first, Lay second, int64_t width, int64_t padded, int64_t from) {
+    const int64_t group = from + blockIdx.x;                                  // (from: of a launch that is not the first)
+    const bool one = group < first.groups;
     const Lay& l = one ? first : second;
-    const int64_t i = ((int64_t)(one ? blockIdx.x : blockIdx.x - first.groups) * 256 + threadIdx.x) * 8;
+    const int64_t i = ((one ? group : group - first.groups) * 256 + threadIdx.x) * 8;
     if (i >= l.rows * padded) return;
     const int64_t r = i / padded, k = i - r * padded;
     uint16_t q[Elem<DT>::planes][8];
@@ -1216,10 +1217,10 @@ template <int DT> __device__ __forceinline__ void finish(const Finish& f, float 
     }
 }
 template <int DT>
-__global__ void __launch_bounds__(256) finish_kernel(Finish dw, Finish dh, FinishBias db, Upstream up) {
+__global__ void __launch_bounds__(256) finish_kernel(Finish dw, Finish dh, FinishBias db, Upstream up, uint32_t from) {
     __shared__ float red[4][64];
     const float scale = up.result();
-    uint32_t b = blockIdx.x;
+    uint32_t b = from + blockIdx.x;                                          // (from: of a launch that is not the first)
     if (b < dw.groups) return finish<DT>(dw, scale, b);
     b -= dw.groups;
     if (b < dh.groups) return finish<DT>(dh, scale, b);

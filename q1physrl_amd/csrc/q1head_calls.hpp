@@ -17,6 +17,9 @@ constexpr uint64_t PIECE_BYTES = 448ull << 20;     // of the gradient of one pie
 constexpr uint64_t laid_bytes(int dt) { return dt == 0 ? 448ull << 20 : 160ull << 20; }
 constexpr int64_t MAX_ROWS = 1 << 22, MAX_WIDTH = 1 << 16, MAX_CLASSES = 1 << 22;
 constexpr int64_t PIECE_STEP = 256;                // pieces are whole tiles of every configuration
+// A launch holds fewer than 2^32 threads.  Tiles whose grid would hold more than half of that are not taken (a quarter for each of the two backward products, which may share a launch), pieces are cut
+// so that Large's always fit, and what only streams goes out in several launches.
+constexpr int64_t MOST_THREADS = 1ll << 31;
 
 typedef Config<256, 256, 2, 4, 64, 2> Large;           // 128 KB of LDS: one workgroup of eight waves per CU
 typedef Config<128, 128, 2, 2, 64, 2> Middle;          // 64 KB: two workgroups of four waves per CU, one computes while the other waits
@@ -75,10 +78,12 @@ Shape shape_of(int64_t m, int64_t n, int64_t k, int products, bool split, const 
     for (int s = LARGE; s <= PAIR; ++s) {
         if (s == PAIR && (starts.pair == 0.0 || products > 1)) continue;
         const int64_t tiles = div_up(m, bm_of((Size)s)) * div_up(n, bn_of((Size)s)), slots = s == LARGE ? 256 : 512;
+        const int64_t threads = s == LARGE || s == PAIR ? 512 : 256, groups_most = (split ? MOST_THREADS / 2 : MOST_THREADS) / threads;
         const double start = s == LARGE ? starts.large : s == MIDDLE ? starts.middle : s == PAIR ? starts.pair : starts.middle / 2;
         const int64_t most = split ? std::min<int64_t>(div_up(k, 256), std::max<int64_t>(1, div_up(4 * slots, tiles))) : 1;
         for (int64_t parts = 1; parts <= most; ++parts) {
             const int64_t len = round_up(div_up(k, parts), PART_STEP), real = div_up(k, len), groups = tiles * real;
+            if (groups > groups_most) break;
             // a term of k of one round; of a round that leaves every workgroup a CU to itself
             const double full = s == LARGE ? 31.0 : s == MIDDLE ? 18.0 : s == PAIR ? 36.0 : 9.5, alone = s == LARGE ? 31.0 : s == MIDDLE ? 11.0 : s == PAIR ? 20.0 : 5.0;
             double t = (double)div_up(groups, slots) * ((double)len * products * (groups <= 256 ? alone : full) + start);
@@ -181,6 +186,7 @@ Plan plan_of(int dt, int64_t rows, int64_t width, int64_t classes, bool backward
     const int64_t laid = planes_of(dt) * 2 * p.padded;                        // bytes of a laid-out row
     if (!w_in_place) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(laid_bytes(dt) / laid) / PIECE_STEP * PIECE_STEP));
     if (backward) piece = std::min<int64_t>(piece, std::max<int64_t>(PIECE_STEP, (int64_t)(PIECE_BYTES / (2 * g_pieces * rows)) / PIECE_STEP * PIECE_STEP));
+    piece = std::min<int64_t>(piece, std::max<int64_t>(1, MOST_THREADS / 512 / div_up(rows, 256)) * PIECE_STEP);          // Large: 512 threads to a tile of 256 x 256
     p.pieces = div_up(classes, piece);
     p.piece = piece = even_piece(piece, p.pieces, classes, rows);
     p.pieces = div_up(classes, piece);
@@ -232,7 +238,7 @@ uint64_t workspace_of(int dt, int64_t rows, int64_t width, int64_t classes, bool
 }
 
 template <class C, auto KERNEL, typename... A> int go(hipStream_t stream, int device, int64_t workgroups, A... args) {
-    if (workgroups <= 0 || workgroups > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
+    if (workgroups <= 0 || workgroups * C::THREADS >= 1ll << 32) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
     static std::atomic<uint64_t> done{0};
     const uint64_t bit = 1ull << (device & 63);
     if (C::ALL_BYTES > 65536 && (device > 63 || !(done.load(std::memory_order_relaxed) & bit))) {        // more than 64 KB of LDS has to be allowed once per kernel and device
@@ -271,7 +277,6 @@ template <class C> int64_t tiles_of(Product& pr, int splits) {
 // dw and dh may each be absent (null out)
 template <class C, int DT, int GP> int products(const Where& at, Product dw, int dw_split, Product dh, int dh_split, const Upstream& up) {
     const int64_t a = dw.out ? tiles_of<C>(dw, dw_split) : 0, b = dh.out ? tiles_of<C>(dh, dh_split) : 0, padded = b > 0 ? round_up(a, 8) : a;
-    if (a > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
     return a + b == 0 ? 0 : go<C, products_kernel<C, DT, GP>>(at.stream, at.device, padded + b, dw, dh, up, (uint32_t)a, (uint32_t)padded);
 }
 template <class C, int DT, int GP> int rows_product(const Where& at, Product dh, int dh_split, const Upstream& up) {
@@ -282,12 +287,20 @@ template <class C, int DT, int GP> int rows_product(const Where& at, Product dh,
 // lays out what has rows, in one launch
 template <int DT> int lay_out(const Where& at, Lay a, Lay b, int64_t width, int64_t padded) {
     const int64_t ga = div_up(a.rows * padded, 2048), gb = div_up(b.rows * padded, 2048);
-    if (ga + gb == 0) return 0;
-    if (ga + gb > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many values");
-    a.groups = (uint32_t)ga;
-    b.groups = (uint32_t)gb;
-    hipLaunchKernelGGL((lay_out_kernel<DT>), dim3((unsigned)(ga + gb)), dim3(256), 0, at.stream, a, b, width, padded);
-    HIP_TRY(hipGetLastError());
+    a.groups = ga;
+    for (int64_t from = 0; from < ga + gb; from += MOST_THREADS / 256) {
+        hipLaunchKernelGGL((lay_out_kernel<DT>), dim3((unsigned)std::min(ga + gb - from, MOST_THREADS / 256)), dim3(256), 0, at.stream, a, b, width, padded, from);
+        HIP_TRY(hipGetLastError());
+    }
+    return 0;
+}
+// adds the parts of the sums up
+template <int DT> int add_parts(const Where& at, const Finish& fw, const Finish& fh, const FinishBias& fb, const Upstream& up) {
+    const int64_t groups = (int64_t)fw.groups + fh.groups + fb.groups;
+    for (int64_t from = 0; from < groups; from += MOST_THREADS / 256) {
+        hipLaunchKernelGGL((finish_kernel<DT>), dim3((unsigned)std::min(groups - from, MOST_THREADS / 256)), dim3(256), 0, at.stream, fw, fh, fb, up, (uint32_t)from);
+        HIP_TRY(hipGetLastError());
+    }
     return 0;
 }
 
@@ -324,7 +337,7 @@ int skinny_product(const Where& at, SkinnyProduct q, bool b_k_major, const Upstr
     q.tiles_n = (uint32_t)div_up(q.n, 32);
     const bool shared = q.part >= 128;                                        // long sums: four waves to a unit
     const int64_t units = (int64_t)q.tiles_m * q.tiles_n * q.splits, groups = shared ? units : div_up(units, 4);
-    if (units > INT32_MAX) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
+    if (groups * 256 >= 1ll << 32) return fail(Q1ENV_ERR_INVALID_ARG, "wide categorical head: too many tiles");
     const dim3 g((unsigned)groups), b(256);
     if (b_k_major) {
         if (shared) hipLaunchKernelGGL((skinny_product_kernel<true, true>), g, b, 0, at.stream, q, up);
@@ -415,11 +428,7 @@ int backward(const Where& at, const q1env_head& q, const Plan& p, bool hp, bool 
             Finish fw{ss, p.dw_split, v, d, nullptr, dw, dw_stride, four(dw, dw_stride) ? 1 : 0, dw && ss ? (uint32_t)div_up(v * d, 1024) : 0};
             Finish fh{hs, p.dh_split, n, d, st.live, dh, dh_stride, four(dh, dh_stride) ? 1 : 0, dh && hs ? (uint32_t)div_up(n * d, 1024) : 0};
             FinishBias fb{db_part, v, (int)p.teams, db, db ? (uint32_t)div_up(v, 64) : 0};
-            if (const uint64_t all = (uint64_t)fw.groups + fh.groups + fb.groups) {
-                hipLaunchKernelGGL((finish_kernel<DT>), dim3((unsigned)all), dim3(256), 0, at.stream, fw, fh, fb, up);
-                HIP_TRY(hipGetLastError());
-            }
-            return Q1ENV_OK;
+            return add_parts<DT>(at, fw, fh, fb, up);
         }
     const Op h = rows_op(DT, hp, q.hidden_dev, q.hidden_stride, n, d, p.padded, ws + p.h_laid);
     uint16_t* g = (uint16_t*)(ws + p.g);
@@ -466,10 +475,7 @@ int backward(const Where& at, const q1env_head& q, const Plan& p, bool hp, bool 
         Finish fw{dw_slab, p.dw_split, len, d, nullptr, pw.out, dw_stride, four(pw.out, dw_stride) ? 1 : 0, dw && dw_slab ? (uint32_t)div_up(len * d, 1024) : 0};
         Finish fh{dh_slab, p.dh_split, n, d, st.live, dh, dh_stride, four(dh, dh_stride) ? 1 : 0, dh && dh_slab && last ? (uint32_t)div_up(n * d, 1024) : 0};
         FinishBias fb{db_part, v, (int)div_up(n, bn_of(p.logits)), db, db && last ? (uint32_t)div_up(v, 64) : 0};
-        if (const uint64_t groups = (uint64_t)fw.groups + fh.groups + fb.groups) {
-            hipLaunchKernelGGL((finish_kernel<DT>), dim3((unsigned)groups), dim3(256), 0, at.stream, fw, fh, fb, up);
-            HIP_TRY(hipGetLastError());
-        }
+        Q1_TRY(add_parts<DT>(at, fw, fh, fb, up));
     }
     return Q1ENV_OK;
 }

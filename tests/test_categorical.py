@@ -678,3 +678,73 @@ def test_refuses_forward_mode_tangents():
     for f in calls[:2]:
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(lambda x: f(x, w, t, b), (h,), (torch.ones_like(h),))
+
+
+def _room(gib):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gib * 2 ** 30:
+        pytest.skip(f"needs {gib} GiB of device memory")
+
+
+@gpu
+def test_more_tiles_than_one_launch_holds():
+    """2^22 rows against 131073 classes: more than 2^32 threads in any tile, so that the classes go in pieces although the weights are taken as they lie"""
+    _room(40)
+    n, d, v = 2 ** 22, 8, 131073
+    g = torch.Generator(device="cuda").manual_seed(1)
+    h = torch.randn(n, d, device="cuda", generator=g).to(torch.bfloat16)
+    w = torch.randn(v, d, device="cuda", generator=g).to(torch.bfloat16)
+    t = torch.randint(0, v, (n,), device="cuda", generator=g)
+    t[5], t[6], t[n - 1] = IGN, v - 1, v - 1
+    logp, ent = categorical.linear_categorical(h, w, t)
+    i = torch.cat([torch.arange(0, n, n // 100, device="cuda"), torch.arange(8, device="cuda"), torch.arange(n - 8, n, device="cuda")])
+    T = Truth(h[i], w, None, t[i])
+    near(logp[i], T.logp, T.elogp, "logp")
+    near(ent[i], T.entropy, T.eent, "entropy")
+    assert bool(torch.isfinite(logp).all() & torch.isfinite(ent).all()) and int((logp == 0).sum()) == 1
+    del logp, ent
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_more_values_than_one_launch_lays_out():
+    """2^22 rows of 8191 halves, which have to be laid out: 2^32 threads"""
+    _room(150)
+    n, d, v = 2 ** 22, 8191, 3
+    h = torch.zeros(n, d, device="cuda", dtype=torch.float16)
+    w = torch.randn(v, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).mul_(0.01).to(torch.float16)
+    i = torch.tensor([0, 1, 2 ** 21 - 1, 2 ** 21, 2 ** 21 + 1, n - 2, n - 1], device="cuda")
+    h[i] = torch.randn(len(i), d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(torch.float16)
+    t = torch.arange(n, device="cuda") % v
+    logp, ent = categorical.linear_categorical(h, w, t)
+    T = Truth(h[i], w, None, t[i])
+    near(logp[i], T.logp, T.elogp, "logp")
+    near(ent[i], T.entropy, T.eent, "entropy")
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[i] = False
+    assert bool(((logp[rest] + math.log(v)).abs() < 1e-6).all())              # zero rows are uniform
+    del h, logp, ent
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_more_parts_than_one_launch_adds_up():
+    """the gradient of 2^22 rows of 4096 values over two pieces of the classes: 2^34 float32 sums, four to a thread"""
+    _room(150)
+    n, d, v = 2 ** 22, 4096, 300
+    h = torch.zeros(n, d, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(v, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).mul_(0.03).to(torch.bfloat16)
+    i = torch.tensor([0, 1, 2 ** 21 - 1, 2 ** 21, 2 ** 21 + 1, n - 2, n - 1], device="cuda")
+    h[i] = torch.randn(len(i), d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(torch.bfloat16)
+    t = torch.full((n,), IGN, device="cuda")
+    t[i] = torch.tensor([0, 299, 255, 256, 257, 1, 298], device="cuda")
+    loss, dh, dw, _ = categorical.linear_cross_entropy_grad(h, w, t, reduction="sum")
+    T = Truth(h[i], w, None, t[i])
+    near(loss, -T.logp.sum(), T.elogp.sum() + 4 * U * T.logp.abs().sum(), "loss")
+    ref = T.grads(torch.full((len(i),), -1.0, device="cuda"), torch.zeros(len(i), device="cuda"))
+    near(dh[i], *ref[0], "dh")
+    near(dw, *ref[1], "dw")
+    dh[i] = 0
+    assert not any(bool(x.any()) for x in dh.split(2 ** 18))
+    del h, dh
+    torch.cuda.empty_cache()
