@@ -221,6 +221,14 @@ __device__ __forceinline__ T div_const_sel(T x, T c, T y) {
     else return div_const<T>(x, c, y);
 }
 
+// m / 12.5 for an integer m, correctly rounded to float32, in two instructions: m 0.08 with the constant in two float32 parts, RN(m hi + RN(m lo)).  hi + lo is 0.08 to 2^-48 (relative) and the inner rounding
+// is below 2^-46 of the result, so the sum the fma rounds is within 2^-45 of 2 m / 25 (relative) - which is a float32 or at least 2^-24 / 25 > 2^-29 away from the middle between two, whatever m is.
+// hi lies ABOVE 0.08 (the nearest float32 lies below), so that lo is negative and m = -0 gives +0: -0 x lo = +0, -0 x hi + +0 = +0.
+__device__ __forceinline__ float div_12_5(float m) {
+    constexpr float hi = 0x1.47ae16p-4f, lo = -0x1.851eb8p-28f;
+    return __builtin_fmaf(m, hi, m * lo);
+}
+
 // a / b for two numerators sharing one denominator: the refined reciprocal (v_rcp_f64 + two Newton steps, the
 // same recurrence the compiler's own f64 division expands to) is computed once; each quotient is then
 // q = a*y, r = a - b*q, q + r*y.  With operands in the normal range (|wish_vel| <= ~2000, speeds <= ~1e4)
@@ -776,8 +784,7 @@ __device__ __forceinline__ void physics_yaw_only(const Params& p, const TickCons
 //        within 2^-29.6 (relative) of a float32 rounding boundary for 0 < |j| < 2^24, and never ON one (that needs j >= 25 * 2^24), so
 //        ANY float64 value within 2^-52 of j / 800 rounds to the same float32: RN32(j * RN64(1 / 800)), one product and one conversion
 //   vel: trunc(v / 16) = m, the reference's value is RN64(16 m / 200) = 2 m / 25 to within 2^-53 and the same argument makes its
-//        float32 rounding equal to the correctly rounded float32 quotient m / 12.5, which one Markstein step on RN32(0.08) delivers
-//        (|12.5 RN32(0.08) - 1| = 0.75 x 2^-25; m = -0 yields +0 like the reference's integer cast)
+//        float32 rounding equal to the correctly rounded float32 quotient m / 12.5 (div_12_5; m = -0 yields +0 like the reference's integer cast)
 // Both are checked EXHAUSTIVELY - every j and every m below 2^24 in magnitude - by tests/test_division_shortcuts.py (NumPy float64
 // emulation, exact for these operand widths) and on the device by q1env_selftest_division.
 // ONE_STEP: time_limit's reciprocal passes the one-step bound (SPEC kernels); 90 always does.
@@ -792,17 +799,9 @@ __device__ __forceinline__ void observe(const Params& p, const Env& e, OBS_T o[6
         o[5] = div_const<double>(trunc((double)(e.vz * 0.0625f)) * 16.0 + 0.0, 200.0, 1.0 / 200.0);
     } else {
         o[2] = (float)(rint(e.z * 8.0) * (1.0 / 800.0));
-        o[3] = div_const1<float>(truncf(e.vx * 0.0625f), 12.5f, 0.08f);
-        // (vel_y, vel_z) as ONE two-wide float32 chain (v_pk_mul / v_pk_fma): columns 4 and 5 are neighbours in the row, so the result
-        // pair is the register pair the row's third 8-byte LDS write takes
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        f2 m = {e.vy, e.vz};
-        m = __builtin_elementwise_trunc(m * 0.0625f);
-        const f2 q = m * 0.08f;
-        const f2 r = __builtin_elementwise_fma(-q, (f2)12.5f, m);
-        const f2 o45 = __builtin_elementwise_fma(r, (f2)0.08f, q);
-        o[4] = o45.x;
-        o[5] = o45.y;
+        o[3] = div_12_5(truncf(e.vx * 0.0625f));
+        o[4] = div_12_5(truncf(e.vy * 0.0625f));
+        o[5] = div_12_5(truncf(e.vz * 0.0625f));
     }
 }
 

@@ -61,7 +61,7 @@ selftest_division_kernel(uint64_t n, uint64_t seed, double c_extra0, double c_ex
     {   // vel column: v float32 -> trunc(v/16)*16 / 200, float64 reference vs float32 shortcut
         const float v = (float)((2.0 * u - 1.0) * 40000.0);
         const double ref = (trunc((double)(v / 16.0f)) * 16.0 + 0.0) / 200.0;
-        const float fast = div_const1<float>(truncf(v * 0.0625f), 12.5f, 0.08f);                  // observe<float>'s vel columns
+        const float fast = div_12_5(truncf(v * 0.0625f));                  // observe<float>'s vel columns
         bad2 += (__float_as_uint((float)ref) != __float_as_uint(fast));
         const double z = 24.03125 + 3000.0 * w;
         const double refz = (rint(z * 8.0) / 8.0) / 100.0;
@@ -73,7 +73,7 @@ selftest_division_kernel(uint64_t n, uint64_t seed, double c_extra0, double c_ex
             const double md = (double)((long long)i - (1ll << 24));
             const float mf = (float)md;
             const double refm = (md * 16.0 + 0.0) / 200.0;
-            bad2 += (__float_as_uint((float)refm) != __float_as_uint(div_const1<float>(mf, 12.5f, 0.08f)));
+            bad2 += (__float_as_uint((float)refm) != __float_as_uint(div_12_5(mf)));
             const double jd = fabs(md);
             const double refj = (jd * 0.125) / 100.0;
             bad3 += (__float_as_uint((float)refj) != __float_as_uint((float)(jd * (1.0 / 800.0))));

@@ -58,3 +58,24 @@ def test_the_bound_is_what_separates_one_step_from_two():
         return abs(F(1.0 / c) * F(c) - 1) <= F(1, 2 ** 54)
     assert ok(10.0) and ok(10.079999923706055) and ok(180.0)
     assert any(not ok(float(k) / 7.0) for k in range(1, 200))
+
+
+def test_vel_columns_two_product_quotient_is_the_reference_value_for_every_m():
+    """div_12_5: RN(m hi + RN(m lo)) with hi + lo = 0.08 in two float32 parts, exhaustively; and the bound of its comment for any m"""
+    hi, lo = float.fromhex("0x1.47ae16p-4"), float.fromhex("-0x1.851eb8p-28")
+    assert float(np.float32(hi)) == hi and float(np.float32(lo)) == lo and abs(F(hi) + F(lo) - F(2, 25)) <= F(2, 25) * F(1, 2 ** 48)
+    m = np.arange(-(1 << 24) + 1, 1 << 24, dtype=np.float64)
+    ref = ((m * 16.0 + 0.0) / 200.0).astype(np.float32)
+    # m hi has 48 bits and is exact in float64; RN(m lo) is 2^-24 of it with 24 bits: their sum spans 53 bits at most, and .astype(float32) is the fma's rounding
+    p = (m * lo).astype(np.float32).astype(np.float64)
+    got = (m * hi + p).astype(np.float32)
+    assert np.array_equal(ref.view(np.uint32), got.view(np.uint32))
+    rnd = random.Random(3)
+    for _ in range(20000):
+        x = F(rnd.randint(1 << 23, (1 << 24) - 1)) * F(2) ** rnd.randint(0, 60)
+        s = x * F(hi) + F(float(np.float32(float(x * F(lo)))))
+        assert abs(s / (x * F(2, 25)) - 1) <= F(1, 2 ** 45)
+    # the signs of zero, as the kernel's two operations give them
+    for z in (0.0, -0.0):
+        q = np.float32(z) * np.float32(lo)
+        assert str(np.float32(z) * np.float32(hi) + q) == "0.0"
