@@ -28,8 +28,11 @@ OBJ_DIR = os.path.join(PKG, "build")
 OUT = os.path.join(PKG, "libq1env.so")
 OUT_CHECK = os.path.join(PKG, "libq1env_check.so")
 
+# No packed float32 instructions, which the compiler otherwise forms from ordinary float code: some of their forms have given wrong results now and then, with no error.  (They are the same IEEE
+# operations in the same order otherwise: every result keeps its bits.  The env core's tick is 239 vector instructions without them and 237 with.)  check_objects refuses a library that has one.
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 COMPILE_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-fvisibility=hidden",
-                 "-Wall", "-Wno-unused-function",
+                 "-Wall", "-Wno-unused-function", *NO_PACKED,
                  "-mllvm", "-amdgpu-kernarg-preload-count=16"]   # leading scalar kernel arguments arrive in SGPRs (step_kernel's state pointers)
 # per translation unit, on top of COMPILE_FLAGS.  q1env_learner.hip: matrix instructions take their C / D operands in the ordinary
 # vector registers wherever the allocator can afford it (round 4): the learner's backward kernel spent 19 % of its vector instructions
@@ -41,10 +44,6 @@ TU_FLAGS = {"q1env_learner.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
             # optimizer: that pass rewrites a uniform-address atomic into a wave reduction + s_waitcnt vmcnt(0) + readfirstlane, i.e. it
             # makes the barrier poll that is requested early and looked at late (q1learner_persist.hpp, barrier 3) synchronous again
             "q1env_plearner.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]}
-# No packed float32 instructions, which the compiler otherwise forms from ordinary float code: some of their forms have given wrong results now and then.  The env core keeps them:
-# its rollout is one wave per SIMD and pays for every instruction (237 a tick with them, 242 without: 90.4e9 and 89.3e9 env steps/s), and every tick is held to the oracle.
-NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-TU_FLAGS = {src: NO_PACKED + TU_FLAGS.get(src, []) for src in map(os.path.basename, SOURCES) if src != "q1env_core.hip"}
 LINK_FLAGS = ["--offload-arch=gfx950", "-shared", "-fPIC"]
 HIPCC_FLAGS = COMPILE_FLAGS + ["-shared"]     # (kept for tools that compile a single file the old way, e.g. tools/asan_check.sh)
 
@@ -103,7 +102,7 @@ def _run(cmd, verbose):
 def build_lib(force=False, verbose=False, check=False, extra_flags=(), out=None, tag=None):
     """Compile the stale translation units (in parallel) and link.  check=True: the -DQ1_CHECK assertion build (libq1env_check.so).
     out / tag: an experimental variant (extra_flags) built next to the product library, e.g. tools/exp_step_large.py.
-    Every library is disassembled and held to q1physrl_amd/isa_check.py's rule before it replaces the previous one (the compiler bug that made
+    Every library is disassembled and held to q1physrl_amd/isa_check.py's rules before it replaces the previous one (the compiler bug that made
     the persistent learner fault once is visible in the machine code and nowhere else)."""
     if out is None:
         out = OUT_CHECK if check else OUT

@@ -257,9 +257,7 @@ __device__ __forceinline__ void store_n(f16x8* dstN, uint32_t t, const f32x16& d
 }
 
 // acc (float32, C/D layout) *= 1 - h^2 with h the matching T-format vectors; returns nothing, acc updated in place
-// (two elements per instruction - v_pk_mul_f32 / v_pk_add_f32 on register pairs: the same IEEE operations in the same order as the scalar
-// form, RN(acc RN(1 - RN(h h))), so the bits are the same; 1.5 instead of 3 vector instructions per element, and this function was 41 % of
-// the backward kernel's vector instructions)
+// (written on pairs of elements; the operations are RN(acc RN(1 - RN(h h))) of each, three scalar vector instructions, since the units are compiled without packed float32 ones: build.py NO_PACKED)
 __device__ __forceinline__ void times_dtanh(f32x16& acc, const f16x8 h0, const f16x8 h1) {
     typedef float f32x2_t __attribute__((ext_vector_type(2)));
     const f32x2_t one = {1.0f, 1.0f};

@@ -314,9 +314,9 @@ __device__ __forceinline__ float adam1(float w, float g, float& m, float& v, flo
     return w - lr_bc1 * (m * __builtin_amdgcn_rcpf(denom));
 }
 
-// two elements at a time: the same operations in the same order (packed float32 multiply / add; square root and reciprocal per element)
+// two elements at a time: the same operations in the same order as one at a time (and the same instructions: build.py NO_PACKED)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-// (An explicitly fused form - v_pk_fma_f32, 13 instead of 17 instructions per pair, -0.1 us per step - was built and is equivalent (391 steps
+// (An explicitly fused form, -0.1 us per step when packed instructions were in use, was built and is equivalent (391 steps
 //  against the four-launch path: the same 1e-4); it is NOT used: at seed 0 the reference-configuration run ended at 5 345 with it instead of
 //  5 666 - seeds 1 and 2 went the other way over their first 300 iterations, i.e. the run is that sensitive to rounding - and the unfused form
 //  keeps this kernel on the trajectory of the round's earlier runs.  STATE.md.)

@@ -24,7 +24,7 @@
 // 2 log2 e folded into the producing layer's weights.
 // Measured on MI355X (tools/trace_mlp.py, gpurun_scratch micro-benchmarks): under this load the shader
 // clock settles at ~1.6 GHz; a tile costs ~7 600 cycles per SIMD against a VALU floor of ~6 500 (512 tanh per lane: 4 250 cycles
-// of v_exp/v_rcp at 8.3 cycles each, the rest packed float32 and f16 converts) and an MFMA floor of 4 864 (152 x 32 cycles).
+// of v_exp/v_rcp at 8.3 cycles each, the rest float32 arithmetic and f16 converts) and an MFMA floor of 4 864 (152 x 32 cycles).
 // What mattered, in order: accumulators in VGPRs (a 256-register budget; with 512 the compiler parks them in AGPRs and pays a
 // v_accvgpr_read per tanh input), layer 1 as one f16 MFMA instead of four dependent float32 ones, MFMA / VALU alternation in the
 // instruction stream (one wave issues in order), both networks in one launch (weight staging overlaps).
@@ -50,13 +50,12 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // tanh(z) = 1 - 2 / (2^(c z) + 1) with c = 2 log2(e).  The factor c is folded into the weights and biases of the layer that
 // PRODUCES z (W1, b1 here at staging; the W2 block of the host-built image; b2 at staging), so the accumulators already hold c z
-// and an activation is v_exp_f32, +1, v_rcp_f32, 1 - 2r: one packed multiply less per pair of values on the VALU that bounds
+// and an activation is v_exp_f32, +1, v_rcp_f32, 1 - 2r: one multiply less per value on the VALU that bounds
 // this kernel.
 constexpr float TANH_PRESCALE = 2.8853900817779268f;                 // 2 log2(e)
 
 // tanh of accumulator registers 8u .. 8u+7 (holding c z) -> the lane's f16 B operand of K-step 2t + u.  Two values at a time:
-// the +1 and the final 1 - 2r are packed float32 instructions (v_pk_add/fma_f32), only v_exp_f32 and v_rcp_f32 are per
-// element; the pair is converted with one v_cvt_pk_f16_f32 (RNE).
+// the pair is converted with one v_cvt_pk_f16_f32 (RNE).
 __device__ __forceinline__ f16x8 activate(const f32x16& acc, int u) {
     union { f16x8 v; f16x2 p[4]; } o;
 #ifdef Q1POL_ACT_PK16

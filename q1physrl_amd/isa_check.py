@@ -24,8 +24,11 @@ exit of a divergent loop (behind `s_andn2_b64 exec, exec, m ; s_cbranch_execnz`)
 (`s_or_b64 exec, exec, x`, `s_or_saveexec_b64`, `s_mov_b64 exec, x`), must not execute a vector instruction before it (v_readlane / v_writelane / v_readfirstlane ignore EXEC and are what the compiler's own
 scalar spills use there: allowed).
 
-build_lib() runs this on the objects it links and refuses to produce a library that violates it; tests/test_isa_exec_restore.py runs it on
-every translation unit's assembly and on a synthetic positive (the faulting form itself, -DQ1PL_ONE_ROW_VAR, is kept compilable for that).
+build_lib() runs this on the library it links and refuses to produce one that violates it; tests/test_isa_exec_restore.py runs it on the libraries that build() made, on
+synthetic blocks and on the faulting block itself (tests/golden/r6_faulting_join_block.s).
+
+A second rule: no packed float32 arithmetic (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32).  Some of their forms have given wrong results now and then; the compile flags turn them off
+(build.py NO_PACKED), and a unit that was compiled without the flag shows here.
 """
 import os
 import re
@@ -173,6 +176,14 @@ def device_disassembly(path, workdir=None):
             shutil.rmtree(tmp, ignore_errors=True)
 
 
+_PACKED = re.compile(r"^\s*(v_pk_(?:add|mul|fma)_f32)\b", re.M)
+
+
+def packed_float32(text):
+    """The packed float32 instructions of an assembly or disassembly."""
+    return _PACKED.findall(text)
+
+
 def format_violations(v, limit=6):
     rows = []
     for func, label, line, pend in v[:limit]:
@@ -186,7 +197,10 @@ def check_objects(paths):
     """Raise RuntimeError naming every violation found in the device code of `paths` (host objects / shared libraries)."""
     bad = []
     for p in paths:
-        v = exec_restore_violations(device_disassembly(p))
+        text = device_disassembly(p)
+        v, packed = exec_restore_violations(text), packed_float32(text)
+        if packed:
+            raise RuntimeError(f"{os.path.basename(p)}: {len(packed)} packed float32 instructions, first {packed[0]}: a unit was compiled without build.NO_PACKED")
         if v:
             bad.append(os.path.basename(p) + ":\n" + format_violations(v))
     if bad:

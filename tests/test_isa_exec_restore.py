@@ -137,3 +137,13 @@ def test_build_refuses_a_violating_library(tmp_path, monkeypatch):
     monkeypatch.setattr(isa_check, "device_disassembly", lambda path, workdir=None: open(GOLDEN).read())
     with pytest.raises(RuntimeError, match="exec restore"):
         isa_check.check_objects([os.path.join(build.PKG, "libq1env.so")])
+
+
+def test_no_packed_float32_arithmetic_in_any_library():
+    """the compile flags turn it off for every translation unit; the rule sees one where it is (the assembly of a unit compiled without them, and the libraries build() made)"""
+    from q1physrl_amd import build
+    assert isa_check.packed_float32("\tv_pk_mul_f32 v[0:1], v[2:3], v[4:5]\n\tv_pk_mul_f16 v0, v1, v2\n\tv_mul_f32_e32 v0, v1, v2\n") == ["v_pk_mul_f32"]
+    assert all(f in build.COMPILE_FLAGS for f in build.NO_PACKED) and not any(f in build.NO_PACKED for flags in build.TU_FLAGS.values() for f in flags)
+    for lib in (build.OUT, build.OUT_CHECK):
+        if os.path.exists(lib):
+            assert isa_check.packed_float32(isa_check.device_disassembly(lib)) == [], lib
