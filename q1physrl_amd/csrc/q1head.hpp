@@ -111,7 +111,7 @@ __device__ __forceinline__ void load_to_lds(const char* base, uint32_t size, uin
     auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };      // (all of it is; the resource has to sit in scalar registers)
     const u32x4 rsrc = {uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffffu), uniform(size), 0x00020000u};
     // (no result registers: what the instruction writes is LDS, waited for with vmcnt before the barrier in front of its use)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(uniform(lds)), "v"(offset), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(uniform(lds)), "v"(offset), "s"(rsrc) : "memory", "m0");
 }
 template <int N> __device__ __forceinline__ void wait_loads() {             // all but the N youngest loads have landed, and this wave's LDS reads are done
     static_assert(N < 64, "vmcnt");

@@ -147,3 +147,18 @@ def test_no_packed_float32_arithmetic_in_any_library():
     for lib in (build.OUT, build.OUT_CHECK):
         if os.path.exists(lib):
             assert isa_check.packed_float32(isa_check.device_disassembly(lib)) == [], lib
+
+
+def test_inline_assembly_names_the_m0_it_writes():
+    """a statement that writes m0 without saying so leaves the compiler free to keep a value of its own there across it"""
+    import glob
+    import re
+    found = 0
+    for path in glob.glob(os.path.join(ROOT, "q1physrl_amd", "csrc", "*.h*")):
+        text = open(path).read()
+        for m in re.finditer(r"asm\s*(?:volatile)?\s*\((.*?)\)\s*;", text, re.S):
+            body = re.sub(r'"v"\([^)]*\)', "", m.group(1))
+            if re.search(r"s_mov_b32 m0|s_add_u32 m0", body):
+                found += 1
+                assert '"m0"' in text[m.start():text.index(";\n", m.start())], (path, m.group(0))
+    assert found >= 1
