@@ -242,7 +242,8 @@ class PPOLearner:
                  optimizer; self.grad_norm holds the last step's norm (a device scalar).  With native=True the optimizer is then torch's, as with several
                  processes (the library's own step goes from gradient sums to new weights in one kernel).
     logits_free: for a discrete mouse with many steps: the loss takes log-probability and entropy of the sampled actions from the network's hidden layer and
-                 last weights (Q1Policy.evaluate_actions) and estimates the KL from them, so that no (samples x 2S+1) array exists; GPU only, not with
+                 last weights (Q1Policy.evaluate_actions) and estimates the KL from them, so that it stores no (samples x 2S+1) array (nor does the trajectory of a
+                 GpuSampler(keep_logits=False); logits that a trajectory has are not read); GPU only, not with
                  native / fused_loss (their kernels walk stored logits) or use_graph (the head's differentiable form cannot be captured).
     native:      the WHOLE step up to the gradients - minibatch gather, both MLPs forward and backward, the loss gradient, the weight
                  gradients - is the library's own gfx950 kernels (NativeStep / q1env_learner_step: float16 matrix-core operands,

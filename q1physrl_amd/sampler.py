@@ -23,8 +23,11 @@ from .tensor_env import TensorVectorEnv
 
 class GpuSampler:
     def __init__(self, env: TensorVectorEnv, policy, horizon: int, autocast_dtype=None, use_graph: bool = False,
-                 fused_tick: bool = True, resident: bool = False):
-        """resident=True: the whole horizon is ONE dispatch (q1env_sample_resident: policy blocks with the network's weights in LDS
+                 fused_tick: bool = True, resident: bool = False, keep_logits: bool = True):
+        """keep_logits=False: the trajectory has no "logits" (what PPOLearner(logits_free=True) does without): one tick's rows exist at a time
+        instead of (T, N, row width) - with a mouse of 4 097 steps and 50 000 samples 820 MB.  Not with resident.
+
+        resident=True: the whole horizon is ONE dispatch (q1env_sample_resident: policy blocks with the network's weights in LDS
         and env blocks with the state in registers, talking through tagged granules) followed by one batched value-network
         forward over the stored observations - bit-identical trajectories, no per-tick launches.  Needs a FusedPolicyForward
         policy (continuous, discrete - up to 24 outputs - or no mouse); any batch size (q1env.h); use_graph is
@@ -36,6 +39,9 @@ class GpuSampler:
         self.resident = bool(resident)
         if self.resident and not hasattr(policy, "_mlp"):
             raise ValueError("GpuSampler(resident=True) needs a policy.FusedPolicyForward")
+        self.keep_logits = bool(keep_logits)
+        if self.resident and not self.keep_logits:
+            raise ValueError("GpuSampler(resident=True) keeps its logits: they are written by the dispatch")
         n, d, t = env.num_envs, env.device, self.T
         self.obs = torch.empty((t + 1, n, 6), dtype=torch.float32, device=d)
         self.keys = torch.empty((t, n), dtype=torch.uint8, device=d)
@@ -43,7 +49,7 @@ class GpuSampler:
         self.logp = torch.empty((t, n), dtype=torch.float32, device=d)
         from .policy import policy_row_width
         width = policy_row_width(env.num_keys, env.config.discrete_yaw_steps, env.config.allow_yaw)
-        self.logits = torch.empty((t, n, width), dtype=torch.float32, device=d)   # behaviour-policy outputs
+        self.logits = torch.empty((t if self.keep_logits else 1, n, width), dtype=torch.float32, device=d)   # behaviour-policy outputs
         self.value = torch.empty((t + 1, n), dtype=torch.float32, device=d)
         self.reward = torch.empty((t, n), dtype=torch.float32, device=d)
         self.done = torch.empty((t, n), dtype=torch.uint8, device=d)
@@ -74,7 +80,7 @@ class GpuSampler:
         cnt = self.tick.data_ptr()
         into = getattr(self.policy, "forward_into", None)
         for t in range(self.T):
-            logits = self.logits[t]                   # what the actions are really sampled from (the learner's "old" policy)
+            logits = self.logits[t if self.keep_logits else 0]      # what the actions are really sampled from (the learner's "old" policy)
             if into is not None:
                 into(self.obs[t], logits, self.value[t])
             else:
@@ -155,7 +161,7 @@ class GpuSampler:
                 self._capture(key)
             else:
                 self._graphs[key].replay()
-        return {"obs": self.obs, "keys": self.keys, "mouse": self.mouse, "logp": self.logp, "logits": self.logits,
+        return {"obs": self.obs, "keys": self.keys, "mouse": self.mouse, "logp": self.logp, **({"logits": self.logits} if self.keep_logits else {}),
                 "value": self.value, "reward": self.reward, "done": self.done}
 
     def _capture(self, deterministic):

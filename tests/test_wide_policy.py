@@ -249,3 +249,56 @@ def test_averaged_and_clipped_gradients_of_mixed_types_and_layouts(monkeypatch):
         for p, w in zip(params, want):
             ref = w.double() * (0.5 / norm)
             assert bool(((p.grad.double() - ref).abs() <= ref.abs() * (2 ** -8 + 2 ** -22 if p.dtype == torch.bfloat16 else 2 ** -22)).all())
+
+
+@gpu
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_from_the_sampler_to_the_logits_free_step(use_graph):
+    """GpuSampler with a mouse of 4 097 steps into PPOLearner(logits_free=True): with and without kept logits the same trajectory and the same step; the sampler's
+    log-probabilities, taken from its logits, are those the head gives for its actions; the statistics of the first step are the stored-logits loss's."""
+    from q1physrl_amd.env import Config
+    from q1physrl_amd.sampler import GpuSampler
+    from q1physrl_amd.tensor_env import TensorVectorEnv
+    steps, n, t = 2048, 64, 6
+    cfg = Config(**{**Config.get_default().__dict__, "num_envs": n, "discrete_yaw_steps": steps})
+
+    def run(keep, logits_free):
+        torch.manual_seed(0)
+        env = TensorVectorEnv(cfg, device=0, seed=1)
+        pol, *_ = make(steps, 1, seed=3)
+        smp = GpuSampler(env, pol, horizon=t, use_graph=use_graph, keep_logits=keep)
+        assert smp.logits.shape == ((t if keep else 1), n, 8 + 2 * steps + 1)
+        smp.collect()
+        traj = smp.collect()
+        assert ("logits" in traj) == keep
+        with torch.no_grad():
+            logp, ent, _ = pol.evaluate_actions(traj["obs"][:t].reshape(-1, 6), (traj["keys"].reshape(-1, 1).long() >> torch.arange(4, device="cuda")) & 1, traj["mouse"].reshape(-1))
+        # both float32 sums over 256 terms of weights around 0.06 and logits of a few units
+        assert float((logp - traj["logp"].reshape(-1)).abs().max()) <= 1e-4
+        adv, vt = smp.advantages(traj, 0.99, 0.95)
+        lrn = ppo.PPOLearner(pol, float(cfg.action_range), lr=1e-4, num_sgd_iter=1, minibatch_size=t * n, discrete_yaw_steps=steps, logits_free=logits_free)
+        kept = {k: v.clone() for k, v in traj.items()}
+        out = lrn.update(traj, adv, vt)
+        grads = [p.grad.clone() for p in pol.parameters()]
+        env.close()
+        return kept, out, grads, float(ent.mean())
+    a, oa, ga, ea = run(True, True)
+    b, ob, gb, _ = run(False, True)
+    assert all(torch.equal(a[k], b[k]) for k in b) and oa == ob and all(map(torch.equal, ga, gb))
+    assert int(a["mouse"].max()) > steps and int(a["mouse"].min()) >= 0
+    _, oc, gc, _ = run(True, False)
+    assert abs(oa["entropy"] - ea) <= 1e-4 * ea
+    for k in ("policy_loss", "vf_loss", "entropy"):
+        assert abs(oa[k] - oc[k]) <= 1e-4 * (1 + abs(oc[k])), k
+    assert abs(oa["kl"]) <= 1e-4 and abs(oc["kl"]) <= 1e-4
+    for x, y in zip(ga, gc):                                     # at the old policy the estimated KL has no gradient, nor has the exact one
+        assert float((x - y).norm()) <= 1e-3 * (float(y.norm()) + 1e-3)
+
+
+def test_a_resident_sampler_keeps_its_logits():
+    from q1physrl_amd.sampler import GpuSampler
+
+    class Fused:
+        _mlp = None
+    with pytest.raises(ValueError, match="keeps its logits"):
+        GpuSampler(None, Fused(), 4, resident=True, keep_logits=False)

@@ -91,7 +91,8 @@ ck = torch.load(args.restore, map_location="cuda", weights_only=False) if args.r
 env = TensorVectorEnv(cfg, device=local, seed=args.seed + 1 + (1000003 * (int(ck["iter"]) + 1) if ck is not None else 0), env_index_base=start)
 pol = P.Q1Policy(discrete_yaw_steps=args.discrete_yaw_steps).cuda()
 fused = P.FusedPolicyForward(pol, env) if args.fused_policy else None
-smp = GpuSampler(env, fused if fused is not None else pol, horizon=args.horizon, use_graph=not args.no_graph, resident=args.resident)
+smp = GpuSampler(env, fused if fused is not None else pol, horizon=args.horizon, use_graph=not args.no_graph, resident=args.resident,
+                 keep_logits=args.resident or not args.logits_free)
 env._dev.learner_set_step_mode(args.step_mode)
 lrn = ppo.PPOLearner(pol, float(cfg.action_range), lr=args.lr, num_sgd_iter=args.epochs, minibatch_size=args.minibatch,
                      entropy_coeff=args.entropy, kl_target=args.kl_target, seed=args.seed + rank, use_graph=not args.no_graph and not args.logits_free, fused_loss=args.fused_loss, env=env,
