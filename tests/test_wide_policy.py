@@ -302,3 +302,48 @@ def test_a_resident_sampler_keeps_its_logits():
         _mlp = None
     with pytest.raises(ValueError, match="keeps its logits"):
         GpuSampler(None, Fused(), 4, resident=True, keep_logits=False)
+
+
+@gpu
+@pytest.mark.parametrize("steps,batch", [(5, 1), (5, 300), (360, 257), (2048, 100)])
+def test_evaluate_actions_term_by_term(steps, batch):
+    """The head's own error, without the layers before it: in float64 from the very hidden rows the call computed (test_categorical.Truth bounds the mouse's part, derived there; a key's
+    logits are off by el, its log-probability and entropy by 2 el and a few roundings).  Log-probability and entropy are differentiated apart, and every part of the gradient is held to its
+    own bound, so that none can be missing."""
+    from tests.test_categorical import Truth, near
+    pol, obs, keys, mouse = make(steps, batch)
+    seen = []
+    pol.pi[-2].register_forward_hook(lambda m, i, o: seen.append(o) or o.retain_grad())
+    logp, ent, value = pol.evaluate_actions(obs, keys, mouse)
+    assert torch.equal(value, pol.vf(obs).squeeze(-1))
+    h = seen[0].detach()
+    w, b = pol.pi[-1].weight.detach(), pol.pi[-1].bias.detach()
+    T = Truth(h, w[8:], b[8:], mouse[:, 0].long())
+    leaves = [x.double().requires_grad_() for x in (h, w[:8], b[:8])]
+    z = torch.nn.functional.log_softmax((leaves[0] @ leaves[1].T + leaves[2]).view(batch, 4, 2), 2)
+    klp, kent = z.gather(2, keys[:, :, None])[:, :, 0].sum(1), -(z.exp() * z).sum((1, 2))
+    S = (h.double().abs() @ w[:8].double().abs().T + b[:8].double().abs()).amax(1)
+    el = (256 + 8) * 2 * U * S
+    ek = 4 * (2 * el + 16 * U * (z.detach().abs().amax((1, 2)) + 1)) + 8 * U * (T.logp.abs() + T.entropy)
+    near(logp, T.logp + klp.detach(), T.elogp + ek, "logp")
+    near(ent, T.entropy + kent.detach(), T.eent + 3 * ek, "entropy")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    A, E, zero = torch.randn(batch, device="cuda", generator=g), torch.randn(batch, device="cuda", generator=g), torch.zeros(batch, device="cuda")
+    for out, ref, A_, E_ in ((logp, klp, A, zero), (ent, kent, zero, E)):
+        pol.zero_grad()
+        seen[0].grad = None
+        out.backward(A_ + E_, retain_graph=True)
+        (dh, th), (dw, tw), (db, tb) = T.grads(A_, E_)
+        kh, kw, kb = torch.autograd.grad(ref, leaves, (A_ + E_).double(), retain_graph=True)
+        # a key's gradient of a logit is off by 3 ek of the upstream at most, and sums of those by that of the absolute products
+        off = 3 * ek * (A_ + E_).double().abs()
+        size = (A_ + E_).double().abs() * 2
+        rounding = (batch + 264) * 2 * U
+        near(seen[0].grad, dh + kh, th + (off + rounding * size)[:, None] * w[:8].double().abs().sum(0) + 8 * U * (dh.abs() + kh.abs()), "dhidden")
+        near(pol.pi[-1].weight.grad[8:], dw, tw * 1.01, "dweight, mouse")
+        near(pol.pi[-1].bias.grad[8:], db, tb * 1.01, "dbias, mouse")
+        near(pol.pi[-1].weight.grad[:8], kw, ((off + rounding * size) @ h.double().abs()).expand(8, -1) + 8 * U * kw.abs(), "dweight, keys")
+        near(pol.pi[-1].bias.grad[:8], kb, (off + rounding * size).sum().expand(8) + 8 * U * kb.abs(), "dbias, keys")
+        assert all(p.grad is not None and bool(p.grad.any()) for p in pol.pi.parameters())
+        # a part that were missing would be over its bound somewhere: it is larger than the bound as a whole
+        assert float(th.norm()) < float(dh.norm()) and float(tw.norm()) < float(dw.norm())
