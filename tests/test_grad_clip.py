@@ -293,3 +293,19 @@ def test_results_carry_no_graph():
     g = x * 3.0
     out = [torch.zeros(50, device="cuda")]
     assert not clip.grad_norm([g]).requires_grad and not clip.clip_grad_norm_([g], 1.0, out=out).requires_grad and not out[0].requires_grad
+
+
+@gpu
+def test_autograd_learns_of_the_write_beside_inference_tensors():
+    """a list that begins with a tensor made in inference mode: the others' versions count all the same"""
+    with torch.inference_mode():
+        first = torch.full((16,), 2.0, device="cuda")
+    x = torch.randn(10, device="cuda", requires_grad=True)
+    z = (x * 2).exp()
+    clip.clip_grad_norm_([first, z.detach()], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        z.sum().backward()
+    out = [torch.zeros(16, device="cuda"), torch.zeros(10, device="cuda")]
+    before = out[1]._version
+    clip.clip_grad_norm_([first, x.detach()], 0.1, out=out)
+    assert out[1]._version > before
