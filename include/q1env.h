@@ -627,7 +627,7 @@ int q1env_head_backward(int device, void* stream, const q1env_head* head, const 
  *   dst = src x scale x (norm <= max_norm ? 1 : max_norm / norm)
  * Tensor i holds values[i] elements of type dtype[i] at src[i] (device addresses in HOST arrays, read before the call returns): contiguous, or -
  * where cols is given and cols[i] != 0 - rows of cols[i] elements, src_pitch[i] / dst_pitch[i] elements apart.  dst[i] == src[i] clips in place (nothing
- * is written when there is nothing to scale); a result that overlaps another tensor is refused.  What is not finite is not hidden: a NaN
+ * is written when there is nothing to scale); a result, the norm or a workspace that overlaps a tensor that is not its own source is refused.  What is not finite is not hidden: a NaN
  * gradient makes the norm and every result NaN, an infinite one makes the norm infinite and turns finite values to zero.  norm: one float on the device; a norm past float32's
  * range is reported as infinite, and the gradients are clipped by its float64 value all the same. */
 uint64_t q1env_grad_norm_workspace_bytes(int count);

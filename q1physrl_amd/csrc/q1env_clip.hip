@@ -208,7 +208,8 @@ struct Job {
 struct Span { Extent x; int i; };
 uintptr_t end_of(const Extent& x) { return x.at + (uintptr_t)(x.rows - 1) * x.pitch + x.row; }
 
-int check_job(const char* who, const Job& j, bool write) {
+// own: the norm and the workspace, which the call writes besides
+int check_job(const char* who, const Job& j, bool write, const Extent (&own)[2]) {
     if (j.count < 0 || j.count > 65536) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": tensor count out of range (0 .. 65536)");
     if (j.count > 0 && (!j.src || !j.values || !j.dtype || (write && !j.dst))) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": null argument");
     if (j.cols && (!j.src_pitch || (write && !j.dst_pitch))) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": pitched tensors need their pitches");
@@ -229,6 +230,16 @@ int check_job(const char* who, const Job& j, bool write) {
         }
     }
     if (total > (int64_t)1 << 42) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": more than 2^42 values");
+    bool free = apart(own[0], own[1]);
+    for (int i = 0; i < j.count && free; ++i) {
+        const uintptr_t es = elem_size(j.dtype[i]);
+        const bool pitched = j.cols && j.cols[i] && j.values[i];
+        const int64_t c = pitched ? j.cols[i] : j.values[i], rows = pitched ? j.values[i] / c : 1;
+        for (const Extent& o : own)
+            free = free && apart(o, Extent{(uintptr_t)j.src[i], rows, c * es, pitched ? (uintptr_t)j.src_pitch[i] * es : 0}) &&
+                   (!write || apart(o, Extent{(uintptr_t)j.dst[i], rows, c * es, pitched ? (uintptr_t)j.dst_pitch[i] * es : 0}));
+    }
+    if (!free) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": the norm or the workspace overlaps a tensor or the other");
     if (!write) return 0;
     // no value is written by one tensor and read or written by another: every destination against all spans
     std::vector<Span> s;
@@ -268,7 +279,8 @@ int64_t unit_of(const Job& j) {
 }
 
 int run(const char* who, int device, hipStream_t stream, const Job& j, bool write, double scale, double max_norm, float* norm, void* ws, uint64_t ws_bytes) {
-    if (int rc = check_job(who, j, write)) return rc;
+    const Extent own[2] = {{(uintptr_t)norm, 1, 4, 0}, {(uintptr_t)ws, 1, q1env_grad_norm_workspace_bytes(j.count), 0}};
+    if (int rc = check_job(who, j, write, own)) return rc;
     if (!norm) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": norm is NULL");
     if (!(scale > 0.0) || std::isinf(scale)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": scale must be positive and finite");
     if (write && !(max_norm >= 0.0)) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": max_norm must not be negative or NaN");

@@ -309,3 +309,23 @@ def test_autograd_learns_of_the_write_beside_inference_tensors():
     before = out[1]._version
     clip.clip_grad_norm_([first, x.detach()], 0.1, out=out)
     assert out[1]._version > before
+
+
+def test_the_library_refuses_a_norm_or_workspace_over_a_tensor():
+    lib = _lib.load()
+    a, b, ws, norm = 1 << 20, 1 << 21, 1 << 24, 1 << 23
+
+    def norm_only(src, values, **kw):
+        k = dict(norm=norm, ws=ws, cols=None, sp=None, device=0)
+        k.update(kw)
+        arr = lambda x, t: None if x is None else np.array(x, t)  # noqa: E731
+        keep = [arr(src, np.uint64), arr(values, np.int64), arr([0] * len(src), np.int32), arr(k["cols"], np.int64), arr(k["sp"], np.int64)]
+        return lib.q1env_grad_norm(k["device"], None, len(src), *[_lib.ptr(x) for x in keep], 1.0, k["norm"], k["ws"], 1 << 20)
+    for kw in (dict(norm=a + 36), dict(ws=a - 16), dict(norm=b), dict(norm=ws + 16)):
+        assert call(lib, src=[a, b], dst=[a, b], values=[10, 10], **{"ws": ws, "norm": norm, **kw}) == -1 and b"the norm or the workspace" in lib.q1env_last_error(), kw
+        assert norm_only([a, b], [10, 10], **kw) == -1 and b"the norm or the workspace" in lib.q1env_last_error(), kw
+    assert call(lib, src=[a], dst=[b], values=[10], ws=ws, norm=b + 4) == -1 and b"the norm or the workspace" in lib.q1env_last_error()
+    assert norm_only([a], [20], cols=[4], sp=[10], norm=a + 12) == -1 and b"the norm or the workspace" in lib.q1env_last_error()
+    # beside them: on to the next check (no such device)
+    for kw in (dict(src=[a, b], values=[10, 10], norm=a + 40), dict(src=[a, 0], values=[10, 0])):
+        assert norm_only(device=99, **kw) != 0 and b"the norm or the workspace" not in lib.q1env_last_error()
