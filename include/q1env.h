@@ -616,8 +616,8 @@ uint64_t q1env_head_workspace_bytes(int dtype, int64_t rows, int64_t width, int6
  * rows that are not ignored (Q1ENV_REDUCE_MEAN; 0 when all are). */
 int q1env_head_forward(int device, void* stream, const q1env_head* head, int reduction, float* logp_dev, float* entropy_dev, float* loss_dev);
 /* The gradients of hidden, weight and bias (each may be NULL) for EITHER dlogp / dentropy (float[rows], one may be NULL) OR dloss (one float: the
- * gradient of the loss the forward call wrote).  The head is the one the forward call had, with its state; results are overwritten.  A result (of either call) may not
- * overlap what the call reads, the workspace or another result (rows of one pitch may interleave); state and workspace are aligned to 16 bytes.  dentropy needs a
+ * gradient of the loss the forward call wrote).  The head is the one the forward call had, with its state; results are overwritten.  What a call writes (results,
+ * the workspace, the forward call's state) may not overlap what it reads or each other (rows of one pitch may interleave); state and workspace are aligned to 16 bytes.  dentropy needs a
  * forward call that was asked for the entropy (results are NaN otherwise). */
 int q1env_head_backward(int device, void* stream, const q1env_head* head, const float* dlogp_dev, const float* dentropy_dev, const float* dloss_dev,
                         void* dhidden_dev, int64_t dhidden_stride, void* dweight_dev, int64_t dweight_stride, void* dbias_dev);

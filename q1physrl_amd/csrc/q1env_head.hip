@@ -27,7 +27,7 @@ int check_head(const char* who, const q1env_head* hd) {
     return 0;
 }
 
-// results against everything that is read, the workspace and each other
+// what the call writes - results, the workspace, the forward call's state - against everything that is read and each other
 int check_apart(const char* who, const Extent* results, int n, const q1env_head& hd, uint64_t ws_bytes, bool backward) {
     const uintptr_t es = elem_size(hd.dtype);
     const Extent others[] = {{(uintptr_t)hd.hidden_dev, hd.rows, (uintptr_t)hd.width * es, (uintptr_t)hd.hidden_stride * es},
@@ -42,6 +42,9 @@ int check_apart(const char* who, const Extent* results, int n, const q1env_head&
         for (int k = 0; k < i; ++k)
             if (!apart(results[i], results[k])) return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": two results overlap");
     }
+    for (int k = 0; k < 4; ++k)
+        if (!apart(others[k], others[5]) || (!backward && !apart(others[k], others[4])))
+            return fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": the state or the workspace overlaps an operand");
     return apart(others[4], others[5]) ? 0 : fail(Q1ENV_ERR_INVALID_ARG, std::string(who) + ": the state overlaps the workspace");
 }
 
@@ -111,9 +114,11 @@ static int head_backward(int device, void* stream, const q1env_head* hd, const f
                               {(uintptr_t)dbias, 1, hd->classes * size, 0}};
     if (int rc = check_apart(who, results, 3, *hd, need, true)) return rc;
     const Extent upstream[] = {{(uintptr_t)dlogp, 1, 4 * (uintptr_t)hd->rows, 0}, {(uintptr_t)dentropy, 1, 4 * (uintptr_t)hd->rows, 0}, {(uintptr_t)dloss, 1, 4, 0}};
-    for (const Extent& r : results)
-        for (const Extent& u : upstream)
+    for (const Extent& u : upstream) {
+        for (const Extent& r : results)
             if (!apart(r, u)) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_backward: a result overlaps an upstream gradient");
+        if (!apart(u, Extent{(uintptr_t)hd->ws_dev, 1, need, 0})) return fail(Q1ENV_ERR_INVALID_ARG, "q1env_head_backward: the workspace overlaps an upstream gradient");
+    }
     if (int rc = guard_device(who, device)) return rc;
     DeviceGuard guard(device);
     if (hd->rows == 0) {                             // no sample: the weights' gradients are zero

@@ -748,3 +748,19 @@ def test_more_parts_than_one_launch_adds_up():
     assert not any(bool(x.any()) for x in dh.split(2 ** 18))
     del h, dh
     torch.cuda.empty_cache()
+
+
+def test_the_library_refuses_a_workspace_or_state_over_an_operand():
+    lib = _lib.load()
+    rows, width, classes, base = 64, 8, 5, 1 << 24
+    at = dict(hidden_dev=base, weight_dev=base + (1 << 16), bias_dev=base + (2 << 16), target_dev=base + (3 << 16), state_dev=base + (4 << 16), ws_dev=base + (1 << 20))
+    free = base + (8 << 16)
+    f, b = lib.q1env_head_forward, lib.q1env_head_backward
+    for name in ("hidden_dev", "weight_dev", "bias_dev", "target_dev"):
+        for what in ("ws_dev", "state_dev"):
+            hd = head(rows=rows, width=width, classes=classes, **{**at, what: at[name]})
+            assert f(0, None, C.byref(hd), 0, free, None, None) == -1 and b"overlaps an operand" in lib.q1env_last_error(), (name, what)
+            if what == "ws_dev" and name != "target_dev":
+                assert b(0, None, C.byref(hd), free, None, None, free + 4096, width, None, width, None) == -1 and b"overlaps an operand" in lib.q1env_last_error(), name
+    ok = head(rows=rows, width=width, classes=classes, **at)
+    assert b(0, None, C.byref(ok), at["ws_dev"] + 64, None, None, free + 4096, width, None, width, None) == -1 and b"workspace overlaps an upstream" in lib.q1env_last_error()
