@@ -91,8 +91,9 @@ def clip_grads_(params, grad_clip):
         from .clip import clip_grad_norm_
         return clip_grad_norm_(grads, grad_clip)
     norm = torch.sqrt(sum((g.double() ** 2).sum() for g in grads)).float()
+    factor = torch.where(norm <= grad_clip, 1.0, grad_clip / norm)
     for g in grads:
-        g.mul_(grad_clip / torch.clamp(norm, min=grad_clip))
+        g.mul_(factor)
     return norm
 
 

@@ -347,3 +347,17 @@ def test_evaluate_actions_term_by_term(steps, batch):
         assert all(p.grad is not None and bool(p.grad.any()) for p in pol.pi.parameters())
         # a part that were missing would be over its bound somewhere: it is larger than the bound as a whole
         assert float(th.norm()) < float(dh.norm()) and float(tw.norm()) < float(dw.norm())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_an_infinite_bound_measures_and_leaves_the_gradients(device):
+    """grad_clip=inf is how a learner asks for the norm alone: inf / inf is no factor"""
+    params = [torch.nn.Parameter(p.detach().to(device)) for p in grads_of(0, 1.0)]
+    for p, q in zip(params, grads_of(0, 1.0)):
+        p.grad = q.grad.to(device)
+    kept = [p.grad.clone() for p in params]
+    norm = float(ppo.clip_grads_(params, float("inf")))
+    assert abs(norm - float(torch.sqrt(sum((k.double() ** 2).sum() for k in kept)))) <= 1e-6 * norm
+    assert all(torch.equal(p.grad, k) for p, k in zip(params, kept))
+    params[0].grad[0, 0] = float("inf")
+    assert ppo.clip_grads_(params, 1.0) == float("inf") and bool((params[1].grad == 0).all()) and bool(torch.isnan(params[0].grad[0, 0]))
