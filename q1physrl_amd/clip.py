@@ -65,6 +65,8 @@ def _layouts(tensors, out):
         o = t if out is None else out[i]
         if t.numel() == 0:
             continue
+        if t.is_neg() != o.is_neg():
+            raise ValueError(f"tensor {i} or its out is a lazily negated view (of a conjugate): call resolve_neg() first")
         a, b = _pitched(t), _pitched(o)
         c = 0 if a is None or b is None else min((x for x in (a[0], b[0]) if x), default=0)
         if a is None or b is None or (out is not None and _order(t) != _order(o)) or (a[0] or c) != c or (b[0] or c) != c:

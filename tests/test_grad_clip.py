@@ -329,3 +329,14 @@ def test_the_library_refuses_a_norm_or_workspace_over_a_tensor():
     # beside them: on to the next check (no such device)
     for kw in (dict(src=[a, b], values=[10, 10], norm=a + 40), dict(src=[a, 0], values=[10, 0])):
         assert norm_only(device=99, **kw) != 0 and b"the norm or the workspace" not in lib.q1env_last_error()
+
+
+def test_lazily_negated_views_are_not_taken_for_their_memory():
+    """the imaginary part of a conjugate holds the opposite of what its memory does"""
+    x = torch.randn(5, 3, dtype=torch.complex64).conj().imag
+    assert x.is_neg()
+    with pytest.raises(ValueError, match="negated"):
+        clip._layouts([x], [torch.zeros(5, 6)[:, ::2]])
+    with pytest.raises(ValueError, match="negated"):
+        clip._layouts([torch.zeros(5, 6)[:, ::2]], [x])
+    clip._layouts([x], None)                                        # in place a factor commutes with the sign
