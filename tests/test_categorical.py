@@ -764,3 +764,47 @@ def test_the_library_refuses_a_workspace_or_state_over_an_operand():
                 assert b(0, None, C.byref(hd), free, None, None, free + 4096, width, None, width, None) == -1 and b"overlaps an operand" in lib.q1env_last_error(), name
     ok = head(rows=rows, width=width, classes=classes, **at)
     assert b(0, None, C.byref(ok), at["ws_dev"] + 64, None, None, free + 4096, width, None, width, None) == -1 and b"workspace overlaps an upstream" in lib.q1env_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(20, 61, 300), (20, 64, 300), (60, 72, 500), (300, 64, 31), (300, 200, 700), (1500, 136, 2100)])
+@pytest.mark.parametrize("gap", [0, 3, 8])
+def test_results_at_a_pitch_and_every_choice_of_them(n, d, v, dtype, gap):
+    """the C call writes rows of `width` values at any pitch and leaves what lies between them, and each of the three gradients is the same whichever others are asked for"""
+    lib = _lib.load()
+    h, w, b, t = make(n, d, v, dtype, seed=n + d)
+    want = categorical.linear_cross_entropy_grad(h, w, t, b)[1:]
+    dev, stream = h.device.index, torch.cuda.current_stream().cuda_stream
+    dt = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+
+    def struct(ws):
+        return _lib.Q1Head(dt, 64, n, d, v, IGN, h.data_ptr(), d, w.data_ptr(), d, b.data_ptr(), t.data_ptr(), state.data_ptr(), ws.data_ptr(), ws.numel())
+    state = torch.empty(lib.q1env_head_state_bytes(n), dtype=torch.uint8, device="cuda")
+    logp, loss, one = torch.empty(n, device="cuda"), torch.empty((), device="cuda"), torch.ones((), device="cuda")
+    ws = torch.empty(lib.q1env_head_workspace_bytes(dt, n, d, v, 0), dtype=torch.uint8, device="cuda")
+    _lib.check(lib.q1env_head_forward(dev, stream, C.byref(struct(ws)), 0, logp.data_ptr(), None, loss.data_ptr()))
+    ws = torch.empty(lib.q1env_head_workspace_bytes(dt, n, d, v, 1), dtype=torch.uint8, device="cuda")
+    for asked in range(1, 8):
+        dh, dw, db = (torch.full(s, 7.0, dtype=dtype, device="cuda") for s in ((n, d + gap), (v, d + gap), (v + 5,)))
+        p = [x.data_ptr() if asked >> k & 1 else None for k, x in enumerate((dh, dw, db))]
+        _lib.check(lib.q1env_head_backward(dev, stream, C.byref(struct(ws)), None, None, one.data_ptr(), p[0], d + gap, p[1], d + gap, p[2]))
+        for k, (x, ref) in enumerate(zip((dh[:, :d], dw[:, :d], db[:v]), want)):
+            if not asked >> k & 1:
+                assert bool((x == 7).all())
+            elif (asked == 7 and gap in (0, 8)) or k == 2:
+                assert torch.equal(x, ref)                                    # the Python call, whole
+            else:                                                             # (sums may be split elsewhere, and stored by other instructions: the same value to a rounding of the type and of the sums)
+                far = (x.double() - ref.double()).abs() - 2.1 * HALF[dtype] * ref.double().abs() - (n + v + 16) * 2 * U * float(ref.abs().max())
+                assert float(far.max()) <= (2.0 ** -24 if dtype == torch.float16 else 0.0)
+        assert bool((dh[:, d:] == 7).all()) and bool((dw[:, d:] == 7).all()) and bool((db[v:] == 7).all())
+
+
+@gpu
+def test_no_rows_and_a_pitch():
+    lib = _lib.load()
+    w, dw, db = torch.randn(50, 24, device="cuda"), torch.full((50, 31), 7.0, device="cuda"), torch.full((53,), 7.0, device="cuda")
+    hd = _lib.Q1Head(0, 64, 0, 24, 50, IGN, None, 24, w.data_ptr(), 24, None, None, None, None, 0)
+    one = torch.ones((), device="cuda")
+    _lib.check(lib.q1env_head_backward(0, torch.cuda.current_stream().cuda_stream, C.byref(hd), None, None, one.data_ptr(), None, 24, dw.data_ptr(), 31, db.data_ptr()))
+    assert not bool(dw[:, :24].any()) and bool((dw[:, 24:] == 7).all()) and not bool(db[:50].any()) and bool((db[50:] == 7).all())
