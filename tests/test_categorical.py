@@ -808,3 +808,13 @@ def test_no_rows_and_a_pitch():
     one = torch.ones((), device="cuda")
     _lib.check(lib.q1env_head_backward(0, torch.cuda.current_stream().cuda_stream, C.byref(hd), None, None, one.data_ptr(), None, 24, dw.data_ptr(), 31, db.data_ptr()))
     assert not bool(dw[:, :24].any()) and bool((dw[:, 24:] == 7).all()) and not bool(db[:50].any()) and bool((db[50:] == 7).all())
+
+
+@gpu
+def test_functional_transforms_are_refused_not_answered_wrongly():
+    h, w, b, t = make(12, 16, 20, torch.float32, ignored=0.0)
+    for f in (lambda: torch.func.grad(lambda x: categorical.linear_cross_entropy(x, w, t, b))(h), lambda: torch.func.jvp(lambda x: categorical.linear_cross_entropy(x, w, t, b), (h,), (h,)),
+              lambda: torch.vmap(lambda x, y: categorical.linear_cross_entropy(x, w, y, b))(h.view(3, 4, 16), t.view(3, 4)),
+              lambda: torch.func.jacrev(lambda x: categorical.linear_categorical(x, w, t, b)[0])(h)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            f()
