@@ -818,3 +818,27 @@ def test_functional_transforms_are_refused_not_answered_wrongly():
               lambda: torch.func.jacrev(lambda x: categorical.linear_categorical(x, w, t, b)[0])(h)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             f()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(5, 8, 2 ** 22), (70, 8, 2 ** 22), (2 ** 22, 4, 3), (2 ** 22, 8, 40), (3, 2 ** 16, 5), (40, 2 ** 16, 70), (300, 2 ** 16, 33)])
+def test_sizes_at_their_limits(n, d, v, dtype):
+    _room(40)
+    h, w, b, t = make(n, d, v, dtype, seed=d, ignored=0.2)
+    leaves = [x.requires_grad_() for x in (h, w, b)]
+    logp, ent = categorical.linear_categorical(h, w, t, b)
+    T = Truth(h, w, b, t)
+    near(logp, T.logp, T.elogp, "logp")
+    near(ent, T.entropy, T.eent, "entropy")
+    A, E = torch.linspace(-1, 1, n, device="cuda"), torch.linspace(0.5, -0.5, n, device="cuda")
+    got = torch.autograd.grad((logp, ent), leaves, (A, E))
+    for name, x, (r, tol) in zip(("dh", "dw", "db"), got, T.grads(A, E)):
+        near(x, r, tol, name)
+    del T, got, leaves, logp, ent
+    torch.cuda.empty_cache()
+    for rows, width, classes in ((n + 1, d, v), (n, d + 1, v), (n, d, v + 1)):
+        if rows > 2 ** 22 or width > 2 ** 16 or classes > 2 ** 22:
+            with pytest.raises(ValueError, match="out of range"):
+                categorical.linear_categorical(torch.empty(rows, width, dtype=dtype, device="cuda"), torch.empty(classes, width, dtype=dtype, device="cuda"),
+                                               torch.zeros(rows, dtype=torch.int64, device="cuda"))
