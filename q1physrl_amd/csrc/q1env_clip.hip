@@ -7,7 +7,7 @@
 // launch - and writes its share, last values first: those the device's last-level cache still holds from the first pass.  Up to SLOTS table slots travel in the kernel
 // arguments; longer lists are first written to the workspace by small launches that carry SLOTS each.  Nothing is uploaded or kept between calls, and a captured
 // launch holds its own table.
-// Bound: memory.  536 870 913 float32 values (2.1 GB read, read again, written): 395 us for the first pass (5.4 TB/s), 794 for the second (5.4 TB/s; a plain copy makes 4.8).
+// Bound: memory.  536 870 913 float32 values (2.1 GB read, read again, written): 366 - 372 us for the first pass (5.8 TB/s), 795 - 807 for the second (5.4 TB/s; a plain copy makes 4.8).
 #include "q1env_host.hpp"
 
 #include <float.h>

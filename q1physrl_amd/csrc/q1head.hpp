@@ -431,8 +431,8 @@ __device__ __forceinline__ void start(Acc<C>& acc, const void* bias, int64_t bas
 // class-tile statistics of each row, and the logit of the row's own class.  The accumulators never leave the registers: one fused multiply-add, one exponential, an addition (and two more
 // instructions for the entropy) per logit, then three floats per row and tile.
 // Bound: the matrix pipe where k is long (8192 x 2048 x 131072 bfloat16: 3.40 ms, 1290 TFLOP/s, the pipe 67 % busy, no bank conflict; a large library product makes 1225 to 1481); the weights
-// where there are few rows (64 x 4096 x 131073: 194 us, 5.5 TB/s); start and epilogue of a tile where k is short (50176 x 256 x 4352: 151 us, 739 TFLOP/s, two workgroups per CU in different phases; 164 with one of
-// 256 x 256).
+// where there are few rows (64 x 4096 x 131073: 193 us, 5.6 TB/s); start and epilogue of a tile where k is short (50000 x 256 x 4097: 156 us in a run of passes, 672 TFLOP/s, two workgroups per CU in different
+// phases, the pipe 32 % busy; 198 in the first passes of an idle card).
 template <class C, int DT, bool ENTROPY>
 __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) statistics_kernel(Head hd, Target target, int64_t tile0, float* __restrict__ part, float* __restrict__ own_logit) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -705,7 +705,7 @@ __device__ __forceinline__ float sums_of_32(float (&v)[32], int lane, int& which
 
 // a piece [c0, c1) of the classes: the logits again, and the gradient of each -> g[row][class - c0] (stride `piece`; 16 bits, float32 as three pieces g_plane values apart), zero
 // up to the end of the last tile; and the sums over this tile's rows -> db_part[row tile][class]
-// Bound: as statistics_kernel, and 16 bits per logit written (8192 x 2048 x 28672: 844 us, 1140 TFLOP/s, 470 MB; 50176 x 256 x 4352: 219 us, 437 MB).  Storing g costs less than a third
+// Bound: as statistics_kernel, and 16 bits per logit written (8192 x 2048 x 28672: 840 us, 1145 TFLOP/s, 470 MB; 50000 x 256 x 4097: 219 us in a run of passes, 268 in the first of an idle card, 416 MB).  Storing g costs less than a third
 // computation of the logits, which both products would otherwise need.
 // GP: pieces the gradient is stored in.  One in 16-bit types: its rounding leaves an error of the size that the result's own rounding leaves anyway (bfloat16, random upstream, 50176 rows:
 // 0.0024 of the results' norm instead of 0.0017), and a second piece would double the products.  Two up to 256 rows, where the few roundings need not even out (2 rows of 2 classes: 0.004 with
@@ -846,7 +846,7 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) gradient_kernel(Head 
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // float32 with few rows or few classes (32 at most): memory decides, the float32 matrix instruction (16 FLOP per byte at 32) is fast enough, and laying pieces out
-// would cost several times the reading: 100000 x 256 x 32 takes 57 us forward and 250 with gradients, 33 classes laid out take 105 and 385; 32 x 4096 x 4096 54 and 166, 33 rows 152 and 363.  No LDS on the way in: a lane loads 16 bytes at k = 8 q + 4 (lane >> 5) of its class, row or column and feeds them to four instructions - which
+// would cost several times the reading: 100000 x 256 x 32 takes 59 us forward and 238 with gradients, 33 classes laid out take 107 and 377; 32 x 4096 x 4096 54 and 166, 33 rows 153 and 356.  No LDS on the way in: a lane loads 16 bytes at k = 8 q + 4 (lane >> 5) of its class, row or column and feeds them to four instructions - which
 // value of k a lane holds does not matter as long as both operands hold the same.
 // What lies outside is loaded from `safe` (any address that may be read) and replaced by zero, without a branch.  Loads of 16 bytes may start at any float.
 typedef f32x4 __attribute__((aligned(4))) f32x4_any;
@@ -993,7 +993,7 @@ __global__ void __launch_bounds__(256) skinny_gradient_kernel(Skinny q, Upstream
 
 // dW = g^T h and dh = g W from the stored gradient, both in one launch where they take the same tiles.  The operands lie with k outermost (h, W, and g for dW): ds_read_tr turns them on the
 // way from the LDS.  A sum is split over workgroups where its tiles would leave CUs idle; the parts are added in order (same bits every time), no atomics.
-// Bound: the matrix pipe (8192 x 2048 x 28672, both: 1.65 ms, 1165 TFLOP/s, 58 % busy; 50000 x 256 x 4097: 250 us, 840 TFLOP/s: 451 units of work on 256 CUs).
+// Bound: the matrix pipe (8192 x 2048 x 28672, both: 1.61 - 1.66 ms, 1195 - 1160 TFLOP/s, 58 % busy; 50000 x 256 x 4097: 243 - 273 us, 865 - 770 TFLOP/s, 41 % busy: two rounds of 256 CUs).
 // out[n][m] (stride out_stride): m = column of the result (width), n = its row.  slab: the sums stay in float32 [split][rows][width] for
 // finish_kernel (accumulate: added to what is there); without it the scaled result is stored.
 struct Product {
@@ -1171,7 +1171,7 @@ __global__ void __launch_bounds__(256) skinny_product_kernel(SkinnyProduct q, Up
     }
 }
 
-// result = scale x sum of the slabs, in their order (22 us for 15 slabs of 4097 x 256 and the bias at 50000 rows); and db[class] = scale x sum over the row tiles: 64 classes per workgroup, wave g takes tiles g, g + 4, ...
+// result = scale x sum of the slabs, in their order (23 us for the slabs of 4097 x 256 and the bias at 50000 rows); and db[class] = scale x sum over the row tiles: 64 classes per workgroup, wave g takes tiles g, g + 4, ...
 struct Finish {
     const float* slab;
     int64_t splits, rows, width;

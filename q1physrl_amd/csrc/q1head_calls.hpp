@@ -11,7 +11,9 @@
 namespace q1head {
 namespace {
 
-constexpr uint64_t PIECE_BYTES = 448ull << 20;     // of the gradient of one piece of the classes (half of it: 15 % slower at 50000 x 256 x 4097 and 4096 x 1024 x 32768, 1 % at 8192 x 2048 x 131072)
+// of the gradient of one piece of the classes, which is 256 classes at least: beyond 305 000 float32 or 917 000 16-bit rows that is more (6.4 GB at 2^22 float32 rows).
+// (Half of it: 15 % slower at 50000 x 256 x 4097 and 4096 x 1024 x 32768, 1 % at 8192 x 2048 x 131072.)
+constexpr uint64_t PIECE_BYTES = 448ull << 20;
 // of the laid-out weights of one piece.  float32 always needs them: a piece of 96 MiB costs 10 to 20 % (1578 x 1344 x 16658: 2115 us against 1726, 64 x 1024 x 50000 forward 238 against 180); 16-bit
 // weights only where they are not aligned
 constexpr uint64_t laid_bytes(int dt) { return dt == 0 ? 448ull << 20 : 160ull << 20; }
@@ -59,7 +61,7 @@ int64_t bn_of(Size s) { return s == LARGE || s == PAIR ? 256 : s == MIDDLE ? 128
 
 // The tile of a product of m x n results with k terms, and into how many parts its sum is split, by what it should take in nanoseconds.  One round of Large workgroups (256,
 // one per CU) was measured at 31 ns per term of k (1075 TFLOP/s), one of Middle (512, two per CU) at 18 (930), of Pair (512) at 36; Start is what a round costs besides, prologue and epilogue:
-// 50176 x 256 x 4352 takes 164 / 189 / 151 us of statistics and 250 / 294 / 219 of gradients in Large / Middle / Pair, 4096 x 1024 x 32768 282 / 356 / 331 of statistics.  The slabs of a split sum
+// 50176 x 256 x 4352 (whole tiles), each kernel alone in a loop, takes 164 / 189 / 151 us of statistics and 250 / 294 / 219 of gradients in Large / Middle / Pair, 4096 x 1024 x 32768 282 / 356 / 331 of statistics.  The slabs of a split sum
 // are written and read once at 4.5 TB/s.
 struct Start { double large, middle, pair; };          // nanoseconds; pair 0: not for this product
 constexpr Start STATISTICS{4500.0, 2600.0, 2400.0}, GRADIENT{11500.0, 6800.0, 7600.0}, PRODUCT{4000.0, 3000.0, 0.0};
