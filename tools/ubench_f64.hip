@@ -3,7 +3,7 @@
 // clock measured in the same launch (s_memtime ticks over wall_clock64's 100 MHz) - the inputs of the VALU-issue roofline of the
 // register-resident kernels (tools/valu_model.py).  Eight independent dependency chains per wave, so the
 // figure is ISSUE cost, not latency.
-// Build + run: hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/ubench_f64.hip -o gpurun_scratch/ubench_f64 && ./gpurun_scratch/ubench_f64
+// Build + run: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 tools/ubench_f64.hip -o gpurun_scratch/ubench_f64 && ./gpurun_scratch/ubench_f64
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

@@ -1,5 +1,5 @@
 // Instruction-rate micro-benchmarks on gfx950 (issue cost per wave64 instruction; MFMA/VALU co-issue) behind DESIGN.md section 8.
-// Build + run: hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/ubench_gfx950.hip -o gpurun_scratch/ubench && gpurun -- ./gpurun_scratch/ubench
+// Build + run: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 tools/ubench_gfx950.hip -o gpurun_scratch/ubench && gpurun -- ./gpurun_scratch/ubench
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>
@@ -32,15 +32,6 @@ __global__ void __launch_bounds__(512) k_fma(float* o, float s) {
                      : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3), "+v"(a4), "+v"(a5), "+v"(a6), "+v"(a7));
     }
     o[blockIdx.x * blockDim.x + threadIdx.x] = a0 + a1 + a2 + a3 + a4 + a5 + a6 + a7;
-}
-__global__ void __launch_bounds__(512) k_pkfma(float* o, float s) {
-    f32x2 a0 = {s + threadIdx.x, s}, a1 = a0 + 1.f, a2 = a0 + 2.f, a3 = a0 + 3.f, a4 = a0 + 4.f, a5 = a0 + 5.f, a6 = a0 + 6.f, a7 = a0 + 7.f;
-    for (int i = 0; i < ITER; ++i) {
-        asm volatile("v_pk_fma_f32 %0, %0, %0, %0\n v_pk_fma_f32 %1, %1, %1, %1\n v_pk_fma_f32 %2, %2, %2, %2\n v_pk_fma_f32 %3, %3, %3, %3\n v_pk_fma_f32 %4, %4, %4, %4\n v_pk_fma_f32 %5, %5, %5, %5\n v_pk_fma_f32 %6, %6, %6, %6\n v_pk_fma_f32 %7, %7, %7, %7\n"
-                     : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3), "+v"(a4), "+v"(a5), "+v"(a6), "+v"(a7));
-    }
-    f32x2 r = a0 + a1 + a2 + a3 + a4 + a5 + a6 + a7;
-    o[blockIdx.x * blockDim.x + threadIdx.x] = r[0] + r[1];
 }
 __global__ void __launch_bounds__(512) k_cvt(float* o, float s) {
     float a0 = s + threadIdx.x, a1 = a0 + 1, a2 = a0 + 2, a3 = a0 + 3, a4 = a0 + 4, a5 = a0 + 5, a6 = a0 + 6, a7 = a0 + 7;
@@ -137,7 +128,6 @@ int main() {
         run(k_exp, "v_exp_f32", 8, threads, d);
         run(k_rcp, "v_rcp_f32", 8, threads, d);
         run(k_fma, "v_fma_f32", 8, threads, d);
-        run(k_pkfma, "v_pk_fma_f32", 8, threads, d);
         run(k_cvt, "v_cvt_pk_bf16_f32", 8, threads, d);
         run(k_accread, "v_accvgpr_read_b32", 8, threads, d);
         run(k_mfma<0>, "mfma 32x32x16 bf16", 8, threads, d);

@@ -3,7 +3,7 @@
 // Eight independent dependency chains per wave (issue cost, not latency), at 1 and 2 waves per SIMD, for float64 FMA / MUL / ADD and
 // float32 FMA, with EXEC = all 64 lanes, the LOW 32 lanes, the EVEN lanes (control: as many active lanes, spread over every pass),
 // and the low 16 lanes.  Prints shader cycles per instruction per wave (s_memtime over wall_clock64, as tools/ubench_f64.hip).
-// Build + run: hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/ubench_halfexec.hip -o tools/_bin/ubench_halfexec && tools/_bin/ubench_halfexec
+// Build + run: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 tools/ubench_halfexec.hip -o tools/_bin/ubench_halfexec && tools/_bin/ubench_halfexec
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

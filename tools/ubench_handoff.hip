@@ -7,7 +7,7 @@
 //   mode 3: both stores; the L2 copy is polled `m` times for every poll of the sc1 copy (placement-independent AND L2-fast when
 //           the pair shares an XCD; a pair that does not pays m wasted L2 polls per hop: slower, not wrong)
 // shift = 0 pairs block b with block B + b (same XCD when B % 8 == 0: blocks are observed to go to XCD id % 8); shift = 1 pairs
-// across XCDs.  Build: hipcc --offload-arch=gfx950 -O3 -o ubench_handoff tools/ubench_handoff.hip ; run: ./ubench_handoff
+// across XCDs.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o ubench_handoff tools/ubench_handoff.hip ; run: ./ubench_handoff
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>

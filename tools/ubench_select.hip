@@ -3,7 +3,7 @@
 // ~45 of them.  This probe separates the causes: mask in VCC vs an SGPR pair, e32 vs e64 encoding, interleaving with other VALU work,
 // a v_cmp in front, and the alternatives a select can be rewritten into (v_bfi_b32 / v_and_b32 with a lane mask in a VGPR, v_med3,
 // v_max / v_min, multiply by 0 / 1).  Eight independent chains per wave: issue cost, not latency; plus single-chain latencies.
-// Build + run: hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/ubench_select.hip -o gpurun_scratch/ubench_select && ./gpurun_scratch/ubench_select
+// Build + run: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 tools/ubench_select.hip -o gpurun_scratch/ubench_select && ./gpurun_scratch/ubench_select
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

@@ -1,6 +1,6 @@
 // ubench_stage.hip - how long does it take every CU to copy the SAME 152 KB weight image from L2 into its LDS (the prologue of the
 // policy / learner kernels), and does the ORDER in which the workgroups walk the image matter?
-//   hipcc --offload-arch=gfx950 -O3 tools/ubench_stage.hip -o /tmp/ubench_stage && /tmp/ubench_stage
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench_stage.hip -o /tmp/ubench_stage && /tmp/ubench_stage
 // mode 0: every workgroup copies chunk k = 0, 1, 2, ... (what stage_image / stage_copy did until round 4)
 // mode 1: workgroup b starts at chunk (b * 5) mod PER and wraps (the workgroups of an XCD address different 4 KB chunks at any moment)
 // mode 2: as 0, but only ONE workgroup per XCD... (grid of 8): the no-contention reference

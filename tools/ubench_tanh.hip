@@ -15,7 +15,7 @@
 //      is clamped to 30 so that the product of four stays finite
 // Per variant: ns per activation per wave at 1 / 2 waves per SIMD (256 workgroups x 256 / 512 threads), and the largest error of the
 // f16 result against tanh in double over z in [-9, 9] (the f16 operand the next layer consumes has 2^-11 relative resolution).
-// Build + run: hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/ubench_tanh.hip -o gpurun_scratch/ubench_tanh && ./gpurun_scratch/ubench_tanh
+// Build + run: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 tools/ubench_tanh.hip -o gpurun_scratch/ubench_tanh && ./gpurun_scratch/ubench_tanh
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdio.h>
